@@ -249,7 +249,7 @@ def _rotated(x, heads, case, freq, positions):
 
 
 class _Cache:
-    """K and V rows as the cache types hold them: codes, with a scale (and an offset) per row or per block of 32."""
+    """K and V rows as the cache types hold them: codes, with a scale per row, or a step and a middle per block of 32."""
 
     def __init__(self, kind, n, kv_dim):
         self.kind = kind
@@ -277,11 +277,11 @@ class _Cache:
                 b = x.reshape(n, -1, 32)
                 lo, hi = b.amin(dim=2), b.amax(dim=2)
                 sc = ((hi - lo) / torch.full_like(lo, 15.0)).clamp(max=512.0).half()
-                off = (lo - 16 * sc.float()).clamp(-65504.0, 65504.0).half()
-                z = (b - off.float()[..., None]) / sc.float()[..., None]
-                code = torch.where(sc[..., None] > 0, (torch.round(z) - 16).clamp(0, 15), torch.zeros_like(z))
+                mid = (lo + 8 * sc.float()).clamp(-65504.0, 65504.0).half()
+                z = (b - mid.float()[..., None]) / sc.float()[..., None]
+                code = torch.where(sc[..., None] > 0, (torch.round(z) + 8).clamp(0, 15), torch.full_like(z, 8))
                 self.codes[which][pos:pos + n] = code.reshape(n, -1).to(torch.uint8)
-                self.scales[which][pos:pos + n, 0], self.scales[which][pos:pos + n, 1] = sc, off
+                self.scales[which][pos:pos + n, 0], self.scales[which][pos:pos + n, 1] = sc, mid
 
     def values(self, which, pos, n):
         c = self.codes[which][pos:pos + n]
@@ -292,7 +292,7 @@ class _Cache:
         sc = self.scales[which][pos:pos + n]
         if self.kind == "q8":
             return c.float() * sc
-        return ((c.float() + 16).reshape(n, -1, 32) * sc[:, 0].float()[..., None] + sc[:, 1].float()[..., None]).reshape(n, -1)
+        return ((c.float() - 8).reshape(n, -1, 32) * sc[:, 0].float()[..., None] + sc[:, 1].float()[..., None]).reshape(n, -1)
 
 
 def _half_bits(x):
@@ -433,9 +433,9 @@ def _stored(x, kind):
     blocks = x.reshape(-1, 32)
     small, large = torch.aminmax(blocks, dim=1, keepdim=True)
     step = torch.minimum(torch.div(large - small, torch.full_like(small, 15)), torch.full_like(small, 512)).to(torch.float16)
-    origin = (small - step.float() * 16).clamp(-65504, 65504).to(torch.float16).float()
-    level = torch.where(step > 0, torch.div(blocks - origin, step.float()), torch.full_like(blocks, 16)).round().clamp(16, 31)
-    return (level.double() * step.double() + origin.double()).reshape(x.shape)
+    middle = (small + step.float() * 8).clamp(-65504, 65504).to(torch.float16).float()
+    level = torch.where(step > 0, torch.div(blocks - middle, step.float()), torch.zeros_like(blocks)).round().clamp(-8, 7)
+    return (level.double() * step.double() + middle.double()).reshape(x.shape)
 
 
 def exact(case, seed):
