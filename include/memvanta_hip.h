@@ -77,6 +77,21 @@ extern "C" {
 #define MVH_KV_F32 0
 #define MVH_KV_F16 1 /* LlamaModel's default */
 #define MVH_KV_Q8 2  /* int8 with one float scale per token and K/V row */
+/* No counterpart in the reference: 4-bit codes n with an fp16 step s and middle c per token and block of 32
+ * channels, x = c + s (n - 8): s = fp16(min((max - min) / 15, 512)), c = fp16(min + 8 s) (at most +-65504), n =
+ * round((x - c) / s) + 8 (ties to even) in 0..15, each step rounded to 32 bits; 5 bits an element.  A block that
+ * holds a NaN or an infinity reads back as NaN.  kv_dim % 32 == 0.  A word of a V page holds 8 rows: writes to
+ * one such cache from several streams must be ordered, also where their positions differ. */
+#define MVH_KV_Q4 3
+
+/* rotary positions: which elements of a head form a pair (rot = the rotated elements, from the head's first) */
+#define MVH_ROPE_HALF 0        /* (i, i + rot/2): LlamaModel::rope_ptr, src/llama_model.cpp:238 */
+#define MVH_ROPE_INTERLEAVED 1 /* (2i, 2i + 1) */
+/* and how the angles f_i = base^(-2i/rot) per position are scaled for contexts longer than the trained one */
+#define MVH_ROPE_SCALE_NONE 0
+#define MVH_ROPE_SCALE_LINEAR 1 /* f_i / factor */
+#define MVH_ROPE_SCALE_TURNS 2  /* g f_i + (1 - g) f_i / factor; g by the turns r = orig_ctx f_i / 2 pi: 0 up to low, 1 from high, linear between */
+#define MVH_ROPE_SCALE_INDEX 3  /* the same with g linear in i: 1 up to the pair (rounded down) of high turns, 0 from that (rounded up) of low */
 
 /* GGML type ids accepted by mvh_tensor_upload */
 #define MVH_TYPE_F32 0
@@ -96,6 +111,7 @@ typedef struct mvh_context mvh_context;
 typedef struct mvh_tensor mvh_tensor;
 typedef struct mvh_kv_cache mvh_kv_cache;
 typedef struct mvh_model mvh_model;
+typedef struct mvh_rope mvh_rope;
 
 /* ---- library / context ---- */
 const char* mvh_last_error(void);
@@ -157,6 +173,15 @@ int mvh_stream_read(mvh_context* ctx, const void* buf, size_t bytes, uint32_t* s
  * the maximum of logits[r*n .. r*n+n) (std::max_element), for rows rows of NaN-free logits; n == 0 fails with
  * "empty logits" */
 int mvh_argmax(mvh_context* ctx, const float* logits, size_t n, size_t rows, int* out, int ptr_kind);
+/* No counterpart in the reference: what the logits say about each row's distribution (softmax), in one pass.
+ * logits [rows][n], targets [rows] token ids (NULL: no logprob), each output may be NULL: logprob [rows] =
+ * log p(target), entropy [rows] in nats, top_ids / top_logprobs [rows][top_k] = the top_k <= 64 most probable
+ * tokens, ties by the lower id.  -inf marks a masked token (log probability -inf); a row of nothing else has
+ * entropy 0 and log probability -inf everywhere; a NaN or +inf makes the row's float results NaN (its top_ids are
+ * then some ids of the row).  A target outside 0..n-1 fails with MVH_E_RANGE for host arrays and gives NaN for
+ * device ones.  Calls of one context share its workspace; see mvh_attn_decode for calls captured into graphs. */
+int mvh_logprobs(mvh_context* ctx, const float* logits, size_t n, size_t rows, const int* targets, size_t top_k,
+                 float* logprob, float* entropy, int* top_ids, float* top_logprobs, int ptr_kind);
 /* fp32_to_fp16 (the reference's rounding, bit for bit) and the exact fp16_to_fp32 */
 int mvh_fp32_to_fp16(mvh_context* ctx, const float* x, uint16_t* out, size_t n, int ptr_kind);
 int mvh_fp16_to_fp32(mvh_context* ctx, const uint16_t* h, float* out, size_t n, int ptr_kind);
@@ -178,27 +203,68 @@ int mvh_matvec_q4_0(mvh_context* ctx, const mvh_tensor* a, const float* x, float
 int mvh_matvec_q8_0(mvh_context* ctx, const mvh_tensor* a, const float* x, float* y, int ptr_kind);
 
 /* ---- paged KV cache (F32 / F16 / Q8 pages): all layers of one model on one device ---- */
-/* parse_kv_cache_type: "f32", "f16", "q8" or "q8_0"; anything else fails with
+/* parse_kv_cache_type: "f32", "f16", "q8" or "q8_0", and "q4"; anything else fails with
  * "unknown KV cache type: <s>" */
 int mvh_kv_parse_type(const char* s, int* kv_type);
-/* kv_cache_type_name: "f32", "f16", "q8", or "?" */
+/* kv_cache_type_name: "f32", "f16", "q8", "q4", or "?" */
 const char* mvh_kv_type_name(int kv_type);
+/* max_tokens up to 16000, of a Q4 cache up to 1048576 */
 int mvh_kv_create(mvh_context* ctx, size_t n_layer, size_t kv_dim, size_t page_tokens, size_t max_tokens,
                   int kv_type, mvh_kv_cache** out);
 int mvh_kv_destroy(mvh_kv_cache* kv);
 int mvh_kv_reset(mvh_kv_cache* kv);
 /* PagedKVCache::bytes_allocated: element bytes of K and V of every page any write touched, plus 4 bytes per
- * slot per Q8 scale array */
+ * slot per Q8 scale array; 5/8 byte an element for Q4 */
 int mvh_kv_bytes_allocated(const mvh_kv_cache* kv, size_t* bytes);
 int mvh_kv_type(const mvh_kv_cache* kv, int* kv_type);
 /* PagedKVCache::write for n_tokens consecutive positions pos..pos+n-1; k/v are [n][kv_dim] fp32 */
 int mvh_kv_write(mvh_context* ctx, mvh_kv_cache* kv, size_t layer, size_t pos, size_t n_tokens, const float* k,
                  const float* v, int ptr_kind);
 /* copy the stored row of (layer, pos): which = 0 for K, 1 for V; out is host memory for kv_dim elements of the
- * cache type (float, fp16 bits or int8); scale (may be NULL) receives the Q8 row scale, 1 for F32/F16 */
+ * cache type (float, fp16 bits or int8; for Q4 the float values the codes stand for); scale (may be NULL) receives
+ * the Q8 row scale, 1 for the other types */
 int mvh_kv_read_row(mvh_context* ctx, const mvh_kv_cache* kv, size_t layer, size_t pos, int which, void* out,
                     float* scale);
-/* decode attention of one layer over positions 0..pos: q[n_head*hd] -> out[n_head*hd] */
+/* No counterpart in the reference: rows pos..pos+n-1 of K and V as fp32 [n][kv_dim] (either may be NULL) */
+int mvh_kv_read(mvh_context* ctx, const mvh_kv_cache* kv, size_t layer, size_t pos, size_t n_tokens, float* k, float* v,
+                int ptr_kind);
+
+/* ---- rotary positions (no counterpart as a call of its own in the reference: LlamaModel::rope_ptr,
+ * src/llama_model.cpp:238, is the MVH_ROPE_HALF layout of a whole head without scaling) ----
+ * A pair (x0, x1) at position p becomes (x0 c - x1 s, x0 s + x1 c), c and s = attn_scale times cos and sin of p f_i.
+ * Angles, cos and sin are formed in 64 bits and rounded to 32 (so far positions keep their precision), products and
+ * sums are fp32, each rounded.  Elements from rot_dim on pass through. */
+typedef struct mvh_rope_config {
+    size_t head_dim;   /* even, up to 1024 */
+    size_t rot_dim;    /* even, 2 .. head_dim; 0: head_dim */
+    int layout;        /* MVH_ROPE_HALF or MVH_ROPE_INTERLEAVED */
+    int scaling;       /* MVH_ROPE_SCALE_* */
+    double base;       /* > 1 */
+    double factor;     /* > 0; read unless scaling is NONE */
+    double orig_ctx;   /* trained context, TURNS and INDEX: > 0 */
+    double low, high;  /* turns, TURNS and INDEX: 0 < low < high */
+    double attn_scale; /* > 0; 1 leaves lengths as they are */
+} mvh_rope_config;
+int mvh_rope_create(mvh_context* ctx, const mvh_rope_config* config, mvh_rope** out);
+int mvh_rope_destroy(mvh_rope* rope);
+/* the scaled f_i: out[rot_dim / 2], host memory */
+int mvh_rope_angles(const mvh_rope* rope, double* out);
+/* out row t = x row t rotated: n_tokens rows of n_head heads, x_pitch / out_pitch floats apart (at least
+ * n_head*head_dim); out may be x with the same pitch, and overlap it in no other way.  The position of row t is
+ * positions[t], or pos + t when positions is NULL. */
+int mvh_rope_apply(mvh_context* ctx, const mvh_rope* rope, const float* x, size_t x_pitch, size_t n_tokens, size_t n_head,
+                   const int* positions, size_t pos, float* out, size_t out_pitch, int ptr_kind);
+/* No counterpart in the reference: mvh_kv_write of k rotated (and v as it is) at positions pos..pos+n-1, rows k_pitch /
+ * v_pitch floats apart, and, when q is not NULL, q's n_head heads rotated to q_out, as mvh_rope_apply does it; any cache
+ * type.  kv_dim must be whole heads of a head_dim that is a multiple of 8.  q_out must not overlap k or v. */
+int mvh_kv_append(mvh_context* ctx, mvh_kv_cache* kv, size_t layer, size_t pos, size_t n_tokens, const mvh_rope* rope,
+                  const float* q, size_t q_pitch, size_t n_head, float* q_out, size_t out_pitch, const float* k,
+                  size_t k_pitch, const float* v, size_t v_pitch, int ptr_kind);
+
+/* decode attention of one layer over positions 0..pos: q[n_head*hd] -> out[n_head*hd].  Over a Q4 cache the calls
+ * of a context share its workspace, which a longer call replaces by a larger one; the old one is kept until the
+ * context is destroyed, so a captured graph stays valid.  Graphs captured from one context must not run at the same
+ * time, and a call whose workspace is not there yet cannot be captured (MVH_E_NOMEM): make it once before. */
 int mvh_attn_decode(mvh_context* ctx, const mvh_kv_cache* kv, size_t layer, const float* q, size_t pos,
                     size_t n_head, size_t n_head_kv, size_t head_dim, float* out, int ptr_kind);
 /* the batched causal attention of LlamaModel::forward_batch_impl (the per-(token, head) loop at
@@ -240,7 +306,7 @@ int mvh_profile_snapshot(mvh_profile_entry* out, size_t cap, size_t* n_total);
 const char* mvh_profile_kind_name(int kind);
 
 /* ---- whole model: LlamaModel on one device (weights, paged KV and activations in HBM) ---- */
-/* kv_type is LlamaModel's kv_type argument (MVH_KV_F16 is its default); act_mode selects the prefill numerics
+/* kv_type is LlamaModel's kv_type argument (MVH_KV_F16 is its default; MVH_KV_Q4 needs kv_dim % 32 == 0); act_mode selects the prefill numerics
  * (MVH_ACT_REF / MVH_ACT_Q8); max_batch bounds the prefill chunk */
 int mvh_model_open(const char* gguf_path, int device, size_t ctx_override, size_t kv_page_tokens, int kv_type,
                    int act_mode, size_t max_batch, mvh_model** out);

@@ -20,8 +20,12 @@ HEADER = os.path.join(os.path.dirname(HERE), "include", "memvanta_hip.h")
 MVH_HOST, MVH_DEVICE = 0, 1
 MVH_ACT_REF, MVH_ACT_Q8 = 0, 1
 MVH_KV_F32, MVH_KV_F16, MVH_KV_Q8 = 0, 1, 2  # KVCacheType order
+MVH_KV_Q4 = 3  # 4-bit codes, a step and a middle per block of 32
+MVH_ROPE_HALF, MVH_ROPE_INTERLEAVED = 0, 1
+MVH_ROPE_SCALE_NONE, MVH_ROPE_SCALE_LINEAR, MVH_ROPE_SCALE_TURNS, MVH_ROPE_SCALE_INDEX = 0, 1, 2, 3
 MVH_TYPE_NATIVE_Q4_0, MVH_TYPE_NATIVE_Q8_0 = 0x1002, 0x1008  # BlockQ4_0 (20 B) / BlockQ8_0 (36 B) of quant.hpp
-KV_DTYPE = {MVH_KV_F32: np.float32, MVH_KV_F16: np.uint16, MVH_KV_Q8: np.int8}
+KV_DTYPE = {MVH_KV_F32: np.float32, MVH_KV_F16: np.uint16, MVH_KV_Q8: np.int8,
+            MVH_KV_Q4: np.float32}
 STATUS = {0: "MVH_OK", 1: "MVH_E_INVALID", 2: "MVH_E_SHAPE", 3: "MVH_E_TYPE", 4: "MVH_E_DEVICE",
           5: "MVH_E_RANGE", 6: "MVH_E_NOMEM"}
 
@@ -76,6 +80,13 @@ _SIGS = {
     "mvh_kv_read_row": (_int, [_vp, _vp, _sz, _sz, _int, _vp, C.POINTER(C.c_float)]),
     "mvh_attn_decode": (_int, [_vp, _vp, _sz, _vp, _sz, _sz, _sz, _sz, _vp, _int]),
     "mvh_attn_batch": (_int, [_vp, _vp, _sz, _vp, _sz, _sz, _sz, _sz, _sz, _vp, _int]),
+    "mvh_kv_read": (_int, [_vp, _vp, _sz, _sz, _sz, _vp, _vp, _int]),
+    "mvh_rope_create": (_int, [_vp, _vp, C.POINTER(_vp)]),
+    "mvh_rope_destroy": (_int, [_vp]),
+    "mvh_rope_angles": (_int, [_vp, _vp]),
+    "mvh_rope_apply": (_int, [_vp, _vp, _vp, _sz, _sz, _sz, _vp, _sz, _vp, _sz, _int]),
+    "mvh_kv_append": (_int, [_vp, _vp, _sz, _sz, _sz, _vp, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _int]),
+    "mvh_logprobs": (_int, [_vp, _vp, _sz, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _int]),
     "mvh_model_open": (_int, [C.c_char_p, _int, _sz, _sz, _int, _int, _sz, C.POINTER(_vp)]),
     "mvh_model_kv_type": (_int, [_vp, C.POINTER(_int)]),
     "mvh_model_close": (_int, [_vp]),
@@ -105,6 +116,15 @@ class ProfileEntry(C.Structure):
 
     _fields_ = [("layer", C.c_int), ("kind", C.c_int), ("tensor", C.c_char * 192), ("calls", C.c_size_t),
                 ("batch", C.c_size_t), ("ms", C.c_double)]
+
+
+class RopeConfig(C.Structure):
+    """mvh_rope_config."""
+
+    _fields_ = [("head_dim", _sz), ("rot_dim", _sz), ("layout", _int), ("scaling", _int), ("base", C.c_double),
+                ("factor", C.c_double), ("orig_ctx", C.c_double), ("low", C.c_double), ("high", C.c_double),
+                ("attn_scale", C.c_double)]
+
 
 _lib = None
 
@@ -170,6 +190,21 @@ def _kind(*arrs) -> int:
     if not any(dev):
         return MVH_HOST
     raise ValueError("mix of host and device buffers in one call")
+
+
+def _rows(a):
+    """(a as rows of fp32 elements, elements from one row to the next): a torch view may keep its row stride."""
+    if isinstance(a, np.ndarray):
+        a = np.ascontiguousarray(a, np.float32)
+        a = a[None] if a.ndim == 1 else a
+        return a, a.shape[1]
+    if a.dim() == 1:
+        a = a[None]
+    if a.element_size() != 4 or not a.is_floating_point():
+        raise ValueError("rows must be float32")
+    if a.dim() != 2 or (a.shape[1] > 1 and a.stride(1) != 1):
+        raise ValueError("rows must be 2-D with consecutive elements")
+    return a, a.stride(0) if a.shape[0] > 1 else a.shape[1]
 
 
 class Context:
@@ -292,6 +327,37 @@ class Context:
         self._check(self.lib.mvh_argmax(self.h, _ptr(logits), n, rows, _ptr(out), _kind(logits, out)))
         return out
 
+    def logprobs(self, logits, targets=None, top_k: int = 0, logprob=None, entropy=None, top_ids=None,
+                 top_logprobs=None):
+        """mvh_logprobs of [rows][n] logits.  Host arrays: {"logprob" (with targets), "entropy", "top_ids",
+        "top_logprobs" (with top_k)} are returned; device buffers: the given outputs are written."""
+        if isinstance(logits, np.ndarray):
+            logits = np.ascontiguousarray(logits, np.float32)
+            logits = logits[None] if logits.ndim == 1 else logits
+            rows, n = logits.shape
+            out = {"entropy": np.empty(rows, np.float32)}
+            if targets is not None:
+                targets = np.ascontiguousarray(targets, np.int32).reshape(rows)
+                out["logprob"] = np.empty(rows, np.float32)
+            if top_k:
+                out["top_ids"] = np.empty((rows, top_k), np.int32)
+                out["top_logprobs"] = np.empty((rows, top_k), np.float32)
+            self._check(self.lib.mvh_logprobs(self.h, _ptr(logits), n, rows, _ptr(targets), top_k,
+                                              _ptr(out.get("logprob")), _ptr(out["entropy"]), _ptr(out.get("top_ids")),
+                                              _ptr(out.get("top_logprobs")), MVH_HOST))
+            return out
+        if not logits.is_contiguous():
+            raise ValueError("logits must be contiguous")
+        rows = 1 if logits.dim() == 1 else logits.shape[0]
+        self._check(self.lib.mvh_logprobs(self.h, _ptr(logits), logits.shape[-1], rows, _ptr(targets), top_k,
+                                          _ptr(logprob), _ptr(entropy), _ptr(top_ids), _ptr(top_logprobs), MVH_DEVICE))
+        return None
+
+    def rope(self, head_dim: int, rot_dim: int = 0, layout: int = MVH_ROPE_HALF, base: float = 10000.0,
+             scaling: int = MVH_ROPE_SCALE_NONE, factor: float = 1.0, orig_ctx: float = 0.0, low: float = 0.0,
+             high: float = 0.0, attn_scale: float = 1.0) -> "Rope":
+        return Rope(self, RopeConfig(head_dim, rot_dim, layout, scaling, base, factor, orig_ctx, low, high, attn_scale))
+
     def fp32_to_fp16(self, x, out=None):
         if out is None:
             x = np.ascontiguousarray(x, np.float32).ravel()
@@ -365,6 +431,49 @@ class Tensor:
         self.ctx._check(self.ctx.lib.mvh_tensor_info(self.h, C.byref(ty), C.byref(n0), C.byref(n1), C.byref(nb),
                                                      C.byref(dp)))
         return ty.value, n0.value, n1.value, nb.value, dp.value
+
+
+class Rope:
+    """Rotary positions (mvh_rope)."""
+
+    def __init__(self, ctx: Context, config: RopeConfig):
+        self.ctx, self.head_dim, self.rot_dim = ctx, config.head_dim, config.rot_dim or config.head_dim
+        h = _vp()
+        ctx._check(ctx.lib.mvh_rope_create(ctx.h, C.byref(config), C.byref(h)))
+        self.h = h.value
+
+    def close(self):
+        if getattr(self, "h", None):
+            self.ctx.lib.mvh_rope_destroy(self.h)
+            self.h = None
+
+    def __del__(self, _fin=_finalize):
+        _fin(self.close)
+
+    def angles(self) -> np.ndarray:
+        """Angle per position of each pair, scaled (float64)."""
+        out = np.empty(self.rot_dim // 2, np.float64)
+        self.ctx._check(self.ctx.lib.mvh_rope_angles(self.h, out.ctypes.data))
+        return out
+
+    def apply(self, x, n_head: int, pos: int = 0, out=None, positions=None):
+        """Rows of n_head heads rotated: row t by position positions[t] (int32), or pos + t.  Device rows may be a
+        view with a row stride; out may be x itself."""
+        x, pitch = _rows(x)
+        if x.shape[1] < n_head * self.head_dim:
+            raise ValueError("rows shorter than n_head heads")
+        if isinstance(x, np.ndarray):
+            out = np.empty((x.shape[0], n_head * self.head_dim), np.float32) if out is None else out
+            if positions is not None:
+                positions = np.ascontiguousarray(positions, np.int32)
+        y, out_pitch = _rows(out) if not isinstance(out, np.ndarray) else (out, out.shape[-1])
+        if y.shape[0] < x.shape[0] or y.shape[1] < n_head * self.head_dim:
+            raise ValueError("out is smaller than the rotated rows")
+        if positions is not None and (len(positions) != x.shape[0] or str(positions.dtype) not in ("int32", "torch.int32")):
+            raise ValueError("positions must be one int32 per row")
+        self.ctx._check(self.ctx.lib.mvh_rope_apply(self.ctx.h, self.h, _ptr(x), pitch, x.shape[0], n_head,
+                                                    _ptr(positions), pos, _ptr(y), out_pitch, _kind(x, y, positions)))
+        return out
 
 
 PROFILE_KINDS = ("q_proj", "k_proj", "v_proj", "o_proj", "ffn_gate", "ffn_up", "ffn_down", "output", "other")
@@ -450,6 +559,36 @@ class KVCache:
         self.ctx._check(self.ctx.lib.mvh_kv_read_row(self.ctx.h, self.h, layer, pos, which, out.ctypes.data,
                                                      C.byref(sc)))
         return out, np.float32(sc.value)
+
+    def append(self, layer, pos, k, v, rope: Rope, q=None, q_out=None):
+        """k rotated and v stored at positions pos.., and q (when given) rotated to q_out (which may be q).  Device
+        rows may be views of one fused buffer."""
+        k, k_pitch = _rows(k)
+        v, v_pitch = _rows(v)
+        n = k.shape[0]
+        if v.shape[0] != n or k.shape[1] != self.kv_dim or v.shape[1] != self.kv_dim:
+            raise ValueError("k and v must be rows of kv_dim elements")
+        y, n_head, q_pitch, out_pitch = None, 0, 0, 0
+        if q is not None:
+            host = isinstance(q, np.ndarray)
+            q, q_pitch = _rows(q)
+            if host and q_out is None:
+                q_out = np.empty_like(q)
+            y, out_pitch = (q_out, q_out.shape[-1]) if host else _rows(q_out)
+            if q.shape[0] != n or q.shape[1] % rope.head_dim or tuple(y.shape) != tuple(q.shape):
+                raise ValueError("q and q_out must be one row of whole heads per row of k")
+            n_head = q.shape[1] // rope.head_dim
+        self.ctx._check(self.ctx.lib.mvh_kv_append(self.ctx.h, self.h, layer, pos, n, rope.h, _ptr(q), q_pitch, n_head,
+                                                   _ptr(y), out_pitch, _ptr(k), k_pitch, _ptr(v), v_pitch,
+                                                   _kind(k, v, q, y)))
+        return q_out
+
+    def read(self, layer, pos, n, k=None, v=None):
+        """Rows pos .. pos+n-1 of K and V as float32 [n][kv_dim]: into device buffers, or returned as host arrays."""
+        if k is None and v is None:
+            k, v = (np.empty((n, self.kv_dim), np.float32) for _ in range(2))
+        self.ctx._check(self.ctx.lib.mvh_kv_read(self.ctx.h, self.h, layer, pos, n, _ptr(k), _ptr(v), _kind(k, v)))
+        return k, v
 
     def type(self) -> int:
         t = _int()

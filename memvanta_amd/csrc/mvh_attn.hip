@@ -1523,6 +1523,8 @@ hipError_t launch_kv_write(int kv_type, void* const* pt_k, void* const* pt_v, co
         kv_write_q8_kernel<<<dim3(static_cast<unsigned>(n_tokens), 2), kKW, 0, st>>>(pt_k, pt_v, k, v, ip, d_pos, ipos,
                                                                                   kd, pt);
         break;
+    case kKvQ4:
+        return launch_kv4_write(pt_k, pt_v, k, v, pitch, d_pos, pos, n_tokens, kv_dim, page_tokens, st);
     default:
         return hipErrorInvalidValue;
     }

@@ -1,0 +1,528 @@
+// mvh_attn_q4.hip -- attention over a paged KV cache held in 4 bits (layout
+// and format: mvh_kv4.hpp), of one token or a chunk of tokens.
+//
+//   y_t = log2(e) / sqrt(hd) * q.K_t,  out = sum_t 2^(y_t - m) V_t / sum_t 2^(y_t - m)
+// over rows t = 0 .. the token's position, in one pass with a running m.  Per
+// block of 32 channels K_t = c + s (n - 8), so
+//   q.K_t       = sum_b s_tb (sum_i q_i (n_ti - 8)) + c_tb sum_i q_i,
+//   sum p_t V_t = sum_t (p_t s_tb) (n_t - 8) + sum_t p_t c_tb :
+// n - 8 is exact in fp16, so the products run on the fp16 matrix pipe with the
+// codes as they are; q and p s are split into two fp16 (22 bits: 2^-22 of
+// the largest, where one fp16 would leave 2^-11), sums are fp32.
+#include "mvh_kernels.hpp"
+#include "mvh_kv4.hpp"
+
+namespace mvh {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+struct Q4Args {
+    const void* const* pt_k;
+    const void* const* pt_v;
+    const float* q;
+    float* out;
+    float* part;  // [row][split][hd], then [row][split][2]: sums and (m, l); null with one split
+    const int* d_pos;
+    size_t q_pitch;
+    int pos, n_tokens, n_head, group, kv_dim, hd;
+    int chunk;  // 32-row steps a split takes; 0: the rows' steps shared out evenly
+    Kv4Map map;
+};
+
+constexpr float kLowest = -3.0e38f;  // m before the first row: finite, so that 2^(-inf - m) is 0
+constexpr float kLog2e = 1.44269504088896340736f;
+// Weights are 2^(y - m + lift), at most 2^lift, so that p s stays clear of both
+// ends of fp16: lift 14 while every step s seen is below 2, then 6 (s <= 512).
+constexpr float kLift = 14.0f, kLiftBig = 6.0f;
+constexpr int kWaves = 4;
+
+__device__ __forceinline__ int steps_of(const Kv4Map& map, int lim) { return map.group_of(lim) / 4 + 1; }
+// a split's steps: whole turns of the workgroup's waves
+__device__ __forceinline__ int split_chunk(const Q4Args& a, int pos, int n_split) {
+    if (a.chunk) return a.chunk;
+    const int per = (steps_of(a.map, pos + a.n_tokens - 1) + n_split - 1) / n_split;
+    return (per + kWaves - 1) / kWaves * kWaves;
+}
+
+// max over the four 16-lane rows of a wave, in every lane
+__device__ __forceinline__ float rows_max(float v) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float rows_sum(float v) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+__device__ __forceinline__ float plus_ror8(float v) { return v + dpp_mov<0x128>(v); }  // + lane (l + 8) % 16 of the row
+__device__ __forceinline__ half2v pk_rtz(float a, float b) { return __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(a, b)); }
+
+// One workgroup: 8 query rows (row = token * group + head of the kv head) of kv
+// head x, tile y, split z.  Its four waves take 32-row steps in turn, each with
+// a running maximum of its own, and join through LDS.
+//
+// The matrix pipe's 16 columns are the 8 query rows twice, the high and the low
+// parts.  Scores come transposed (rows of the operand = cache rows), so a lane
+// then holds p of 8 consecutive cache rows of one query row: with the cache
+// rows in that order in V's words too, p is the next product's operand as it
+// is.  sum p c and sum p are one more product whose operand rows are the
+// blocks' c, and ones.
+template <int NB, bool UNI>
+__global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4Args a) {
+    constexpr int HD = 32 * NB, PITCH = HD + 4;
+    __shared__ float s_o[kWaves][8][PITCH];
+    __shared__ float s_c[kWaves][8][12];  // [0..NB) sum p c of the blocks, [NB] sum p
+    __shared__ float s_m[kWaves][8];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 15, j = lane >> 4;
+    const int kh = blockIdx.x, row0 = blockIdx.y * 8, rows = a.n_tokens * a.group;
+    const int pos = a.d_pos ? *a.d_pos : a.pos;
+    const int tile_lim = pos + (min(row0 + 8, rows) - 1) / a.group, first_lim = pos + row0 / a.group;
+    const int n_split = gridDim.z, chunk = split_chunk(a, pos, n_split);
+    const int begin = blockIdx.z * chunk, end = min(begin + chunk, steps_of(a.map, tile_lim));
+    if (begin >= end) return;  // rows past the tile's last position
+
+    // q: lane (col, j) holds channels 8 j .. of each block of row col % 8; scaled by a power of two to [1, 2)
+    const int r = min(row0 + (col & 7), rows - 1), lim = pos + r / a.group;
+    const float* qr = a.q + static_cast<size_t>(r / a.group) * a.q_pitch + static_cast<size_t>(kh * a.group + r % a.group) * HD;
+    half8 qf[NB];
+    float qs[NB], y_scale;
+    {
+        float f[NB][8], top = 0.0f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                f[b][i] = qr[32 * b + 8 * j + i];
+                top = fmaxf(top, fabsf(f[b][i]));
+            }
+        }
+        top = rows_max(top);
+        const int e = top > 0.0f && top <= 3.402823466e38f ? __builtin_amdgcn_frexp_expf(top) - 1 : 0;
+        y_scale = ldexpf(__fdiv_rn(kLog2e, sqrt_rn(static_cast<float>(HD))), e);
+        const bool low = col >= 8;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float z = ldexpf(f[b][i], -e);
+                sum += z;
+                const _Float16 hi = static_cast<_Float16>(z);
+                const int at = (i & 3) * 2 + (i >> 2);  // nibble order of q4_unpack
+                qf[b][at] = low ? static_cast<_Float16>(z - static_cast<float>(hi)) : hi;
+            }
+            sum = rows_sum(sum);
+            qs[b] = low ? 0.0f : sum;
+        }
+    }
+
+    const int last_group = a.map.group_of(tile_lim);
+    const size_t sc_off = kv4_scales(a.map.page_tokens, a.kv_dim);
+    // group g (of 4) of step st: its page's base, and the group's index there
+    auto locate = [&](const void* const* pt, int st, int g, const uint8_t*& base, int& at) {
+        const int vg = UNI ? 4 * st : min(4 * st + g, last_group);
+        const int page = UNI ? __builtin_amdgcn_readfirstlane(a.map.page_of(vg)) : a.map.page_of(vg);
+        base = static_cast<const uint8_t*>(pt[page]);
+        at = vg - page * a.map.groups + (UNI ? g : 0);
+    };
+    uint2 kn[NB], vn[NB];
+    uint4 ks[NB], kc[NB], vs[NB], vc;
+    auto load_k = [&](int st) {
+        const uint8_t *bn, *bs;
+        int gn, gs;
+        locate(a.pt_k, st, col >> 2, bn, gn);
+        locate(a.pt_k, st, j, bs, gs);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const size_t blk = static_cast<size_t>(kh * NB + b) * a.map.groups;
+            kn[b] = ld_global8(bn + (blk + gn) * 128 + (j * 4 + (col & 3)) * 8);
+            ks[b] = ld_global16(bs + sc_off + (blk + gs) * 32);
+            kc[b] = ld_global16(bs + sc_off + (blk + gs) * 32 + 16);
+        }
+    };
+    auto load_v = [&](int st) {
+        const uint8_t* base;
+        int g;
+        locate(a.pt_v, st, j, base, g);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const size_t blk = static_cast<size_t>(kh * NB + b) * a.map.groups;
+            vn[b] = ld_global8(base + (blk + g) * 128 + col * 8);
+            vs[b] = ld_global16(base + sc_off + (blk + g) * 32);
+        }
+        vc = ld_global16(base + sc_off + (static_cast<size_t>(kh * NB + min(col, NB - 1)) * a.map.groups + g) * 32 + 16);
+    };
+
+    f32x4 o[NB][2], oc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int b = 0; b < NB; ++b) o[b][0] = o[b][1] = oc;
+    float m = kLowest, lift = kLift;
+    const uint32_t low_mask = col >= 8 ? 0xffffffffu : 0u;
+
+    int st = begin + wave;
+    if (st < end) load_k(st);
+    for (; st < end; st += kWaves) {
+        load_v(st);
+        f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
+        const f32x4 zero = s0;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const f32x4 c0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(q4_unpack(kn[b].x), qf[b], zero, 0, 0, 0);
+            const f32x4 c1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(q4_unpack(kn[b].y), qf[b], zero, 0, 0, 0);
+            const uint32_t sp[4] = {ks[b].x, ks[b].y, ks[b].z, ks[b].w}, cp[4] = {kc[b].x, kc[b].y, kc[b].z, kc[b].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const half2v s = as_half2(sp[i]), c = as_half2(cp[i]);
+                s0[i] = fmaf(static_cast<float>(c.x), qs[b], fmaf(static_cast<float>(s.x), c0[i], s0[i]));
+                s1[i] = fmaf(static_cast<float>(c.y), qs[b], fmaf(static_cast<float>(s.y), c1[i], s1[i]));
+            }
+        }
+        if (st + kWaves < end) load_k(st + kWaves);
+        float y0[4], y1[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            y0[i] = plus_ror8(s0[i]) * y_scale;
+            y1[i] = plus_ror8(s1[i]) * y_scale;
+        }
+        // rows of the step that a query row does not see: p = 0, whatever is stored there
+        uint32_t seen[4] = {~0u, ~0u, ~0u, ~0u}, seen_c[4] = {~0u, ~0u, ~0u, ~0u};
+        const int lp = a.map.page_of(4 * st + 3), lg = 4 * st + 3 - lp * a.map.groups;
+        if ((!UNI && (a.map.page_tokens & 7)) || lp * a.map.page_tokens + lg * 8 + 7 > first_lim) {
+            const int page = a.map.page_of(4 * st + j), g = 4 * st + j - page * a.map.groups;
+            const int p0 = page * a.map.page_tokens + g * 8, room = a.map.page_tokens - g * 8;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool in0 = i < room, in1 = i + 4 < room;
+                const bool v0 = in0 && p0 + i <= lim, v1 = in1 && p0 + i + 4 <= lim;
+                if (!v0) y0[i] = -INFINITY;
+                if (!v1) y1[i] = -INFINITY;
+                seen[i] = (v0 ? 0xffffu : 0u) | (v1 ? 0xffff0000u : 0u);
+                seen_c[i] = (in0 && p0 + i <= tile_lim ? 0xffffu : 0u) | (in1 && p0 + i + 4 <= tile_lim ? 0xffff0000u : 0u);
+            }
+        }
+        float mx = fmaxf(fmaxf(fmaxf(y0[0], y0[1]), fmaxf(y0[2], y0[3])), fmaxf(fmaxf(y1[0], y1[1]), fmaxf(y1[2], y1[3])));
+        mx = rows_max(mx);
+        // a step of 2 and more (fp16 bit 14) among the rows that the query row sees
+        uint32_t big = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t w = 0;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) w |= i == 0 ? vs[b].x : i == 1 ? vs[b].y : i == 2 ? vs[b].z : vs[b].w;
+            big |= w & seen[i];
+        }
+        big &= 0x40004000u;
+        if (__any(mx > m || (big && lift == kLift))) {
+            const float top = fmaxf(m, mx), down = rows_max(big ? 1.0f : 0.0f) > 0.0f ? kLiftBig : lift;
+            const float f = __builtin_amdgcn_exp2f((m - top) + (down - lift));
+            m = top;
+            lift = down;
+            oc *= f;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                o[b][0] *= f;
+                o[b][1] *= f;
+            }
+        }
+        half2v hi[4], lo[4];
+        u32x4 pf;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float p0 = __builtin_amdgcn_exp2f(y0[i] - (m - lift)), p1 = __builtin_amdgcn_exp2f(y1[i] - (m - lift));
+            hi[i] = pk_rtz(p0, p1);
+            lo[i] = as_half2(as_u32(pk_rtz(p0 - static_cast<float>(hi[i].x), p1 - static_cast<float>(hi[i].y))) & low_mask);
+            pf[i] = low_mask ? as_u32(lo[i]) : as_u32(hi[i]);
+        }
+        {
+            u32x4 cf = {vc.x & seen_c[0], vc.y & seen_c[1], vc.z & seen_c[2], vc.w & seen_c[3]};
+            const uint32_t fill = col == NB ? 0x3c003c00u : 0u;  // ones: sum p
+#pragma unroll
+            for (int i = 0; i < 4; ++i) cf[i] = col < NB ? cf[i] : fill;
+            oc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, cf), __builtin_bit_cast(half8, pf), oc, 0, 0, 0);
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            // p s in two parts: the rounded product of the high part, and what it lost plus the low part's
+            const uint32_t sp[4] = {vs[b].x, vs[b].y, vs[b].z, vs[b].w};
+            u32x4 f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const half2v s = as_half2(sp[i]), t = hi[i] * s;
+                const half2v taken = as_half2(as_u32(t) & low_mask);
+                half2v w = __builtin_elementwise_fma(hi[i], s, -taken);
+                w = __builtin_elementwise_fma(lo[i], s, w);
+                f[i] = as_u32(w) & seen[i];
+            }
+            const half8 ps = __builtin_bit_cast(half8, f);
+            o[b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q4_unpack(vn[b].x), ps, o[b][0], 0, 0, 0);
+            o[b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q4_unpack(vn[b].y), ps, o[b][1], 0, 0, 0);
+        }
+    }
+
+    // the two parts' columns added, the waves joined
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float4 v = make_float4(plus_ror8(o[b][h][0]), plus_ror8(o[b][h][1]), plus_ror8(o[b][h][2]), plus_ror8(o[b][h][3]));
+            if (col < 8) *reinterpret_cast<float4*>(&s_o[wave][col][32 * b + 16 * h + 4 * j]) = v;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float v = plus_ror8(oc[i]);
+        if (col < 8 && 4 * j + i <= NB) s_c[wave][col][4 * j + i] = v;
+    }
+    if (lane < 8) s_m[wave][lane] = m - lift;
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < 8 * HD; idx += 64 * kWaves) {
+        const int c = idx / HD, d = idx % HD, row = row0 + c;
+        if (row >= rows) break;
+        float top = s_m[0][c], sum = 0.0f, l = 0.0f;
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) top = fmaxf(top, s_m[w][c]);
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float f = __builtin_amdgcn_exp2f(s_m[w][c] - top);
+            sum = fmaf(f, s_o[w][c][d] + s_c[w][c][d / 32], sum);
+            l = fmaf(f, s_c[w][c][NB], l);
+        }
+        const size_t out_row = static_cast<size_t>(row / a.group) * a.n_head + kh * a.group + row % a.group;
+        if (!a.part) {
+            a.out[out_row * HD + d] = __fdiv_rn(sum, l);
+        } else {
+            const size_t at = out_row * n_split + blockIdx.z;
+            a.part[at * HD + d] = sum;
+            if (d == 0) {
+                float* ml = a.part + static_cast<size_t>(a.n_tokens) * a.n_head * n_split * HD + 2 * at;
+                ml[0] = top;
+                ml[1] = l;
+            }
+        }
+    }
+}
+
+// Head sizes that are not whole blocks (48: a block then belongs to two heads)
+// or have no kernel above: a workgroup per (head, token, split), a thread a row
+// for the scores, a thread a channel for the values, 256 rows at a time.
+constexpr int kAny = 256;
+__global__ __launch_bounds__(kAny) void attn_q4_any_kernel(Q4Args a) {
+    extern __shared__ float s_q[];  // [hd] q, then [hd] sums
+    __shared__ float s_p[kAny];
+    __shared__ float s_red[kAny / 64];
+    const int tid = threadIdx.x, h = blockIdx.x, t = blockIdx.y, hd = a.hd, n_split = gridDim.z;
+    const int pos = a.d_pos ? *a.d_pos : a.pos, lim = pos + t;
+    const int chunk = split_chunk(a, pos, n_split);
+    const int begin = blockIdx.z * chunk * 4, end = min(begin + chunk * 4, a.map.group_of(lim) + 1);  // groups
+    if (begin >= end) return;
+    float* s_o = s_q + hd;
+    for (int d = tid; d < hd; d += kAny) {
+        s_q[d] = a.q[static_cast<size_t>(t) * a.q_pitch + static_cast<size_t>(h) * hd + d];
+        s_o[d] = 0.0f;
+    }
+    __syncthreads();
+    const int e0 = h / a.group * hd;  // the head's first element of a row
+    const size_t sc_off = kv4_scales(a.map.page_tokens, a.kv_dim);
+    const float y_scale = __fdiv_rn(kLog2e, sqrt_rn(static_cast<float>(hd)));
+    float m = kLowest, l = 0.0f;
+    for (int g0 = begin; g0 < end; g0 += kAny / 8) {
+        const int vg = min(g0 + tid / 8, end - 1), i = tid & 7;
+        const int page = a.map.page_of(vg), g = vg - page * a.map.groups;
+        const bool seen = g0 + tid / 8 < end && g * 8 + i < a.map.page_tokens && page * a.map.page_tokens + g * 8 + i <= lim;
+        float y = -INFINITY;
+        if (seen) {
+            const uint8_t* base = static_cast<const uint8_t*>(a.pt_k[page]);
+            float sum = 0.0f;
+            for (int d = 0; d < hd; d += 8) {
+                const int b = (e0 + d) / 32, kq = (e0 + d) % 32 / 8;
+                const size_t at = static_cast<size_t>(b) * a.map.groups + g;
+                const uint32_t w = kv4_nat(reinterpret_cast<const uint32_t*>(base + at * 128)[kv4_k_word(i, kq)]);
+                const float s = kv4_step(base + sc_off + at * 32, i), c = kv4_middle(base + sc_off + at * 32, i);
+                float dot = 0.0f, qsum = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float qv = s_q[d + k];
+                    dot = fmaf(qv, static_cast<float>((w >> (4 * k)) & 15u) - 8.0f, dot);
+                    qsum += qv;
+                }
+                sum = fmaf(s, dot, fmaf(c, qsum, sum));
+            }
+            y = sum * y_scale;
+        }
+        float mx = wave_max_all(y);
+        if ((tid & 63) == 0) s_red[tid >> 6] = mx;
+        __syncthreads();
+        mx = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+        // a NaN score reaches the sums through p, not through the maximum
+        const float top = fmaxf(m, mx), f = __builtin_amdgcn_exp2f(m - top);
+        const float p = seen ? __builtin_amdgcn_exp2f(y - top) : 0.0f;
+        s_p[tid] = p;
+        __syncthreads();
+        float part = 0.0f;
+        for (int k = tid & 63; k < kAny; k += 64) part += s_p[k];
+        part += __shfl_xor(part, 32);
+        part += __shfl_xor(part, 16);
+        part += __shfl_xor(part, 8);
+        part += __shfl_xor(part, 4);
+        part += __shfl_xor(part, 2);
+        part += __shfl_xor(part, 1);
+        l = fmaf(l, f, part);
+        m = top;
+        const int groups = min(kAny / 8, end - g0);
+        for (int d = tid; d < hd; d += kAny) {
+            const int b = (e0 + d) / 32, ch = (e0 + d) % 32;
+            float acc = s_o[d] * f;
+            for (int k = 0; k < groups; ++k) {
+                const int pg = a.map.page_of(g0 + k), gg = g0 + k - pg * a.map.groups;
+                const int n = min(min(8, a.map.page_tokens - gg * 8), lim - (pg * a.map.page_tokens + gg * 8) + 1);
+                const uint8_t* base = static_cast<const uint8_t*>(a.pt_v[pg]);
+                const size_t at = static_cast<size_t>(b) * a.map.groups + gg;
+                const uint32_t w = kv4_nat(reinterpret_cast<const uint32_t*>(base + at * 128)[kv4_v_word(ch)]);
+                for (int r = 0; r < n; ++r) {
+                    const float s = kv4_step(base + sc_off + at * 32, r), c = kv4_middle(base + sc_off + at * 32, r);
+                    acc = fmaf(s_p[8 * k + r], fmaf(s, static_cast<float>((w >> (4 * r)) & 15u) - 8.0f, c), acc);
+                }
+            }
+            s_o[d] = acc;
+        }
+        __syncthreads();
+    }
+    const size_t row = static_cast<size_t>(t) * a.n_head + h;
+    for (int d = tid; d < hd; d += kAny) {
+        if (a.part) a.part[(row * n_split + blockIdx.z) * hd + d] = s_o[d];
+        else a.out[row * hd + d] = __fdiv_rn(s_o[d], l);
+    }
+    if (a.part && tid == 0) {
+        float* ml = a.part + static_cast<size_t>(a.n_tokens) * a.n_head * n_split * hd + 2 * (row * n_split + blockIdx.z);
+        ml[0] = m;
+        ml[1] = l;
+    }
+}
+
+// The splits of a row joined: weights 2^(m - max) once in LDS, a thread a channel.
+constexpr int kMaxSplit = 256;
+__global__ __launch_bounds__(256) void attn_q4_join_kernel(Q4Args a, int n_split) {
+    __shared__ float s_w[kMaxSplit];
+    __shared__ float s_l;
+    const size_t row = blockIdx.x;
+    const int pos = a.d_pos ? *a.d_pos : a.pos, lim = pos + static_cast<int>(row) / a.n_head;
+    const int chunk = split_chunk(a, pos, n_split);
+    const int used = (steps_of(a.map, lim) + chunk - 1) / chunk;
+    const float* ml = a.part + static_cast<size_t>(a.n_tokens) * a.n_head * n_split * a.hd + 2 * row * n_split;
+    const float* o = a.part + row * n_split * a.hd;
+    if (threadIdx.x < 64) {
+        float mv[kMaxSplit / 64], top = kLowest, sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kMaxSplit / 64; ++k) {
+            const int s = threadIdx.x + 64 * k;
+            mv[k] = s < used ? ml[2 * s] : kLowest;
+            top = fmaxf(top, mv[k]);
+        }
+        top = wave_max_all(top);
+#pragma unroll
+        for (int k = 0; k < kMaxSplit / 64; ++k) {
+            const int s = threadIdx.x + 64 * k;
+            if (s < used) {
+                const float w = __builtin_amdgcn_exp2f(mv[k] - top);
+                s_w[s] = w;
+                sum = fmaf(w, ml[2 * s + 1], sum);
+            }
+        }
+#pragma unroll
+        for (int x = 32; x >= 1; x >>= 1) sum += __shfl_xor(sum, x);
+        if (threadIdx.x == 0) s_l = sum;
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < a.hd; d += blockDim.x) {
+        float acc = 0.0f;
+#pragma unroll 8
+        for (int s = 0; s < used; ++s) acc = fmaf(s_w[s], o[static_cast<size_t>(s) * a.hd + d], acc);
+        a.out[row * a.hd + d] = __fdiv_rn(acc, s_l);
+    }
+}
+
+bool q4_tiles(size_t hd) { return hd % 32 == 0 && (hd <= 128 || hd == 192 || hd == 256); }
+
+// Splits of a call: enough workgroups for two a CU, each wave at least one step, at most kMaxSplit.
+size_t q4_splits(size_t max_pos, size_t n_tokens, size_t n_head, size_t n_head_kv, size_t hd, size_t page_tokens,
+                 size_t chunk) {
+    const Kv4Map map = kv4_map(page_tokens);
+    const size_t steps = static_cast<size_t>(map.group_of(static_cast<int>(max_pos - 1)) / 4 + 1);
+    if (chunk) return (steps + chunk - 1) / chunk;
+    const size_t tiles = q4_tiles(hd) ? n_head_kv * ((n_tokens * (n_head / n_head_kv) + 7) / 8) : n_head * n_tokens;
+    return std::max<size_t>(1, std::min({512 / tiles, (steps + kWaves - 1) / kWaves, static_cast<size_t>(kMaxSplit)}));
+}
+
+template <int NB>
+void q4_launch(const Q4Args& a, dim3 grid, hipStream_t st) {
+    if (a.map.page_tokens % 32 == 0) attn_q4_kernel<NB, true><<<grid, 64 * kWaves, 0, st>>>(a);
+    else attn_q4_kernel<NB, false><<<grid, 64 * kWaves, 0, st>>>(a);
+}
+
+}  // namespace
+
+// 512 positions a split (whole 8-row groups), more where they would be over kMaxSplit
+size_t attn_q4_chunk(size_t max_pos, size_t page_tokens) {
+    const size_t steps = static_cast<size_t>(kv4_map(page_tokens).group_of(static_cast<int>(max_pos - 1)) / 4 + 1);
+    size_t chunk = 16;
+    while (steps > chunk * kMaxSplit) chunk *= 2;
+    return chunk;
+}
+
+size_t attn_q4_scratch(size_t max_pos, size_t n_tokens, size_t n_head, size_t n_head_kv, size_t hd, size_t page_tokens,
+                       size_t chunk) {
+    const size_t n = q4_splits(max_pos, n_tokens, n_head, n_head_kv, hd, page_tokens, chunk);
+    return n > 1 ? n * n_tokens * n_head * (hd + 2) : 0;
+}
+
+hipError_t launch_attn_q4(const void* const* pt_k, const void* const* pt_v, const float* q, size_t q_pitch, float* part,
+                          float* out, const int* d_pos, size_t pos, size_t max_pos, size_t n_tokens, size_t n_head,
+                          size_t n_head_kv, size_t hd, size_t kv_dim, size_t page_tokens, size_t chunk, hipStream_t st) {
+    if (!n_tokens) return hipSuccess;
+    const size_t splits = q4_splits(max_pos, n_tokens, n_head, n_head_kv, hd, page_tokens, chunk);
+    if (hd % 8 || kv_dim % 32 || splits > static_cast<size_t>(kMaxSplit) || (splits > 1 && !part)) return hipErrorInvalidValue;
+    Q4Args a{};
+    a.pt_k = pt_k;
+    a.pt_v = pt_v;
+    a.q = q;
+    a.out = out;
+    a.part = splits > 1 ? part : nullptr;
+    a.d_pos = d_pos;
+    a.q_pitch = q_pitch;
+    a.pos = static_cast<int>(pos);
+    a.n_tokens = static_cast<int>(n_tokens);
+    a.n_head = static_cast<int>(n_head);
+    a.group = static_cast<int>(n_head / n_head_kv);
+    a.kv_dim = static_cast<int>(kv_dim);
+    a.hd = static_cast<int>(hd);
+    a.chunk = static_cast<int>(chunk);
+    a.map = kv4_map(page_tokens);
+    const unsigned z = static_cast<unsigned>(splits);
+    if (q4_tiles(hd)) {
+        const dim3 grid(static_cast<unsigned>(n_head_kv), static_cast<unsigned>((n_tokens * a.group + 7) / 8), z);
+        switch (hd / 32) {
+        case 1: q4_launch<1>(a, grid, st); break;
+        case 2: q4_launch<2>(a, grid, st); break;
+        case 3: q4_launch<3>(a, grid, st); break;
+        case 4: q4_launch<4>(a, grid, st); break;
+        case 6: q4_launch<6>(a, grid, st); break;
+        default: q4_launch<8>(a, grid, st); break;
+        }
+    } else {
+        attn_q4_any_kernel<<<dim3(static_cast<unsigned>(n_head), static_cast<unsigned>(n_tokens), z), kAny,
+                             2 * hd * sizeof(float), st>>>(a);
+    }
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    if (splits > 1) {
+        attn_q4_join_kernel<<<static_cast<unsigned>(n_tokens * n_head), hd <= 64 ? 64 : hd <= 128 ? 128 : 256, 0, st>>>(
+            a, static_cast<int>(splits));
+        return hipGetLastError();
+    }
+    return hipSuccess;
+}
+
+}  // namespace mvh

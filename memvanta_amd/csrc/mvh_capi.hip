@@ -10,6 +10,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -30,6 +31,8 @@ struct mvh_context {
     Buf xin;      // host-pointer staging of inputs
     Buf yout;     // host-pointer staging of outputs
     Buf scores;   // attention scores
+    Buf work;     // partial results of the 4-bit attention and the log probabilities (grow_kept)
+    std::vector<void*> retired;  // smaller work buffers that captured graphs may still use
     // pinned host memory of a one-token call with host vectors: the first
     // kPinIn bytes for the input, kPinOut for the output.  Borrowed for the
     // call; kept where the call failed with work perhaps still in flight, or
@@ -45,6 +48,12 @@ struct mvh_tensor {
     uint64_t ne0 = 0, ne1 = 0, nbytes = 0;
     void* d = nullptr;
     bool owned = false;
+};
+
+struct mvh_rope {
+    int device = 0;
+    std::vector<double> freq;  // angle per position of each pair
+    mvh::RopeView view;        // with the device's copy
 };
 
 struct mvh_kv_cache {
@@ -137,6 +146,34 @@ int grow(mvh_context* c, mvh_context::Buf& b, size_t bytes) {
         (void)hipGetLastError();
         return fail(MVH_E_NOMEM, "device allocation of %zu bytes failed", cap);
     }
+    b.cap = cap;
+    return MVH_OK;
+}
+
+// grow() for memory whose address captured graphs hold: the old buffer stays
+// until the context goes (sizes double, so all of them together take at most
+// what the largest takes), and a stream under capture gets no allocation.
+int grow_kept(mvh_context* c, mvh_context::Buf& b, size_t bytes) {
+    if (bytes <= b.cap) return MVH_OK;
+    hipStreamCaptureStatus state = hipStreamCaptureStatusNone;
+    MVH_HIP(hipStreamIsCapturing(c->stream, &state));
+    if (state != hipStreamCaptureStatusNone)
+        return fail(MVH_E_NOMEM, "workspace of %zu bytes is not there yet: make the call once before capturing it", bytes);
+    const size_t cap = std::max({bytes, 2 * b.cap, static_cast<size_t>(1) << 20});
+    void* p = nullptr;
+    if (hipMalloc(&p, cap) != hipSuccess) {
+        (void)hipGetLastError();
+        return fail(MVH_E_NOMEM, "device allocation of %zu bytes failed", cap);
+    }
+    if (b.p) {
+        try {
+            c->retired.push_back(b.p);
+        } catch (const std::bad_alloc&) {
+            (void)hipFree(p);
+            return fail(MVH_E_NOMEM, "host allocation failed");
+        }
+    }
+    b.p = p;
     b.cap = cap;
     return MVH_OK;
 }
@@ -302,6 +339,23 @@ int check_kv(const mvh_kv_cache* kv, size_t layer) {
     return MVH_OK;
 }
 
+constexpr size_t kMaxKv4Tokens = size_t{1} << 20, kMaxKv4Dim = size_t{1} << 16;
+
+// The cache is on the context's device, and layer is one of its layers.
+int check_kv_on(const mvh_context* c, const mvh_kv_cache* kv, size_t layer) {
+    if (int rc = check_kv(kv, layer)) return rc;
+    if (kv->device != c->device)
+        return fail(MVH_E_INVALID, "KV cache of device %d used with a context of device %d", kv->device, c->device);
+    return MVH_OK;
+}
+
+// Every page of positions first..last of the layer is there.
+int check_pages(const mvh_kv_cache* kv, size_t layer, size_t first, size_t last) {
+    for (size_t p = first / kv->page_tokens; p <= last / kv->page_tokens; ++p)
+        if (!kv->hk[layer * kv->max_pages + p]) return fail(MVH_E_RANGE, "KV key page missing");
+    return MVH_OK;
+}
+
 int ensure_page(mvh_kv_cache* kv, size_t layer, size_t p) {
     const size_t slot = layer * kv->max_pages + p;
     if (kv->hk[slot]) return MVH_OK;
@@ -392,8 +446,9 @@ int mvh_context_destroy(mvh_context* c) {
     if (!c) return MVH_OK;
     (void)hipSetDevice(c->device);
     if (hipStreamSynchronize(c->stream) == hipSuccess) pin_done(c);
-    for (auto* b : {&c->act, &c->xin, &c->yout, &c->scores})
+    for (auto* b : {&c->act, &c->xin, &c->yout, &c->scores, &c->work})
         if (b->p) (void)hipFree(b->p);
+    for (void* p : c->retired) (void)hipFree(p);
     if (c->pin) (void)hipHostFree(c->pin);
     if (--g_contexts == 0) pins().trim(1);
     (void)hipStreamDestroy(c->stream);
@@ -894,6 +949,7 @@ int mvh_kv_parse_type(const char* s, int* type) {
     if (t == "f32") *type = MVH_KV_F32;
     else if (t == "f16") *type = MVH_KV_F16;
     else if (t == "q8" || t == "q8_0") *type = MVH_KV_Q8;
+    else if (t == "q4") *type = MVH_KV_Q4;
     else return fail(MVH_E_INVALID, "unknown KV cache type: %s", s);
     return MVH_OK;
 }
@@ -903,6 +959,7 @@ const char* mvh_kv_type_name(int type) {
     case MVH_KV_F32: return "f32";
     case MVH_KV_F16: return "f16";
     case MVH_KV_Q8: return "q8";
+    case MVH_KV_Q4: return "q4";
     }
     return "?";
 }
@@ -912,12 +969,19 @@ int mvh_kv_create(mvh_context* c, size_t n_layer, size_t kv_dim, size_t page_tok
     CHECK_CTX(c);
     if (!out) return fail(MVH_E_INVALID, "null out");
     *out = nullptr;
-    if (kv_type != MVH_KV_F32 && kv_type != MVH_KV_F16 && kv_type != MVH_KV_Q8)
+    if (kv_type != MVH_KV_F32 && kv_type != MVH_KV_F16 && kv_type != MVH_KV_Q8 && kv_type != MVH_KV_Q4)
         return fail(MVH_E_INVALID, "unknown KV cache type id %d", kv_type);
     if (!page_tokens) page_tokens = 128;  // PagedKVCache default (src/llama_model.cpp:19)
     if (!n_layer || !kv_dim || !max_tokens) return fail(MVH_E_INVALID, "KV cache needs layers, kv_dim and max_tokens");
     if (kv_dim % 8) return fail(MVH_E_SHAPE, "kv_dim must be a multiple of 8");
-    if (max_tokens > 16000) return fail(MVH_E_RANGE, "max_tokens above 16000 is not supported");
+    if (kv_type == MVH_KV_Q4) {
+        if (kv_dim % 32) return fail(MVH_E_SHAPE, "kv_dim of a 4-bit KV cache must be a multiple of 32");
+        if (kv_dim > kMaxKv4Dim) return fail(MVH_E_RANGE, "kv_dim above %zu is not supported", kMaxKv4Dim);
+        if (max_tokens > kMaxKv4Tokens || page_tokens > kMaxKv4Tokens)
+            return fail(MVH_E_RANGE, "max_tokens and page_tokens above %zu are not supported", kMaxKv4Tokens);
+    } else if (max_tokens > 16000) {
+        return fail(MVH_E_RANGE, "max_tokens above 16000 is not supported");
+    }
     auto* kv = new (std::nothrow) mvh_kv_cache;
     if (!kv) return fail(MVH_E_NOMEM, "host allocation failed");
     kv->device = c->device;
@@ -1022,6 +1086,11 @@ int mvh_kv_read_row(mvh_context* c, const mvh_kv_cache* kv, size_t layer, size_t
     const size_t slot = layer * kv->max_pages + pos / kv->page_tokens, i = pos % kv->page_tokens;
     const uint8_t* page = which ? kv->hv[slot] : kv->hk[slot];
     if (!page) return fail(MVH_E_RANGE, which ? "KV value page missing" : "KV key page missing");
+    if (kv->type == MVH_KV_Q4) {
+        if (scale) *scale = 1.0f;
+        float* row = static_cast<float*>(out);
+        return mvh_kv_read(c, kv, layer, pos, 1, which ? nullptr : row, which ? row : nullptr, MVH_HOST);
+    }
     const size_t eb = mvh::kv_elem_bytes(kv->type);
     MVH_HIP(hipStreamSynchronize(c->stream));
     MVH_HIP(hipMemcpy(out, page + i * kv->kv_dim * eb, kv->kv_dim * eb, hipMemcpyDeviceToHost));
@@ -1032,6 +1101,284 @@ int mvh_kv_read_row(mvh_context* c, const mvh_kv_cache* kv, size_t layer, size_t
                               hipMemcpyDeviceToHost));
     }
     return MVH_OK;
+}
+
+int mvh_kv_read(mvh_context* c, const mvh_kv_cache* kv, size_t layer, size_t pos, size_t n_tokens, float* k, float* v,
+                int kind) {
+    CHECK_CTX(c);
+    if (int rc = check_kv_on(c, kv, layer)) return rc;
+    if (kind != MVH_HOST && kind != MVH_DEVICE) return fail(MVH_E_INVALID, "ptr_kind must be MVH_HOST or MVH_DEVICE");
+    if (!n_tokens) return MVH_OK;
+    if (!k && !v) return fail(MVH_E_INVALID, "null k and v");
+    if (n_tokens > kv->max_tokens || pos > kv->max_tokens - n_tokens) return fail(MVH_E_RANGE, "KV position out of range");
+    if (int rc = check_pages(kv, layer, pos, pos + n_tokens - 1)) return rc;
+    const size_t bytes = n_tokens * kv->kv_dim * 4;
+    float *kd = k, *vd = v;
+    if (kind == MVH_HOST) {
+        if (int rc = grow(c, c->yout, 2 * bytes)) return rc;
+        kd = k ? static_cast<float*>(c->yout.p) : nullptr;
+        vd = v ? reinterpret_cast<float*>(static_cast<uint8_t*>(c->yout.p) + bytes) : nullptr;
+    }
+    const size_t base = layer * kv->max_pages;
+    MVH_HIP(mvh::launch_kv_read(kv->type, kv->dk + base, kv->dv + base, pos, n_tokens, kv->kv_dim, kv->page_tokens, kd, vd,
+                                c->stream));
+    if (kind == MVH_HOST && k) MVH_HIP(hipMemcpyAsync(k, kd, bytes, hipMemcpyDeviceToHost, c->stream));
+    if (kind == MVH_HOST && v) MVH_HIP(hipMemcpyAsync(v, vd, bytes, hipMemcpyDeviceToHost, c->stream));
+    if (kind == MVH_HOST) MVH_HIP(hipStreamSynchronize(c->stream));
+    return MVH_OK;
+}
+
+// ---- rotary positions ----
+
+int mvh_rope_create(mvh_context* c, const mvh_rope_config* cfg, mvh_rope** out) {
+    CHECK_CTX(c);
+    if (!cfg || !out) return fail(MVH_E_INVALID, "null argument");
+    *out = nullptr;
+    const size_t hd = cfg->head_dim, rot = cfg->rot_dim ? cfg->rot_dim : hd;
+    if (!hd || hd % 2 || hd > 1024) return fail(MVH_E_SHAPE, "rope head_dim must be even and at most 1024");
+    if (rot % 2 || rot > hd) return fail(MVH_E_SHAPE, "rope rot_dim must be even and at most head_dim");
+    if (cfg->layout != MVH_ROPE_HALF && cfg->layout != MVH_ROPE_INTERLEAVED)
+        return fail(MVH_E_INVALID, "bad rope layout %d", cfg->layout);
+    if (cfg->scaling < MVH_ROPE_SCALE_NONE || cfg->scaling > MVH_ROPE_SCALE_INDEX)
+        return fail(MVH_E_INVALID, "bad rope scaling %d", cfg->scaling);
+    auto positive = [](double v) { return v > 0.0 && std::isfinite(v); };
+    if (!positive(cfg->base) || cfg->base <= 1.0) return fail(MVH_E_INVALID, "rope base must be above 1");
+    if (!positive(cfg->attn_scale)) return fail(MVH_E_INVALID, "rope attn_scale must be positive");
+    const bool blend = cfg->scaling == MVH_ROPE_SCALE_TURNS || cfg->scaling == MVH_ROPE_SCALE_INDEX;
+    if (cfg->scaling != MVH_ROPE_SCALE_NONE && !positive(cfg->factor))
+        return fail(MVH_E_INVALID, "rope factor must be positive");
+    if (blend && (!positive(cfg->orig_ctx) || !positive(cfg->low) || !positive(cfg->high) || cfg->low >= cfg->high))
+        return fail(MVH_E_INVALID, "rope scaling needs orig_ctx > 0 and 0 < low < high");
+    auto* r = new (std::nothrow) mvh_rope;
+    if (!r) return fail(MVH_E_NOMEM, "host allocation failed");
+    constexpr double two_pi = 6.283185307179586476925;
+    r->device = c->device;
+    try {
+        r->freq.resize(rot / 2);
+    } catch (const std::bad_alloc&) {
+        delete r;
+        return fail(MVH_E_NOMEM, "host allocation failed");
+    }
+    double a = 0.0, b = 0.0;
+    if (cfg->scaling == MVH_ROPE_SCALE_INDEX) {  // pair index at which f turns `t` times over orig_ctx
+        auto at = [&](double t) { return rot * std::log(cfg->orig_ctx / (two_pi * t)) / (2.0 * std::log(cfg->base)); };
+        a = std::max(std::floor(at(cfg->high)), 0.0);
+        b = std::min(std::ceil(at(cfg->low)), static_cast<double>(rot) - 1.0);
+    }
+    for (size_t i = 0; i < rot / 2; ++i) {
+        const double f = std::pow(cfg->base, -2.0 * static_cast<double>(i) / static_cast<double>(rot));
+        double keep = 1.0;
+        if (cfg->scaling == MVH_ROPE_SCALE_LINEAR) keep = 0.0;
+        else if (cfg->scaling == MVH_ROPE_SCALE_TURNS)
+            keep = std::clamp((cfg->orig_ctx / two_pi * f - cfg->low) / (cfg->high - cfg->low), 0.0, 1.0);
+        else if (cfg->scaling == MVH_ROPE_SCALE_INDEX)
+            keep = 1.0 - std::clamp((static_cast<double>(i) - a) / std::max(b - a, 0.001), 0.0, 1.0);
+        r->freq[i] = cfg->scaling == MVH_ROPE_SCALE_NONE ? f : f * keep + f / cfg->factor * (1.0 - keep);
+    }
+    double* d = nullptr;
+    if (hipMalloc(&d, r->freq.size() * sizeof(double)) != hipSuccess) {
+        (void)hipGetLastError();
+        delete r;
+        return fail(MVH_E_NOMEM, "rope table allocation failed");
+    }
+    if (hipMemcpy(d, r->freq.data(), r->freq.size() * sizeof(double), hipMemcpyHostToDevice) != hipSuccess) {
+        (void)hipFree(d);
+        delete r;
+        return fail(MVH_E_DEVICE, "rope table upload failed");
+    }
+    r->view.freq = d;
+    r->view.scale = cfg->attn_scale;
+    r->view.head_dim = static_cast<int>(hd);
+    r->view.rot = static_cast<int>(rot);
+    r->view.layout = cfg->layout == MVH_ROPE_HALF ? mvh::kRopeHalf : mvh::kRopeInterleaved;
+    *out = r;
+    return MVH_OK;
+}
+
+int mvh_rope_destroy(mvh_rope* r) {
+    if (!r) return MVH_OK;
+    (void)hipSetDevice(r->device);
+    (void)hipDeviceSynchronize();
+    (void)hipFree(const_cast<double*>(r->view.freq));
+    delete r;
+    return MVH_OK;
+}
+
+int mvh_rope_angles(const mvh_rope* r, double* out) {
+    if (!r || !out) return fail(MVH_E_INVALID, "null argument");
+    std::copy(r->freq.begin(), r->freq.end(), out);
+    return MVH_OK;
+}
+
+// The rotation belongs to the context's device, and rows of n_head heads at this pitch are sound.
+static int check_rope(const mvh_context* c, const mvh_rope* r, size_t n_tokens, size_t n_head, size_t pitch_in,
+                      size_t pitch_out) {
+    if (!r) return fail(MVH_E_INVALID, "null rope");
+    if (r->device != c->device)
+        return fail(MVH_E_INVALID, "rope of device %d used with a context of device %d", r->device, c->device);
+    const size_t width = n_head * r->view.head_dim;
+    if (n_head > (size_t{1} << 20) || width > (size_t{1} << 24)) return fail(MVH_E_RANGE, "rows above 16777216 elements");
+    if (n_tokens > (size_t{1} << 24)) return fail(MVH_E_RANGE, "more than 16777216 tokens");
+    if (pitch_in < width || pitch_out < width) return fail(MVH_E_SHAPE, "row pitch below n_head*head_dim");
+    return MVH_OK;
+}
+
+int mvh_rope_apply(mvh_context* c, const mvh_rope* r, const float* x, size_t x_pitch, size_t n_tokens, size_t n_head,
+                   const int* positions, size_t pos, float* out, size_t out_pitch, int kind) {
+    CHECK_CTX(c);
+    if (int rc = check_rope(c, r, n_tokens, n_head, x_pitch, out_pitch)) return rc;
+    if (kind != MVH_HOST && kind != MVH_DEVICE) return fail(MVH_E_INVALID, "ptr_kind must be MVH_HOST or MVH_DEVICE");
+    if (!n_tokens || !n_head) return MVH_OK;
+    if (!x || !out) return fail(MVH_E_INVALID, "null x/out");
+    if (x == out && x_pitch != out_pitch) return fail(MVH_E_INVALID, "rotation in place needs equal pitches");
+    if (!positions && pos > 0x7fffffff - n_tokens) return fail(MVH_E_RANGE, "position out of range");
+    const float* xd = x;
+    float* od = out;
+    const int* pd = positions;
+    const size_t width = n_head * r->view.head_dim * 4;
+    if (kind == MVH_HOST) {
+        const size_t bytes = up16(n_tokens * width);
+        if (int rc = grow(c, c->xin, bytes + n_tokens * 4)) return rc;
+        if (int rc = grow(c, c->yout, bytes)) return rc;
+        auto* base = static_cast<uint8_t*>(c->xin.p);
+        MVH_HIP(hipMemcpy2DAsync(base, width, x, x_pitch * 4, width, n_tokens, hipMemcpyHostToDevice, c->stream));
+        if (positions) {
+            MVH_HIP(hipMemcpyAsync(base + bytes, positions, n_tokens * 4, hipMemcpyHostToDevice, c->stream));
+            pd = reinterpret_cast<const int*>(base + bytes);
+        }
+        xd = reinterpret_cast<const float*>(base);
+        od = static_cast<float*>(c->yout.p);
+        x_pitch = width / 4;
+    }
+    MVH_HIP(mvh::launch_rope(r->view, xd, x_pitch, od, kind == MVH_HOST ? width / 4 : out_pitch, pd, pos, n_tokens, n_head,
+                             c->stream));
+    if (kind == MVH_HOST) {
+        MVH_HIP(hipMemcpy2DAsync(out, out_pitch * 4, od, width, width, n_tokens, hipMemcpyDeviceToHost, c->stream));
+        MVH_HIP(hipStreamSynchronize(c->stream));
+    }
+    return MVH_OK;
+}
+
+int mvh_kv_append(mvh_context* c, mvh_kv_cache* kv, size_t layer, size_t pos, size_t n_tokens, const mvh_rope* r,
+                  const float* q, size_t q_pitch, size_t n_head, float* q_out, size_t out_pitch, const float* k,
+                  size_t k_pitch, const float* v, size_t v_pitch, int kind) {
+    CHECK_CTX(c);
+    if (int rc = check_kv_on(c, kv, layer)) return rc;
+    if (!q) n_head = 0;
+    if (int rc = check_rope(c, r, n_tokens, n_head, q ? q_pitch : 0, q ? out_pitch : 0)) return rc;
+    if (kind != MVH_HOST && kind != MVH_DEVICE) return fail(MVH_E_INVALID, "ptr_kind must be MVH_HOST or MVH_DEVICE");
+    const size_t hd = static_cast<size_t>(r->view.head_dim), kv_dim = kv->kv_dim;
+    if (hd % 8 || kv_dim % hd) return fail(MVH_E_SHAPE, "kv_dim must be whole heads of a multiple of 8 elements");
+    if (k_pitch < kv_dim || v_pitch < kv_dim) return fail(MVH_E_SHAPE, "row pitch below kv_dim");
+    if (kv->type == MVH_KV_Q8 && kv_dim > 16384) return fail(MVH_E_SHAPE, "kv_dim of Q8 rows above 16384 is not supported");
+    if (!n_tokens) return MVH_OK;
+    if (!k || !v) return fail(MVH_E_INVALID, "null k/v");
+    if (q && !q_out) return fail(MVH_E_INVALID, "null q_out");
+    if (q && q == q_out && q_pitch != out_pitch) return fail(MVH_E_INVALID, "rotation in place needs equal pitches");
+    if (n_tokens > kv->max_tokens || pos > kv->max_tokens - n_tokens) return fail(MVH_E_RANGE, "context exhausted");
+    for (size_t p = pos / kv->page_tokens; p <= (pos + n_tokens - 1) / kv->page_tokens; ++p)
+        if (int rc = ensure_page(kv, layer, p)) return rc;
+    const size_t qw = n_head * hd * 4, kw = kv_dim * 4;
+    const float *qd = q, *kd = k, *vd = v;
+    float* od = q_out;
+    if (kind == MVH_HOST) {
+        if (int rc = grow(c, c->xin, n_tokens * (qw + 2 * kw))) return rc;
+        if (int rc = grow(c, c->yout, n_tokens * qw)) return rc;
+        auto* base = static_cast<uint8_t*>(c->xin.p);
+        if (q) MVH_HIP(hipMemcpy2DAsync(base, qw, q, q_pitch * 4, qw, n_tokens, hipMemcpyHostToDevice, c->stream));
+        qd = q ? reinterpret_cast<const float*>(base) : nullptr;
+        base += n_tokens * qw;
+        MVH_HIP(hipMemcpy2DAsync(base, kw, k, k_pitch * 4, kw, n_tokens, hipMemcpyHostToDevice, c->stream));
+        kd = reinterpret_cast<const float*>(base);
+        base += n_tokens * kw;
+        MVH_HIP(hipMemcpy2DAsync(base, kw, v, v_pitch * 4, kw, n_tokens, hipMemcpyHostToDevice, c->stream));
+        vd = reinterpret_cast<const float*>(base);
+        od = static_cast<float*>(c->yout.p);
+        q_pitch = qw / 4;
+        k_pitch = v_pitch = kv_dim;
+    }
+    const size_t base = layer * kv->max_pages;
+    MVH_HIP(mvh::launch_kv_append(kv->type, r->view, kv->dk + base, kv->dv + base, qd, q_pitch, od,
+                                  kind == MVH_HOST ? qw / 4 : out_pitch, kd, k_pitch, vd, v_pitch, pos, n_tokens, n_head,
+                                  kv_dim, kv->page_tokens, c->stream));
+    if (kind == MVH_HOST) {
+        if (q) MVH_HIP(hipMemcpy2DAsync(q_out, out_pitch * 4, od, qw, qw, n_tokens, hipMemcpyDeviceToHost, c->stream));
+        MVH_HIP(hipStreamSynchronize(c->stream));
+    }
+    return MVH_OK;
+}
+
+int mvh_logprobs(mvh_context* c, const float* logits, size_t n, size_t rows, const int* targets, size_t top_k,
+                 float* logprob, float* entropy, int* top_ids, float* top_logprobs, int kind) {
+    CHECK_CTX(c);
+    if (kind != MVH_HOST && kind != MVH_DEVICE) return fail(MVH_E_INVALID, "ptr_kind must be MVH_HOST or MVH_DEVICE");
+    if (!n) return fail(MVH_E_INVALID, "empty logits");
+    if (n > 0x7fffffff) return fail(MVH_E_RANGE, "logits row too long");
+    if (top_k > 64 || top_k > n) return fail(MVH_E_RANGE, "top_k above 64 or the row's length");
+    if (!rows) return MVH_OK;
+    if (!logits) return fail(MVH_E_INVALID, "null logits");
+    if (logprob && !targets) return fail(MVH_E_INVALID, "logprob needs targets");
+    if (!top_k) top_ids = nullptr, top_logprobs = nullptr;
+    if (!top_ids && !top_logprobs) top_k = 0;
+    if (!logprob && !entropy && !top_k) return MVH_OK;
+    const size_t tops = rows * top_k * 4;
+    const float* ld = logits;
+    const int* td = targets;
+    float *lpd = logprob, *ed = entropy, *tld = top_logprobs;
+    int* tid = top_ids;
+    if (kind == MVH_HOST) {
+        if (logprob)
+            for (size_t r = 0; r < rows; ++r)
+                if (targets[r] < 0 || static_cast<size_t>(targets[r]) >= n)
+                    return fail(MVH_E_RANGE, "target %d of row %zu out of range", targets[r], r);
+        const size_t lb = up16(rows * n * 4);
+        if (int rc = grow(c, c->xin, lb + rows * 4)) return rc;
+        if (int rc = grow(c, c->yout, 2 * rows * 4 + 2 * tops)) return rc;
+        auto* base = static_cast<uint8_t*>(c->xin.p);
+        MVH_HIP(hipMemcpyAsync(base, logits, rows * n * 4, hipMemcpyHostToDevice, c->stream));
+        if (logprob) MVH_HIP(hipMemcpyAsync(base + lb, targets, rows * 4, hipMemcpyHostToDevice, c->stream));
+        ld = reinterpret_cast<const float*>(base);
+        td = reinterpret_cast<const int*>(base + lb);
+        auto* y = static_cast<uint8_t*>(c->yout.p);
+        if (logprob) lpd = reinterpret_cast<float*>(y);
+        if (entropy) ed = reinterpret_cast<float*>(y + rows * 4);
+        if (top_ids) tid = reinterpret_cast<int*>(y + 2 * rows * 4);
+        if (top_logprobs) tld = reinterpret_cast<float*>(y + 2 * rows * 4 + tops);
+    }
+    if (int rc = grow_kept(c, c->work, mvh::logprobs_scratch(n, rows, top_k))) return rc;
+    MVH_HIP(mvh::launch_logprobs(ld, n, n, rows, td, top_k, lpd, ed, tid, tld, c->work.p, c->stream));
+    if (kind == MVH_HOST) {
+        if (logprob) MVH_HIP(hipMemcpyAsync(logprob, lpd, rows * 4, hipMemcpyDeviceToHost, c->stream));
+        if (entropy) MVH_HIP(hipMemcpyAsync(entropy, ed, rows * 4, hipMemcpyDeviceToHost, c->stream));
+        if (top_ids) MVH_HIP(hipMemcpyAsync(top_ids, tid, tops, hipMemcpyDeviceToHost, c->stream));
+        if (top_logprobs) MVH_HIP(hipMemcpyAsync(top_logprobs, tld, tops, hipMemcpyDeviceToHost, c->stream));
+        MVH_HIP(hipStreamSynchronize(c->stream));
+    }
+    return MVH_OK;
+}
+
+// mvh_attn_decode / mvh_attn_batch over 4-bit pages, past their checks
+static int attend_q4(mvh_context* c, const mvh_kv_cache* kv, size_t layer, const float* q, size_t pos, size_t n_tokens,
+                     size_t n_head, size_t n_head_kv, size_t head_dim, float* out, int kind) {
+    if (int rc = check_kv_on(c, kv, layer)) return rc;
+    if (n_head > (size_t{1} << 16) || head_dim > 1024) return fail(MVH_E_RANGE, "n_head above 65536 or head_dim above 1024");
+    if (n_tokens * (n_head / n_head_kv) > 8 * 65535 || n_tokens > 65535)
+        return fail(MVH_E_RANGE, "a 4-bit cache takes chunks of up to 65535 tokens and 524280 rows a kv head");
+    const size_t qn = n_tokens * n_head * head_dim;
+    const void* qd = nullptr;
+    if (int rc = stage_in(c, c->xin, q, qn * 4, kind, &qd)) return rc;
+    float* od = out;
+    if (kind == MVH_HOST) {
+        if (int rc = grow(c, c->yout, qn * 4)) return rc;
+        od = static_cast<float*>(c->yout.p);
+    }
+    const size_t need = mvh::attn_q4_scratch(pos + n_tokens, n_tokens, n_head, n_head_kv, head_dim, kv->page_tokens, 0);
+    if (int rc = grow_kept(c, c->work, need * 4)) return rc;
+    const size_t base = layer * kv->max_pages;
+    MVH_HIP(mvh::launch_attn_q4(kv->dk + base, kv->dv + base, static_cast<const float*>(qd), n_head * head_dim,
+                                static_cast<float*>(c->work.p), od, nullptr, pos, pos + n_tokens, n_tokens, n_head,
+                                n_head_kv, head_dim, kv->kv_dim, kv->page_tokens, 0, c->stream));
+    return finish_out(c, out, od, qn * 4, kind);
 }
 
 int mvh_attn_decode(mvh_context* c, const mvh_kv_cache* kv, size_t layer, const float* q, size_t pos, size_t n_head,
@@ -1046,6 +1393,7 @@ int mvh_attn_decode(mvh_context* c, const mvh_kv_cache* kv, size_t layer, const 
     if (pos >= kv->max_tokens) return fail(MVH_E_RANGE, "context exhausted");
     for (size_t p = 0; p <= pos / kv->page_tokens; ++p)
         if (!kv->hk[layer * kv->max_pages + p]) return fail(MVH_E_RANGE, "KV key page missing");
+    if (kv->type == MVH_KV_Q4) return attend_q4(c, kv, layer, q, pos, 1, n_head, n_head_kv, head_dim, out, kind);
     const size_t qn = n_head * head_dim;
     const void* qd = nullptr;
     if (int rc = stage_in(c, c->xin, q, qn * 4, kind, &qd)) return rc;
@@ -1076,6 +1424,7 @@ int mvh_attn_batch(mvh_context* c, const mvh_kv_cache* kv, size_t layer, const f
     const size_t last = pos + n_tokens - 1;
     for (size_t p = 0; p <= last / kv->page_tokens; ++p)
         if (!kv->hk[layer * kv->max_pages + p]) return fail(MVH_E_RANGE, "KV key page missing");
+    if (kv->type == MVH_KV_Q4) return attend_q4(c, kv, layer, q, pos, n_tokens, n_head, n_head_kv, head_dim, out, kind);
     const size_t qn = n_tokens * n_head * head_dim;
     const void* qd = nullptr;
     if (int rc = stage_in(c, c->xin, q, qn * 4, kind, &qd)) return rc;
@@ -1127,7 +1476,7 @@ int mvh_model_open(const char* path, int device, size_t ctx_override, size_t pag
     if (!path || !out) return fail(MVH_E_INVALID, "null argument");
     *out = nullptr;
     if (act_mode != MVH_ACT_REF && act_mode != MVH_ACT_Q8) return fail(MVH_E_INVALID, "bad act_mode %d", act_mode);
-    if (kv_type != MVH_KV_F32 && kv_type != MVH_KV_F16 && kv_type != MVH_KV_Q8)
+    if (kv_type != MVH_KV_F32 && kv_type != MVH_KV_F16 && kv_type != MVH_KV_Q8 && kv_type != MVH_KV_Q4)
         return fail(MVH_E_INVALID, "unknown KV cache type id %d", kv_type);
     return guarded([&] {
         auto mode = act_mode == MVH_ACT_Q8 ? memvanta::hip::PrefillMode::Q8 : memvanta::hip::PrefillMode::Reference;

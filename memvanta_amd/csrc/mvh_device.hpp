@@ -330,21 +330,25 @@ __device__ __forceinline__ void rmsnorm_row(float* __restrict__ xr_, const float
 
 // ---- paged KV cache element types ------------------------------------------
 //
-// PagedKVCache's KVCacheType (F32, F16, Q8 in that order).  One page of K (or
-// V) is [page_tokens][kv_dim] elements of the type: float, fp16 bits, or int8;
-// a Q8 page then holds its page_tokens float row scales at a 16-byte aligned
-// offset after the elements.
-enum KvType : int { kKvF32 = 0, kKvF16 = 1, kKvQ8 = 2 };
+// PagedKVCache's KVCacheType (F32, F16, Q8 in that order), and Q4, which the
+// reference has not.  One page of K (or V) is [page_tokens][kv_dim] elements of
+// the type: float, fp16 bits, or int8; a Q8 page then holds its page_tokens
+// float row scales at a 16-byte aligned offset after the elements.  A Q4 page
+// has a layout of its own (mvh_kv4.hpp), 160 bytes per block of 32 channels
+// and 8 rows.
+enum KvType : int { kKvF32 = 0, kKvF16 = 1, kKvQ8 = 2, kKvQ4 = 3 };
 __host__ __device__ constexpr size_t kv_elem_bytes(int kt) { return kt == kKvF32 ? 4 : kt == kKvF16 ? 2 : 1; }
 __host__ __device__ constexpr size_t kv_scale_offset(size_t page_tokens, size_t kv_dim) {
     return (page_tokens * kv_dim + 15) / 16 * 16;
 }
 __host__ __device__ constexpr size_t kv_page_bytes(int kt, size_t page_tokens, size_t kv_dim) {
+    if (kt == kKvQ4) return kv_dim / 32 * ((page_tokens + 7) / 8) * 160;
     return kt == kKvQ8 ? kv_scale_offset(page_tokens, kv_dim) + 4 * page_tokens : page_tokens * kv_dim * kv_elem_bytes(kt);
 }
 // bytes PagedKVCache::bytes_allocated counts per page index (K and V; the
-// Q8 alignment padding is not counted)
+// Q8 alignment padding and a Q4 page's rounding to 8 rows are not counted)
 __host__ __device__ constexpr size_t kv_page_pair_bytes_ref(int kt, size_t page_tokens, size_t kv_dim) {
+    if (kt == kKvQ4) return 2 * page_tokens * kv_dim / 8 * 5;
     return 2 * (page_tokens * kv_dim * kv_elem_bytes(kt) + (kt == kKvQ8 ? 4 * page_tokens : 0));
 }
 

@@ -1,6 +1,7 @@
 // mvh_kernels.hpp -- launchers of the gfx950 kernels (host-callable).
 #pragma once
 #include "mvh_device.hpp"
+#include "mvh_rope.hpp"
 
 #include <algorithm>
 
@@ -130,6 +131,46 @@ hipError_t launch_attn_decode_fused(const float* q, const float* k, const float*
 hipError_t launch_attn_decode(int kv_type, const void* const* pt_k, const void* const* pt_v, const float* q,
                               float* scores, float* out, size_t pos, size_t n_head, size_t n_head_kv, size_t hd,
                               size_t kv_dim, size_t page_tokens, hipStream_t st);
+
+// ---- 4-bit pages: attention (mvh_attn_q4.hip) ----
+// The attention of launch_attn over kKvQ4 pages, any hd % 8 == 0, kv_dim % 32
+// == 0: n_tokens query tokens at positions pos.. (*d_pos when d_pos != null),
+// max_pos > last position.  Splits of `chunk` 32-row steps (a token's bits then
+// depend on nothing but its q and the rows up to it), or, with 0, as many as
+// fill the chip.  part: attn_q4_scratch(...) floats for the same arguments.
+size_t attn_q4_chunk(size_t max_pos, size_t page_tokens);  // a fixed chunk for positions below max_pos
+size_t attn_q4_scratch(size_t max_pos, size_t n_tokens, size_t n_head, size_t n_head_kv, size_t hd, size_t page_tokens,
+                       size_t chunk);
+hipError_t launch_attn_q4(const void* const* pt_k, const void* const* pt_v, const float* q, size_t q_pitch, float* part,
+                          float* out, const int* d_pos, size_t pos, size_t max_pos, size_t n_tokens, size_t n_head,
+                          size_t n_head_kv, size_t hd, size_t kv_dim, size_t page_tokens, size_t chunk, hipStream_t st);
+
+// ---- rotary positions and rotated appends (mvh_rope.hip) ----
+// out row t = x row t (n_head heads) rotated by position positions[t], or pos +
+// t when positions == null; out == x with equal pitches is allowed
+hipError_t launch_rope(const RopeView& rope, const float* x, size_t x_pitch, float* out, size_t out_pitch,
+                       const int* positions, size_t pos, size_t n_tokens, size_t n_head, hipStream_t st);
+// q (n_head heads; may be none) rotated to q_out, k rotated and v as it is
+// stored at positions pos.. in pages of kv_type; kv_dim = whole heads
+hipError_t launch_kv_append(int kv_type, const RopeView& rope, void* const* pt_k, void* const* pt_v, const float* q,
+                            size_t q_pitch, float* q_out, size_t out_pitch, const float* k, size_t k_pitch,
+                            const float* v, size_t v_pitch, size_t pos, size_t n_tokens, size_t n_head, size_t kv_dim,
+                            size_t page_tokens, hipStream_t st);
+// the kKvQ4 case of launch_kv_write
+hipError_t launch_kv4_write(void* const* pt_k, void* const* pt_v, const float* k, const float* v, size_t pitch,
+                            const int* d_pos, size_t pos, size_t n_tokens, size_t kv_dim, size_t page_tokens,
+                            hipStream_t st);
+// rows pos.. of K and V (either may be null) as fp32 [n_tokens][kv_dim]
+hipError_t launch_kv_read(int kv_type, const void* const* pt_k, const void* const* pt_v, size_t pos, size_t n_tokens,
+                          size_t kv_dim, size_t page_tokens, float* k, float* v, hipStream_t st);
+
+// ---- log probabilities (mvh_logprobs.hip) ----
+// per row of n logits (pitch apart): log probability of targets[row], entropy,
+// the k <= 64 most probable tokens; any output may be null; scratch of
+// logprobs_scratch(n, rows, k) bytes, 8-byte aligned
+size_t logprobs_scratch(size_t n, size_t rows, size_t k);
+hipError_t launch_logprobs(const float* logits, size_t pitch, size_t n, size_t rows, const int* targets, size_t k,
+                           float* logprob, float* entropy, int* top_ids, float* top_lp, void* scratch, hipStream_t st);
 
 // ---- measurement probe (mvh_probe.hip) ----
 // reads bytes (a multiple of 16) of buf once; sink holds sink_words words (at

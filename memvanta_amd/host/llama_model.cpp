@@ -58,7 +58,7 @@ LlamaModel::LlamaModel(const std::string& path, int device, std::size_t ctx_over
                        int kv_type, PrefillMode mode, std::size_t max_batch)
     : file_(std::make_unique<GgufFile>(path)), device_(device), kv_type_(kv_type), mode_(mode),
       page_tokens_(kv_page_tokens ? kv_page_tokens : 128), max_batch_(std::max<std::size_t>(1, max_batch)) {
-    if (kv_type != mvh::kKvF32 && kv_type != mvh::kKvF16 && kv_type != mvh::kKvQ8)
+    if (kv_type != mvh::kKvF32 && kv_type != mvh::kKvF16 && kv_type != mvh::kKvQ8 && kv_type != mvh::kKvQ4)
         throw std::runtime_error("unknown KV cache type id " + std::to_string(kv_type));
     const auto arch = file_->get_string("general.architecture").value_or("");
     if (arch != "llama")
@@ -84,6 +84,8 @@ LlamaModel::LlamaModel(const std::string& path, int device, std::size_t ctx_over
         throw std::runtime_error("invalid Llama head configuration");
     if (c_.n_embd % 32 || c_.n_ff % 32 || c_.head_dim() % 8)
         throw std::runtime_error("device path needs n_embd, n_ff % 32 == 0 and head_dim % 8 == 0");
+    if (kv_type_ == mvh::kKvQ4 && c_.kv_dim() % 32)
+        throw std::runtime_error("kv_dim of a 4-bit KV cache must be a multiple of 32");
 
     check(hipSetDevice(device_), "hipSetDevice");
     check(hipStreamCreateWithFlags(&lanes_[0].st, hipStreamNonBlocking), "hipStreamCreate");
@@ -147,6 +149,7 @@ LlamaModel::LlamaModel(const std::string& path, int device, std::size_t ctx_over
     check(hipMemcpy(rope_sin_, si.data(), si.size() * 4, hipMemcpyHostToDevice), "upload rope");
     rope_cur_ = static_cast<float*>(dalloc(c_.head_dim() * 4));
 
+    q4_chunk_ = kv_type_ == mvh::kKvQ4 ? mvh::attn_q4_chunk(c_.n_ctx, page_tokens_) : 0;
     // paged KV cache: the pages of every layer preallocated in HBM, addressed
     // through per-layer page tables; page stride 256-byte aligned (a Q8 page
     // ends with its float row scales)
@@ -193,7 +196,7 @@ LlamaModel::LlamaModel(const std::string& path, int device, std::size_t ctx_over
             l.proj = static_cast<float*>(take(B * D * 4));
             l.gu = static_cast<float*>(take(B * 2 * F * 4));
             l.ff = static_cast<float*>(take(B * F * 4));
-            l.scores = static_cast<float*>(take(B * c_.n_head * c_.n_ctx * 4));
+            l.scores = static_cast<float*>(take(kv_type_ == mvh::kKvQ4 ? q4_scratch(B) * 4 : B * c_.n_head * c_.n_ctx * 4));
             l.ffo = static_cast<float*>(take(B * D * 4));
             l.q8 = static_cast<int8_t*>(take(mvh::q8_op_bytes(B, W)));  // row-major or operand order
             l.q8d = static_cast<float*>(take(B * (W / 32) * 4));
@@ -302,6 +305,13 @@ LlamaModel::QkvLayout LlamaModel::qkv_layout(const Layer& L, std::size_t B) cons
     const std::size_t D = c_.n_embd, KV = c_.kv_dim();
     if (L.fused_qkv) return {ln_->qkv, ln_->qkv + D, ln_->qkv + D + KV, D + 2 * KV, D + 2 * KV};
     return {ln_->qkv, ln_->qkv + B * D, ln_->qkv + B * (D + KV), D, KV};
+}
+
+// Floats of workspace that the attention over 4-bit pages of a chunk of up to B tokens takes, or of a decode step.
+std::size_t LlamaModel::q4_scratch(std::size_t B) const {
+    const std::size_t hd = c_.head_dim();
+    return std::max(mvh::attn_q4_scratch(c_.n_ctx, B, c_.n_head, c_.n_head_kv, hd, page_tokens_, q4_chunk_),
+                    mvh::attn_q4_scratch(c_.n_ctx, 1, c_.n_head, c_.n_head_kv, hd, page_tokens_, 0));
 }
 
 float* LlamaModel::upload_vector(const std::string& name) {
@@ -469,8 +479,13 @@ void LlamaModel::decode_step(const int* d_token, bool logits, bool argmax) {
         void* const* pk = pt_k_ + li * max_pages_;
         void* const* pv = pt_v_ + li * max_pages_;
         // the attention kernels write the o projection's Q8 activations (32-element head slices are Q8 blocks)
-        const bool o_q8 = L.o.type == 2 && hd % 32 == 0 && L.o.cols == c_.n_head * hd;
-        if (fused_attn_) {
+        const bool o_q8 = L.o.type == 2 && hd % 32 == 0 && L.o.cols == c_.n_head * hd && kv_type_ != mvh::kKvQ4;
+        if (kv_type_ == mvh::kKvQ4) {
+            store_kv(lay, pk, pv, d_pos_, 0, 1);
+            check(mvh::launch_attn_q4(pk, pv, lay.q, lay.q_pitch, a.scores, a.att, d_pos_, 0, c_.n_ctx, 1, c_.n_head,
+                                      c_.n_head_kv, hd, c_.kv_dim(), page_tokens_, 0, a.st),
+                  "attention");
+        } else if (fused_attn_) {
             const std::size_t layer_off = li * max_pages_ * kv_stride_;
             check(mvh::launch_attn_decode_fused(lay.q, lay.k, lay.v, rope_cur_, d_pos_,
                                                 reinterpret_cast<uint16_t*>(kslab_ + layer_off),
@@ -549,20 +564,31 @@ void LlamaModel::batch_step(const int* d_tokens, std::size_t B, bool logits, int
         }
         void* const* pk = pt_k_ + li * max_pages_;
         void* const* pv = pt_v_ + li * max_pages_;
-        store_kv(lay, pk, pv, nullptr, pos_, B);
         // this chunk's attention of the layer reads the rows of every earlier
         // chunk: it waits for the previous chunk's event, and records its own
         // only after that wait, so the event of chunk c stands for the rows
-        // of chunks 0..c (with three lanes chunk c - 2 runs on a third stream)
-        if (prev_lane >= 0)
-            check(hipStreamWaitEvent(a.st, kv_done_[prev_lane * c_.n_layer + li], 0), "event wait");
+        // of chunks 0..c (with three lanes chunk c - 2 runs on a third stream).
+        // A word of a Q4 page holds rows of two chunks where they meet within
+        // 8 rows: there the store waits too
+        auto wait = [&] {
+            if (prev_lane >= 0)
+                check(hipStreamWaitEvent(a.st, kv_done_[prev_lane * c_.n_layer + li], 0), "event wait");
+        };
+        const bool wait_first = kv_type_ == mvh::kKvQ4;
+        if (wait_first) wait();
+        store_kv(lay, pk, pv, nullptr, pos_, B);
+        if (!wait_first) wait();
         check(hipEventRecord(kv_done_[lane * c_.n_layer + li], a.st), "event record");
         // the softmax-V kernel also writes the o projection's Q8 activations
         // (32-element head slices are Q8 blocks), in the MFMA GEMM's operand
         // order when the projection runs there
-        const bool o_q8 = q8mode && L.o.type == 2 && hd % 32 == 0 && L.o.cols == c_.n_head * hd;
+        const bool o_q8 = q8mode && L.o.type == 2 && hd % 32 == 0 && L.o.cols == c_.n_head * hd && kv_type_ != mvh::kKvQ4;
         const bool o_op = o_q8 && mfma_gemm(L.o);
-        if (hd % 32 == 0) {  // scores + softmax once per (token, head), V tiles shared by the chunk's tokens
+        if (kv_type_ == mvh::kKvQ4) {
+            check(mvh::launch_attn_q4(pk, pv, lay.q, lay.q_pitch, a.scores, a.att, nullptr, pos_, pos_ + B, B, c_.n_head,
+                                      c_.n_head_kv, hd, c_.kv_dim(), page_tokens_, q4_chunk_, a.st),
+                  "attention");
+        } else if (hd % 32 == 0) {  // scores + softmax once per (token, head), V tiles shared by the chunk's tokens
             check(mvh::launch_attn_prefill(kv_type_, pk, pv, lay.q, lay.q_pitch, a.scores, a.att, o_q8 ? a.q8 : nullptr,
                                            a.q8d,
                                            o_op, nullptr, pos_, pos_ + B, B, c_.n_head, c_.n_head_kv, hd,
@@ -618,8 +644,8 @@ std::size_t LlamaModel::kv_bytes_allocated() const {
 void LlamaModel::store_kv(const QkvLayout& lay, void* const* pk, void* const* pv, const int* d_pos, std::size_t pos,
                           std::size_t B) {
     // F16 and F32 rows are written by the RoPE launch; a Q8 row's scale
-    // spans every head, so Q8 pages get their own write launch
-    const bool fused = kv_type_ != mvh::kKvQ8;
+    // spans every head and a Q4 word several rows, so these get their own write launch
+    const bool fused = kv_type_ != mvh::kKvQ8 && kv_type_ != mvh::kKvQ4;
     check(mvh::launch_rope_kv(lay.q, lay.q_pitch, lay.k, lay.v, lay.kv_pitch, rope_cos_, rope_sin_, d_pos, pos, B,
                               c_.n_head, c_.n_head_kv, c_.head_dim(), kv_type_, fused ? pk : nullptr,
                               fused ? pv : nullptr, page_tokens_, ln_->st),

@@ -34,7 +34,7 @@ enum class PrefillMode { Reference = 0, Q8 = 1 };  // Q8 = MEMVANTA_FORCE_Q8_ACT
 
 class LlamaModel {
 public:
-    // kv_type: KVCacheType order, 0 = F32, 1 = F16 (the reference's default), 2 = Q8
+    // kv_type: KVCacheType order, 0 = F32, 1 = F16 (the reference's default), 2 = Q8; 3 = Q4 (not in the reference)
     LlamaModel(const std::string& gguf_path, int device = 0, std::size_t ctx_override = 0,
                std::size_t kv_page_tokens = 128, int kv_type = 1, PrefillMode mode = PrefillMode::Q8,
                std::size_t max_batch = 64);
@@ -81,6 +81,7 @@ private:
     void upload(Tensor& t, const std::string& name);
     bool upload_fused(Tensor& t, const std::vector<std::string>& names);
     float* upload_vector(const std::string& name);
+    std::size_t q4_scratch(std::size_t B) const;
     void gemv(const Tensor& w, const float* x, const int8_t* q8, const float* q8d, float* y);
     // q8/q8d: the Q8 activations of x when already quantized (null: quantize
     // here); q8_op: q8 is in the MFMA GEMM's operand order (mfma_gemm(w) holds)
@@ -141,6 +142,7 @@ private:
     float* rope_cur_{};                  // cos/sin row of the decode position (written by the embedding launch)
     uint8_t *kslab_{}, *vslab_{};        // every layer's KV pages, page i of layer l at slab + (l * max_pages_ + i) * kv_stride_
     std::size_t kv_stride_{};
+    std::size_t q4_chunk_{};             // 4-bit pages: mvh::attn_q4_chunk
     float* logits_d_{};
     int *d_tok_{}, *d_pos_{}, *d_hist_{};  // d_hist_[p] = greedy token sampled at position p
     int* d_prompt_{};                       // token ids of a prefill call, chunk i's at d_prompt_ + i
