@@ -12,6 +12,8 @@
 #include "mvh_kernels.hpp"
 #include "mvh_kv4.hpp"
 
+#include <type_traits>
+
 namespace mvh {
 namespace {
 
@@ -30,7 +32,7 @@ struct Q4Args {
     Kv4Map map;
 };
 
-constexpr float kLowest = -3.0e38f;  // m before the first row: finite, so that 2^(-inf - m) is 0
+constexpr float kLowest = -1.0e12f;  // m before the first row: finite, so that 2^(-inf - m) is 0; scores stay above it
 constexpr float kLog2e = 1.44269504088896340736f;
 // Weights are 2^(y - m + lift), at most 2^lift, so that p s stays clear of both
 // ends of fp16: lift 14 while every step s seen is below 2, then 6 (s <= 512).
@@ -58,8 +60,39 @@ __device__ __forceinline__ float rows_sum(float v) {
     auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
-__device__ __forceinline__ float plus_ror8(float v) { return v + dpp_mov<0x128>(v); }  // + lane (l + 8) % 16 of the row
-__device__ __forceinline__ half2v pk_rtz(float a, float b) { return __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(a, b)); }
+__device__ __forceinline__ float plus_ror8(float v) {  // + lane (l + 8) % 16 of the 16
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, true));
+}
+
+// Loads at a base that is the same in every lane plus a 32-bit offset: the base
+// stays in scalar registers.
+__device__ __forceinline__ uint2 ld8_at(const uint8_t* base, uint32_t off) {
+    const auto* b = (const __attribute__((address_space(1))) uint8_t*)(reinterpret_cast<uintptr_t>(base));
+    const u32x2 v = *(const __attribute__((address_space(1))) u32x2*)(b + off);
+    return make_uint2(v.x, v.y);
+}
+__device__ __forceinline__ uint32_t ld4_at(const uint8_t* base, uint32_t off) {
+    const auto* b = (const __attribute__((address_space(1))) uint8_t*)(reinterpret_cast<uintptr_t>(base));
+    return *(const __attribute__((address_space(1))) uint32_t*)(b + off);
+}
+__device__ __forceinline__ u32x4 ld16_at(const uint8_t* base, uint32_t off) {
+    const auto* b = (const __attribute__((address_space(1))) uint8_t*)(reinterpret_cast<uintptr_t>(base));
+    return *(const __attribute__((address_space(1))) u32x4*)(b + off);
+}
+// An entry of a page table through the scalar cache (page: the same in every lane)
+__device__ __forceinline__ const uint8_t* page_at(const void* const* pt, int page) {
+    typedef const __attribute__((address_space(4))) uint64_t* entry;
+    return reinterpret_cast<const uint8_t*>(*reinterpret_cast<entry>(reinterpret_cast<uintptr_t>(pt + page)));
+}
+
+// Two floats as fp16, rounded to nearest
+__device__ __forceinline__ half2v pk_half(float a, float b) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    const f32x2 v = {a, b};
+    return __builtin_convertvector(v, half2v);
+}
+// p - h (exact where h is p rounded, or 0): the conversion inside the addition
+__device__ __forceinline__ float less(float p, _Float16 h, float minus1) { return fmaf(static_cast<float>(h), minus1, p); }
 
 // One workgroup: 8 query rows (row = token * group + head of the kv head) of kv
 // head x, tile y, split z.  Its four waves take 32-row steps in turn, each with
@@ -77,7 +110,7 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
     __shared__ float s_o[kWaves][8][PITCH];
     __shared__ float s_c[kWaves][8][12];  // [0..NB) sum p c of the blocks, [NB] sum p
     __shared__ float s_m[kWaves][8];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 15, j = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, j = lane >> 4;
     const int kh = blockIdx.x, row0 = blockIdx.y * 8, rows = a.n_tokens * a.group;
     const int pos = a.d_pos ? *a.d_pos : a.pos;
     const int tile_lim = pos + (min(row0 + 8, rows) - 1) / a.group, first_lim = pos + row0 / a.group;
@@ -85,11 +118,104 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
     const int begin = blockIdx.z * chunk, end = min(begin + chunk, steps_of(a.map, tile_lim));
     if (begin >= end) return;  // rows past the tile's last position
 
+    const int groups = a.map.groups, last_group = a.map.group_of(tile_lim);
+    const size_t sc_off = kv4_scales(a.map.page_tokens, a.kv_dim);
+    const size_t n_head_off = static_cast<size_t>(kh * NB) * groups * 128, s_head_off = sc_off + static_cast<size_t>(kh * NB) * groups * 32;
+    const size_t n_blk = static_cast<size_t>(groups) * 128, s_blk = static_cast<size_t>(groups) * 32;
+    const uint32_t kn_lane = (col >> 2) * 128 + (j * 4 + (col & 3)) * 8, vn_lane = j * 128 + col * 8, s_lane = j * 32;
+    const uint32_t vc_lane = static_cast<uint32_t>(min(col, NB - 1)) * static_cast<uint32_t>(s_blk) + j * 32 + 16;
+    uint32_t kc_lane[(NB + 3) / 4];
+#pragma unroll
+    for (int k = 0; k < (NB + 3) / 4; ++k)
+        kc_lane[k] = static_cast<uint32_t>(min(j + 4 * k, NB - 1)) * static_cast<uint32_t>(s_blk) + (col >> 2) * 32 + 16 + (col & 3) * 4;
+
+    // the page of group g (of 4) of step st, and the group's index there (UNI: whole steps lie in a page)
+    auto locate = [&](const void* const* pt, int st, int g, const uint8_t*& base, int& at) {
+        const int vg = min(4 * st + g, last_group), page = a.map.page_of(vg);
+        base = static_cast<const uint8_t*>(pt[page]);
+        at = vg - page * groups;
+    };
+    constexpr int NQ = (NB + 3) / 4;  // blocks j, j + 4 of a lane's share of the c
+    uint2 kn[NB], vn[NB];
+    u32x4 ks[NB], vs[NB], vc;
+    uint32_t kc[NQ];  // c of the lane's two cache rows, blocks j and j + 4
+    auto load_k = [&](const uint8_t* page, int st) {
+        if constexpr (UNI) {
+            const int g0 = 4 * st - a.map.page_of(4 * st) * groups;
+            const uint8_t* nb = page + n_head_off + static_cast<size_t>(g0) * 128;
+            const uint8_t* sb = page + s_head_off + static_cast<size_t>(g0) * 32;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                kn[b] = ld8_at(nb + b * n_blk, kn_lane);
+                ks[b] = ld16_at(sb + b * s_blk, s_lane);
+            }
+#pragma unroll
+            for (int k = 0; k < NQ; ++k) kc[k] = ld4_at(sb, kc_lane[k]);
+        } else {
+            const uint8_t *bn, *bs;
+            int gn, gs;
+            locate(a.pt_k, st, col >> 2, bn, gn);
+            locate(a.pt_k, st, j, bs, gs);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                kn[b] = ld8_at(bn + n_head_off + b * n_blk + static_cast<size_t>(gn) * 128, (j * 4 + (col & 3)) * 8);
+                ks[b] = ld16_at(bs + s_head_off + b * s_blk + static_cast<size_t>(gs) * 32, 0);
+            }
+#pragma unroll
+            for (int k = 0; k < NQ; ++k)
+                kc[k] = ld4_at(bn + s_head_off + min(j + 4 * k, NB - 1) * s_blk + static_cast<size_t>(gn) * 32, 16 + (col & 3) * 4);
+        }
+    };
+    auto load_v = [&](const uint8_t* page, int st) {
+        if constexpr (UNI) {
+            const int g0 = 4 * st - a.map.page_of(4 * st) * groups;
+            const uint8_t* nb = page + n_head_off + static_cast<size_t>(g0) * 128;
+            const uint8_t* sb = page + s_head_off + static_cast<size_t>(g0) * 32;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                vn[b] = ld8_at(nb + b * n_blk, vn_lane);
+                vs[b] = ld16_at(sb + b * s_blk, s_lane);
+            }
+            vc = ld16_at(sb, vc_lane);
+        } else {
+            const uint8_t* base;
+            int g;
+            locate(a.pt_v, st, j, base, g);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                vn[b] = ld8_at(base + n_head_off + b * n_blk + static_cast<size_t>(g) * 128, col * 8);
+                vs[b] = ld16_at(base + s_head_off + b * s_blk + static_cast<size_t>(g) * 32, 0);
+            }
+            vc = ld16_at(base + s_head_off + min(col, NB - 1) * s_blk + static_cast<size_t>(g) * 32, 16);
+        }
+    };
+    auto page_of_step = [&](const void* const* pt, int st) -> const uint8_t* {
+        if constexpr (UNI) return page_at(pt, a.map.page_of(4 * st));
+        else return nullptr;
+    };
+
+    int st = begin + wave;
+    if (st < end) {
+        load_k(page_of_step(a.pt_k, st), st);
+        load_v(page_of_step(a.pt_v, st), st);
+    }
+
     // q: lane (col, j) holds channels 8 j .. of each block of row col % 8; scaled by a power of two to [1, 2)
     const int r = min(row0 + (col & 7), rows - 1), lim = pos + r / a.group;
     const float* qr = a.q + static_cast<size_t>(r / a.group) * a.q_pitch + static_cast<size_t>(kh * a.group + r % a.group) * HD;
-    half8 qf[NB];
-    float qs[NB], y_scale;
+    // masks and constants that the compiler is not to see: as selects and literals they take more operations
+    uint32_t low_mask = col >= 8 ? 0xffffffffu : 0u;
+    uint32_t c_mask = col < NB ? 0xffffffffu : 0u, c_fill = col == NB ? 0x3c003c00u : 0u;  // ones: sum p
+    float minus1 = -1.0f;
+    Q4Ones ones;
+    asm("" : "+v"(low_mask), "+v"(ones.c16), "+v"(ones.c256), "+v"(c_mask), "+v"(c_fill), "+v"(minus1));
+    // two numbers as the column holds them: rounded to fp16, or what the rounding left
+    auto part = [&](float a, float b) {
+        const half2v h = as_half2(as_u32(pk_half(a, b)) & low_mask);
+        return as_u32(pk_half(less(a, h.x, minus1), less(b, h.y, minus1)));
+    };
+    u32x4 qf[NB], qc = {0u, 0u, 0u, 0u};  // qc: block sums of q, one or two a lane: the operand that meets kc
+    float y_scale;
     {
         float f[NB][8], top = 0.0f;
 #pragma unroll
@@ -101,110 +227,97 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
             }
         }
         top = rows_max(top);
-        const int e = top > 0.0f && top <= 3.402823466e38f ? __builtin_amdgcn_frexp_expf(top) - 1 : 0;
+        const int e = top > 0.0f && top <= 3.402823466e38f ? max(__builtin_amdgcn_frexp_expf(top) - 1, -120) : 0;
+        const float down = ldexpf(1.0f, -e);
         y_scale = ldexpf(__fdiv_rn(kLog2e, sqrt_rn(static_cast<float>(HD))), e);
-        const bool low = col >= 8;
+        float mine[NQ];
+#pragma unroll
+        for (int k = 0; k < NQ; ++k) mine[k] = 0.0f;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float z = ldexpf(f[b][i], -e);
-                sum += z;
-                const _Float16 hi = static_cast<_Float16>(z);
-                const int at = (i & 3) * 2 + (i >> 2);  // nibble order of q4_unpack
-                qf[b][at] = low ? static_cast<_Float16>(z - static_cast<float>(hi)) : hi;
+                f[b][i] *= down;
+                sum += f[b][i];
             }
             sum = rows_sum(sum);
-            qs[b] = low ? 0.0f : sum;
+            if ((b & 3) == j) mine[b / 4] = sum;
+            // the order of q4_unpack
+            qf[b] = u32x4{part(f[b][0], f[b][4]), part(f[b][1], f[b][5]), part(f[b][2], f[b][6]), part(f[b][7], f[b][3])};
         }
+        qc[0] = part(mine[0], NQ > 1 ? mine[NQ - 1] : 0.0f);
     }
-
-    const int last_group = a.map.group_of(tile_lim);
-    const size_t sc_off = kv4_scales(a.map.page_tokens, a.kv_dim);
-    // group g (of 4) of step st: its page's base, and the group's index there
-    auto locate = [&](const void* const* pt, int st, int g, const uint8_t*& base, int& at) {
-        const int vg = UNI ? 4 * st : min(4 * st + g, last_group);
-        const int page = UNI ? __builtin_amdgcn_readfirstlane(a.map.page_of(vg)) : a.map.page_of(vg);
-        base = static_cast<const uint8_t*>(pt[page]);
-        at = vg - page * a.map.groups + (UNI ? g : 0);
-    };
-    uint2 kn[NB], vn[NB];
-    uint4 ks[NB], kc[NB], vs[NB], vc;
-    auto load_k = [&](int st) {
-        const uint8_t *bn, *bs;
-        int gn, gs;
-        locate(a.pt_k, st, col >> 2, bn, gn);
-        locate(a.pt_k, st, j, bs, gs);
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const size_t blk = static_cast<size_t>(kh * NB + b) * a.map.groups;
-            kn[b] = ld_global8(bn + (blk + gn) * 128 + (j * 4 + (col & 3)) * 8);
-            ks[b] = ld_global16(bs + sc_off + (blk + gs) * 32);
-            kc[b] = ld_global16(bs + sc_off + (blk + gs) * 32 + 16);
-        }
-    };
-    auto load_v = [&](int st) {
-        const uint8_t* base;
-        int g;
-        locate(a.pt_v, st, j, base, g);
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const size_t blk = static_cast<size_t>(kh * NB + b) * a.map.groups;
-            vn[b] = ld_global8(base + (blk + g) * 128 + col * 8);
-            vs[b] = ld_global16(base + sc_off + (blk + g) * 32);
-        }
-        vc = ld_global16(base + sc_off + (static_cast<size_t>(kh * NB + min(col, NB - 1)) * a.map.groups + g) * 32 + 16);
-    };
 
     f32x4 o[NB][2], oc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int b = 0; b < NB; ++b) o[b][0] = o[b][1] = oc;
-    float m = kLowest, lift = kLift;
-    const uint32_t low_mask = col >= 8 ? 0xffffffffu : 0u;
+    float m = kLowest, lift = kLift;  // m: of the scores before y_scale
+    const uint32_t c_turn = (col & 3) == 3 ? 16 : 0;  // rows 3 and 7 are stored the other way round
 
-    int st = begin + wave;
-    if (st < end) load_k(st);
-    for (; st < end; st += kWaves) {
-        load_v(st);
-        f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
-        const f32x4 zero = s0;
+    const u32x4 zero_words = {0u, 0u, 0u, 0u};
+    auto step = [&](auto edge_tag) {
+        constexpr bool EDGE = decltype(edge_tag)::value;
+        const uint8_t *next_k = nullptr, *next_v = nullptr;
+        const bool more = st + kWaves < end;
+        if (more) {
+            next_k = page_of_step(a.pt_k, st + kWaves);
+            next_v = page_of_step(a.pt_v, st + kWaves);
+        }
+        // scores of rows 8 j + i (s0) and 8 j + 4 + i (s1): the c first, then block by block
+        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+        f32x4 s0, s1;
+        {
+            u32x4 c0 = zero_words, c1 = zero_words;
+            uint32_t w0 = __builtin_amdgcn_alignbit(kc[0], kc[0], c_turn);
+            if constexpr (NQ == 1) {
+                c0[0] = w0 & 0xffffu;
+                c1[0] = w0 >> 16;
+            } else {
+                const uint32_t w1 = __builtin_amdgcn_alignbit(kc[NQ - 1], kc[NQ - 1], c_turn);
+                c0[0] = (w0 & 0xffffu) | (w1 << 16);
+                c1[0] = (w0 >> 16) | (w1 & 0xffff0000u);
+            }
+            s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, c0), __builtin_bit_cast(half8, qc), zero, 0, 0, 0);
+            s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, c1), __builtin_bit_cast(half8, qc), zero, 0, 0, 0);
+        }
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            const f32x4 c0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(q4_unpack(kn[b].x), qf[b], zero, 0, 0, 0);
-            const f32x4 c1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(q4_unpack(kn[b].y), qf[b], zero, 0, 0, 0);
-            const uint32_t sp[4] = {ks[b].x, ks[b].y, ks[b].z, ks[b].w}, cp[4] = {kc[b].x, kc[b].y, kc[b].z, kc[b].w};
+            const half8 q = __builtin_bit_cast(half8, qf[b]);
+            const f32x4 c0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(q4_unpack(kn[b].x, ones), q, zero, 0, 0, 0);
+            const f32x4 c1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(q4_unpack(kn[b].y, ones), q, zero, 0, 0, 0);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const half2v s = as_half2(sp[i]), c = as_half2(cp[i]);
-                s0[i] = fmaf(static_cast<float>(c.x), qs[b], fmaf(static_cast<float>(s.x), c0[i], s0[i]));
-                s1[i] = fmaf(static_cast<float>(c.y), qs[b], fmaf(static_cast<float>(s.y), c1[i], s1[i]));
+                const half2v s = as_half2(ks[b][i]);
+                s0[i] = fmaf(static_cast<float>(i < 3 ? s.x : s.y), c0[i], s0[i]);
+                s1[i] = fmaf(static_cast<float>(i < 3 ? s.y : s.x), c1[i], s1[i]);
             }
         }
-        if (st + kWaves < end) load_k(st + kWaves);
-        float y0[4], y1[4];
+        if (more) load_k(next_k, st + kWaves);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            y0[i] = plus_ror8(s0[i]) * y_scale;
-            y1[i] = plus_ror8(s1[i]) * y_scale;
+            s0[i] = plus_ror8(s0[i]);
+            s1[i] = plus_ror8(s1[i]);
         }
         // rows of the step that a query row does not see: p = 0, whatever is stored there
-        uint32_t seen[4] = {~0u, ~0u, ~0u, ~0u}, seen_c[4] = {~0u, ~0u, ~0u, ~0u};
-        const int lp = a.map.page_of(4 * st + 3), lg = 4 * st + 3 - lp * a.map.groups;
-        if ((!UNI && (a.map.page_tokens & 7)) || lp * a.map.page_tokens + lg * 8 + 7 > first_lim) {
-            const int page = a.map.page_of(4 * st + j), g = 4 * st + j - page * a.map.groups;
+        uint32_t seen[4], seen_c[4];
+        if constexpr (EDGE) {
+            const int page = a.map.page_of(4 * st + j), g = 4 * st + j - page * groups;
             const int p0 = page * a.map.page_tokens + g * 8, room = a.map.page_tokens - g * 8;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const bool in0 = i < room, in1 = i + 4 < room;
                 const bool v0 = in0 && p0 + i <= lim, v1 = in1 && p0 + i + 4 <= lim;
-                if (!v0) y0[i] = -INFINITY;
-                if (!v1) y1[i] = -INFINITY;
-                seen[i] = (v0 ? 0xffffu : 0u) | (v1 ? 0xffff0000u : 0u);
-                seen_c[i] = (in0 && p0 + i <= tile_lim ? 0xffffu : 0u) | (in1 && p0 + i + 4 <= tile_lim ? 0xffff0000u : 0u);
+                if (!v0) s0[i] = -INFINITY;
+                if (!v1) s1[i] = -INFINITY;
+                const uint32_t first = i < 3 ? 0xffffu : 0xffff0000u;
+                seen[i] = (v0 ? first : 0u) | (v1 ? ~first : 0u);
+                seen_c[i] = (in0 && p0 + i <= tile_lim ? first : 0u) | (in1 && p0 + i + 4 <= tile_lim ? ~first : 0u);
             }
         }
-        float mx = fmaxf(fmaxf(fmaxf(y0[0], y0[1]), fmaxf(y0[2], y0[3])), fmaxf(fmaxf(y1[0], y1[1]), fmaxf(y1[2], y1[3])));
+        float mx = s0[0];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = fmaxf(fmaxf(mx, s0[i]), s1[i]);
         mx = rows_max(mx);
         // a step of 2 and more (fp16 bit 14) among the rows that the query row sees
         uint32_t big = 0;
@@ -212,13 +325,13 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
         for (int i = 0; i < 4; ++i) {
             uint32_t w = 0;
 #pragma unroll
-            for (int b = 0; b < NB; ++b) w |= i == 0 ? vs[b].x : i == 1 ? vs[b].y : i == 2 ? vs[b].z : vs[b].w;
-            big |= w & seen[i];
+            for (int b = 0; b < NB; ++b) w |= vs[b][i];
+            big |= EDGE ? w & seen[i] : w;
         }
         big &= 0x40004000u;
         if (__any(mx > m || (big && lift == kLift))) {
             const float top = fmaxf(m, mx), down = rows_max(big ? 1.0f : 0.0f) > 0.0f ? kLiftBig : lift;
-            const float f = __builtin_amdgcn_exp2f((m - top) + (down - lift));
+            const float f = __builtin_amdgcn_exp2f(fmaf(m - top, y_scale, down - lift));
             m = top;
             lift = down;
             oc *= f;
@@ -228,40 +341,41 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
                 o[b][1] *= f;
             }
         }
-        half2v hi[4], lo[4];
-        u32x4 pf;
+        const float below = fmaf(-m, y_scale, lift);
+        half2v hi[4], lo[4], hl[4];
+        u32x4 pf, cf;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float p0 = __builtin_amdgcn_exp2f(y0[i] - (m - lift)), p1 = __builtin_amdgcn_exp2f(y1[i] - (m - lift));
-            hi[i] = pk_rtz(p0, p1);
-            lo[i] = as_half2(as_u32(pk_rtz(p0 - static_cast<float>(hi[i].x), p1 - static_cast<float>(hi[i].y))) & low_mask);
-            pf[i] = low_mask ? as_u32(lo[i]) : as_u32(hi[i]);
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(s0[i], y_scale, below)), p1 = __builtin_amdgcn_exp2f(fmaf(s1[i], y_scale, below));
+            const float pa = i < 3 ? p0 : p1, pb = i < 3 ? p1 : p0;
+            hi[i] = pk_half(pa, pb);
+            hl[i] = as_half2(as_u32(hi[i]) & low_mask);
+            pf[i] = as_u32(pk_half(less(pa, hl[i].x, minus1), less(pb, hl[i].y, minus1)));
+            lo[i] = as_half2(pf[i] & low_mask);
+            cf[i] = ((EDGE ? vc[i] & seen_c[i] : vc[i]) & c_mask) | c_fill;
         }
-        {
-            u32x4 cf = {vc.x & seen_c[0], vc.y & seen_c[1], vc.z & seen_c[2], vc.w & seen_c[3]};
-            const uint32_t fill = col == NB ? 0x3c003c00u : 0u;  // ones: sum p
-#pragma unroll
-            for (int i = 0; i < 4; ++i) cf[i] = col < NB ? cf[i] : fill;
-            oc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, cf), __builtin_bit_cast(half8, pf), oc, 0, 0, 0);
-        }
+        oc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, cf), __builtin_bit_cast(half8, pf), oc, 0, 0, 0);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            // p s in two parts: the rounded product of the high part, and what it lost plus the low part's
-            const uint32_t sp[4] = {vs[b].x, vs[b].y, vs[b].z, vs[b].w};
+            // p s in two parts: high columns hi s, rounded; low ones what that lost, plus lo s
             u32x4 f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const half2v s = as_half2(sp[i]), t = hi[i] * s;
-                const half2v taken = as_half2(as_u32(t) & low_mask);
+                const half2v s = as_half2(vs[b][i]), taken = hl[i] * s;
                 half2v w = __builtin_elementwise_fma(hi[i], s, -taken);
                 w = __builtin_elementwise_fma(lo[i], s, w);
-                f[i] = as_u32(w) & seen[i];
+                f[i] = EDGE ? as_u32(w) & seen[i] : as_u32(w);
             }
             const half8 ps = __builtin_bit_cast(half8, f);
-            o[b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q4_unpack(vn[b].x), ps, o[b][0], 0, 0, 0);
-            o[b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q4_unpack(vn[b].y), ps, o[b][1], 0, 0, 0);
+            o[b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q4_unpack(vn[b].x, ones), ps, o[b][0], 0, 0, 0);
+            o[b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q4_unpack(vn[b].y, ones), ps, o[b][1], 0, 0, 0);
         }
-    }
+        if (more) load_v(next_v, st + kWaves);
+    };
+    // steps that every query row sees whole; none where pages end inside a group
+    const int full = a.map.page_tokens & 7 ? 0 : (first_lim + 1) / 32;
+    for (; st < min(end, full); st += kWaves) step(std::false_type{});
+    for (; st < end; st += kWaves) step(std::true_type{});
 
     // the two parts' columns added, the waves joined
 #pragma unroll
@@ -277,7 +391,7 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
         const float v = plus_ror8(oc[i]);
         if (col < 8 && 4 * j + i <= NB) s_c[wave][col][4 * j + i] = v;
     }
-    if (lane < 8) s_m[wave][lane] = m - lift;
+    if (lane < 8) s_m[wave][lane] = fmaf(m, y_scale, -lift);
     __syncthreads();
     for (int idx = threadIdx.x; idx < 8 * HD; idx += 64 * kWaves) {
         const int c = idx / HD, d = idx % HD, row = row0 + c;

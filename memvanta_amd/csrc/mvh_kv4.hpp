@@ -15,12 +15,14 @@
 //   V: a word holds the 8 rows of one channel; channel c + 16 h at word c * 2
 //      + h, so that one 8-byte load gives a lane its two 16-channel tiles.
 // The page is [block][group] of these 128 bytes, then [block][group] of the
-// rows' scales: four dwords (s of row i, s of row i + 4), four dwords of c in
-// the same order.  Consecutive rows of a block are consecutive in memory.
+// rows' scales: dwords of s for rows (0, 4), (1, 5), (2, 6), (7, 3), then four
+// dwords of c in the same order.  Consecutive rows of a block are consecutive
+// in memory.
 //
 // A word is stored rotated left by 6, which puts nibbles 0 and 4 where the
-// upper four mantissa bits of two fp16 are: unpacking is a rotation, and-or
-// and a packed subtraction (q4_unpack).
+// upper four mantissa bits of two fp16 are, and 7 and 3 four bits below: with
+// the word rotated by 8 once, four and-ors and packed subtractions unpack all
+// eight (q4_unpack), in the order of the scales.
 #pragma once
 #include "mvh_device.hpp"
 
@@ -46,24 +48,27 @@ __host__ __device__ constexpr uint32_t kv4_store(uint32_t nat) { return (nat << 
 __host__ __device__ constexpr uint32_t kv4_nat(uint32_t w) { return (w >> 6) | (w << 26); }
 
 // The 8 values n - 8 of a stored word as fp16 (exact), in the order of
-// nibbles 0 4 1 5 2 6 3 7: 0x4c00 | n << 6 is 16 + n.
-__device__ __forceinline__ half8 q4_unpack(uint32_t w) {
-    u32x4 r;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const uint32_t v = j ? __builtin_amdgcn_alignbit(w, w, 4 * j) : w;
-        const half2v off = {static_cast<_Float16>(-24.0f), static_cast<_Float16>(-24.0f)};
-        r[j] = as_u32(as_half2((v & 0x03c003c0u) | 0x4c004c00u) + off);
-    }
-    return __builtin_bit_cast(half8, r);
+// nibbles 0 4 1 5 2 6 7 3: 0x4c00 | n << 6 is 16 + n, 0x5c00 | n << 2 is 256 + n.
+// The or's constants come in registers (an instruction takes one literal).
+struct Q4Ones {
+    uint32_t c16 = 0x4c004c00u, c256 = 0x5c005c00u;
+};
+__device__ __forceinline__ half8 q4_unpack(uint32_t w, const Q4Ones& k) {
+    const uint32_t r = __builtin_amdgcn_alignbit(w, w, 8);
+    const _Float16 m24 = static_cast<_Float16>(-24.0f), m264 = static_cast<_Float16>(-264.0f);
+    const u32x4 v = {as_u32(as_half2((w & 0x03c003c0u) | k.c16) + m24), as_u32(as_half2((r & 0x003c003cu) | k.c256) + m264),
+                     as_u32(as_half2((r & 0x03c003c0u) | k.c16) + m24), as_u32(as_half2((w & 0x003c003cu) | k.c256) + m264)};
+    return __builtin_bit_cast(half8, v);
 }
 
-// Step and middle of row `row` (0..7) of a group: base = the group's 32 bytes of scales
+// Index of row `row` (0..7) of a group among its 8 steps (or middles)
+__host__ __device__ constexpr int kv4_scale(int row) { return (row & 3) * 2 + ((row >> 2) ^ ((row & 3) == 3 ? 1 : 0)); }
+// Step and middle of a row: base = the group's 32 bytes of scales
 __device__ __forceinline__ float kv4_step(const uint8_t* base, int row) {
-    return h2f(reinterpret_cast<const uint16_t*>(base)[(row & 3) * 2 + (row >> 2)]);
+    return h2f(reinterpret_cast<const uint16_t*>(base)[kv4_scale(row)]);
 }
 __device__ __forceinline__ float kv4_middle(const uint8_t* base, int row) {
-    return h2f(reinterpret_cast<const uint16_t*>(base)[8 + (row & 3) * 2 + (row >> 2)]);
+    return h2f(reinterpret_cast<const uint16_t*>(base)[8 + kv4_scale(row)]);
 }
 
 // Row order with each page's rows rounded up to whole groups: group index of a

@@ -293,7 +293,7 @@ __global__ __launch_bounds__(kA4) void append_q4_kernel(RotArgs a, Kv4Map map, i
         if (live && c4 == 0) {
             uint16_t* sc = reinterpret_cast<uint16_t*>(base + kv4_scales(map.page_tokens, a.kv_dim) +
                                                        (static_cast<size_t>(b) * map.groups + g) * 32);
-            const int at = (i & 3) * 2 + (i >> 2);
+            const int at = kv4_scale(i);
             sc[at] = __builtin_bit_cast(uint16_t, s16);
             sc[8 + at] = __builtin_bit_cast(uint16_t, c16);
         }
