@@ -38,6 +38,7 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // ends of fp16: lift 14 while every step s seen is below 2, then 6 (s <= 512).
 constexpr float kLift = 14.0f, kLiftBig = 6.0f;
 constexpr int kWaves = 4;
+constexpr int kTile = 16;  // query rows of a workgroup
 
 __device__ __forceinline__ int steps_of(const Kv4Map& map, int lim) { return map.group_of(lim) / 4 + 1; }
 // a split's steps: whole turns of the workgroup's waves
@@ -59,9 +60,6 @@ __device__ __forceinline__ float rows_sum(float v) {
     v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
     auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-__device__ __forceinline__ float plus_ror8(float v) {  // + lane (l + 8) % 16 of the 16
-    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, true));
 }
 
 // Loads at a base that is the same in every lane plus a 32-bit offset: the base
@@ -91,15 +89,21 @@ __device__ __forceinline__ half2v pk_half(float a, float b) {
     const f32x2 v = {a, b};
     return __builtin_convertvector(v, half2v);
 }
+// a times (high + low) + c, the low parts first
+__device__ __forceinline__ f32x4 mfma2(u32x4 a, u32x4 high, u32x4 low, f32x4 c) {
+    const half8 m = __builtin_bit_cast(half8, a);
+    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(m, __builtin_bit_cast(half8, low), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(m, __builtin_bit_cast(half8, high), c, 0, 0, 0);
+}
 // p - h (exact where h is p rounded, or 0): the conversion inside the addition
 __device__ __forceinline__ float less(float p, _Float16 h, float minus1) { return fmaf(static_cast<float>(h), minus1, p); }
 
-// One workgroup: 8 query rows (row = token * group + head of the kv head) of kv
-// head x, tile y, split z.  Its four waves take 32-row steps in turn, each with
-// a running maximum of its own, and join through LDS.
+// One workgroup: 16 query rows (row = token * group + head of the kv head) of
+// kv head x, tile y, split z.  Its four waves take 32-row steps in turn, each
+// with a running maximum of its own, and join through LDS.
 //
-// The matrix pipe's 16 columns are the 8 query rows twice, the high and the low
-// parts.  Scores come transposed (rows of the operand = cache rows), so a lane
+// The matrix pipe's 16 columns are the query rows; the high and the low parts
+// go through it one after the other.  Scores come transposed (rows of the operand = cache rows), so a lane
 // then holds p of 8 consecutive cache rows of one query row: with the cache
 // rows in that order in V's words too, p is the next product's operand as it
 // is.  sum p c and sum p are one more product whose operand rows are the
@@ -107,13 +111,13 @@ __device__ __forceinline__ float less(float p, _Float16 h, float minus1) { retur
 template <int NB, bool UNI>
 __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4Args a) {
     constexpr int HD = 32 * NB, PITCH = HD + 4;
-    __shared__ float s_o[kWaves][8][PITCH];
-    __shared__ float s_c[kWaves][8][12];  // [0..NB) sum p c of the blocks, [NB] sum p
-    __shared__ float s_m[kWaves][8];
+    __shared__ float s_o[kWaves][kTile][PITCH];
+    __shared__ float s_c[kWaves][kTile][12];  // [0..NB) sum p c of the blocks, [NB] sum p
+    __shared__ float s_m[kWaves][kTile];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, j = lane >> 4;
-    const int kh = blockIdx.x, row0 = blockIdx.y * 8, rows = a.n_tokens * a.group;
+    const int kh = blockIdx.x, row0 = blockIdx.y * kTile, rows = a.n_tokens * a.group;
     const int pos = a.d_pos ? *a.d_pos : a.pos;
-    const int tile_lim = pos + (min(row0 + 8, rows) - 1) / a.group, first_lim = pos + row0 / a.group;
+    const int tile_lim = pos + (min(row0 + kTile, rows) - 1) / a.group, first_lim = pos + row0 / a.group;
     const int n_split = gridDim.z, chunk = split_chunk(a, pos, n_split);
     const int begin = blockIdx.z * chunk, end = min(begin + chunk, steps_of(a.map, tile_lim));
     if (begin >= end) return;  // rows past the tile's last position
@@ -200,21 +204,21 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
         load_v(page_of_step(a.pt_v, st), st);
     }
 
-    // q: lane (col, j) holds channels 8 j .. of each block of row col % 8; scaled by a power of two to [1, 2)
-    const int r = min(row0 + (col & 7), rows - 1), lim = pos + r / a.group;
+    // q: lane (col, j) holds channels 8 j .. of each block of row col; scaled by a power of two to [1, 2)
+    const int r = min(row0 + col, rows - 1), lim = pos + r / a.group;
     const float* qr = a.q + static_cast<size_t>(r / a.group) * a.q_pitch + static_cast<size_t>(kh * a.group + r % a.group) * HD;
     // masks and constants that the compiler is not to see: as selects and literals they take more operations
-    uint32_t low_mask = col >= 8 ? 0xffffffffu : 0u;
     uint32_t c_mask = col < NB ? 0xffffffffu : 0u, c_fill = col == NB ? 0x3c003c00u : 0u;  // ones: sum p
     float minus1 = -1.0f;
     Q4Ones ones;
-    asm("" : "+v"(low_mask), "+v"(ones.c16), "+v"(ones.c256), "+v"(c_mask), "+v"(c_fill), "+v"(minus1));
-    // two numbers as the column holds them: rounded to fp16, or what the rounding left
-    auto part = [&](float a, float b) {
-        const half2v h = as_half2(as_u32(pk_half(a, b)) & low_mask);
-        return as_u32(pk_half(less(a, h.x, minus1), less(b, h.y, minus1)));
+    asm("" : "+v"(ones.c16), "+v"(ones.c256), "+v"(c_mask), "+v"(c_fill), "+v"(minus1));
+    // two numbers in two fp16 each: rounded, and what the rounding left
+    auto part = [&](float a, float b, uint32_t& hi, uint32_t& lo) {
+        const half2v h = pk_half(a, b);
+        hi = as_u32(h);
+        lo = as_u32(pk_half(less(a, h.x, minus1), less(b, h.y, minus1)));
     };
-    u32x4 qf[NB], qc = {0u, 0u, 0u, 0u};  // qc: block sums of q, one or two a lane: the operand that meets kc
+    u32x4 qh[NB], ql[NB], qch = {0u, 0u, 0u, 0u}, qcl = qch;  // qc: block sums of q, one or two a lane: the operand that meets kc
     float y_scale;
     {
         float f[NB][8], top = 0.0f;
@@ -243,10 +247,18 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
             }
             sum = rows_sum(sum);
             if ((b & 3) == j) mine[b / 4] = sum;
-            // the order of q4_unpack
-            qf[b] = u32x4{part(f[b][0], f[b][4]), part(f[b][1], f[b][5]), part(f[b][2], f[b][6]), part(f[b][7], f[b][3])};
+            uint32_t h[4], l[4];  // the order of q4_unpack
+            part(f[b][0], f[b][4], h[0], l[0]);
+            part(f[b][1], f[b][5], h[1], l[1]);
+            part(f[b][2], f[b][6], h[2], l[2]);
+            part(f[b][7], f[b][3], h[3], l[3]);
+            qh[b] = u32x4{h[0], h[1], h[2], h[3]};
+            ql[b] = u32x4{l[0], l[1], l[2], l[3]};
         }
-        qc[0] = part(mine[0], NQ > 1 ? mine[NQ - 1] : 0.0f);
+        uint32_t h, l;
+        part(mine[0], NQ > 1 ? mine[NQ - 1] : 0.0f, h, l);
+        qch[0] = h;
+        qcl[0] = l;
     }
 
     f32x4 o[NB][2], oc = {0.f, 0.f, 0.f, 0.f};
@@ -278,14 +290,13 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
                 c0[0] = (w0 & 0xffffu) | (w1 << 16);
                 c1[0] = (w0 >> 16) | (w1 & 0xffff0000u);
             }
-            s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, c0), __builtin_bit_cast(half8, qc), zero, 0, 0, 0);
-            s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, c1), __builtin_bit_cast(half8, qc), zero, 0, 0, 0);
+            s0 = mfma2(c0, qch, qcl, zero);
+            s1 = mfma2(c1, qch, qcl, zero);
         }
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            const half8 q = __builtin_bit_cast(half8, qf[b]);
-            const f32x4 c0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(q4_unpack(kn[b].x, ones), q, zero, 0, 0, 0);
-            const f32x4 c1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(q4_unpack(kn[b].y, ones), q, zero, 0, 0, 0);
+            const f32x4 c0 = mfma2(__builtin_bit_cast(u32x4, q4_unpack(kn[b].x, ones)), qh[b], ql[b], zero);
+            const f32x4 c1 = mfma2(__builtin_bit_cast(u32x4, q4_unpack(kn[b].y, ones)), qh[b], ql[b], zero);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const half2v s = as_half2(ks[b][i]);
@@ -294,11 +305,6 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
             }
         }
         if (more) load_k(next_k, st + kWaves);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            s0[i] = plus_ror8(s0[i]);
-            s1[i] = plus_ror8(s1[i]);
-        }
         // rows of the step that a query row does not see: p = 0, whatever is stored there
         uint32_t seen[4], seen_c[4];
         if constexpr (EDGE) {
@@ -342,33 +348,34 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
             }
         }
         const float below = fmaf(-m, y_scale, lift);
-        half2v hi[4], lo[4], hl[4];
-        u32x4 pf, cf;
+        half2v hi[4], lo[4];
+        u32x4 ph, pl, cf;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float p0 = __builtin_amdgcn_exp2f(fmaf(s0[i], y_scale, below)), p1 = __builtin_amdgcn_exp2f(fmaf(s1[i], y_scale, below));
-            const float pa = i < 3 ? p0 : p1, pb = i < 3 ? p1 : p0;
-            hi[i] = pk_half(pa, pb);
-            hl[i] = as_half2(as_u32(hi[i]) & low_mask);
-            pf[i] = as_u32(pk_half(less(pa, hl[i].x, minus1), less(pb, hl[i].y, minus1)));
-            lo[i] = as_half2(pf[i] & low_mask);
+            uint32_t h, l;
+            part(i < 3 ? p0 : p1, i < 3 ? p1 : p0, h, l);
+            ph[i] = h;
+            pl[i] = l;
+            hi[i] = as_half2(h);
+            lo[i] = as_half2(l);
             cf[i] = ((EDGE ? vc[i] & seen_c[i] : vc[i]) & c_mask) | c_fill;
         }
-        oc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, cf), __builtin_bit_cast(half8, pf), oc, 0, 0, 0);
+        oc = mfma2(cf, ph, pl, oc);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            // p s in two parts: high columns hi s, rounded; low ones what that lost, plus lo s
-            u32x4 f;
+            // p s in two parts: hi s rounded, and what that lost plus lo s
+            u32x4 fh, fl;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const half2v s = as_half2(vs[b][i]), taken = hl[i] * s;
-                half2v w = __builtin_elementwise_fma(hi[i], s, -taken);
+                const half2v s = as_half2(vs[b][i]), t = hi[i] * s;
+                half2v w = __builtin_elementwise_fma(hi[i], s, -t);
                 w = __builtin_elementwise_fma(lo[i], s, w);
-                f[i] = EDGE ? as_u32(w) & seen[i] : as_u32(w);
+                fh[i] = EDGE ? as_u32(t) & seen[i] : as_u32(t);
+                fl[i] = EDGE ? as_u32(w) & seen[i] : as_u32(w);
             }
-            const half8 ps = __builtin_bit_cast(half8, f);
-            o[b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q4_unpack(vn[b].x, ones), ps, o[b][0], 0, 0, 0);
-            o[b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q4_unpack(vn[b].y, ones), ps, o[b][1], 0, 0, 0);
+            o[b][0] = mfma2(__builtin_bit_cast(u32x4, q4_unpack(vn[b].x, ones)), fh, fl, o[b][0]);
+            o[b][1] = mfma2(__builtin_bit_cast(u32x4, q4_unpack(vn[b].y, ones)), fh, fl, o[b][1]);
         }
         if (more) load_v(next_v, st + kWaves);
     };
@@ -377,23 +384,21 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
     for (; st < min(end, full); st += kWaves) step(std::false_type{});
     for (; st < end; st += kWaves) step(std::true_type{});
 
-    // the two parts' columns added, the waves joined
+    // the waves joined
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            float4 v = make_float4(plus_ror8(o[b][h][0]), plus_ror8(o[b][h][1]), plus_ror8(o[b][h][2]), plus_ror8(o[b][h][3]));
-            if (col < 8) *reinterpret_cast<float4*>(&s_o[wave][col][32 * b + 16 * h + 4 * j]) = v;
+            const f32x4 v = o[b][h];
+            *reinterpret_cast<float4*>(&s_o[wave][col][32 * b + 16 * h + 4 * j]) = make_float4(v[0], v[1], v[2], v[3]);
         }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float v = plus_ror8(oc[i]);
-        if (col < 8 && 4 * j + i <= NB) s_c[wave][col][4 * j + i] = v;
-    }
-    if (lane < 8) s_m[wave][lane] = fmaf(m, y_scale, -lift);
+    for (int i = 0; i < 4; ++i)
+        if (4 * j + i <= NB) s_c[wave][col][4 * j + i] = oc[i];
+    if (lane < kTile) s_m[wave][lane] = fmaf(m, y_scale, -lift);
     __syncthreads();
-    for (int idx = threadIdx.x; idx < 8 * HD; idx += 64 * kWaves) {
+    for (int idx = threadIdx.x; idx < kTile * HD; idx += 64 * kWaves) {
         const int c = idx / HD, d = idx % HD, row = row0 + c;
         if (row >= rows) break;
         float top = s_m[0][c], sum = 0.0f, l = 0.0f;
@@ -567,7 +572,7 @@ size_t q4_splits(size_t max_pos, size_t n_tokens, size_t n_head, size_t n_head_k
     const Kv4Map map = kv4_map(page_tokens);
     const size_t steps = static_cast<size_t>(map.group_of(static_cast<int>(max_pos - 1)) / 4 + 1);
     if (chunk) return (steps + chunk - 1) / chunk;
-    const size_t tiles = q4_tiles(hd) ? n_head_kv * ((n_tokens * (n_head / n_head_kv) + 7) / 8) : n_head * n_tokens;
+    const size_t tiles = q4_tiles(hd) ? n_head_kv * ((n_tokens * (n_head / n_head_kv) + kTile - 1) / kTile) : n_head * n_tokens;
     return std::max<size_t>(1, std::min({512 / tiles, (steps + kWaves - 1) / kWaves, static_cast<size_t>(kMaxSplit)}));
 }
 
@@ -617,7 +622,7 @@ hipError_t launch_attn_q4(const void* const* pt_k, const void* const* pt_v, cons
     a.map = kv4_map(page_tokens);
     const unsigned z = static_cast<unsigned>(splits);
     if (q4_tiles(hd)) {
-        const dim3 grid(static_cast<unsigned>(n_head_kv), static_cast<unsigned>((n_tokens * a.group + 7) / 8), z);
+        const dim3 grid(static_cast<unsigned>(n_head_kv), static_cast<unsigned>((n_tokens * a.group + kTile - 1) / kTile), z);
         switch (hd / 32) {
         case 1: q4_launch<1>(a, grid, st); break;
         case 2: q4_launch<2>(a, grid, st); break;
