@@ -18,6 +18,11 @@ namespace mvh {
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half4v __attribute__((ext_vector_type(4)));
+template <int NB>
+struct NQuad {  // registers that hold a number per block in four lanes
+    static constexpr int value = (NB + 3) / 4;
+};
 
 struct Q4Args {
     const void* const* pt_k;
@@ -41,11 +46,11 @@ constexpr int kWaves = 4;
 constexpr int kTile = 16;  // query rows of a workgroup
 
 __device__ __forceinline__ int steps_of(const Kv4Map& map, int lim) { return map.group_of(lim) / 4 + 1; }
-// a split's steps: whole turns of the workgroup's waves
+// a split's steps: whole turns of the workgroup's waves, by two steps at a time
 __device__ __forceinline__ int split_chunk(const Q4Args& a, int pos, int n_split) {
     if (a.chunk) return a.chunk;
     const int per = (steps_of(a.map, pos + a.n_tokens - 1) + n_split - 1) / n_split;
-    return (per + kWaves - 1) / kWaves * kWaves;
+    return (per + 2 * kWaves - 1) / (2 * kWaves) * (2 * kWaves);
 }
 
 // max over the four 16-lane rows of a wave, in every lane
@@ -97,6 +102,22 @@ __device__ __forceinline__ f32x4 mfma2(u32x4 a, u32x4 high, u32x4 low, f32x4 c) 
 }
 // p - h (exact where h is p rounded, or 0): the conversion inside the addition
 __device__ __forceinline__ float less(float p, _Float16 h, float minus1) { return fmaf(static_cast<float>(h), minus1, p); }
+
+// A workgroup's result for channel d of query row `row`: the output, or the split's part of it
+__device__ __forceinline__ void write_sum(const Q4Args& a, int kh, int row, int d, int hd, int n_split, float sum, float l, float top) {
+    const size_t out_row = static_cast<size_t>(row / a.group) * a.n_head + kh * a.group + row % a.group;
+    if (!a.part) {
+        a.out[out_row * hd + d] = __fdiv_rn(sum, l);
+        return;
+    }
+    const size_t at = out_row * n_split + blockIdx.z;
+    a.part[at * hd + d] = sum;
+    if (d == 0) {
+        float* ml = a.part + static_cast<size_t>(a.n_tokens) * a.n_head * n_split * hd + 2 * at;
+        ml[0] = top;
+        ml[1] = l;
+    }
+}
 
 // One workgroup: 16 query rows (row = token * group + head of the kv head) of
 // kv head x, tile y, split z.  Its four waves take 32-row steps in turn, each
@@ -410,18 +431,386 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
             sum = fmaf(f, s_o[w][c][d] + s_c[w][c][d / 32], sum);
             l = fmaf(f, s_c[w][c][NB], l);
         }
-        const size_t out_row = static_cast<size_t>(row / a.group) * a.n_head + kh * a.group + row % a.group;
-        if (!a.part) {
-            a.out[out_row * HD + d] = __fdiv_rn(sum, l);
+        write_sum(a, kh, row, d, HD, n_split, sum, l, top);
+    }
+}
+
+// Few query rows (token * group + head <= 4: decoding with up to four heads a kv
+// head): of the kernel above's 16 columns most would be empty, while its work
+// per lane stays the same.  Here the matrix pipe takes 16 products of 4 x 4 at
+// once, with the query rows as their short side and 64 cache rows a step:
+//   scores  16 quads of cache rows (a lane's own row) by 4 query rows, 4
+//           channels at a time; q comes from one of four 16-lane groups, so
+//           that a register holds four channel steps of it;
+//   values  64 channels (a lane's own) by 4 query rows, one quad of cache rows
+//           at a time: its p s is broadcast to the 8 channel quads of a block.
+// The scores leave a lane with four cache rows of one query row, which is the
+// operand that the values take.  Rows of a group go in the order of the scales
+// (0 4 1 5, 2 6 7 3), as the words unpack.  Against the kernel above (65000
+// rows of 8 kv heads of 128, 4 heads each): 26.5 us.
+template <int NB, bool UNI>
+__global__ __launch_bounds__(64 * kWaves, 2) void attn_q4_narrow_kernel(Q4Args a) {
+    constexpr int HD = 32 * NB, NH = NB / 2, NR = 2 * NB;  // 64-channel halves; q registers (of four channel steps)
+    __shared__ float s_o[kWaves][4][HD];
+    __shared__ float s_c[kWaves][4][NB];
+    __shared__ float s_l[kWaves][4], s_m[kWaves][4];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int head = lane & 3, half32 = lane >> 5, g8 = lane >> 3, odd = (lane >> 2) & 1;  // odd: the group's second quad
+    const int kh = blockIdx.x, row0 = blockIdx.y * 4, rows = a.n_tokens * a.group;
+    const int pos = a.d_pos ? *a.d_pos : a.pos;
+    const int tile_lim = pos + (min(row0 + 4, rows) - 1) / a.group, first_lim = pos + row0 / a.group;
+    const int n_split = gridDim.z, chunk = split_chunk(a, pos, n_split);
+    const int begin = blockIdx.z * chunk, end = min(begin + chunk, steps_of(a.map, tile_lim));
+    if (begin >= end) return;  // rows past the tile's last position
+
+    const int groups = a.map.groups, last_group = a.map.group_of(tile_lim);
+    const size_t sc_off = kv4_scales(a.map.page_tokens, a.kv_dim);
+    const size_t n_head_off = static_cast<size_t>(kh * NB) * groups * 128, s_head_off = sc_off + static_cast<size_t>(kh * NB) * groups * 32;
+    const uint32_t n_blk = static_cast<uint32_t>(groups) * 128, s_blk = static_cast<uint32_t>(groups) * 32;
+    const int in_group = lane & 7;
+    const uint32_t k_word = (in_group < 6 ? in_group : 13 - in_group) * 4;  // the lane's row among a group's words
+
+    uint32_t kn[NB][4], vn[NH][8];
+    uint2 ks[NB], kc[NB], vs[NH][2], vc[NQuad<NB>::value];
+    auto group_at = [&](const void* const* pt, int vg, int& at) -> const uint8_t* {
+        const int v = min(vg, last_group), page = a.map.page_of(v);
+        at = v - page * groups;
+        return static_cast<const uint8_t*>(pt[page]);
+    };
+    auto load_k = [&](const uint8_t* page, int it) {
+        const uint8_t *nb, *sb;
+        uint32_t on, os;
+        if constexpr (UNI) {
+            const int g0 = 8 * it - a.map.page_of(8 * it) * groups;
+            nb = page + n_head_off + static_cast<size_t>(g0) * 128;
+            sb = page + s_head_off + static_cast<size_t>(g0) * 32;
+            on = g8 * 128 + k_word;
+            os = g8 * 32 + odd * 8;
         } else {
-            const size_t at = out_row * n_split + blockIdx.z;
-            a.part[at * HD + d] = sum;
-            if (d == 0) {
-                float* ml = a.part + static_cast<size_t>(a.n_tokens) * a.n_head * n_split * HD + 2 * at;
-                ml[0] = top;
-                ml[1] = l;
+            int g;
+            const uint8_t* base = group_at(a.pt_k, 8 * it + g8, g);
+            nb = base + n_head_off + static_cast<size_t>(g) * 128;
+            sb = base + s_head_off + static_cast<size_t>(g) * 32;
+            on = k_word;
+            os = odd * 8;
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+#pragma unroll
+            for (int kq = 0; kq < 4; ++kq) kn[b][kq] = ld4_at(nb + static_cast<size_t>(b) * n_blk, on + kq * 32);
+            ks[b] = ld8_at(sb + static_cast<size_t>(b) * s_blk, os);
+            kc[b] = ld8_at(sb + static_cast<size_t>(b) * s_blk, os + 16);
+        }
+    };
+    auto load_v = [&](const uint8_t* page, int it) {
+        if constexpr (UNI) {
+            const int g0 = 8 * it - a.map.page_of(8 * it) * groups;
+            const uint8_t* nb = page + n_head_off + static_cast<size_t>(g0) * 128;
+            const uint8_t* sb = page + s_head_off + static_cast<size_t>(g0) * 32;
+#pragma unroll
+            for (int h = 0; h < NH; ++h) {
+#pragma unroll
+                for (int g = 0; g < 8; ++g) vn[h][g] = ld4_at(nb + static_cast<size_t>(2 * h) * n_blk, half32 * n_blk + (lane & 31) * 4 + g * 128);
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+                    vs[h][t] = ld8_at(sb + static_cast<size_t>(2 * h) * s_blk, half32 * s_blk + (4 * t + (g8 & 3)) * 32 + odd * 8);
+            }
+#pragma unroll
+            for (int k = 0; k < NQuad<NB>::value; ++k)
+                vc[k] = ld8_at(sb, static_cast<uint32_t>(min(head + 4 * k, NB - 1)) * s_blk + g8 * 32 + 16 + odd * 8);
+        } else {
+#pragma unroll
+            for (int g = 0; g < 8; ++g) {
+                const int v = min(8 * it + g, last_group), p = a.map.page_of(v);
+                const uint8_t* nb = page_at(a.pt_v, p) + n_head_off + static_cast<size_t>(v - p * groups) * 128;
+#pragma unroll
+                for (int h = 0; h < NH; ++h) vn[h][g] = ld4_at(nb + static_cast<size_t>(2 * h) * n_blk, half32 * n_blk + (lane & 31) * 4);
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                int g;
+                const uint8_t* sb = group_at(a.pt_v, 8 * it + 4 * t + (g8 & 3), g) + s_head_off;
+#pragma unroll
+                for (int h = 0; h < NH; ++h)
+                    vs[h][t] = ld8_at(sb + static_cast<size_t>(2 * h + half32) * s_blk + static_cast<size_t>(g) * 32, odd * 8);
+            }
+            int g;
+            const uint8_t* sb = group_at(a.pt_v, 8 * it + g8, g) + s_head_off;
+#pragma unroll
+            for (int k = 0; k < NQuad<NB>::value; ++k)
+                vc[k] = ld8_at(sb + static_cast<size_t>(min(head + 4 * k, NB - 1)) * s_blk + static_cast<size_t>(g) * 32, 16 + odd * 8);
+        }
+    };
+    auto page_of_it = [&](const void* const* pt, int it) -> const uint8_t* {
+        if constexpr (UNI) return page_at(pt, a.map.page_of(8 * it));
+        else return nullptr;
+    };
+
+    const int it_end = (end + 1) / 2;
+    int it = begin / 2 + wave;
+    if (it < it_end) {
+        load_k(page_of_it(a.pt_k, it), it);
+        load_v(page_of_it(a.pt_v, it), it);
+    }
+
+    // q: register R of the 16-lane group w holds, for row `head`, channels 8 kq .. of block R / 2, kq = 2 (R % 2) + w / 2,
+    // in unpacked order the first four (w even) or the last
+    const int r = min(row0 + head, rows - 1), lim = pos + r / a.group;
+    const float* qr = a.q + static_cast<size_t>(r / a.group) * a.q_pitch + static_cast<size_t>(kh * a.group + r % a.group) * HD;
+    float minus1 = -1.0f;
+    Q4Ones ones;
+    asm("" : "+v"(ones.c16), "+v"(ones.c256), "+v"(minus1));
+    auto part = [&](float x, float y, uint32_t& hi, uint32_t& lo) {
+        const half2v h = pk_half(x, y);
+        hi = as_u32(h);
+        lo = as_u32(pk_half(less(x, h.x, minus1), less(y, h.y, minus1)));
+    };
+    half4v qh[NR], ql[NR];
+    float qs[NB], y_scale;
+    {
+        float f[NR][4], top = 0.0f;
+        const int w = lane >> 4;
+#pragma unroll
+        for (int R = 0; R < NR; ++R) {
+            const float* x = qr + 32 * (R / 2) + 8 * (2 * (R % 2) + (w >> 1));
+            f[R][0] = x[w & 1 ? 2 : 0];
+            f[R][1] = x[w & 1 ? 6 : 4];
+            f[R][2] = x[w & 1 ? 7 : 1];
+            f[R][3] = x[w & 1 ? 3 : 5];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(f[R][i]));
+        }
+        top = rows_max(top);
+        const int e = top > 0.0f && top <= 3.402823466e38f ? max(__builtin_amdgcn_frexp_expf(top) - 1, -120) : 0;
+        const float down = ldexpf(1.0f, -e);
+        y_scale = ldexpf(__fdiv_rn(kLog2e, sqrt_rn(static_cast<float>(HD))), e);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) qs[b] = 0.0f;
+#pragma unroll
+        for (int R = 0; R < NR; ++R) {
+            u32x2 hi, lo;
+            uint32_t x, y;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                f[R][i] *= down;
+                qs[R / 2] += f[R][i];
+            }
+            part(f[R][0], f[R][1], x, y);
+            hi[0] = x, lo[0] = y;
+            part(f[R][2], f[R][3], x, y);
+            hi[1] = x, lo[1] = y;
+            qh[R] = __builtin_bit_cast(half4v, hi);
+            ql[R] = __builtin_bit_cast(half4v, lo);
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) qs[b] = rows_sum(qs[b]);
+    }
+
+    f32x4 oh[NH], ol[NH], oc[NQuad<NB>::value];
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int h = 0; h < NH; ++h) oh[h] = ol[h] = zero;
+#pragma unroll
+    for (int k = 0; k < NQuad<NB>::value; ++k) oc[k] = zero;
+    float m = kLowest, l = 0.0f, lift = kLift;
+
+    auto step = [&](auto edge_tag) {
+        constexpr bool EDGE = decltype(edge_tag)::value;
+        const bool more = it + kWaves < it_end;
+        const uint8_t *next_k = nullptr, *next_v = nullptr;
+        if (more) {
+            next_k = page_of_it(a.pt_k, it + kWaves);
+            next_v = page_of_it(a.pt_v, it + kWaves);
+        }
+        f32x4 sc = zero;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            f32x4 c = zero;
+#pragma unroll
+            for (int kq = 0; kq < 4; ++kq) {
+                const u32x4 w = __builtin_bit_cast(u32x4, q4_unpack(kn[b][kq], ones));
+                const half4v w0 = __builtin_bit_cast(half4v, u32x2{w[0], w[1]}), w1 = __builtin_bit_cast(half4v, u32x2{w[2], w[3]});
+                const int R = 2 * b + kq / 2;
+                if (kq & 1) {
+                    c = __builtin_amdgcn_mfma_f32_4x4x4f16(w0, ql[R], c, 0, 0, 6);
+                    c = __builtin_amdgcn_mfma_f32_4x4x4f16(w1, ql[R], c, 0, 0, 7);
+                    c = __builtin_amdgcn_mfma_f32_4x4x4f16(w0, qh[R], c, 0, 0, 6);
+                    c = __builtin_amdgcn_mfma_f32_4x4x4f16(w1, qh[R], c, 0, 0, 7);
+                } else {
+                    c = __builtin_amdgcn_mfma_f32_4x4x4f16(w0, ql[R], c, 0, 0, 4);
+                    c = __builtin_amdgcn_mfma_f32_4x4x4f16(w1, ql[R], c, 0, 0, 5);
+                    c = __builtin_amdgcn_mfma_f32_4x4x4f16(w0, qh[R], c, 0, 0, 4);
+                    c = __builtin_amdgcn_mfma_f32_4x4x4f16(w1, qh[R], c, 0, 0, 5);
+                }
+            }
+            const half2v sa = as_half2(ks[b].x), sb = as_half2(ks[b].y), ca = as_half2(kc[b].x), cb = as_half2(kc[b].y);
+            sc[0] = fmaf(static_cast<float>(ca.x), qs[b], fmaf(static_cast<float>(sa.x), c[0], sc[0]));
+            sc[1] = fmaf(static_cast<float>(ca.y), qs[b], fmaf(static_cast<float>(sa.y), c[1], sc[1]));
+            sc[2] = fmaf(static_cast<float>(cb.x), qs[b], fmaf(static_cast<float>(sb.x), c[2], sc[2]));
+            sc[3] = fmaf(static_cast<float>(cb.y), qs[b], fmaf(static_cast<float>(sb.y), c[3], sc[3]));
+        }
+        if (more) load_k(next_k, it + kWaves);
+        // rows that a query row does not see: p = 0, whatever is stored there
+        uint32_t seen[2][2], seen_c[2];  // of quad pairs (the value operand: rows 32 t ..), of the lane's own quad
+        if constexpr (EDGE) {
+            const int ia[4] = {0, 4, 1, 5}, ib[4] = {2, 6, 7, 3};
+            auto place = [&](int vg, int& p0, int& room) {
+                const int page = a.map.page_of(vg), g = vg - page * groups;
+                p0 = page * a.map.page_tokens + g * 8;
+                room = a.map.page_tokens - g * 8;
+            };
+            int p0, room;
+            place(8 * it + g8, p0, room);
+            seen_c[0] = seen_c[1] = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = odd ? ib[i] : ia[i];
+                if (row >= room || p0 + row > lim) sc[i] = -INFINITY;
+                if (row < room && p0 + row <= tile_lim) seen_c[i / 2] |= 0xffffu << (16 * (i & 1));
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                place(8 * it + 4 * t + (g8 & 3), p0, room);
+                seen[t][0] = seen[t][1] = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = odd ? ib[i] : ia[i];
+                    if (row < room && p0 + row <= lim) seen[t][i / 2] |= 0xffffu << (16 * (i & 1));
+                }
             }
         }
+        float mx = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
+        mx = fmaxf(mx, dpp_mov<0x124>(mx));  // over the quads: lanes 4 and 8 on, then the 16-lane rows
+        mx = fmaxf(mx, dpp_mov<0x128>(mx));
+        mx = rows_max(mx);
+        uint32_t big = 0;
+#pragma unroll
+        for (int h = 0; h < NH; ++h)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+                big |= EDGE ? (vs[h][t].x & seen[t][0]) | (vs[h][t].y & seen[t][1]) : vs[h][t].x | vs[h][t].y;
+        big &= 0x40004000u;
+        if (__any(mx > m || (big && lift == kLift))) {
+            float any_big = big ? 1.0f : 0.0f;
+            any_big = fmaxf(any_big, dpp_mov<0x124>(any_big));
+            any_big = fmaxf(any_big, dpp_mov<0x128>(any_big));
+            const float top = fmaxf(m, mx), down = rows_max(any_big) > 0.0f ? kLiftBig : lift;
+            const float f = __builtin_amdgcn_exp2f(fmaf(m - top, y_scale, down - lift));
+            m = top;
+            lift = down;
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float fi = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), i));
+#pragma unroll
+                for (int h = 0; h < NH; ++h) {
+                    oh[h][i] *= fi;
+                    ol[h][i] *= fi;
+                }
+#pragma unroll
+                for (int k = 0; k < NQuad<NB>::value; ++k) oc[k][i] *= fi;
+            }
+        }
+        const float below = fmaf(-m, y_scale, lift);
+        u32x2 ph, pl;
+        {
+            float p[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], y_scale, below));
+            l += (p[0] + p[1]) + (p[2] + p[3]);
+            uint32_t x, y;
+            part(p[0], p[1], x, y);
+            ph[0] = x, pl[0] = y;
+            part(p[2], p[3], x, y);
+            ph[1] = x, pl[1] = y;
+        }
+#pragma unroll
+        for (int k = 0; k < NQuad<NB>::value; ++k) {
+            const u32x2 c = {EDGE ? vc[k].x & seen_c[0] : vc[k].x, EDGE ? vc[k].y & seen_c[1] : vc[k].y};
+            oc[k] = __builtin_amdgcn_mfma_f32_4x4x4f16(__builtin_bit_cast(half4v, pl), __builtin_bit_cast(half4v, c), oc[k], 0, 0, 0);
+            oc[k] = __builtin_amdgcn_mfma_f32_4x4x4f16(__builtin_bit_cast(half4v, ph), __builtin_bit_cast(half4v, c), oc[k], 0, 0, 0);
+        }
+        // rows 0..31 and 32..63 of the step, each in both halves of the wave
+        uint32_t dh[2][2], dl[2][2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const auto x = __builtin_amdgcn_permlane32_swap(ph[k], ph[k], false, false);
+            const auto y = __builtin_amdgcn_permlane32_swap(pl[k], pl[k], false, false);
+            dh[0][k] = x[0], dh[1][k] = x[1];
+            dl[0][k] = y[0], dl[1][k] = y[1];
+        }
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                u32x2 fh, fl;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const half2v s = as_half2(k ? vs[h][t].y : vs[h][t].x), x = as_half2(dh[t][k]), z = x * s;
+                    half2v w = __builtin_elementwise_fma(x, s, -z);
+                    w = __builtin_elementwise_fma(as_half2(dl[t][k]), s, w);
+                    fh[k] = EDGE ? as_u32(z) & seen[t][k] : as_u32(z);
+                    fl[k] = EDGE ? as_u32(w) & seen[t][k] : as_u32(w);
+                }
+                const half4v ah = __builtin_bit_cast(half4v, fh), al = __builtin_bit_cast(half4v, fl);
+                auto quads = [&](auto g_tag) {
+                    constexpr int G = decltype(g_tag)::value;
+                    const u32x4 w = __builtin_bit_cast(u32x4, q4_unpack(vn[h][4 * t + G], ones));
+                    const half4v w0 = __builtin_bit_cast(half4v, u32x2{w[0], w[1]}), w1 = __builtin_bit_cast(half4v, u32x2{w[2], w[3]});
+                    ol[h] = __builtin_amdgcn_mfma_f32_4x4x4f16(al, w0, ol[h], 3, 2 * G, 0);
+                    oh[h] = __builtin_amdgcn_mfma_f32_4x4x4f16(ah, w0, oh[h], 3, 2 * G, 0);
+                    ol[h] = __builtin_amdgcn_mfma_f32_4x4x4f16(al, w1, ol[h], 3, 2 * G + 1, 0);
+                    oh[h] = __builtin_amdgcn_mfma_f32_4x4x4f16(ah, w1, oh[h], 3, 2 * G + 1, 0);
+                };
+                quads(std::integral_constant<int, 0>{});
+                quads(std::integral_constant<int, 1>{});
+                quads(std::integral_constant<int, 2>{});
+                quads(std::integral_constant<int, 3>{});
+            }
+        }
+        if (more) load_v(next_v, it + kWaves);
+    };
+    // steps that every query row sees whole; none where pages end inside a group
+    const int full = a.map.page_tokens & 7 ? 0 : (first_lim + 1) / 64;
+    for (; it < min(it_end, full); it += kWaves) step(std::false_type{});
+    for (; it < it_end; it += kWaves) step(std::true_type{});
+
+    // the quads' sums of p and p c, then the waves joined
+    auto over_quads = [&](float v) {
+        v += dpp_mov<0x124>(v);
+        v += dpp_mov<0x128>(v);
+        return rows_sum(v);
+    };
+    l = over_quads(l);
+    const int ch = 32 * half32 + 16 * (lane & 1) + ((lane & 31) >> 1);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int h = 0; h < NH; ++h) s_o[wave][i][64 * h + ch] = oh[h][i] + ol[h][i];
+#pragma unroll
+        for (int k = 0; k < NQuad<NB>::value; ++k) {
+            const float v = over_quads(oc[k][i]);
+            if (lane < 4 && lane + 4 * k < NB) s_c[wave][i][lane + 4 * k] = v;
+        }
+    }
+    if (lane < 4) {
+        s_m[wave][lane] = fmaf(m, y_scale, -lift);
+        s_l[wave][lane] = l;
+    }
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < 4 * HD; idx += 64 * kWaves) {
+        const int c = idx / HD, d = idx % HD, row = row0 + c;
+        if (row >= rows) break;
+        float top = s_m[0][c], sum = 0.0f, den = 0.0f;
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) top = fmaxf(top, s_m[w][c]);
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float f = __builtin_amdgcn_exp2f(s_m[w][c] - top);
+            sum = fmaf(f, s_o[w][c][d] + s_c[w][c][d / 32], sum);
+            den = fmaf(f, s_l[w][c], den);
+        }
+        write_sum(a, kh, row, d, HD, n_split, sum, den, top);
     }
 }
 
@@ -565,6 +954,8 @@ __global__ __launch_bounds__(256) void attn_q4_join_kernel(Q4Args a, int n_split
 }
 
 bool q4_tiles(size_t hd) { return hd % 32 == 0 && (hd <= 128 || hd == 192 || hd == 256); }
+// A chunk of fixed splits is to give a token the bits it has in any other chunk: one kernel for all
+bool q4_narrow(size_t hd, size_t rows, size_t chunk) { return (hd == 64 || hd == 128) && rows <= 4 && !chunk; }
 
 // Splits of a call: enough workgroups for two a CU, each wave at least one step, at most kMaxSplit.
 size_t q4_splits(size_t max_pos, size_t n_tokens, size_t n_head, size_t n_head_kv, size_t hd, size_t page_tokens,
@@ -573,7 +964,7 @@ size_t q4_splits(size_t max_pos, size_t n_tokens, size_t n_head, size_t n_head_k
     const size_t steps = static_cast<size_t>(map.group_of(static_cast<int>(max_pos - 1)) / 4 + 1);
     if (chunk) return (steps + chunk - 1) / chunk;
     const size_t tiles = q4_tiles(hd) ? n_head_kv * ((n_tokens * (n_head / n_head_kv) + kTile - 1) / kTile) : n_head * n_tokens;
-    return std::max<size_t>(1, std::min({512 / tiles, (steps + kWaves - 1) / kWaves, static_cast<size_t>(kMaxSplit)}));
+    return std::max<size_t>(1, std::min({512 / tiles, (steps + 2 * kWaves - 1) / (2 * kWaves), static_cast<size_t>(kMaxSplit)}));
 }
 
 template <int NB>
@@ -621,7 +1012,14 @@ hipError_t launch_attn_q4(const void* const* pt_k, const void* const* pt_v, cons
     a.chunk = static_cast<int>(chunk);
     a.map = kv4_map(page_tokens);
     const unsigned z = static_cast<unsigned>(splits);
-    if (q4_tiles(hd)) {
+    if (q4_narrow(hd, n_tokens * a.group, chunk)) {
+        const dim3 grid(static_cast<unsigned>(n_head_kv), 1, z);
+        const bool uni = page_tokens % 64 == 0;
+        if (hd == 128 && uni) attn_q4_narrow_kernel<4, true><<<grid, 64 * kWaves, 0, st>>>(a);
+        else if (hd == 128) attn_q4_narrow_kernel<4, false><<<grid, 64 * kWaves, 0, st>>>(a);
+        else if (uni) attn_q4_narrow_kernel<2, true><<<grid, 64 * kWaves, 0, st>>>(a);
+        else attn_q4_narrow_kernel<2, false><<<grid, 64 * kWaves, 0, st>>>(a);
+    } else if (q4_tiles(hd)) {
         const dim3 grid(static_cast<unsigned>(n_head_kv), static_cast<unsigned>((n_tokens * a.group + kTile - 1) / kTile), z);
         switch (hd / 32) {
         case 1: q4_launch<1>(a, grid, st); break;
