@@ -192,19 +192,28 @@ def _kind(*arrs) -> int:
     raise ValueError("mix of host and device buffers in one call")
 
 
+def _host_rows(a):
+    """A host array as [rows][elements] of float32."""
+    a = np.ascontiguousarray(a, np.float32)
+    return a[None] if a.ndim == 1 else a
+
+
 def _rows(a):
-    """(a as rows of fp32 elements, elements from one row to the next): a torch view may keep its row stride."""
+    """(address, rows, elements of a row, elements from one row to the next) of float32 rows: a host array from
+    _host_rows, or a device tensor, which may be a view with a row stride."""
+    shape = a.shape
     if isinstance(a, np.ndarray):
-        a = np.ascontiguousarray(a, np.float32)
-        a = a[None] if a.ndim == 1 else a
-        return a, a.shape[1]
-    if a.dim() == 1:
-        a = a[None]
-    if a.element_size() != 4 or not a.is_floating_point():
-        raise ValueError("rows must be float32")
-    if a.dim() != 2 or (a.shape[1] > 1 and a.stride(1) != 1):
+        if a.dtype != np.float32 or a.ndim != 2 or not a.flags["C_CONTIGUOUS"]:
+            raise ValueError("host rows must be 2-D, C-contiguous and float32")
+        return a.ctypes.data, shape[0], shape[1], shape[1]
+    if a.dtype is not sys.modules["torch"].float32:
+        raise ValueError("device rows must be float32")
+    stride = a.stride()
+    if len(shape) == 1:
+        shape, stride = (1, shape[0]), (shape[0], stride[0])
+    if len(shape) != 2 or (stride[1] != 1 and shape[1] > 1):
         raise ValueError("rows must be 2-D with consecutive elements")
-    return a, a.stride(0) if a.shape[0] > 1 else a.shape[1]
+    return a.data_ptr(), shape[0], shape[1], stride[0] if shape[0] > 1 else shape[1]
 
 
 class Context:
@@ -346,11 +355,26 @@ class Context:
                                               _ptr(out.get("logprob")), _ptr(out["entropy"]), _ptr(out.get("top_ids")),
                                               _ptr(out.get("top_logprobs")), MVH_HOST))
             return out
-        if not logits.is_contiguous():
-            raise ValueError("logits must be contiguous")
-        rows = 1 if logits.dim() == 1 else logits.shape[0]
-        self._check(self.lib.mvh_logprobs(self.h, _ptr(logits), logits.shape[-1], rows, _ptr(targets), top_k,
-                                          _ptr(logprob), _ptr(entropy), _ptr(top_ids), _ptr(top_logprobs), MVH_DEVICE))
+        torch = sys.modules["torch"]
+        shape = logits.shape
+        rows, n = (1, shape[0]) if len(shape) == 1 else shape
+        if logits.dtype is not torch.float32 or not logits.is_contiguous():
+            raise ValueError("logits must be contiguous float32 rows")
+
+        def at(a, dtype, count, name):
+            if a is None:
+                return None
+            if isinstance(a, np.ndarray):
+                raise ValueError("mix of host and device buffers in one call")
+            if a.dtype is not dtype or a.numel() < count or not a.is_contiguous():
+                raise ValueError(f"{name} must be {count} contiguous elements of {dtype}")
+            return a.data_ptr()
+
+        f32, i32 = torch.float32, torch.int32
+        self._check(self.lib.mvh_logprobs(self.h, logits.data_ptr(), n, rows, at(targets, i32, rows, "targets"), top_k,
+                                          at(logprob, f32, rows, "logprob"), at(entropy, f32, rows, "entropy"),
+                                          at(top_ids, i32, rows * top_k, "top_ids"),
+                                          at(top_logprobs, f32, rows * top_k, "top_logprobs"), MVH_DEVICE))
         return None
 
     def rope(self, head_dim: int, rot_dim: int = 0, layout: int = MVH_ROPE_HALF, base: float = 10000.0,
@@ -459,20 +483,32 @@ class Rope:
     def apply(self, x, n_head: int, pos: int = 0, out=None, positions=None):
         """Rows of n_head heads rotated: row t by position positions[t] (int32), or pos + t.  Device rows may be a
         view with a row stride; out may be x itself."""
-        x, pitch = _rows(x)
-        if x.shape[1] < n_head * self.head_dim:
-            raise ValueError("rows shorter than n_head heads")
-        if isinstance(x, np.ndarray):
+        host = isinstance(x, np.ndarray)
+        if host:
+            x = _host_rows(x)
             out = np.empty((x.shape[0], n_head * self.head_dim), np.float32) if out is None else out
             if positions is not None:
                 positions = np.ascontiguousarray(positions, np.int32)
-        y, out_pitch = _rows(out) if not isinstance(out, np.ndarray) else (out, out.shape[-1])
-        if y.shape[0] < x.shape[0] or y.shape[1] < n_head * self.head_dim:
-            raise ValueError("out is smaller than the rotated rows")
-        if positions is not None and (len(positions) != x.shape[0] or str(positions.dtype) not in ("int32", "torch.int32")):
-            raise ValueError("positions must be one int32 per row")
-        self.ctx._check(self.ctx.lib.mvh_rope_apply(self.ctx.h, self.h, _ptr(x), pitch, x.shape[0], n_head,
-                                                    _ptr(positions), pos, _ptr(y), out_pitch, _kind(x, y, positions)))
+        elif out is None:
+            raise ValueError("device rows need an out")
+        if isinstance(out, np.ndarray) != host:
+            raise ValueError("mix of host and device buffers in one call")
+        x_at, n, width, pitch = _rows(x)
+        y_at, out_n, out_width, out_pitch = _rows(out)
+        if min(width, out_width) < n_head * self.head_dim or out_n < n:
+            raise ValueError("rows shorter than n_head heads, or fewer out than x")
+        at = None
+        if positions is not None:
+            if isinstance(positions, np.ndarray) != host:
+                raise ValueError("mix of host and device buffers in one call")
+            if len(positions) != n or str(positions.dtype) not in ("int32", "torch.int32"):
+                raise ValueError("positions must be one int32 per row")
+            if not host and not positions.is_contiguous():
+                raise ValueError("positions must be contiguous")
+            at = _ptr(positions)
+        ctx = self.ctx
+        ctx._check(ctx.lib.mvh_rope_apply(ctx.h, self.h, x_at, pitch, n, n_head, at, pos, y_at, out_pitch,
+                                          MVH_HOST if host else MVH_DEVICE))
         return out
 
 
@@ -563,31 +599,44 @@ class KVCache:
     def append(self, layer, pos, k, v, rope: Rope, q=None, q_out=None):
         """k rotated and v stored at positions pos.., and q (when given) rotated to q_out (which may be q).  Device
         rows may be views of one fused buffer."""
-        k, k_pitch = _rows(k)
-        v, v_pitch = _rows(v)
-        n = k.shape[0]
-        if v.shape[0] != n or k.shape[1] != self.kv_dim or v.shape[1] != self.kv_dim:
+        host = isinstance(k, np.ndarray)
+        if host:
+            k, v = _host_rows(k), _host_rows(v)
+        k_at, n, k_width, k_pitch = _rows(k)
+        v_at, v_n, v_width, v_pitch = _rows(v)
+        if v_n != n or k_width != self.kv_dim or v_width != self.kv_dim:
             raise ValueError("k and v must be rows of kv_dim elements")
-        y, n_head, q_pitch, out_pitch = None, 0, 0, 0
+        q_at, y_at, n_head, q_pitch, out_pitch = None, None, 0, 0, 0
         if q is not None:
-            host = isinstance(q, np.ndarray)
-            q, q_pitch = _rows(q)
-            if host and q_out is None:
-                q_out = np.empty_like(q)
-            y, out_pitch = (q_out, q_out.shape[-1]) if host else _rows(q_out)
-            if q.shape[0] != n or q.shape[1] % rope.head_dim or tuple(y.shape) != tuple(q.shape):
+            if host:
+                q = _host_rows(q)
+                q_out = np.empty_like(q) if q_out is None else q_out
+            elif q_out is None:
+                raise ValueError("device rows need a q_out")
+            q_at, q_n, q_width, q_pitch = _rows(q)
+            y_at, y_n, y_width, out_pitch = _rows(q_out)
+            if q_n != n or y_n != n or q_width % rope.head_dim or y_width != q_width:
                 raise ValueError("q and q_out must be one row of whole heads per row of k")
-            n_head = q.shape[1] // rope.head_dim
-        self.ctx._check(self.ctx.lib.mvh_kv_append(self.ctx.h, self.h, layer, pos, n, rope.h, _ptr(q), q_pitch, n_head,
-                                                   _ptr(y), out_pitch, _ptr(k), k_pitch, _ptr(v), v_pitch,
-                                                   _kind(k, v, q, y)))
+            n_head = q_width // rope.head_dim
+        if isinstance(v, np.ndarray) != host or (q is not None and (isinstance(q, np.ndarray) != host
+                                                                    or isinstance(q_out, np.ndarray) != host)):
+            raise ValueError("mix of host and device buffers in one call")
+        ctx = self.ctx
+        ctx._check(ctx.lib.mvh_kv_append(ctx.h, self.h, layer, pos, n, rope.h, q_at, q_pitch, n_head, y_at, out_pitch, k_at,
+                                         k_pitch, v_at, v_pitch, MVH_HOST if host else MVH_DEVICE))
         return q_out
 
     def read(self, layer, pos, n, k=None, v=None):
         """Rows pos .. pos+n-1 of K and V as float32 [n][kv_dim]: into device buffers, or returned as host arrays."""
         if k is None and v is None:
             k, v = (np.empty((n, self.kv_dim), np.float32) for _ in range(2))
-        self.ctx._check(self.ctx.lib.mvh_kv_read(self.ctx.h, self.h, layer, pos, n, _ptr(k), _ptr(v), _kind(k, v)))
+        for a in (k, v):
+            if a is not None:
+                _, rows, width, pitch = _rows(a)
+                if rows < n or width != self.kv_dim or pitch != width:
+                    raise ValueError("k and v must be n contiguous rows of kv_dim float32 elements")
+        ctx = self.ctx
+        ctx._check(ctx.lib.mvh_kv_read(ctx.h, self.h, layer, pos, n, _ptr(k), _ptr(v), _kind(k, v)))
         return k, v
 
     def type(self) -> int:

@@ -8,20 +8,44 @@
 // pass is bound by reading the logits (~10 operations an element); few rows are
 // cut into parts, whose sums and candidates a second kernel joins.
 //
-// The most probable tokens: a wave keeps the best 64 keys (value, then lower
-// index) sorted across its lanes, and sets aside elements that beat the k-th;
-// once 64 wait they are sorted and merged in.  A row of n random elements sets
-// aside about k ln(n / k) of them, a sorted one all.
+// The most probable tokens, a tile of the row (32 elements a lane) at a time:
+// the k-th of the largest elements of 64 groups of lanes is a bound that at
+// least k elements reach, and few more (24 of 32000 random ones for k = 20);
+// what reaches it is set aside in LDS, and the first wave sorts that by value,
+// then index, into the best 64 so far.  In later
+// tiles the bound is the k-th best so far.  Where too many are equal (a masked
+// row) every wave sorts its own elements 64 at a time instead.
 #include "mvh_kernels.hpp"
+
+#include <type_traits>
 
 namespace mvh {
 namespace {
 
-constexpr int kLT = 256, kLW = kLT / 64;
-constexpr int kPer = 16;               // elements a lane holds at once
-constexpr int kBatch = kLT * kPer;     // a workgroup's elements at once
+constexpr int kPer = 32;  // elements a lane holds at once
+constexpr int kSetAside = 1024;  // candidates of a tile that have room
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr float kFar = -1.0e4f;        // e^kFar is 0; keeps 0 * (l - m) from being 0 * inf
+constexpr float kFar = -1.0e4f;  // e^kFar is 0; keeps 0 * (l - m) from being 0 * inf
+
+// lane ^ X of a wave, by lane moves (no LDS round trip)
+template <int X>
+__device__ __forceinline__ int lane_xor(int v, int lane) {
+    if constexpr (X == 1) return dpp_mov<0xb1>(v);
+    else if constexpr (X == 2) return dpp_mov<0x4e>(v);
+    else if constexpr (X == 4) return dpp_mov<0x1b>(dpp_mov<0x141>(v));  // ^ 7, then ^ 3
+    else if constexpr (X == 8) return dpp_mov<0x128>(v);                 // 8 on within 16
+    else if constexpr (X == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return static_cast<int>(lane & 16 ? r[0] : r[1]);
+    } else {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return static_cast<int>(lane & 32 ? r[0] : r[1]);
+    }
+}
+template <int X>
+__device__ __forceinline__ float lane_xor(float v, int lane) {
+    return __int_as_float(lane_xor<X>(__float_as_int(v), lane));
+}
 
 struct Sums {
     float m, s, t;
@@ -34,10 +58,13 @@ __device__ __forceinline__ Sums join(Sums a, Sums b) {
     const float ra = __builtin_amdgcn_exp2f((a.m - m) * kLog2e), rb = __builtin_amdgcn_exp2f((b.m - m) * kLog2e);
     return {m, fmaf(a.s, ra, b.s * rb), fmaf(ra, fmaf(da, a.s, a.t), rb * fmaf(db, b.s, b.t))};
 }
-__device__ __forceinline__ Sums wave_join(Sums a) {
-#pragma unroll
-    for (int x = 1; x < 64; x <<= 1) a = join(a, Sums{__shfl_xor(a.m, x), __shfl_xor(a.s, x), __shfl_xor(a.t, x)});
-    return a;
+template <int X>
+__device__ __forceinline__ Sums join_xor(Sums a, int lane) {
+    return join(a, Sums{lane_xor<X>(a.m, lane), lane_xor<X>(a.s, lane), lane_xor<X>(a.t, lane)});
+}
+__device__ __forceinline__ Sums wave_join(Sums a, int lane) {
+    a = join_xor<8>(join_xor<4>(join_xor<2>(join_xor<1>(a, lane), lane), lane), lane);
+    return join_xor<32>(join_xor<16>(a, lane), lane);
 }
 
 typedef unsigned long long u64;
@@ -54,36 +81,51 @@ __device__ __forceinline__ float key_value(u64 k) {
 }
 __device__ __forceinline__ int key_index(u64 k) { return static_cast<int>(~static_cast<uint32_t>(k)); }
 
-__device__ __forceinline__ u64 key_xor(u64 k, int x) {
-    return (static_cast<u64>(static_cast<uint32_t>(__shfl_xor(static_cast<int>(k >> 32), x))) << 32) |
-           static_cast<uint32_t>(__shfl_xor(static_cast<int>(k), x));
+template <int X>
+__device__ __forceinline__ u64 key_xor(u64 k, int lane) {
+    return (static_cast<u64>(static_cast<uint32_t>(lane_xor<X>(static_cast<int>(k >> 32), lane))) << 32) |
+           static_cast<uint32_t>(lane_xor<X>(static_cast<int>(k), lane));
 }
-__device__ __forceinline__ u64 key_at(u64 k, int lane) {
-    return (static_cast<u64>(static_cast<uint32_t>(__shfl(static_cast<int>(k >> 32), lane))) << 32) |
-           static_cast<uint32_t>(__shfl(static_cast<int>(k), lane));
+// lane's key, or the same of float maxima: the element of a compared pair that comes first or last
+__device__ __forceinline__ u64 lesser(u64 a, u64 b, bool less) { return less == (b < a) ? b : a; }
+__device__ __forceinline__ float lesser(float a, float b, bool less) { return less ? fminf(a, b) : fmaxf(a, b); }
+template <int X>
+__device__ __forceinline__ u64 other(u64 k, int lane) { return key_xor<X>(k, lane); }
+template <int X>
+__device__ __forceinline__ float other(float k, int lane) { return lane_xor<X>(k, lane); }
+
+// bitonic steps X, X/2 .. 1 of blocks of SIZE lanes
+template <int SIZE, int X, typename T>
+__device__ __forceinline__ T sort_steps(T k, int lane) {
+    k = lesser(k, other<X>(k, lane), !(lane & X) == !(lane & SIZE));
+    if constexpr (X > 1) k = sort_steps<SIZE, X / 2>(k, lane);
+    return k;
 }
-// 64 keys, one a lane, sorted ascending (lane 0 the smallest)
-__device__ __forceinline__ u64 sort_ascending(u64 k, int lane) {
-#pragma unroll
-    for (int size = 2; size <= 64; size <<= 1) {
-#pragma unroll
-        for (int x = size / 2; x >= 1; x >>= 1) {
-            const u64 o = key_xor(k, x);
-            const bool up = !(lane & size), first = !(lane & x);
-            k = (first == up) == (o < k) ? o : k;
-        }
-    }
+// 64 values, one a lane, sorted ascending (lane 0 the smallest)
+template <typename T>
+__device__ __forceinline__ T sort_ascending(T k, int lane) {
+    k = sort_steps<2, 1>(k, lane);
+    k = sort_steps<4, 2>(k, lane);
+    k = sort_steps<8, 4>(k, lane);
+    k = sort_steps<16, 8>(k, lane);
+    k = sort_steps<32, 16>(k, lane);
+    return sort_steps<64, 32>(k, lane);
+}
+template <int X>
+__device__ __forceinline__ u64 merge_steps(u64 k, int lane) {
+    k = lesser(k, key_xor<X>(k, lane), (lane & X) != 0);
+    if constexpr (X > 1) k = merge_steps<X / 2>(k, lane);
     return k;
 }
 // best (descending) and more (ascending): the best 64 of both, descending
-__device__ __forceinline__ u64 merge_best(u64 best, u64 more, int lane) {
-    u64 k = best > more ? best : more;
-#pragma unroll
-    for (int x = 32; x >= 1; x >>= 1) {
-        const u64 o = key_xor(k, x);
-        k = !(lane & x) == (o > k) ? o : k;
-    }
-    return k;
+__device__ __forceinline__ u64 merge_best(u64 best, u64 more, int lane) { return merge_steps<32>(best > more ? best : more, lane); }
+__device__ __forceinline__ u64 key_reversed(u64 k, int lane) {  // lane 63 - l's
+    return (static_cast<u64>(static_cast<uint32_t>(__shfl(static_cast<int>(k >> 32), 63 - lane))) << 32) |
+           static_cast<uint32_t>(__shfl(static_cast<int>(k), 63 - lane));
+}
+__device__ __forceinline__ u64 key_at(u64 k, int lane) {  // lane: the same in every lane
+    return (static_cast<u64>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(k >> 32), lane))) << 32) |
+           static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(k), lane));
 }
 
 // A wave's best k so far, and the candidates set aside for it.
@@ -133,7 +175,7 @@ struct __attribute__((packed, aligned(4))) Quad {
     float f[4];
 };
 
-// What the row's results are, from its sums (in every lane of the first wave) and its best keys
+// What the row's results are, from its sums and its best keys (one a lane of one wave)
 template <bool TOP>
 __device__ __forceinline__ void write_row(const LpArgs& a, size_t row, Sums r, u64 best, int lane) {
     // no finite logit at all: every token has probability 0
@@ -152,30 +194,32 @@ __device__ __forceinline__ void write_row(const LpArgs& a, size_t row, Sums r, u
     if constexpr (TOP) {
         if (lane < a.k) {
             const size_t at = row * a.k + lane;
-            if (a.top_ids) a.top_ids[at] = key_index(best);
+            // no key: a row with NaN, whose ids are any
+            if (a.top_ids) a.top_ids[at] = best ? key_index(best) : lane;
             if (a.top_lp) a.top_lp[at] = empty ? -INFINITY : (key_value(best) - r.m) - ln_s;
         }
     }
 }
 
-template <bool TOP>
-__global__ __launch_bounds__(kLT) void logprobs_kernel(LpArgs a) {
-    __shared__ u64 s_buf[TOP ? kLW : 1][128];
-    __shared__ Sums s_sums[kLW];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+// A workgroup: one part of a row, tile by tile; a thread takes every NT-th quad of a tile.
+template <int NT, bool TOP>
+__global__ __launch_bounds__(NT) void logprobs_kernel(LpArgs a) {
+    constexpr int NW = NT / 64, TILE = NT * kPer, KEYS = TOP ? (NW * 128 > kSetAside ? NW * 128 : kSetAside) : 1;
+    __shared__ u64 s_key[KEYS];
+    __shared__ float s_top[64];
+    __shared__ float s_bound;
+    __shared__ int s_count;
+    __shared__ Sums s_sums[NW];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const size_t row = blockIdx.y, begin = blockIdx.x * a.chunk, end = min(begin + a.chunk, a.n);
     const float* x = a.logits + row * a.pitch;
     Sums r = {-3.402823466e38f, 0.0f, 0.0f};
-    Best top;
-    top.buf = s_buf[TOP ? wave : 0];
-    top.lane = lane;
-    top.k = a.k;
-    float v[kPer], w[kPer];
-    // batch b of this wave: four times 256 consecutive elements, four a lane
-    auto load = [&](size_t at, float (&d)[kPer]) {
+    u64 best = 0;  // first wave: the best 64 so far, descending
+    float v[kPer], w[NT == 256 ? kPer : 1];
+    auto load = [&](size_t at, float* d) {
 #pragma unroll
         for (int c = 0; c < kPer / 4; ++c) {
-            const size_t i = at + c * 256 + lane * 4;
+            const size_t i = at + c * (4 * NT);
             if (i + 4 <= end) {
                 const Quad q = *reinterpret_cast<const Quad*>(x + i);
 #pragma unroll
@@ -186,15 +230,21 @@ __global__ __launch_bounds__(kLT) void logprobs_kernel(LpArgs a) {
             }
         }
     };
-    size_t at = begin + static_cast<size_t>(wave) * (kBatch / kLW);
-    if (at < end) load(at, v);
-    bool first = true;
-    for (; at < end; at += kBatch) {
-        if (at + kBatch < end) load(at + kBatch, w);
-        float bm = v[0];
+    size_t at = begin + threadIdx.x * 4;
+    load(at, v);
+    if (TOP && threadIdx.x == 0) s_count = 0;
+    for (size_t tile = begin; tile < end; tile += TILE, at += TILE) {  // the same number of turns for every wave
+        const bool more = tile + TILE < end, first = tile == begin;
+        if constexpr (NT == 256) {
+            if (more) load(at + TILE, w);
+        }
+        float quad[kPer / 4];
 #pragma unroll
-        for (int i = 1; i < kPer; ++i) bm = fmaxf(bm, v[i]);
-        const float m = fmaxf(r.m, bm), dm = fmaxf(r.m - m, kFar), f = __builtin_amdgcn_exp2f(dm * kLog2e);
+        for (int c = 0; c < kPer / 4; ++c) quad[c] = fmaxf(fmaxf(v[4 * c], v[4 * c + 1]), fmaxf(v[4 * c + 2], v[4 * c + 3]));
+        float top = quad[0];
+#pragma unroll
+        for (int c = 1; c < kPer / 4; ++c) top = fmaxf(top, quad[c]);
+        const float m = fmaxf(r.m, top), dm = fmaxf(r.m - m, kFar), f = __builtin_amdgcn_exp2f(dm * kLog2e);
         float s = r.s * f, t = f * fmaf(dm, r.s, r.t);
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
@@ -204,45 +254,95 @@ __global__ __launch_bounds__(kLT) void logprobs_kernel(LpArgs a) {
         }
         r = {m, s, t};
         if constexpr (TOP) {
+            float bound;
             if (first) {
-                // the k-th largest of the lanes' largest is at most the k-th best of the batch
-                u64 mine = 0;
-#pragma unroll
-                for (int c = 0; c < kPer; ++c) {
-                    const size_t i = at + (c / 4) * 256 + lane * 4 + c % 4;
-                    const u64 key = i < end ? key_of(v[c], static_cast<int>(i)) : 0;
-                    mine = key > mine ? key : mine;
+                // the largest elements of 64 groups of NW lanes: of these, the k-th
+                const float mine = group_max<NW>(fmaxf(top, -INFINITY));
+                if (lane % NW == 0) s_top[wave * (64 / NW) + lane / NW] = mine;
+                __syncthreads();
+                if (wave == 0) {
+                    const float all = sort_ascending(s_top[lane], lane);
+                    if (lane == 64 - a.k) s_bound = all;
                 }
-                const u64 floor_key = key_at(sort_ascending(mine, lane), 64 - a.k);
-                top.least = floor_key ? floor_key - 1 : 0;
+                __syncthreads();
+                bound = s_bound;
+            } else {
+                bound = s_bound;  // the k-th best so far: later equal ones lose, their index is higher
             }
-            // equal values of later batches have higher indices: they lose
-            if (first || top.least == 0 || __any(bm > key_value(top.least))) {
+            // elements of later tiles have to be above it; -inf: fewer than k so far, all are taken
+            const bool all_in = first || bound == -INFINITY;
+            auto reaches = [&](float f) { return all_in ? f >= bound : f > bound; };
+            if (__any(reaches(top))) {
 #pragma unroll
-                for (int c = 0; c < kPer; ++c) {
-                    const size_t i = at + (c / 4) * 256 + lane * 4 + c % 4;
-                    top.offer(i < end ? key_of(v[c], static_cast<int>(i)) : 0);
+                for (int c = 0; c < kPer / 4; ++c) {
+                    if (!__any(reaches(quad[c]))) continue;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const size_t i = at + c * (4 * NT) + j;
+                        if (reaches(v[4 * c + j]) && i < end) {
+                            const int slot = atomicAdd(&s_count, 1);
+                            if (slot < kSetAside) s_key[slot] = key_of(v[4 * c + j], static_cast<int>(i));
+                        }
+                    }
                 }
             }
-            first = false;
+            __syncthreads();
+            const int count = s_count;
+            if (count <= kSetAside) {
+                if (wave == 0) {
+                    for (int c = 0; c < count; c += 64) {
+                        const u64 more_keys = sort_ascending(c + lane < count ? s_key[c + lane] : u64{0}, lane);
+                        best = first && !c ? key_reversed(more_keys, lane) : merge_best(best, more_keys, lane);
+                    }
+                }
+            } else {  // many equal ones
+                __syncthreads();
+                Best own;
+                own.buf = s_key + wave * 128;
+                own.lane = lane;
+                own.k = a.k;
+#pragma unroll 1
+                for (int c = 0; c < kPer; ++c) {
+                    float vc = v[0];
+#pragma unroll
+                    for (int i = 1; i < kPer; ++i) vc = c == i ? v[i] : vc;
+                    const size_t i = at + (c / 4) * (4 * NT) + c % 4;
+                    own.offer(i < end ? key_of(vc, static_cast<int>(i)) : 0);
+                }
+                while (own.waiting > 0) own.flush();
+                __syncthreads();
+                s_key[wave * 64 + lane] = own.best;
+                __syncthreads();
+                if (wave == 0)
+                    for (int k = 0; k < NW; ++k) best = merge_best(best, s_key[k * 64 + 63 - lane], lane);
+            }
+            if (more) {
+                if (wave == 0) {
+                    const u64 kth = key_at(best, a.k - 1);
+                    if (lane == 0) {
+                        s_bound = kth ? key_value(kth) : -INFINITY;
+                        s_count = 0;
+                    }
+                }
+                __syncthreads();
+            }
         }
+        if constexpr (NT == 256) {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) v[i] = w[i];
+            for (int i = 0; i < kPer; ++i) v[i] = w[i];
+        } else if (more) {
+            load(at + TILE, v);
+        }
     }
-    if constexpr (TOP) {
-        while (top.waiting > 0) top.flush();
-        __syncthreads();
-        s_buf[wave][lane] = top.best;
-    }
-    r = wave_join(r);
+    r = wave_join(r, lane);
     if (lane == 0) s_sums[wave] = r;
     __syncthreads();
     if (wave) return;
-    u64 best = top.best;
-    for (int k = 1; k < kLW; ++k) {
-        r = join(r, s_sums[k]);
-        if constexpr (TOP) best = merge_best(best, s_buf[k][63 - lane], lane);
-    }
+    r = lane < NW ? s_sums[lane] : Sums{-3.402823466e38f, 0.0f, 0.0f};
+    r = join_xor<2>(join_xor<1>(r, lane), lane);
+    if constexpr (NW > 4) r = join_xor<8>(join_xor<4>(r, lane), lane);
+    auto lane0 = [](float f) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(f))); };
+    r = {lane0(r.m), lane0(r.s), lane0(r.t)};
     if (a.parts == 1) {
         write_row<TOP>(a, row, r, best, lane);
         return;
@@ -266,7 +366,7 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(LpArgs a) {
         const float* q = a.part_sums + 3 * (row * a.parts + p);
         r = join(r, Sums{q[0], q[1], q[2]});
     }
-    r = wave_join(r);
+    r = wave_join(r, lane);
     u64 best = 0;
     if constexpr (TOP) {
         const u64* keys = a.part_keys + 64 * row * a.parts;
@@ -276,10 +376,13 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(LpArgs a) {
     write_row<TOP>(a, row, r, best, lane);
 }
 
-// Parts of a row: about two workgroups a CU over all rows, each at least one batch
+// Few long rows take workgroups of 1024 threads, whose tile (32768 elements) is
+// a whole row of most vocabularies: one launch, no parts.  (32000 logits, 20
+// tops: TIME1; with 256 threads and 8 parts joined by a second kernel 14.3 us.)
+bool lp_wide(size_t n, size_t rows) { return n > 256 * kPer && rows < 512; }
 size_t lp_parts(size_t n, size_t rows) {
-    const size_t most = (n + kBatch - 1) / kBatch;
-    return std::max<size_t>(1, std::min({most, 512 / rows, size_t{64}}));
+    if (!lp_wide(n, rows) || n <= 2 * 1024 * kPer) return 1;
+    return std::max<size_t>(1, std::min({(n + 1024 * kPer - 1) / (1024 * kPer), 512 / rows, size_t{64}}));
 }
 
 }  // namespace
@@ -304,7 +407,8 @@ hipError_t launch_logprobs(const float* logits, size_t pitch, size_t n, size_t r
     a.pitch = pitch;
     a.k = static_cast<int>(k);
     const size_t parts = lp_parts(n, rows);
-    a.chunk = ((n + parts - 1) / parts + kBatch - 1) / kBatch * kBatch;
+    const size_t tile = (lp_wide(n, rows) ? 1024 : 256) * kPer;
+    a.chunk = ((n + parts - 1) / parts + tile - 1) / tile * tile;
     a.parts = static_cast<int>((n + a.chunk - 1) / a.chunk);
     if (a.parts > 1) {
         if (!scratch) return hipErrorInvalidValue;
@@ -322,8 +426,13 @@ hipError_t launch_logprobs(const float* logits, size_t pitch, size_t n, size_t r
         if (b.top_ids) b.top_ids += r0 * k;
         if (b.top_lp) b.top_lp += r0 * k;
         const dim3 grid(static_cast<unsigned>(b.parts), nr);
-        if (k) logprobs_kernel<true><<<grid, kLT, 0, st>>>(b);
-        else logprobs_kernel<false><<<grid, kLT, 0, st>>>(b);
+        if (lp_wide(n, rows)) {
+            if (k) logprobs_kernel<1024, true><<<grid, 1024, 0, st>>>(b);
+            else logprobs_kernel<1024, false><<<grid, 1024, 0, st>>>(b);
+        } else {
+            if (k) logprobs_kernel<256, true><<<grid, 256, 0, st>>>(b);
+            else logprobs_kernel<256, false><<<grid, 256, 0, st>>>(b);
+        }
         if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
         if (b.parts > 1) {
             if (k) logprobs_join_kernel<true><<<nr, 64, 0, st>>>(b);

@@ -157,7 +157,7 @@ def test_captured_step(ctx):
 
 def test_no_workspace_under_capture():
     c = capi.Context(0)
-    x = torch.randn(1, 50000, device="cuda")
+    x = torch.randn(1, 200000, device="cuda")  # long enough for parts, which take a workspace
     out, y = torch.empty(1, device="cuda"), torch.empty(1, device="cuda")
     torch.cuda.synchronize()
     stream = torch.cuda.ExternalStream(c.stream)
