@@ -226,95 +226,225 @@ __global__ __launch_bounds__(kQT) void append_q8_kernel(RotArgs a, bool vec) {
     if (threadIdx.x == 0) reinterpret_cast<float*>(page + kv_scale_offset(a.page_tokens, a.kv_dim))[slot] = s;
 }
 
+// A quad of a head and what it turns with: loaded first, turned once the turns
+// are there.  LAYOUT < 0: no rotation; VEC as in rope_quad.
+template <int LAYOUT, bool VEC>
+struct TurnQuad {
+    float4 own, mate;  // the quad; the one its pairs' other elements are in (half layout)
+    int d;
+    const float* head;  // the head's first element
+
+    __device__ __forceinline__ void load(const RopeView& r, const float* x, int at) {
+        head = x;
+        d = at;
+        if constexpr (VEC || LAYOUT < 0) {
+            const int half = r.rot / 2;
+            if constexpr (VEC) own = *reinterpret_cast<const float4*>(x + d);
+            else own = make_float4(x[d], x[d + 1], x[d + 2], x[d + 3]);
+            if constexpr (LAYOUT == kRopeHalf) mate = *reinterpret_cast<const float4*>(x + (d >= r.rot ? d : d < half ? d + half : d - half));
+        }
+    }
+    __device__ __forceinline__ float4 turned(const RopeView& r, const float2* cs) const {
+        if constexpr (LAYOUT < 0) return own;
+        if constexpr (!VEC) return rope_quad(r, head, d, cs, false);
+        if (d >= r.rot) return own;
+        const float x[4] = {own.x, own.y, own.z, own.w};
+        float y[4];
+        if constexpr (LAYOUT == kRopeHalf) {
+            const int half = r.rot / 2;
+            const bool low = d < half;
+            const float m[4] = {mate.x, mate.y, mate.z, mate.w}, sgn = low ? -1.0f : 1.0f;
+            const float2* t = cs + (low ? d : d - half);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = x[j] * t[j].x + sgn * (m[j] * t[j].y);
+        } else {
+            const float2 t0 = cs[d / 2], t1 = cs[d / 2 + 1];
+            y[0] = x[0] * t0.x - x[1] * t0.y;
+            y[1] = x[0] * t0.y + x[1] * t0.x;
+            y[2] = x[2] * t1.x - x[3] * t1.y;
+            y[3] = x[2] * t1.y + x[3] * t1.x;
+        }
+        return make_float4(y[0], y[1], y[2], y[3]);
+    }
+};
+
+// The codes, step and middle of a block of 32 held as four elements in each of
+// 8 lanes.  Divisions by the format's definition: range / 15 in double (a
+// 24-bit number over 15 is no closer to a rounding border than 2^-29 of it, so
+// one rounding of the double product is the correct one); (x - c) / s as a
+// product with 1 / s, off by 2^-22 of it, and by division itself only where
+// that is within 4e-6 of a border between two codes (1 in 10^5 elements).
+struct Q4Quad {
+    uint32_t code[4];
+    uint16_t step, middle;
+};
+__device__ __forceinline__ Q4Quad quantize_q4_x4(float4 v) {
+    const float f[4] = {v.x, v.y, v.z, v.w};
+    float mn = fminf(fminf(f[0], f[1]), fminf(f[2], f[3])), mx = fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3]));
+    float bad = fmaf(f[0], 0.0f, fmaf(f[1], 0.0f, fmaf(f[2], 0.0f, f[3] * 0.0f)));  // 0, or NaN
+    mn = -group_max<8>(-mn);
+    mx = group_max<8>(mx);
+    bad = bad + dpp_mov<0xb1>(bad);
+    bad = bad + dpp_mov<0x4e>(bad);
+    bad = bad + dpp_mov<0x141>(bad);
+    const float fifteenth = static_cast<float>(static_cast<double>(mx - mn) * (1.0 / 15.0));
+    const _Float16 s16 = static_cast<_Float16>(fminf(fifteenth, kQ4MaxStep));
+    const float s = static_cast<float>(s16);
+    const _Float16 c16 = static_cast<_Float16>(fminf(fmaxf(fmaf(8.0f, s, mn), -65504.0f), 65504.0f));
+    const float c = static_cast<float>(c16), inv = __builtin_amdgcn_rcpf(s);
+    float n[4];
+    bool near = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float q = (f[j] - c) * inv;
+        n[j] = __builtin_rintf(q);
+        near = near || fabsf(q - n[j]) > 0.5f - 4.0e-6f;
+    }
+    if (__any(near && s > 0.0f)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) n[j] = __builtin_rintf(__fdiv_rn(f[j] - c, s));
+    }
+    Q4Quad r;
+    const bool fine = s > 0.0f && bad == 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        r.code[j] = fine ? static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(n[j] + 8.0f, 0.0f), 15.0f))) : 8u;
+    r.step = bad == 0.0f ? __builtin_bit_cast(uint16_t, s16) : static_cast<uint16_t>(0x7e00);
+    r.middle = bad == 0.0f ? __builtin_bit_cast(uint16_t, c16) : static_cast<uint16_t>(0);
+    return r;
+}
+
 // Q4 pages (layout and rounding: mvh_kv4.hpp).  Workgroup (x, y): the x-th
 // group of 8 rows that the call touches; y < kv_parts a share of the K blocks,
-// then of the V blocks, then of q.  A wave takes a block: lane = (row i, four
-// channels), the block's minimum and maximum by DPP over 8 lanes.  A V word
-// holds the group's 8 rows of a channel: rows of the group that this call does
-// not write keep their nibbles (the word is this wave's alone).
+// then of the V blocks, then of q (a token's heads in q_parts shares).  A wave
+// takes two blocks at a time: lane = (row i, four channels), the block's
+// minimum and maximum by DPP over 8 lanes.  A V word holds the group's 8 rows
+// of a channel: rows of the group that this call does not write keep their
+// nibbles (the word is this wave's alone).
 constexpr int kA4 = 256;
-__global__ __launch_bounds__(kA4) void append_q4_kernel(RotArgs a, Kv4Map map, int kv_parts, const int* d_pos, bool rotate,
-                                                        bool vec) {
+template <int LAYOUT, bool VEC>
+__global__ __launch_bounds__(kA4) void append_q4_kernel(RotArgs a, Kv4Map map, int kv_parts, int q_parts, uint64_t hd_recip,
+                                                        const int* d_pos) {
     extern __shared__ float2 s_cs[];
-    const int pos = d_pos ? *d_pos : a.pos;
-    a.pos = pos;
-    const int vg = map.group_of(pos) + blockIdx.x, page = map.page_of(vg), g = vg - page * map.groups;
+    a.pos = d_pos ? *d_pos : a.pos;
+    const int vg = map.group_of(a.pos) + blockIdx.x, page = map.page_of(vg), g = vg - page * map.groups;
     const int row0 = page * map.page_tokens + g * 8;  // position of the group's first row
-    const int lo = max(pos - row0, 0);
-    const int hi = min(min(pos + a.n_tokens - row0, 8), map.page_tokens - g * 8);  // rows lo .. hi-1 are written
+    const int lo = max(a.pos - row0, 0);
+    const int hi = min(min(a.pos + a.n_tokens - row0, 8), map.page_tokens - g * 8);  // rows lo .. hi-1 are written
     if (lo >= hi) return;  // a device position that starts later in its group than the grid allows for
-    const int t0 = row0 + lo - pos, kind = blockIdx.y / kv_parts;  // token of row lo; 0 K, 1 V, 2.. q
-    const int half = a.rope.rot / 2;
-    if (rotate && kind != 1) {
-        fill_turns(a, t0, hi - lo, s_cs);
-        __syncthreads();
+    const int t0 = row0 + lo - a.pos;  // token of row lo
+    const int half = a.rope.rot / 2, hd = a.rope.head_dim;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, nblk = a.kv_dim / 32;
+    const int part = blockIdx.y;
+    if constexpr (LAYOUT >= 0) {
+        if (part >= 2 * kv_parts) {  // a token's q heads: a thread keeps its quad of the head
+            const int p = part - 2 * kv_parts, t = p / q_parts, hp = p - t * q_parts;
+            if (t >= hi - lo) return;
+            const int quads = hd / 4, per = kA4 / quads, h0 = threadIdx.x / quads, d = (threadIdx.x - h0 * quads) * 4;
+            const float* x = a.q + static_cast<size_t>(t0 + t) * a.q_pitch;
+            float* y = a.q_out + static_cast<size_t>(t0 + t) * a.out_pitch + d;
+            int h = h0 + hp * per;
+            const bool live = h0 < per;
+            TurnQuad<LAYOUT, VEC> quad;
+            if (live && h < a.n_head) quad.load(a.rope, x + static_cast<size_t>(h) * hd, d);
+            fill_turns(a, t0 + t, 1, s_cs);
+            __syncthreads();
+            while (live && h < a.n_head) {
+                const float4 v = quad.turned(a.rope, s_cs);
+                float* dst = y + static_cast<size_t>(h) * hd;
+                h += per * q_parts;
+                if (h < a.n_head) quad.load(a.rope, x + static_cast<size_t>(h) * hd, d);
+                if constexpr (VEC) {
+                    *reinterpret_cast<float4*>(dst) = v;
+                } else {
+                    dst[0] = v.x, dst[1] = v.y, dst[2] = v.z, dst[3] = v.w;
+                }
+            }
+            return;
+        }
     }
-    if (kind >= 2) {
-        rotate_q(a, t0, hi - lo, blockIdx.y - 2 * kv_parts, gridDim.y - 2 * kv_parts, s_cs, vec);
+    const bool is_v = part >= kv_parts;
+    const int i = lane >> 3, c4 = lane & 7;
+    const bool live = i >= lo && i < hi;
+    const int tok = t0 + (live ? i - lo : 0), step = kv_parts * (kA4 / 64);
+    uint8_t* const base = static_cast<uint8_t*>((is_v ? a.pt_v : a.pt_k)[page]);
+    uint8_t* const nibbles = base + static_cast<size_t>(g) * 128;
+    uint16_t* const scales = reinterpret_cast<uint16_t*>(base + kv4_scales(map.page_tokens, a.kv_dim) + static_cast<size_t>(g) * 32) + kv4_scale(i);
+    const size_t n_blk = static_cast<size_t>(map.groups) * 128, s_blk = static_cast<size_t>(map.groups) * 16;
+    int b = (is_v ? part - kv_parts : part) * (kA4 / 64) + wave;
+    auto put_scales = [&](int blk, const Q4Quad& q) {
+        if (live && c4 == 0) {
+            scales[blk * s_blk] = q.step;
+            scales[blk * s_blk + 8] = q.middle;
+        }
+    };
+    if (!is_v) {
+        const float* x = a.k + static_cast<size_t>(tok) * a.k_pitch;
+        TurnQuad<LAYOUT, VEC> quad[2];
+        auto load = [&](int blk, TurnQuad<LAYOUT, VEC>& q) {
+            const int e = blk * 32 + 4 * c4;
+            if constexpr (LAYOUT < 0) {
+                q.load(a.rope, x, e);
+            } else {
+                const int h = static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(e)) * hd_recip) >> 40);
+                q.load(a.rope, x + h * hd, e - h * hd);
+            }
+        };
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            if (b + u * step < nblk) load(b + u * step, quad[u]);
+        if constexpr (LAYOUT >= 0) {
+            fill_turns(a, t0, hi - lo, s_cs);
+            __syncthreads();
+        }
+        const float2* cs = s_cs + (live ? i - lo : 0) * half;
+        for (; b < nblk; b += 2 * step) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int blk = b + u * step;
+                if (blk >= nblk) break;
+                const Q4Quad q = quantize_q4_x4(quad[u].turned(a.rope, cs));
+                if (blk + 2 * step < nblk) load(blk + 2 * step, quad[u]);
+                put_scales(blk, q);
+                const uint32_t own = q.code[0] | (q.code[1] << 4) | (q.code[2] << 8) | (q.code[3] << 12);
+                const uint32_t mate = static_cast<uint32_t>(dpp_mov<0xb1>(static_cast<int>(own)));
+                if (live && !(c4 & 1)) reinterpret_cast<uint32_t*>(nibbles + blk * n_blk)[kv4_k_word(i, c4 >> 1)] = kv4_store(own | (mate << 16));
+            }
+        }
         return;
     }
-    const int lane = threadIdx.x & 63, i = lane >> 3, c4 = lane & 7, nblk = a.kv_dim / 32;
-    const bool live = i >= lo && i < hi;
-    uint8_t* const base = static_cast<uint8_t*>((kind ? a.pt_v : a.pt_k)[page]);
-    const int tok = t0 + (live ? i - lo : 0);
-    const float* x = kind ? a.v + static_cast<size_t>(tok) * a.v_pitch : a.k + static_cast<size_t>(tok) * a.k_pitch;
+    const float* x = a.v + static_cast<size_t>(tok) * a.v_pitch;
     const uint32_t mask = ~((hi == 8 ? 0u : 0xffffffffu << (4 * hi)) | ((1u << (4 * lo)) - 1u));  // the nibbles it writes
-    for (int b = (blockIdx.y % kv_parts) * (kA4 / 64) + (threadIdx.x >> 6); b < nblk; b += kv_parts * (kA4 / 64)) {
-        uint32_t* const words = reinterpret_cast<uint32_t*>(base + (static_cast<size_t>(b) * map.groups + g) * 128);
-        uint32_t old = 0;
-        const int ch = 4 * c4 + (i & 3);  // the channel whose V word lanes i < 4 write
-        if (kind && i < 4 && mask != 0xffffffffu) old = words[kv4_v_word(ch)];
-        const float4 y = row_quad(a, x, b * 32 + 4 * c4, s_cs + (live ? i - lo : 0) * half, rotate && kind == 0, vec);
-        const float f[4] = {y.x, y.y, y.z, y.w};
-        float mn = f[0], mx = f[0], bad = 0.0f;
+    const int ch = 4 * c4 + (i & 3), word = kv4_v_word(ch);  // the channel whose word lanes i < 4 write
+    const uint32_t pick = (i & 3) | ((4 + (i & 3)) << 8);
+    TurnQuad<-1, VEC> quad[2];
+    uint32_t old[2] = {0u, 0u};
+    auto load = [&](int blk, int u) {
+        quad[u].load(a.rope, x, blk * 32 + 4 * c4);
+        if (mask != 0xffffffffu && i < 4) old[u] = reinterpret_cast<const uint32_t*>(nibbles + blk * n_blk)[word];
+    };
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            mn = fminf(mn, f[j]);
-            mx = fmaxf(mx, f[j]);
-            bad = fabsf(f[j]) <= 3.402823466e38f ? bad : 1.0f;
-        }
-        mn = -group_max<8>(-mn);
-        mx = group_max<8>(mx);
-        bad = group_max<8>(bad);
-        _Float16 s16 = static_cast<_Float16>(fminf(__fdiv_rn(mx - mn, 15.0f), kQ4MaxStep));
-        const float s = static_cast<float>(s16);
-        _Float16 c16 = static_cast<_Float16>(fminf(fmaxf(mn + 8.0f * s, -65504.0f), 65504.0f));
-        const float c = static_cast<float>(c16);
-        uint32_t code[4];
+    for (int u = 0; u < 2; ++u)
+        if (b + u * step < nblk) load(b + u * step, u);
+    for (; b < nblk; b += 2 * step) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float n = s > 0.0f ? fminf(fmaxf(__builtin_rintf(__fdiv_rn(f[j] - c, s)) + 8.0f, 0.0f), 15.0f) : 8.0f;
-            code[j] = bad > 0.0f ? 8u : static_cast<uint32_t>(static_cast<int>(n));
-        }
-        if (bad > 0.0f) {
-            s16 = __builtin_bit_cast(_Float16, static_cast<uint16_t>(0x7e00));
-            c16 = static_cast<_Float16>(0.0f);
-        }
-        if (live && c4 == 0) {
-            uint16_t* sc = reinterpret_cast<uint16_t*>(base + kv4_scales(map.page_tokens, a.kv_dim) +
-                                                       (static_cast<size_t>(b) * map.groups + g) * 32);
-            const int at = kv4_scale(i);
-            sc[at] = __builtin_bit_cast(uint16_t, s16);
-            sc[8 + at] = __builtin_bit_cast(uint16_t, c16);
-        }
-        if (kind == 0) {
-            const uint32_t own = code[0] | (code[1] << 4) | (code[2] << 8) | (code[3] << 12);
-            const uint32_t mate = static_cast<uint32_t>(dpp_mov<0xb1>(static_cast<int>(own)));
-            if (live && !(c4 & 1)) words[kv4_k_word(i, c4 >> 1)] = kv4_store(own | (mate << 16));
-        } else {
-            uint32_t w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                int v = live ? static_cast<int>(code[j] << (4 * i)) : 0;
-                v |= __shfl_xor(v, 8);
-                v |= __shfl_xor(v, 16);
-                v |= __shfl_xor(v, 32);
-                w[j] = static_cast<uint32_t>(v);
-            }
-            if (i < 4) {
-                const uint32_t nat = i == 0 ? w[0] : i == 1 ? w[1] : i == 2 ? w[2] : w[3];
-                words[kv4_v_word(ch)] = kv4_store((kv4_nat(old) & ~mask) | nat);
-            }
+        for (int u = 0; u < 2; ++u) {
+            const int blk = b + u * step;
+            if (blk >= nblk) break;
+            const Q4Quad q = quantize_q4_x4(quad[u].own);
+            const uint32_t kept = kv4_nat(old[u]) & ~mask;
+            if (blk + 2 * step < nblk) load(blk + 2 * step, u);
+            put_scales(blk, q);
+            // 8 rows of 4 channels turned into 4 words: two rows a byte (lanes 8 on), then rows 2 and 3, 4 to 7 (16, 32 on)
+            uint32_t p = q.code[0] | (q.code[1] << 8) | (q.code[2] << 16) | (q.code[3] << 24);
+            p = live ? p << (4 * (i & 1)) : 0u;
+            p |= static_cast<uint32_t>(dpp_mov<0x128>(static_cast<int>(p)));
+            const auto r16 = __builtin_amdgcn_permlane16_swap(p, p, false, false);
+            const auto ra = __builtin_amdgcn_permlane32_swap(r16[0], r16[0], false, false);
+            const auto rb = __builtin_amdgcn_permlane32_swap(r16[1], r16[1], false, false);
+            const uint32_t w_lo = __builtin_amdgcn_perm(rb[0], ra[0], pick), w_hi = __builtin_amdgcn_perm(rb[1], ra[1], pick);
+            const uint32_t nat = __builtin_amdgcn_perm(w_hi, w_lo, 0x05040100u);
+            if (i < 4) reinterpret_cast<uint32_t*>(nibbles + blk * n_blk)[word] = kv4_store(kept | nat);
         }
     }
 }
@@ -382,6 +512,26 @@ hipError_t rotate_typed(const RotArgs& a, hipStream_t st) {
     return hipGetLastError();
 }
 
+template <int LAYOUT, bool VEC>
+hipError_t append_q4(const RotArgs& a, const int* d_pos, hipStream_t st) {
+    const Kv4Map map = kv4_map(a.page_tokens);
+    const int groups = d_pos ? 1 : map.group_of(a.pos + a.n_tokens - 1) - map.group_of(a.pos) + 1;
+    const int nblk = a.kv_dim / 32, rows = std::min(8, a.n_tokens);
+    // a wave two blocks, or one where the chip has room for that (few rows: the shortest path counts)
+    const int per = groups * nblk >= 2048 ? 8 : 4, kv_parts = (nblk + per - 1) / per;
+    int q_parts = 0;
+    uint64_t recip = 0;
+    if constexpr (LAYOUT >= 0) {
+        const int heads_at_once = kA4 / (a.rope.head_dim / 4);
+        if (a.n_head) q_parts = std::max(1, (a.n_head + 4 * heads_at_once - 1) / (4 * heads_at_once));
+        recip = (uint64_t{1} << 40) / static_cast<uint64_t>(a.rope.head_dim) + 1;  // exact below 2^16 elements, heads up to 2^10
+    }
+    const dim3 grid(static_cast<unsigned>(groups), static_cast<unsigned>(2 * kv_parts + rows * q_parts));
+    const size_t lds = LAYOUT >= 0 ? rows * (a.rope.rot / 2) * sizeof(float2) : 0;
+    append_q4_kernel<LAYOUT, VEC><<<grid, kA4, lds, st>>>(a, map, kv_parts, q_parts, recip, d_pos);
+    return hipGetLastError();
+}
+
 RopeView no_rope() { return RopeView{}; }
 
 }  // namespace
@@ -444,14 +594,9 @@ hipError_t launch_kv_append(int kv_type, const RopeView& rope, void* const* pt_k
         return hipGetLastError();
     }
     if (kv_type != kKvQ4) return hipErrorInvalidValue;
-    const Kv4Map map = kv4_map(page_tokens);
-    const int groups = map.group_of(static_cast<int>(pos + n_tokens - 1)) - map.group_of(static_cast<int>(pos)) + 1;
-    const int kv_parts = static_cast<int>((kv_dim / 32 + 3) / 4);
-    const size_t rows = std::min<size_t>(8, n_tokens);
-    const int parts = a.n_head ? static_cast<int>(std::min<size_t>(16, (rows * q_quads + kA4 - 1) / kA4)) : 0;
-    append_q4_kernel<<<dim3(static_cast<unsigned>(groups), static_cast<unsigned>(2 * kv_parts + parts)), kA4,
-                       rows * (rope.rot / 2) * sizeof(float2), st>>>(a, map, kv_parts, nullptr, true, vec);
-    return hipGetLastError();
+    const int layout = rope.layout;
+    if (vec) return layout == kRopeHalf ? append_q4<kRopeHalf, true>(a, nullptr, st) : append_q4<kRopeInterleaved, true>(a, nullptr, st);
+    return layout == kRopeHalf ? append_q4<kRopeHalf, false>(a, nullptr, st) : append_q4<kRopeInterleaved, false>(a, nullptr, st);
 }
 
 hipError_t launch_kv4_write(void* const* pt_k, void* const* pt_v, const float* k, const float* v, size_t pitch,
@@ -470,14 +615,8 @@ hipError_t launch_kv4_write(void* const* pt_k, void* const* pt_v, const float* k
     a.pt_v = pt_v;
     a.page_tokens = static_cast<int>(page_tokens);
     a.kv_dim = static_cast<int>(kv_dim);
-    const Kv4Map map = kv4_map(page_tokens);
-    const int groups =
-        d_pos ? 1 : map.group_of(static_cast<int>(pos + n_tokens - 1)) - map.group_of(static_cast<int>(pos)) + 1;
-    const int kv_parts = static_cast<int>((kv_dim / 32 + 3) / 4);
     const bool vec = al16(k) && al16(v) && pitch % 4 == 0;
-    append_q4_kernel<<<dim3(static_cast<unsigned>(groups), static_cast<unsigned>(2 * kv_parts)), kA4, 0, st>>>(
-        a, map, kv_parts, d_pos, false, vec);
-    return hipGetLastError();
+    return vec ? append_q4<-1, true>(a, d_pos, st) : append_q4<-1, false>(a, d_pos, st);
 }
 
 hipError_t launch_kv_read(int kv_type, const void* const* pt_k, const void* const* pt_v, size_t pos, size_t n_tokens,
