@@ -192,6 +192,16 @@ def _kind(*arrs) -> int:
     raise ValueError("mix of host and device buffers in one call")
 
 
+_f32 = None
+
+
+def _torch_f32():
+    global _f32
+    if _f32 is None:
+        _f32 = sys.modules["torch"].float32
+    return _f32
+
+
 def _host_rows(a):
     """A host array as [rows][elements] of float32."""
     a = np.ascontiguousarray(a, np.float32)
@@ -201,19 +211,26 @@ def _host_rows(a):
 def _rows(a):
     """(address, rows, elements of a row, elements from one row to the next) of float32 rows: a host array from
     _host_rows, or a device tensor, which may be a view with a row stride."""
-    shape = a.shape
     if isinstance(a, np.ndarray):
         if a.dtype != np.float32 or a.ndim != 2 or not a.flags["C_CONTIGUOUS"]:
             raise ValueError("host rows must be 2-D, C-contiguous and float32")
-        return a.ctypes.data, shape[0], shape[1], shape[1]
-    if a.dtype is not sys.modules["torch"].float32:
+        n, width = a.shape
+        return a.ctypes.data, n, width, width
+    if a.dtype is not _torch_f32():
         raise ValueError("device rows must be float32")
-    stride = a.stride()
+    shape = a.shape
     if len(shape) == 1:
-        shape, stride = (1, shape[0]), (shape[0], stride[0])
-    if len(shape) != 2 or (stride[1] != 1 and shape[1] > 1):
-        raise ValueError("rows must be 2-D with consecutive elements")
-    return a.data_ptr(), shape[0], shape[1], stride[0] if shape[0] > 1 else shape[1]
+        n, width = 1, shape[0]
+    elif len(shape) == 2:
+        n, width = shape
+    else:
+        raise ValueError("rows must be 2-D")
+    if a.is_contiguous():
+        return a.data_ptr(), n, width, width
+    stride = a.stride()
+    if stride[-1] != 1 and width > 1:
+        raise ValueError("a row's elements must be consecutive")
+    return a.data_ptr(), n, width, stride[0] if n > 1 else width
 
 
 class Context:
@@ -630,13 +647,20 @@ class KVCache:
         """Rows pos .. pos+n-1 of K and V as float32 [n][kv_dim]: into device buffers, or returned as host arrays."""
         if k is None and v is None:
             k, v = (np.empty((n, self.kv_dim), np.float32) for _ in range(2))
-        for a in (k, v):
-            if a is not None:
-                _, rows, width, pitch = _rows(a)
-                if rows < n or width != self.kv_dim or pitch != width:
-                    raise ValueError("k and v must be n contiguous rows of kv_dim float32 elements")
+        k_at = v_at = None
+        if k is not None:
+            k_at, rows, width, pitch = _rows(k)
+            if rows < n or width != self.kv_dim or pitch != width:
+                raise ValueError("k must be n contiguous rows of kv_dim elements")
+        if v is not None:
+            v_at, rows, width, pitch = _rows(v)
+            if rows < n or width != self.kv_dim or pitch != width:
+                raise ValueError("v must be n contiguous rows of kv_dim elements")
+        host = isinstance(k if k is not None else v, np.ndarray)
+        if k is not None and v is not None and isinstance(v, np.ndarray) != host:
+            raise ValueError("mix of host and device buffers in one call")
         ctx = self.ctx
-        ctx._check(ctx.lib.mvh_kv_read(ctx.h, self.h, layer, pos, n, _ptr(k), _ptr(v), _kind(k, v)))
+        ctx._check(ctx.lib.mvh_kv_read(ctx.h, self.h, layer, pos, n, k_at, v_at, MVH_HOST if host else MVH_DEVICE))
         return k, v
 
     def type(self) -> int:
