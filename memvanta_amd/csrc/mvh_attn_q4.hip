@@ -39,9 +39,11 @@ struct Q4Args {
 
 constexpr float kLowest = -1.0e12f;  // m before the first row: finite, so that 2^(-inf - m) is 0; scores stay above it
 constexpr float kLog2e = 1.44269504088896340736f;
-// Weights are 2^(y - m + lift), at most 2^lift, so that p s stays clear of both
-// ends of fp16: lift 14 while every step s seen is below 2, then 6 (s <= 512).
-constexpr float kLift = 14.0f, kLiftBig = 6.0f;
+// Weights are 2^(y - m + lift), and m follows the maximum only when that is
+// kSlack ahead (the sums are rescaled seldom, the decision is each row's own): at
+// most 2^(lift + kSlack), so that p s stays clear of both ends of fp16 with lift
+// 10 while every step s seen is below 2, then 2 (s <= 512).
+constexpr float kLift = 10.0f, kLiftBig = 2.0f, kSlack = 4.0f;
 constexpr int kWaves = 4;
 constexpr int kTile = 16;  // query rows of a workgroup
 
@@ -356,8 +358,8 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
             big |= EDGE ? w & seen[i] : w;
         }
         big &= 0x40004000u;
-        if (__any(mx > m || (big && lift == kLift))) {
-            const float top = fmaxf(m, mx), down = rows_max(big ? 1.0f : 0.0f) > 0.0f ? kLiftBig : lift;
+        if (__any((mx - m) * y_scale > kSlack || (big && lift == kLift))) {
+            const float top = (mx - m) * y_scale > kSlack ? mx : m, down = rows_max(big ? 1.0f : 0.0f) > 0.0f ? kLiftBig : lift;
             const float f = __builtin_amdgcn_exp2f(fmaf(m - top, y_scale, down - lift));
             m = top;
             lift = down;
@@ -690,11 +692,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_q4_narrow_kernel(Q4Args a
             for (int t = 0; t < 2; ++t)
                 big |= EDGE ? (vs[h][t].x & seen[t][0]) | (vs[h][t].y & seen[t][1]) : vs[h][t].x | vs[h][t].y;
         big &= 0x40004000u;
-        if (__any(mx > m || (big && lift == kLift))) {
+        if (__any((mx - m) * y_scale > kSlack || (big && lift == kLift))) {
             float any_big = big ? 1.0f : 0.0f;
             any_big = fmaxf(any_big, dpp_mov<0x124>(any_big));
             any_big = fmaxf(any_big, dpp_mov<0x128>(any_big));
-            const float top = fmaxf(m, mx), down = rows_max(any_big) > 0.0f ? kLiftBig : lift;
+            const float top = (mx - m) * y_scale > kSlack ? mx : m, down = rows_max(any_big) > 0.0f ? kLiftBig : lift;
             const float f = __builtin_amdgcn_exp2f(fmaf(m - top, y_scale, down - lift));
             m = top;
             lift = down;
@@ -811,6 +813,347 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_q4_narrow_kernel(Q4Args a
             den = fmaf(f, s_l[w][c], den);
         }
         write_sum(a, kh, row, d, HD, n_split, sum, den, top);
+    }
+}
+
+// Many query rows (a prefill chunk): 32 a workgroup, on 32 x 32 products, each
+// of its eight waves over every eighth step of 32 cache rows.  Against 16 rows
+// a tile the unpacking of a step, a third of its operations, serves twice the
+// rows.  The products' rows are the step's cache rows in the order that leaves a
+// lane (query row lane % 32, half j2) with those of groups j2 and 2 + j2 in the
+// order of the scales: again the next product's operand, and one 16-byte load
+// of steps or middles.  q lies in LDS for all waves; a step's scales go
+// through LDS too, where 32 lanes read the same ones (from the caches such
+// loads would take as long as the arithmetic).
+constexpr int kRows32 = 32, kWaves32 = 8;
+template <int NB, bool UNI>
+__global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a) {
+    constexpr int HD = 32 * NB, NO = 16 * NB, SCALES = NB * 128;  // bytes of a step's scales of K, or of V
+    typedef float f32x16 __attribute__((ext_vector_type(16)));
+    __shared__ __align__(16) uint8_t s_mem[kWaves32 * NO * 256 + kWaves32 * 6 * 256];
+    static_assert(kWaves32 * NO * 256 >= NB * 4 * 1024 + kWaves32 * 2 * SCALES);
+    u32x4(*s_q)[2][64] = reinterpret_cast<u32x4(*)[2][64]>(s_mem);  // [block * 2 + ks][high, low][lane]
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, j2 = lane >> 5;
+    uint8_t* const s_sc = s_mem + NB * 4 * 1024 + wave * 2 * SCALES;  // this wave's [K, V][block][group][s, c]
+    const int kh = blockIdx.x, row0 = blockIdx.y * kRows32, rows = a.n_tokens * a.group;
+    const int pos = a.d_pos ? *a.d_pos : a.pos;
+    const int tile_lim = pos + (min(row0 + kRows32, rows) - 1) / a.group, first_lim = pos + row0 / a.group;
+    const int n_split = gridDim.z, chunk = split_chunk(a, pos, n_split);
+    const int begin = blockIdx.z * chunk, end = min(begin + chunk, steps_of(a.map, tile_lim));
+    if (begin >= end) return;  // rows past the tile's last position
+
+    const int groups = a.map.groups, last_group = a.map.group_of(tile_lim);
+    const size_t sc_off = kv4_scales(a.map.page_tokens, a.kv_dim);
+    const size_t n_head_off = static_cast<size_t>(kh * NB) * groups * 128, s_head_off = sc_off + static_cast<size_t>(kh * NB) * groups * 32;
+    const size_t n_blk = static_cast<size_t>(groups) * 128, s_blk = static_cast<size_t>(groups) * 32;
+    // the cache row that row `col` of the score product is: its group of the step, its place in the scales' order, its word
+    const int kg = (col >> 4) * 2 + ((col >> 2) & 1), kr = ((col >> 3) & 1) * 4 + (col & 3);
+    const uint32_t k_word = (kr < 6 ? kr : 13 - kr) * 4, v_word = kv4_v_word(col) * 4;
+    const int sl_b = (lane >> 4) & (NB - 1), sl_g = (lane >> 2) & 3, sl_p = (lane & 3) * 8;  // the lane's 8 bytes of scales
+
+    uint32_t kn[NB][2], vn[NB][2];
+    uint2 ksc, vsc;
+    auto group_at = [&](const void* const* pt, int vg, int& at) -> const uint8_t* {
+        const int v = min(vg, last_group), page = a.map.page_of(v);
+        at = v - page * groups;
+        return static_cast<const uint8_t*>(pt[page]);
+    };
+    auto load = [&](const void* const* pt, const uint8_t* page, int st, uint32_t (&w)[NB][2], uint2& sc, bool is_k) {
+        if constexpr (UNI) {
+            const int g0 = 4 * st - a.map.page_of(4 * st) * groups;
+            const uint8_t* nb = page + n_head_off + static_cast<size_t>(g0) * 128;
+            const uint8_t* sb = page + s_head_off + static_cast<size_t>(g0) * 32;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    w[b][k] = ld4_at(nb + b * n_blk, is_k ? kg * 128 + (2 * k + j2) * 32 + k_word : (2 * k + j2) * 128 + v_word);
+            sc = ld8_at(sb, sl_b * static_cast<uint32_t>(s_blk) + sl_g * 32 + sl_p);
+        } else {
+            int g;
+            const uint8_t* base = group_at(pt, 4 * st + (is_k ? kg : j2), g) + n_head_off;
+            const uint8_t* base1 = base;
+            int g1 = g;
+            if (!is_k) base1 = group_at(pt, 4 * st + 2 + j2, g1) + n_head_off;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                w[b][0] = ld4_at(base + b * n_blk + static_cast<size_t>(g) * 128, is_k ? j2 * 32 + k_word : v_word);
+                w[b][1] = ld4_at(base1 + b * n_blk + static_cast<size_t>(g1) * 128, is_k ? (2 + j2) * 32 + k_word : v_word);
+            }
+            const uint8_t* sb = group_at(pt, 4 * st + sl_g, g) + s_head_off;
+            sc = ld8_at(sb + sl_b * s_blk + static_cast<size_t>(g) * 32, sl_p);
+        }
+    };
+    auto page_of_step = [&](const void* const* pt, int st) -> const uint8_t* {
+        if constexpr (UNI) return page_at(pt, a.map.page_of(4 * st));
+        else return nullptr;
+    };
+    int st = begin + wave;
+    if (st < end) {
+        load(a.pt_k, page_of_step(a.pt_k, st), st, kn, ksc, true);
+        load(a.pt_v, page_of_step(a.pt_v, st), st, vn, vsc, false);
+    }
+
+    // masks and constants that the compiler is not to see: as selects and literals they take more operations
+    uint32_t c_mask = col < NB ? 0xffffffffu : 0u, c_fill = col == NB ? 0x3c003c00u : 0u;  // ones: sum p
+    float minus1 = -1.0f;
+    Q4Ones ones;
+    asm("" : "+v"(ones.c16), "+v"(ones.c256), "+v"(c_mask), "+v"(c_fill), "+v"(minus1));
+    auto part = [&](float x, float y, uint32_t& hi, uint32_t& lo) {
+        const half2v h = pk_half(x, y);
+        hi = as_u32(h);
+        lo = as_u32(pk_half(less(x, h.x, minus1), less(y, h.y, minus1)));
+    };
+    // q: lane (col, j2) has channels 8 (2 k + j2) .. of each block of row col, scaled by a power of two to [1, 2); every wave
+    // forms all of them for the row's maximum and the block sums, and stores its share
+    const int r = min(row0 + col, rows - 1), lim = pos + r / a.group;
+    u32x4 qch = {0u, 0u, 0u, 0u}, qcl = qch;  // block sums of blocks j2 and j2 + 2: the operand that meets the c of K
+    float y_scale;
+    {
+        const float* qr = a.q + static_cast<size_t>(r / a.group) * a.q_pitch + static_cast<size_t>(kh * a.group + r % a.group) * HD;
+        float f[2 * NB][8], top = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 2 * NB; ++k)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                f[k][i] = qr[32 * (k / 2) + 8 * (2 * (k & 1) + j2) + i];
+                top = fmaxf(top, fabsf(f[k][i]));
+            }
+        const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+        top = fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
+        const int e = top > 0.0f && top <= 3.402823466e38f ? max(__builtin_amdgcn_frexp_expf(top) - 1, -120) : 0;
+        const float down = ldexpf(1.0f, -e);
+        y_scale = ldexpf(__fdiv_rn(kLog2e, sqrt_rn(static_cast<float>(HD))), e);
+        float mine[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    f[2 * b + k][i] *= down;
+                    sum += f[2 * b + k][i];
+                }
+                if ((2 * b + k) % kWaves32 != wave) continue;
+                uint32_t h[4], l[4];
+                const float* x = f[2 * b + k];
+                part(x[0], x[4], h[0], l[0]);
+                part(x[1], x[5], h[1], l[1]);
+                part(x[2], x[6], h[2], l[2]);
+                part(x[7], x[3], h[3], l[3]);
+                s_q[2 * b + k][0][lane] = u32x4{h[0], h[1], h[2], h[3]};
+                s_q[2 * b + k][1][lane] = u32x4{l[0], l[1], l[2], l[3]};
+            }
+            const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
+            sum = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+            if ((b & 1) == j2) mine[b / 2] = sum;
+        }
+        uint32_t h, l;
+        part(mine[0], mine[1], h, l);
+        qch[0] = h;
+        qcl[0] = l;
+    }
+    __syncthreads();
+
+    f32x16 o[NB], oc;
+    const f32x16 zero = {};
+    oc = zero;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) o[b] = zero;
+    float m = kLowest, lift = kLift;
+    auto mfma = [](u32x4 x, u32x4 y, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, x), __builtin_bit_cast(half8, y), c, 0, 0, 0);
+    };
+    // steps (c == 0) or middles of the rows that the lane's scores belong to: half k of them
+    auto scales = [&](int which, int b, int k, int c) {
+        return *reinterpret_cast<const u32x4*>(s_sc + which * SCALES + (b * 4 + 2 * k + j2) * 32 + 16 * c);
+    };
+
+    auto step = [&](auto edge_tag) {
+        constexpr bool EDGE = decltype(edge_tag)::value;
+        const bool more = st + kWaves32 < end;
+        const uint8_t *next_k = nullptr, *next_v = nullptr;
+        if (more) {
+            next_k = page_of_step(a.pt_k, st + kWaves32);
+            next_v = page_of_step(a.pt_v, st + kWaves32);
+        }
+        // this wave's own memory: its reads of the last step are done, and reads follow writes in order
+        if (NB == 4 || lane < 32) {
+            *reinterpret_cast<uint2*>(s_sc + (sl_b * 4 + sl_g) * 32 + sl_p) = ksc;
+            *reinterpret_cast<uint2*>(s_sc + SCALES + (sl_b * 4 + sl_g) * 32 + sl_p) = vsc;
+        }
+        __builtin_amdgcn_wave_barrier();
+        f32x16 sc;
+        {
+            const uint16_t* c = reinterpret_cast<const uint16_t*>(s_sc + (j2 * 4 + kg) * 32 + 16) + kr;
+            u32x4 w = {c[0], 0u, 0u, 0u};
+            if constexpr (NB == 4) w[0] |= static_cast<uint32_t>(c[2 * 4 * 16]) << 16;
+            sc = mfma(w, qcl, zero);
+            sc = mfma(w, qch, sc);
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            f32x16 x = zero;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const u32x4 w = __builtin_bit_cast(u32x4, q4_unpack(kn[b][k], ones));
+                x = mfma(w, s_q[2 * b + k][1][lane], x);
+                x = mfma(w, s_q[2 * b + k][0][lane], x);
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const u32x4 s = scales(0, b, k, 0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const half2v h = as_half2(s[i]);
+                    sc[8 * k + 2 * i] = fmaf(static_cast<float>(h.x), x[8 * k + 2 * i], sc[8 * k + 2 * i]);
+                    sc[8 * k + 2 * i + 1] = fmaf(static_cast<float>(h.y), x[8 * k + 2 * i + 1], sc[8 * k + 2 * i + 1]);
+                }
+            }
+        }
+        if (more) load(a.pt_k, next_k, st + kWaves32, kn, ksc, true);
+        // rows that a query row does not see: p = 0, whatever is stored there
+        uint32_t seen[2][4], seen_c[2][4];
+        if constexpr (EDGE) {
+            const int order[8] = {0, 4, 1, 5, 2, 6, 7, 3};
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int vg = 4 * st + 2 * k + j2, page = a.map.page_of(vg), g = vg - page * groups;
+                const int p0 = page * a.map.page_tokens + g * 8, room = a.map.page_tokens - g * 8;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    seen[k][i] = seen_c[k][i] = 0;
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const int row = order[2 * i + x];
+                        const uint32_t bits = x ? 0xffff0000u : 0xffffu;
+                        if (row < room && p0 + row <= tile_lim) seen_c[k][i] |= bits;
+                        if (row < room && p0 + row <= lim) seen[k][i] |= bits;
+                        else sc[8 * k + 2 * i + x] = -INFINITY;
+                    }
+                }
+            }
+        }
+        float mx = sc[0];
+#pragma unroll
+        for (int i = 1; i < 15; i += 2) mx = fmaxf(fmaxf(mx, sc[i]), sc[i + 1]);
+        mx = fmaxf(mx, sc[15]);
+        {
+            const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+            mx = fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
+        }
+        uint32_t big = 0;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const u32x4 s = scales(1, b, k, 0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) big |= EDGE ? s[i] & seen[k][i] : s[i];
+            }
+        big &= 0x40004000u;
+        if (__any((mx - m) * y_scale > kSlack || (big && lift == kLift))) {
+            const auto t = __builtin_amdgcn_permlane32_swap(big, big, false, false);
+            const float top = (mx - m) * y_scale > kSlack ? mx : m, down = (t[0] | t[1]) ? kLiftBig : lift;
+            const float f = __builtin_amdgcn_exp2f(fmaf(m - top, y_scale, down - lift));
+            m = top;
+            lift = down;
+            oc *= f;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) o[b] *= f;
+        }
+        const float below = fmaf(-m, y_scale, lift);
+        u32x4 ph[2], pl[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t h, l;
+                part(__builtin_amdgcn_exp2f(fmaf(sc[8 * k + 2 * i], y_scale, below)),
+                     __builtin_amdgcn_exp2f(fmaf(sc[8 * k + 2 * i + 1], y_scale, below)), h, l);
+                ph[k][i] = h;
+                pl[k][i] = l;
+            }
+            u32x4 c = *reinterpret_cast<const u32x4*>(s_sc + SCALES + (min(col, NB - 1) * 4 + 2 * k + j2) * 32 + 16);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c[i] = ((EDGE ? c[i] & seen_c[k][i] : c[i]) & c_mask) | c_fill;
+            oc = mfma(c, pl[k], oc);
+            oc = mfma(c, ph[k], oc);
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const u32x4 s = scales(1, b, k, 0);
+                u32x4 fh, fl;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const half2v z = as_half2(s[i]), x = as_half2(ph[k][i]), t = x * z;
+                    half2v w = __builtin_elementwise_fma(x, z, -t);
+                    w = __builtin_elementwise_fma(as_half2(pl[k][i]), z, w);
+                    fh[i] = EDGE ? as_u32(t) & seen[k][i] : as_u32(t);
+                    fl[i] = EDGE ? as_u32(w) & seen[k][i] : as_u32(w);
+                }
+                const u32x4 w = __builtin_bit_cast(u32x4, q4_unpack(vn[b][k], ones));
+                o[b] = mfma(w, fl, o[b]);
+                o[b] = mfma(w, fh, o[b]);
+            }
+        }
+        if (more) load(a.pt_v, next_v, st + kWaves32, vn, vsc, false);
+        __builtin_amdgcn_wave_barrier();
+    };
+    // steps that every query row sees whole; none where pages end inside a group
+    const int full = a.map.page_tokens & 7 ? 0 : (first_lim + 1) / 32;
+    for (; st < min(end, full); st += kWaves32) step(std::false_type{});
+    for (; st < end; st += kWaves32) step(std::true_type{});
+
+    // the waves joined: every wave's sums by register and lane, then each wave a quarter of the registers
+    __syncthreads();
+    float(*s_o)[NO][64] = reinterpret_cast<float(*)[NO][64]>(s_mem);
+    float(*s_x)[6][64] = reinterpret_cast<float(*)[6][64]>(s_mem + kWaves32 * NO * 256);  // sums of p c and p (rows 0..7), m
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s_o[wave][16 * b + i][lane] = o[b][i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s_x[wave][i][lane] = oc[i];
+    s_x[wave][4][lane] = fmaf(m, y_scale, -lift);
+    __syncthreads();
+    float w[kWaves32], top = s_x[0][4][lane], l = 0.0f;
+#pragma unroll
+    for (int k = 1; k < kWaves32; ++k) top = fmaxf(top, s_x[k][4][lane]);
+    auto extra = [&](int k, int row) { return s_x[k][row & 3][col + 32 * (row >> 2)]; };
+#pragma unroll
+    for (int k = 0; k < kWaves32; ++k) {
+        w[k] = __builtin_amdgcn_exp2f(s_x[k][4][lane] - top);
+        l = fmaf(w[k], extra(k, NB), l);
+    }
+    const int row = row0 + col;
+    if (row >= rows) return;
+    const size_t out_row = static_cast<size_t>(row / a.group) * a.n_head + kh * a.group + row % a.group;
+    const size_t at = out_row * n_split + blockIdx.z;
+    float* dst = a.part ? a.part + at * HD : a.out + out_row * HD;
+    const float scale = a.part ? 1.0f : __fdiv_rn(1.0f, l);
+#pragma unroll
+    for (int i = 0; i < NO / kWaves32; i += 4) {
+        const int reg = wave * (NO / kWaves32) + i, b = reg / 16;
+        float c = 0.0f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < kWaves32; ++k) {
+            c = fmaf(w[k], extra(k, b), c);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) v[x] = fmaf(w[k], s_o[k][reg + x][lane], v[x]);
+        }
+        // registers 4 q .. of a block: channels 8 q + 4 j2 ..; rows of the output are only known to be 4-byte aligned
+        float* p = dst + 32 * b + 2 * (reg % 16) + 4 * j2;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) p[x] = (v[x] + c) * scale;
+    }
+    if (a.part && wave == 0 && j2 == 0) {
+        float* ml = a.part + static_cast<size_t>(a.n_tokens) * a.n_head * n_split * HD + 2 * at;
+        ml[0] = top;
+        ml[1] = l;
     }
 }
 
@@ -956,6 +1299,7 @@ __global__ __launch_bounds__(256) void attn_q4_join_kernel(Q4Args a, int n_split
 bool q4_tiles(size_t hd) { return hd % 32 == 0 && (hd <= 128 || hd == 192 || hd == 256); }
 // A chunk of fixed splits is to give a token the bits it has in any other chunk: one kernel for all
 bool q4_narrow(size_t hd, size_t rows, size_t chunk) { return (hd == 64 || hd == 128) && rows <= 4 && !chunk; }
+bool q4_tile32(size_t hd, size_t rows, size_t chunk) { return (hd == 64 || hd == 128) && (rows > kTile || chunk); }
 
 // Splits of a call: enough workgroups for two a CU, each wave at least one step, at most kMaxSplit.
 size_t q4_splits(size_t max_pos, size_t n_tokens, size_t n_head, size_t n_head_kv, size_t hd, size_t page_tokens,
@@ -963,7 +1307,12 @@ size_t q4_splits(size_t max_pos, size_t n_tokens, size_t n_head, size_t n_head_k
     const Kv4Map map = kv4_map(page_tokens);
     const size_t steps = static_cast<size_t>(map.group_of(static_cast<int>(max_pos - 1)) / 4 + 1);
     if (chunk) return (steps + chunk - 1) / chunk;
-    const size_t tiles = q4_tiles(hd) ? n_head_kv * ((n_tokens * (n_head / n_head_kv) + kTile - 1) / kTile) : n_head * n_tokens;
+    const size_t rows = n_tokens * (n_head / n_head_kv);
+    if (q4_tile32(hd, rows, chunk)) {  // a workgroup a CU: more splits cost more in parts than they gain
+        const size_t tiles = n_head_kv * ((rows + kRows32 - 1) / kRows32);
+        return std::max<size_t>(1, std::min({256 / tiles, (steps + 2 * kWaves - 1) / (2 * kWaves), static_cast<size_t>(kMaxSplit)}));
+    }
+    const size_t tiles = q4_tiles(hd) ? n_head_kv * ((rows + kTile - 1) / kTile) : n_head * n_tokens;
     return std::max<size_t>(1, std::min({512 / tiles, (steps + 2 * kWaves - 1) / (2 * kWaves), static_cast<size_t>(kMaxSplit)}));
 }
 
@@ -1019,6 +1368,13 @@ hipError_t launch_attn_q4(const void* const* pt_k, const void* const* pt_v, cons
         else if (hd == 128) attn_q4_narrow_kernel<4, false><<<grid, 64 * kWaves, 0, st>>>(a);
         else if (uni) attn_q4_narrow_kernel<2, true><<<grid, 64 * kWaves, 0, st>>>(a);
         else attn_q4_narrow_kernel<2, false><<<grid, 64 * kWaves, 0, st>>>(a);
+    } else if (q4_tile32(hd, n_tokens * a.group, chunk)) {
+        const dim3 grid(static_cast<unsigned>(n_head_kv), static_cast<unsigned>((n_tokens * a.group + kRows32 - 1) / kRows32), z);
+        const bool uni = page_tokens % 32 == 0;
+        if (hd == 128 && uni) attn_q4_tile_kernel<4, true><<<grid, 64 * kWaves32, 0, st>>>(a);
+        else if (hd == 128) attn_q4_tile_kernel<4, false><<<grid, 64 * kWaves32, 0, st>>>(a);
+        else if (uni) attn_q4_tile_kernel<2, true><<<grid, 64 * kWaves32, 0, st>>>(a);
+        else attn_q4_tile_kernel<2, false><<<grid, 64 * kWaves32, 0, st>>>(a);
     } else if (q4_tiles(hd)) {
         const dim3 grid(static_cast<unsigned>(n_head_kv), static_cast<unsigned>((n_tokens * a.group + kTile - 1) / kTile), z);
         switch (hd / 32) {

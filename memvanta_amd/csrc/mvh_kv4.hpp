@@ -29,7 +29,7 @@
 namespace mvh {
 
 constexpr int kQ4Block = 32;
-constexpr float kQ4MaxStep = 512.0f;  // keeps 2^6 p s within fp16 in the attention kernels
+constexpr float kQ4MaxStep = 512.0f;  // keeps 64 p s within fp16 in the attention kernels
 
 __host__ __device__ constexpr size_t kv4_groups(size_t page_tokens) { return (page_tokens + 7) / 8; }
 __host__ __device__ constexpr size_t kv4_scales(size_t page_tokens, size_t kv_dim) {  // offset of the scales
