@@ -858,17 +858,15 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
         at = v - page * groups;
         return static_cast<const uint8_t*>(pt[page]);
     };
-    auto load = [&](const void* const* pt, const uint8_t* page, int st, uint32_t (&w)[NB][2], uint2& sc, bool is_k) {
+    auto load = [&](const void* const* pt, const uint8_t* page, int st, uint32_t (&w)[NB][2], bool is_k) {
         if constexpr (UNI) {
             const int g0 = 4 * st - a.map.page_of(4 * st) * groups;
             const uint8_t* nb = page + n_head_off + static_cast<size_t>(g0) * 128;
-            const uint8_t* sb = page + s_head_off + static_cast<size_t>(g0) * 32;
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
                     w[b][k] = ld4_at(nb + b * n_blk, is_k ? kg * 128 + (2 * k + j2) * 32 + k_word : (2 * k + j2) * 128 + v_word);
-            sc = ld8_at(sb, sl_b * static_cast<uint32_t>(s_blk) + sl_g * 32 + sl_p);
         } else {
             int g;
             const uint8_t* base = group_at(pt, 4 * st + (is_k ? kg : j2), g) + n_head_off;
@@ -880,20 +878,26 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
                 w[b][0] = ld4_at(base + b * n_blk + static_cast<size_t>(g) * 128, is_k ? j2 * 32 + k_word : v_word);
                 w[b][1] = ld4_at(base1 + b * n_blk + static_cast<size_t>(g1) * 128, is_k ? (2 + j2) * 32 + k_word : v_word);
             }
+        }
+    };
+    auto load_scales = [&](const void* const* pt, const uint8_t* page, int st) {
+        if constexpr (UNI) {
+            const int g0 = 4 * st - a.map.page_of(4 * st) * groups;
+            return ld8_at(page + s_head_off + static_cast<size_t>(g0) * 32, sl_b * static_cast<uint32_t>(s_blk) + sl_g * 32 + sl_p);
+        } else {
+            int g;
             const uint8_t* sb = group_at(pt, 4 * st + sl_g, g) + s_head_off;
-            sc = ld8_at(sb + sl_b * s_blk + static_cast<size_t>(g) * 32, sl_p);
+            return ld8_at(sb + sl_b * s_blk + static_cast<size_t>(g) * 32, sl_p);
         }
     };
     auto page_of_step = [&](const void* const* pt, int st) -> const uint8_t* {
         if constexpr (UNI) return page_at(pt, a.map.page_of(4 * st));
         else return nullptr;
     };
+    // each wave's loads run a step ahead (past its last step: the same rows again), page addresses two
     int st = begin + wave;
-    if (st < end) {
-        load(a.pt_k, page_of_step(a.pt_k, st), st, kn, ksc, true);
-        load(a.pt_v, page_of_step(a.pt_v, st), st, vn, vsc, false);
-    }
-
+    auto after = [&](int s) { return s + kWaves32 < end ? s + kWaves32 : s; };
+    const uint8_t *next_k = nullptr, *next_v = nullptr;
     // masks and constants that the compiler is not to see: as selects and literals they take more operations
     uint32_t c_mask = col < NB ? 0xffffffffu : 0u, c_fill = col == NB ? 0x3c003c00u : 0u;  // ones: sum p
     float minus1 = -1.0f;
@@ -904,57 +908,65 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
         hi = as_u32(h);
         lo = as_u32(pk_half(less(x, h.x, minus1), less(y, h.y, minus1)));
     };
-    // q: lane (col, j2) has channels 8 (2 k + j2) .. of each block of row col, scaled by a power of two to [1, 2); every wave
-    // forms all of them for the row's maximum and the block sums, and stores its share
+    // q: pieces of 16 channels, half of a block, a wave's own one (lane (col, j2): channels 8 j2 .. of row col); the row's
+    // maximum and the block sums go through LDS.  Scaled by a power of two to [1, 2)
     const int r = min(row0 + col, rows - 1), lim = pos + r / a.group;
-    u32x4 qch = {0u, 0u, 0u, 0u}, qcl = qch;  // block sums of blocks j2 and j2 + 2: the operand that meets the c of K
+    uint32_t qch, qcl;  // block sums of blocks j2 and j2 + 2, in two parts: the operand that meets the c of K
     float y_scale;
     {
+        static_assert(2 * NB <= kWaves32);
         const float* qr = a.q + static_cast<size_t>(r / a.group) * a.q_pitch + static_cast<size_t>(kh * a.group + r % a.group) * HD;
-        float f[2 * NB][8], top = 0.0f;
+        float(*s_top)[64] = reinterpret_cast<float(*)[64]>(s_mem + kWaves32 * NO * 256), (*s_sum)[64] = s_top + 2 * NB;
+        float f[8], top = 0.0f;
+        if (wave < 2 * NB) {
 #pragma unroll
-        for (int k = 0; k < 2 * NB; ++k)
+            for (int i = 0; i < 8; ++i) f[i] = qr[16 * wave + 8 * j2 + i];
+        }
+        if (st < end) {
+            const uint8_t *pk = page_of_step(a.pt_k, st), *pv = page_of_step(a.pt_v, st);
+            next_k = page_of_step(a.pt_k, after(st));
+            next_v = page_of_step(a.pt_v, after(st));
+            ksc = load_scales(a.pt_k, pk, st);
+            vsc = load_scales(a.pt_v, pv, st);
+            load(a.pt_k, pk, st, kn, true);
+            load(a.pt_v, pv, st, vn, false);
+        }
+        if (wave < 2 * NB) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                f[k][i] = qr[32 * (k / 2) + 8 * (2 * (k & 1) + j2) + i];
-                top = fmaxf(top, fabsf(f[k][i]));
-            }
-        const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-        top = fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(f[i]));
+            s_top[wave][lane] = top;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 2 * NB; ++k) top = fmaxf(top, fmaxf(s_top[k][col], s_top[k][col + 32]));
         const int e = top > 0.0f && top <= 3.402823466e38f ? max(__builtin_amdgcn_frexp_expf(top) - 1, -120) : 0;
         const float down = ldexpf(1.0f, -e);
         y_scale = ldexpf(__fdiv_rn(kLog2e, sqrt_rn(static_cast<float>(HD))), e);
-        float mine[2] = {0.0f, 0.0f};
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
+        if (wave < 2 * NB) {
             float sum = 0.0f;
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    f[2 * b + k][i] *= down;
-                    sum += f[2 * b + k][i];
-                }
-                if ((2 * b + k) % kWaves32 != wave) continue;
-                uint32_t h[4], l[4];
-                const float* x = f[2 * b + k];
-                part(x[0], x[4], h[0], l[0]);
-                part(x[1], x[5], h[1], l[1]);
-                part(x[2], x[6], h[2], l[2]);
-                part(x[7], x[3], h[3], l[3]);
-                s_q[2 * b + k][0][lane] = u32x4{h[0], h[1], h[2], h[3]};
-                s_q[2 * b + k][1][lane] = u32x4{l[0], l[1], l[2], l[3]};
+            for (int i = 0; i < 8; ++i) {
+                f[i] *= down;
+                sum += f[i];
             }
-            const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
-            sum = __uint_as_float(x[0]) + __uint_as_float(x[1]);
-            if ((b & 1) == j2) mine[b / 2] = sum;
+            s_sum[wave][lane] = sum;
+            uint32_t h[4], l[4];
+            part(f[0], f[4], h[0], l[0]);
+            part(f[1], f[5], h[1], l[1]);
+            part(f[2], f[6], h[2], l[2]);
+            part(f[7], f[3], h[3], l[3]);
+            s_q[wave][0][lane] = u32x4{h[0], h[1], h[2], h[3]};
+            s_q[wave][1][lane] = u32x4{l[0], l[1], l[2], l[3]};
         }
-        uint32_t h, l;
-        part(mine[0], mine[1], h, l);
-        qch[0] = h;
-        qcl[0] = l;
+        __syncthreads();
+        float mine[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int x = 0; x < NB / 2; ++x) {
+            const int k = 2 * (j2 + 2 * x);
+            mine[x] = (s_sum[k][col] + s_sum[k][col + 32]) + (s_sum[k + 1][col] + s_sum[k + 1][col + 32]);
+        }
+        part(mine[0], mine[1], qch, qcl);
     }
-    __syncthreads();
 
     f32x16 o[NB], oc;
     const f32x16 zero = {};
@@ -972,47 +984,60 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
 
     auto step = [&](auto edge_tag) {
         constexpr bool EDGE = decltype(edge_tag)::value;
-        const bool more = st + kWaves32 < end;
-        const uint8_t *next_k = nullptr, *next_v = nullptr;
-        if (more) {
-            next_k = page_of_step(a.pt_k, st + kWaves32);
-            next_v = page_of_step(a.pt_v, st + kWaves32);
-        }
+        const int nst = after(st);
+        u32x4 qv[2][4], ks[2][2];
+        auto load_q = [&](int b, u32x4 (&v)[4], u32x4 (&s)[2]) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                v[2 * k] = s_q[2 * b + k][1][lane];
+                v[2 * k + 1] = s_q[2 * b + k][0][lane];
+                s[k] = scales(0, b, k, 0);
+            }
+        };
         // this wave's own memory: its reads of the last step are done, and reads follow writes in order
+        bool big_step = false;
         if (NB == 4 || lane < 32) {
             *reinterpret_cast<uint2*>(s_sc + (sl_b * 4 + sl_g) * 32 + sl_p) = ksc;
             *reinterpret_cast<uint2*>(s_sc + SCALES + (sl_b * 4 + sl_g) * 32 + sl_p) = vsc;
+            big_step = sl_p < 16 && ((vsc.x | vsc.y) & 0x40004000u);
         }
         __builtin_amdgcn_wave_barrier();
-        f32x16 sc;
-        {
-            const uint16_t* c = reinterpret_cast<const uint16_t*>(s_sc + (j2 * 4 + kg) * 32 + 16) + kr;
-            u32x4 w = {c[0], 0u, 0u, 0u};
-            if constexpr (NB == 4) w[0] |= static_cast<uint32_t>(c[2 * 4 * 16]) << 16;
-            sc = mfma(w, qcl, zero);
-            sc = mfma(w, qch, sc);
-        }
+        const uint16_t* c = reinterpret_cast<const uint16_t*>(s_sc + (j2 * 4 + kg) * 32 + 16) + kr;
+        uint32_t cw = c[0];
+        if constexpr (NB == 4) cw |= static_cast<uint32_t>(c[2 * 4 * 16]) << 16;
+        load_q(0, qv[0], ks[0]);
+        ksc = load_scales(a.pt_k, next_k, nst);
+        vsc = load_scales(a.pt_v, next_v, nst);
+        asm("" : "+v"(qch), "+v"(qcl));  // or the operand's four registers are kept over the loop, and others spilled
+        f32x16 sc = mfma(u32x4{cw, cw, 0u, 0u}, u32x4{qch, qcl, 0u, 0u}, zero), xs[2];
+        auto add = [&](const f32x16& x, const u32x4 (&s)[2]) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const half2v h = as_half2(s[k][i]);
+                    sc[8 * k + 2 * i] = fmaf(static_cast<float>(h.x), x[8 * k + 2 * i], sc[8 * k + 2 * i]);
+                    sc[8 * k + 2 * i + 1] = fmaf(static_cast<float>(h.y), x[8 * k + 2 * i + 1], sc[8 * k + 2 * i + 1]);
+                }
+        };
+        // a block's products run while the last one's are scaled and the next one's q is read
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
+            u32x4 sb[2] = {ks[(b + 1) & 1][0], ks[(b + 1) & 1][1]};
+            if (b + 1 < NB) load_q(b + 1, qv[(b + 1) & 1], ks[(b + 1) & 1]);
             f32x16 x = zero;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const u32x4 w = __builtin_bit_cast(u32x4, q4_unpack(kn[b][k], ones));
-                x = mfma(w, s_q[2 * b + k][1][lane], x);
-                x = mfma(w, s_q[2 * b + k][0][lane], x);
+                x = mfma(w, qv[b & 1][2 * k], x);
+                x = mfma(w, qv[b & 1][2 * k + 1], x);
             }
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const u32x4 s = scales(0, b, k, 0);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const half2v h = as_half2(s[i]);
-                    sc[8 * k + 2 * i] = fmaf(static_cast<float>(h.x), x[8 * k + 2 * i], sc[8 * k + 2 * i]);
-                    sc[8 * k + 2 * i + 1] = fmaf(static_cast<float>(h.y), x[8 * k + 2 * i + 1], sc[8 * k + 2 * i + 1]);
-                }
-            }
+            xs[b & 1] = x;
+            if (b > 0) add(xs[(b + 1) & 1], sb);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        if (more) load(a.pt_k, next_k, st + kWaves32, kn, ksc, true);
+        load(a.pt_k, next_k, nst, kn, true);
+        add(xs[(NB - 1) & 1], ks[(NB - 1) & 1]);
         // rows that a query row does not see: p = 0, whatever is stored there
         uint32_t seen[2][4], seen_c[2][4];
         if constexpr (EDGE) {
@@ -1043,16 +1068,18 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
             const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
             mx = fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
         }
-        uint32_t big = 0;
+        uint32_t big = __any(big_step);
+        if (EDGE && big) {  // of the rows that the query row sees
+            big = 0;
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+            for (int k = 0; k < 2; ++k)
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const u32x4 s = scales(1, b, k, 0);
+                for (int b = 0; b < NB; ++b) {
+                    const u32x4 s = scales(1, b, k, 0);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) big |= EDGE ? s[i] & seen[k][i] : s[i];
-            }
-        big &= 0x40004000u;
+                    for (int i = 0; i < 4; ++i) big |= s[i] & seen[k][i] & 0x40004000u;
+                }
+        }
         if (__any((mx - m) * y_scale > kSlack || (big && lift == kLift))) {
             const auto t = __builtin_amdgcn_permlane32_swap(big, big, false, false);
             const float top = (mx - m) * y_scale > kSlack ? mx : m, down = (t[0] | t[1]) ? kLiftBig : lift;
@@ -1100,7 +1127,9 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
                 o[b] = mfma(w, fh, o[b]);
             }
         }
-        if (more) load(a.pt_v, next_v, st + kWaves32, vn, vsc, false);
+        load(a.pt_v, next_v, nst, vn, false);
+        next_k = page_of_step(a.pt_k, after(nst));
+        next_v = page_of_step(a.pt_v, after(nst));
         __builtin_amdgcn_wave_barrier();
     };
     // steps that every query row sees whole; none where pages end inside a group
@@ -1146,9 +1175,9 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
             for (int x = 0; x < 4; ++x) v[x] = fmaf(w[k], s_o[k][reg + x][lane], v[x]);
         }
         // registers 4 q .. of a block: channels 8 q + 4 j2 ..; rows of the output are only known to be 4-byte aligned
-        float* p = dst + 32 * b + 2 * (reg % 16) + 4 * j2;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) p[x] = (v[x] + c) * scale;
+        typedef f32x4 f32x4_at4 __attribute__((aligned(4)));
+        *reinterpret_cast<f32x4_at4*>(dst + 32 * b + 2 * (reg % 16) + 4 * j2) =
+            f32x4{(v[0] + c) * scale, (v[1] + c) * scale, (v[2] + c) * scale, (v[3] + c) * scale};
     }
     if (a.part && wave == 0 && j2 == 0) {
         float* ml = a.part + static_cast<size_t>(a.n_tokens) * a.n_head * n_split * HD + 2 * at;
