@@ -448,8 +448,8 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
 //           at a time: its p s is broadcast to the 8 channel quads of a block.
 // The scores leave a lane with four cache rows of one query row, which is the
 // operand that the values take.  Rows of a group go in the order of the scales
-// (0 4 1 5, 2 6 7 3), as the words unpack.  Against the kernel above (65000
-// rows of 8 kv heads of 128, 4 heads each): 26.5 us.
+// (0 4 1 5, 2 6 7 3), as the words unpack.  65000 rows of 8 kv heads of 128, 4
+// heads each: 21.4 us (3.9 TB/s), with the kernel above 26.5.
 template <int NB, bool UNI>
 __global__ __launch_bounds__(64 * kWaves, 2) void attn_q4_narrow_kernel(Q4Args a) {
     constexpr int HD = 32 * NB, NH = NB / 2, NR = 2 * NB;  // 64-channel halves; q registers (of four channel steps)
@@ -1357,23 +1357,48 @@ __global__ __launch_bounds__(kJoin) void attn_q4_join_kernel(Q4Args a, int n_spl
 }
 
 bool q4_tiles(size_t hd) { return hd % 32 == 0 && (hd <= 128 || hd == 192 || hd == 256); }
-// A chunk of fixed splits is to give a token the bits it has in any other chunk: one kernel for all
-bool q4_narrow(size_t hd, size_t rows, size_t chunk) { return (hd == 64 || hd == 128) && rows <= 4 && !chunk; }
-bool q4_tile32(size_t hd, size_t rows, size_t chunk) { return (hd == 64 || hd == 128) && (rows > kTile || chunk); }
+
+// Which kernel takes a call.  A chunk of fixed splits is to give a token the
+// bits it has in any other chunk: one kernel for all (the tiles of 32 rows, where
+// they take the head).  Else, by query rows of a kv head and steps of 32 cache rows:
+//   up to 4 rows, from 32 steps on, the 4 x 4 products.  8 kv heads of 128,
+//     1 / 4 rows, against the tiles of 16: position 1500 9.1 / 10.3 us against
+//     9.5 / 10.3, 30000 15.0 / 17.2 against 16.6 / 17.6; below, fewer of the waves
+//     have a step: position 100 5.5 / 6.4 against 5.0 / 5.5;
+//   the tiles of 32 rows from 16 rows and 32768 rows x steps x kv heads on (they
+//     unpack a step for twice the rows, but start and end slower): position 1500,
+//     64 / 256 rows 14.4 / 19.0 us against 13.1 / 21.5; 16000, 8 / 16 / 32 rows
+//     15.1 / 15.5 / 16.4 against 14.5 / 16.9 / 20.8; 100, 256 / 1024 rows 10.1 /
+//     12.1 against 8.9 / 13.7; 4 kv heads of 64, 16000, 16 / 32 rows 11.4 / 11.5
+//     against 10.5 / 12.6.
+enum class Q4Kind { kNarrow, kTile16, kTile32, kAny };
+Q4Kind q4_kind(size_t hd, size_t rows, size_t steps, size_t n_head_kv, size_t chunk) {
+    if (!q4_tiles(hd)) return Q4Kind::kAny;
+    if (hd != 64 && hd != 128) return Q4Kind::kTile16;
+    if (chunk) return Q4Kind::kTile32;
+    if (rows <= 4) return steps >= 32 ? Q4Kind::kNarrow : Q4Kind::kTile16;
+    return rows >= 16 && rows * steps * n_head_kv >= 32768 ? Q4Kind::kTile32 : Q4Kind::kTile16;
+}
+size_t q4_steps(size_t max_pos, size_t page_tokens) {
+    return static_cast<size_t>(kv4_map(page_tokens).group_of(static_cast<int>(max_pos - 1)) / 4 + 1);
+}
 
 // Splits of a call: enough workgroups for two a CU, each wave at least one step, at most kMaxSplit.
 size_t q4_splits(size_t max_pos, size_t n_tokens, size_t n_head, size_t n_head_kv, size_t hd, size_t page_tokens,
                  size_t chunk) {
-    const Kv4Map map = kv4_map(page_tokens);
-    const size_t steps = static_cast<size_t>(map.group_of(static_cast<int>(max_pos - 1)) / 4 + 1);
+    const size_t steps = q4_steps(max_pos, page_tokens);
     if (chunk) return (steps + chunk - 1) / chunk;
     const size_t rows = n_tokens * (n_head / n_head_kv);
-    if (q4_tile32(hd, rows, chunk)) {  // a workgroup a CU: more splits cost more in parts than they gain
-        const size_t tiles = n_head_kv * ((rows + kRows32 - 1) / kRows32);
-        return std::max<size_t>(1, std::min({256 / tiles, (steps + 2 * kWaves - 1) / (2 * kWaves), static_cast<size_t>(kMaxSplit)}));
+    size_t tiles = n_head_kv * ((rows + kTile - 1) / kTile), room = 512;
+    switch (q4_kind(hd, rows, steps, n_head_kv, chunk)) {
+    case Q4Kind::kTile32:  // a workgroup a CU: more splits cost more in parts than they gain
+        tiles = n_head_kv * ((rows + kRows32 - 1) / kRows32);
+        room = 256;
+        break;
+    case Q4Kind::kAny: tiles = n_head * n_tokens; break;
+    default: break;
     }
-    const size_t tiles = q4_tiles(hd) ? n_head_kv * ((rows + kTile - 1) / kTile) : n_head * n_tokens;
-    return std::max<size_t>(1, std::min({512 / tiles, (steps + 2 * kWaves - 1) / (2 * kWaves), static_cast<size_t>(kMaxSplit)}));
+    return std::max<size_t>(1, std::min({room / tiles, (steps + 2 * kWaves - 1) / (2 * kWaves), static_cast<size_t>(kMaxSplit)}));
 }
 
 template <int NB>
@@ -1386,7 +1411,7 @@ void q4_launch(const Q4Args& a, dim3 grid, hipStream_t st) {
 
 // 512 positions a split (whole 8-row groups), more where they would be over kMaxSplit
 size_t attn_q4_chunk(size_t max_pos, size_t page_tokens) {
-    const size_t steps = static_cast<size_t>(kv4_map(page_tokens).group_of(static_cast<int>(max_pos - 1)) / 4 + 1);
+    const size_t steps = q4_steps(max_pos, page_tokens);
     size_t chunk = 16;
     while (steps > chunk * kMaxSplit) chunk *= 2;
     return chunk;
@@ -1421,21 +1446,26 @@ hipError_t launch_attn_q4(const void* const* pt_k, const void* const* pt_v, cons
     a.chunk = static_cast<int>(chunk);
     a.map = kv4_map(page_tokens);
     const unsigned z = static_cast<unsigned>(splits);
-    if (q4_narrow(hd, n_tokens * a.group, chunk)) {
+    switch (q4_kind(hd, n_tokens * a.group, q4_steps(max_pos, page_tokens), n_head_kv, chunk)) {
+    case Q4Kind::kNarrow: {
         const dim3 grid(static_cast<unsigned>(n_head_kv), 1, z);
         const bool uni = page_tokens % 64 == 0;
         if (hd == 128 && uni) attn_q4_narrow_kernel<4, true><<<grid, 64 * kWaves, 0, st>>>(a);
         else if (hd == 128) attn_q4_narrow_kernel<4, false><<<grid, 64 * kWaves, 0, st>>>(a);
         else if (uni) attn_q4_narrow_kernel<2, true><<<grid, 64 * kWaves, 0, st>>>(a);
         else attn_q4_narrow_kernel<2, false><<<grid, 64 * kWaves, 0, st>>>(a);
-    } else if (q4_tile32(hd, n_tokens * a.group, chunk)) {
+        break;
+    }
+    case Q4Kind::kTile32: {
         const dim3 grid(static_cast<unsigned>(n_head_kv), static_cast<unsigned>((n_tokens * a.group + kRows32 - 1) / kRows32), z);
         const bool uni = page_tokens % 32 == 0;
         if (hd == 128 && uni) attn_q4_tile_kernel<4, true><<<grid, 64 * kWaves32, 0, st>>>(a);
         else if (hd == 128) attn_q4_tile_kernel<4, false><<<grid, 64 * kWaves32, 0, st>>>(a);
         else if (uni) attn_q4_tile_kernel<2, true><<<grid, 64 * kWaves32, 0, st>>>(a);
         else attn_q4_tile_kernel<2, false><<<grid, 64 * kWaves32, 0, st>>>(a);
-    } else if (q4_tiles(hd)) {
+        break;
+    }
+    case Q4Kind::kTile16: {
         const dim3 grid(static_cast<unsigned>(n_head_kv), static_cast<unsigned>((n_tokens * a.group + kTile - 1) / kTile), z);
         switch (hd / 32) {
         case 1: q4_launch<1>(a, grid, st); break;
@@ -1445,7 +1475,9 @@ hipError_t launch_attn_q4(const void* const* pt_k, const void* const* pt_v, cons
         case 6: q4_launch<6>(a, grid, st); break;
         default: q4_launch<8>(a, grid, st); break;
         }
-    } else {
+        break;
+    }
+    case Q4Kind::kAny:
         attn_q4_any_kernel<<<dim3(static_cast<unsigned>(n_head), static_cast<unsigned>(n_tokens), z), kAny,
                              2 * hd * sizeof(float), st>>>(a);
     }

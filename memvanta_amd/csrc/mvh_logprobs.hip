@@ -5,8 +5,9 @@
 //   s = sum e^(l - m), t = sum (l - m) e^(l - m),
 //   log p_i = (l_i - m) - ln s,  entropy = ln s - t / s,
 // all in fp32 per thread, joined across threads with the usual rescaling.  The
-// pass is bound by reading the logits (~10 operations an element); few rows are
-// cut into parts, whose sums and candidates a second kernel joins.
+// pass is bound by reading the logits (~10 operations an element); few
+// rows of more than 65536 are cut into parts, whose sums and candidates a second
+// kernel joins.
 //
 // The most probable tokens, a tile of the row (32 elements a lane) at a time:
 // the k-th of the largest elements of 64 groups of lanes is a bound that at
@@ -377,18 +378,20 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(LpArgs a) {
 }
 
 // Few long rows take workgroups of 1024 threads, whose tile (32768 elements) is
-// a whole row of most vocabularies: one launch, no parts.  (32000 logits, 20
-// tops: 8.5 us; with 256 threads and 8 parts joined by a second kernel 14.3 us.)
-bool lp_wide(size_t n, size_t rows) { return n > 256 * kPer && rows < 512; }
-size_t lp_parts(size_t n, size_t rows) {
-    if (!lp_wide(n, rows) || n <= 2 * 1024 * kPer) return 1;
+// a whole row of most vocabularies: one launch, no parts.  That is up to a
+// workgroup a CU without top tokens, two with (the search for them waits more).
+// 32000 logits, 256 / 400 rows without: 6.5 / 12.2 us against 7.5 / 11.1 with 256
+// threads; with 20 top tokens 1 / 512 / 768 rows: 8.6 / 22.8 / 32.4 against 17.5 / 25.0 / 29.4.
+bool lp_wide(size_t n, size_t rows, size_t k) { return n > 256 * kPer && rows <= (k ? 512 : 256); }
+size_t lp_parts(size_t n, size_t rows, size_t k) {
+    if (!lp_wide(n, rows, k) || n <= 2 * 1024 * kPer) return 1;
     return std::max<size_t>(1, std::min({(n + 1024 * kPer - 1) / (1024 * kPer), 512 / rows, size_t{64}}));
 }
 
 }  // namespace
 
 size_t logprobs_scratch(size_t n, size_t rows, size_t k) {
-    const size_t parts = lp_parts(n, rows);
+    const size_t parts = lp_parts(n, rows, k);
     return parts > 1 ? rows * parts * (16 + (k ? 64 * sizeof(u64) : 0)) : 0;
 }
 
@@ -406,8 +409,8 @@ hipError_t launch_logprobs(const float* logits, size_t pitch, size_t n, size_t r
     a.n = n;
     a.pitch = pitch;
     a.k = static_cast<int>(k);
-    const size_t parts = lp_parts(n, rows);
-    const size_t tile = (lp_wide(n, rows) ? 1024 : 256) * kPer;
+    const size_t parts = lp_parts(n, rows, k);
+    const size_t tile = (lp_wide(n, rows, k) ? 1024 : 256) * kPer;
     a.chunk = ((n + parts - 1) / parts + tile - 1) / tile * tile;
     a.parts = static_cast<int>((n + a.chunk - 1) / a.chunk);
     if (a.parts > 1) {
@@ -426,7 +429,7 @@ hipError_t launch_logprobs(const float* logits, size_t pitch, size_t n, size_t r
         if (b.top_ids) b.top_ids += r0 * k;
         if (b.top_lp) b.top_lp += r0 * k;
         const dim3 grid(static_cast<unsigned>(b.parts), nr);
-        if (lp_wide(n, rows)) {
+        if (lp_wide(n, rows, k)) {
             if (k) logprobs_kernel<1024, true><<<grid, 1024, 0, st>>>(b);
             else logprobs_kernel<1024, false><<<grid, 1024, 0, st>>>(b);
         } else {
