@@ -360,14 +360,26 @@ int check_pages(const mvh_kv_cache* kv, size_t layer, size_t first, size_t last)
 // Pages first..last of the layer are there.  Those a call misses come from the
 // free ones, else from one allocation, and reach the device's tables in one
 // copy: a prompt of 65000 tokens in pages of 128 took 512 allocations and 1024
-// copies (13 ms), and its pages lay apart in memory.
-int ensure_pages(mvh_kv_cache* kv, size_t layer, size_t first, size_t last) {
+// copies (13 ms), and its pages lay apart in memory.  The host's table, which
+// calls go by, takes them last: a failed copy leaves them missing.
+int ensure_pages(const mvh_context* c, mvh_kv_cache* kv, size_t layer, size_t first, size_t last) {
     const size_t row = layer * kv->max_pages;
-    size_t missing = 0;
-    for (size_t p = first; p <= last; ++p) missing += !kv->hk[row + p];
+    size_t missing = 0, lo = last, hi = first;
+    for (size_t p = first; p <= last; ++p) {
+        if (kv->hk[row + p]) continue;
+        ++missing;
+        lo = std::min(lo, p);
+        hi = p;
+    }
     if (!missing) return MVH_OK;
+    hipStreamCaptureStatus state = hipStreamCaptureStatusNone;
+    MVH_HIP(hipStreamIsCapturing(c->stream, &state));
+    if (state != hipStreamCaptureStatusNone)
+        return fail(MVH_E_NOMEM, "KV page is not there yet: write its positions once before capturing the call");
     const size_t bytes = 2 * kv->page_stride();
+    std::vector<void*> table;  // K's entries lo .. hi, then V's
     try {
+        table.resize(2 * (hi - lo + 1));
         kv->pool.reserve(kv->hk.size());  // what reset() returns has its place
         while (kv->pool.size() < missing) {
             // all at once, or one by one where memory is short
@@ -388,20 +400,26 @@ int ensure_pages(mvh_kv_cache* kv, size_t layer, size_t first, size_t last) {
     } catch (const std::bad_alloc&) {
         return fail(MVH_E_NOMEM, "host allocation failed");
     }
-    size_t lo = last, hi = first;
-    for (size_t p = first; p <= last; ++p) {
-        if (kv->hk[row + p]) continue;
-        uint8_t* page = kv->pool.back();
-        kv->pool.pop_back();
-        kv->hk[row + p] = page;
-        kv->hv[row + p] = page + kv->page_stride();
-        ++kv->live_pages;
-        lo = std::min(lo, p);
-        hi = p;
+    const size_t n = hi - lo + 1;
+    size_t taken = 0;
+    for (size_t i = 0; i < n; ++i) {
+        uint8_t* k = kv->hk[row + lo + i];
+        uint8_t* v = kv->hv[row + lo + i];
+        if (!k) {
+            k = kv->pool[kv->pool.size() - ++taken];
+            v = k + kv->page_stride();
+        }
+        table[i] = k;
+        table[n + i] = v;
     }
-    const size_t n = (hi - lo + 1) * sizeof(void*);
-    MVH_HIP(hipMemcpy(kv->dk + row + lo, &kv->hk[row + lo], n, hipMemcpyHostToDevice));
-    MVH_HIP(hipMemcpy(kv->dv + row + lo, &kv->hv[row + lo], n, hipMemcpyHostToDevice));
+    MVH_HIP(hipMemcpy(kv->dk + row + lo, table.data(), n * sizeof(void*), hipMemcpyHostToDevice));
+    MVH_HIP(hipMemcpy(kv->dv + row + lo, table.data() + n, n * sizeof(void*), hipMemcpyHostToDevice));
+    kv->pool.resize(kv->pool.size() - taken);
+    kv->live_pages += taken;
+    for (size_t i = 0; i < n; ++i) {
+        kv->hk[row + lo + i] = static_cast<uint8_t*>(table[i]);
+        kv->hv[row + lo + i] = static_cast<uint8_t*>(table[n + i]);
+    }
     return MVH_OK;
 }
 
@@ -1012,6 +1030,9 @@ int mvh_kv_create(mvh_context* c, size_t n_layer, size_t kv_dim, size_t page_tok
     } else if (max_tokens > 16000) {
         return fail(MVH_E_RANGE, "max_tokens above 16000 is not supported");
     }
+    const size_t max_pages = (max_tokens - 1) / page_tokens + 1;
+    if (n_layer > (size_t{1} << 31) / max_pages)
+        return fail(MVH_E_RANGE, "KV cache of more than 2147483648 pages");
     auto* kv = new (std::nothrow) mvh_kv_cache;
     if (!kv) return fail(MVH_E_NOMEM, "host allocation failed");
     kv->device = c->device;
@@ -1020,10 +1041,15 @@ int mvh_kv_create(mvh_context* c, size_t n_layer, size_t kv_dim, size_t page_tok
     kv->kv_dim = kv_dim;
     kv->page_tokens = page_tokens;
     kv->max_tokens = max_tokens;
-    kv->max_pages = (max_tokens + page_tokens - 1) / page_tokens;
+    kv->max_pages = max_pages;
     const size_t n = n_layer * kv->max_pages;
-    kv->hk.assign(n, nullptr);
-    kv->hv.assign(n, nullptr);
+    try {
+        kv->hk.assign(n, nullptr);
+        kv->hv.assign(n, nullptr);
+    } catch (const std::bad_alloc&) {
+        delete kv;
+        return fail(MVH_E_NOMEM, "host allocation failed");
+    }
     if (hipMalloc(&kv->dk, n * sizeof(void*)) != hipSuccess || hipMalloc(&kv->dv, n * sizeof(void*)) != hipSuccess) {
         (void)hipGetLastError();
         if (kv->dk) (void)hipFree(kv->dk);
@@ -1078,11 +1104,11 @@ int mvh_kv_type(const mvh_kv_cache* kv, int* type) {
 int mvh_kv_write(mvh_context* c, mvh_kv_cache* kv, size_t layer, size_t pos, size_t n_tokens, const float* k,
                  const float* v, int kind) {
     CHECK_CTX(c);
-    if (int rc = check_kv(kv, layer)) return rc;
+    if (int rc = kv && kv->type == MVH_KV_Q4 ? check_kv_on(c, kv, layer) : check_kv(kv, layer)) return rc;
     if (!n_tokens) return MVH_OK;
     if (!k || !v) return fail(MVH_E_INVALID, "null k/v");
-    if (pos + n_tokens > kv->max_tokens) return fail(MVH_E_RANGE, "context exhausted");
-    if (int rc = ensure_pages(kv, layer, pos / kv->page_tokens, (pos + n_tokens - 1) / kv->page_tokens)) return rc;
+    if (n_tokens > kv->max_tokens || pos > kv->max_tokens - n_tokens) return fail(MVH_E_RANGE, "context exhausted");
+    if (int rc = ensure_pages(c, kv, layer, pos / kv->page_tokens, (pos + n_tokens - 1) / kv->page_tokens)) return rc;
     const size_t bytes = n_tokens * kv->kv_dim * 4;
     const void* kd = nullptr;
     const void* vd = nullptr;
@@ -1303,7 +1329,7 @@ int mvh_kv_append(mvh_context* c, mvh_kv_cache* kv, size_t layer, size_t pos, si
     if (q && !q_out) return fail(MVH_E_INVALID, "null q_out");
     if (q && q == q_out && q_pitch != out_pitch) return fail(MVH_E_INVALID, "rotation in place needs equal pitches");
     if (n_tokens > kv->max_tokens || pos > kv->max_tokens - n_tokens) return fail(MVH_E_RANGE, "context exhausted");
-    if (int rc = ensure_pages(kv, layer, pos / kv->page_tokens, (pos + n_tokens - 1) / kv->page_tokens)) return rc;
+    if (int rc = ensure_pages(c, kv, layer, pos / kv->page_tokens, (pos + n_tokens - 1) / kv->page_tokens)) return rc;
     const size_t qw = n_head * hd * 4, kw = kv_dim * 4;
     const float *qd = q, *kd = k, *vd = v;
     float* od = q_out;
@@ -1446,7 +1472,7 @@ int mvh_attn_batch(mvh_context* c, const mvh_kv_cache* kv, size_t layer, const f
         return fail(MVH_E_SHAPE, "invalid Llama head configuration");
     if (head_dim % 8 || n_head_kv * head_dim > kv->kv_dim)
         return fail(MVH_E_SHAPE, "head_dim must be a multiple of 8 and n_head_kv*head_dim <= kv_dim");
-    if (pos + n_tokens > kv->max_tokens) return fail(MVH_E_RANGE, "context exhausted");
+    if (n_tokens > kv->max_tokens || pos > kv->max_tokens - n_tokens) return fail(MVH_E_RANGE, "context exhausted");
     const size_t last = pos + n_tokens - 1;
     for (size_t p = 0; p <= last / kv->page_tokens; ++p)
         if (!kv->hk[layer * kv->max_pages + p]) return fail(MVH_E_RANGE, "KV key page missing");

@@ -56,6 +56,39 @@ def test_batch(ctx, n_head, n_kv, hd, page):
     kv.close()
 
 
+# pages of one row (every row a group of 8 of its own), of no whole groups, of whole groups, steps and pairs of steps; one to
+# 40 heads a kv head; rows, steps and pages on both sides of what the kernels split at
+@pytest.mark.parametrize("hd,page", [(64, 20), (128, 96), (64, 9), (128, 1), (128, 128), (64, 64), (128, 16), (64, 32)])
+def test_rows_and_steps(ctx, hd, page):
+    rng = np.random.default_rng(hd * page)
+    n_kv = 2
+    kv, k, v = _case(ctx, rng, n_kv, hd, page, 2300)
+    for group, pos, n in ((1, 990, 1), (1, 991, 1), (1, 992, 1), (1, 2200, 1), (4, 1500, 1), (4, 2111, 1), (2, 2000, 2), (1, 2100, 4),
+                          (5, 2000, 1), (3, 2001, 5), (4, 2100, 4), (8, 1900, 40), (4, 2000, 200), (40, 2290, 9), (1, 1600, 700)):
+        q = rng.standard_normal((n, group * n_kv, hd), dtype=np.float32) * np.float32(1.5)
+        got = kv.attn_batch(0, q.reshape(n, -1), pos, n, group * n_kv, n_kv, hd).reshape(q.shape)
+        _check(got, attend(q, k, v, pos, group), (group, pos, n))
+    kv.close()
+
+
+def test_page_past_4_gib(ctx):
+    """Pages of 5 GiB: rows and heads beyond offsets of 32 bits."""
+    rng = np.random.default_rng(40)
+    n_kv, hd, rows = 64, 128, 2 ** 20
+    kv = ctx.kv_cache(1, n_kv * hd, rows, rows, kv_type=capi.MVH_KV_Q4)
+    k, v = (rng.standard_normal((41, n_kv * hd), dtype=np.float32) for _ in range(2))
+    for pos in (0, rows - 41):
+        kv.write(0, pos, k, v)
+        for got, want in zip(kv.read(0, pos, 41), (k, v)):
+            assert (got == q4_values(want)).all()
+        k, v = v, k
+    k, v = (q4_values(x).reshape(41, n_kv, hd) for x in (k, v))
+    for n in (1, 3, 41):  # 41 - n rows before the chunk
+        q = rng.standard_normal((n, n_kv, hd), dtype=np.float32)
+        _check(kv.attn_batch(0, q.reshape(n, -1), 41 - n, n, n_kv, n_kv, hd).reshape(q.shape), attend(q, k, v, 41 - n, 1), n)
+    kv.close()
+
+
 @pytest.mark.parametrize("n_head,n_kv,hd,n", [(8, 2, 128, 40001), (4, 4, 64, 70000), (2, 2, 48, 9000)])
 def test_long(ctx, n_head, n_kv, hd, n):
     """Past 16000 positions (and 2^16), several pages of scores a split, and a page table of its own layer."""
@@ -173,5 +206,9 @@ def test_refusals(ctx):
     refused(2, "head_dim", kv.attn_decode, 0, q[0], 0, 4, 2, 60)
     refused(2, "head_dim", kv.attn_decode, 0, q[0], 0, 4, 2, 128)
     refused(5, "layer", kv.attn_decode, 1, q[0], 0, 4, 2, 64)
+    for far in (2 ** 64 - 1, 2 ** 64 - 2, 2 ** 63):
+        refused(5, "exhausted", kv.attn_batch, 0, q, far, 2, 4, 2, 64)
+        refused(5, "exhausted", kv.write, 0, far, q[:, :128], q[:, :128])
+    refused(5, "pages", ctx.kv_cache, 2 ** 60, 128, 16, 2 ** 20, capi.MVH_KV_Q4)
     assert (kv.attn_decode(0, q[0], 0, 4, 2, 64) == 0).all()
     kv.close()

@@ -51,7 +51,7 @@ def _check(got, x, targets, top):
 
 # rows of one element, of no whole quad, of one batch and around it, of several parts; few and many rows
 @pytest.mark.parametrize("rows,n", [(1, 1), (3, 2), (1, 63), (2, 64), (5, 65), (1, 1000), (4, 4095), (1, 4096), (3, 4097),
-                                    (1, 32000), (7, 32003), (600, 513), (300, 5000), (2, 130001)])
+                                    (1, 32000), (7, 32003), (600, 513), (300, 5000), (2, 130001), (300, 9001), (520, 8500)])
 @pytest.mark.parametrize("top", [0, 1, 5, 20, 64])
 def test_random(ctx, rows, n, top):
     rng = np.random.default_rng(rows + n)

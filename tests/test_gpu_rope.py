@@ -151,6 +151,41 @@ def test_q4_format(ctx):
         kv.close()
 
 
+@pytest.mark.parametrize("kind", ["normal", "steps", "halves", "wide", "tiny", "huge"])
+def test_q4_codes(ctx, kind):
+    """Every code of half a million elements, also values on and next to the borders between two codes; by a write, and by a
+    rotated append at position 0, which leaves finite rows as they are."""
+    rng = np.random.default_rng(len(kind))
+    n, f = 1024, np.float32
+    x = rng.standard_normal((n, 512), dtype=f)
+    if kind in ("steps", "halves"):  # lo + s (i or i + 1/2), exact, and their neighbours
+        s = np.exp2(rng.integers(-14, 9, (n, 16, 1))).astype(f) * rng.integers(1, 1024, (n, 16, 1)).astype(f) / f(512)
+        i = rng.integers(0, 16, (n, 16, 32)).astype(f)
+        i[:, :, 0], i[:, :, 1] = 0, 15
+        half = np.where((i > 0) & (i < 15), f(0.5) if kind == "halves" else f(0), f(0))
+        x = (rng.integers(-20, 4, (n, 16, 1)).astype(f) * s + s * (i + half)).reshape(n, 512)
+        off = rng.integers(-1, 2, x.shape)
+        x = np.where(off > 0, np.nextafter(x, f(np.inf)), np.where(off < 0, np.nextafter(x, f(-np.inf)), x))
+    elif kind == "wide":
+        x *= np.exp(rng.uniform(-30, 30, (n, 1))).astype(f)
+    elif kind == "tiny":
+        x *= f(2.0 ** -22) * np.exp2(rng.integers(-20, 4, (n, 1))).astype(f)
+    elif kind == "huge":
+        x *= f(3e37)
+    want = q4_values(x)
+    kv = ctx.kv_cache(1, 512, 128, n, kv_type=capi.MVH_KV_Q4)
+    kv.write(0, 0, x, x[::-1])
+    k, v = kv.read(0, 0, n)
+    assert (k == want).all() and (v == want[::-1]).all()
+    r = ctx.rope(64)
+    for row in range(0, 64):
+        kv.append(0, 0, x[row:row + 1], x[row + 1:row + 2], r)
+        k, v = kv.read(0, 0, 1)
+        assert (k == want[row]).all() and (v == want[row + 1]).all(), row
+    r.close()
+    kv.close()
+
+
 def test_refusals(ctx):
     def refused(code, text, f, *a, **k):
         with pytest.raises(capi.MvhError, match=text) as e:

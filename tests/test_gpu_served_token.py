@@ -174,6 +174,41 @@ def test_no_workspace_under_capture():
     c.close()
 
 
+def test_no_page_under_capture():
+    """A position whose page is not there cannot be captured, also where freed pages wait; it is missing afterwards too."""
+    c = capi.Context(0)
+    kv = c.kv_cache(1, 64, 8, 64, kv_type=capi.MVH_KV_Q4)
+    rope = c.rope(64)
+    rows = torch.randn(16, 64, device="cuda")
+    out = torch.empty(64, device="cuda")
+    torch.cuda.synchronize()
+    kv.append(0, 0, rows, rows, rope)
+    c.synchronize()
+    kv.reset()  # the pages of positions 0..15 are free ones now
+    kv.append(0, 0, rows[:8], rows[:8], rope)
+    stream = torch.cuda.ExternalStream(c.stream)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream):
+        with pytest.raises(capi.MvhError, match="before capturing") as e:
+            kv.append(0, 8, rows[8:], rows[8:], rope)
+        assert e.value.code == 6
+        kv.attn_decode(0, rows[0], 7, 1, 1, 64, out)
+    with pytest.raises(capi.MvhError, match="missing"):
+        kv.attn_decode(0, rows[0], 8, 1, 1, 64, out)
+    with torch.cuda.stream(stream):
+        g.replay()
+    c.synchronize()
+    captured = out.clone()
+    kv.append(0, 8, rows[8:], rows[8:], rope)
+    kv.attn_decode(0, rows[0], 7, 1, 1, 64, out)
+    c.synchronize()
+    assert torch.equal(out, captured)
+    del g
+    kv.close()
+    rope.close()
+    c.close()
+
+
 def test_two_contexts(ctx):
     """Two contexts' steps in flight together give the bits of each alone."""
     other = capi.Context(0)
