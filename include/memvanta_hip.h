@@ -202,7 +202,7 @@ int mvh_matmul_q4_0_batch(mvh_context* ctx, const mvh_tensor* a, const float* x,
 int mvh_matvec_q4_0(mvh_context* ctx, const mvh_tensor* a, const float* x, float* y, int ptr_kind);
 int mvh_matvec_q8_0(mvh_context* ctx, const mvh_tensor* a, const float* x, float* y, int ptr_kind);
 
-/* ---- paged KV cache (F32 / F16 / Q8 pages): all layers of one model on one device ---- */
+/* ---- paged KV cache (F32 / F16 / Q8 / Q4 pages): all layers of one model on one device ---- */
 /* parse_kv_cache_type: "f32", "f16", "q8" or "q8_0", and "q4"; anything else fails with
  * "unknown KV cache type: <s>" */
 int mvh_kv_parse_type(const char* s, int* kv_type);
@@ -264,7 +264,8 @@ int mvh_kv_append(mvh_context* ctx, mvh_kv_cache* kv, size_t layer, size_t pos, 
 /* decode attention of one layer over positions 0..pos: q[n_head*hd] -> out[n_head*hd].  Over a Q4 cache the calls
  * of a context share its workspace, which a longer call replaces by a larger one; the old one is kept until the
  * context is destroyed, so a captured graph stays valid.  Graphs captured from one context must not run at the same
- * time, and a call whose workspace is not there yet cannot be captured (MVH_E_NOMEM): make it once before. */
+ * time, and a call whose workspace is not there yet cannot be captured (MVH_E_NOMEM): make it once before.  The same
+ * goes for a write or append whose pages are not there yet. */
 int mvh_attn_decode(mvh_context* ctx, const mvh_kv_cache* kv, size_t layer, const float* q, size_t pos,
                     size_t n_head, size_t n_head_kv, size_t head_dim, float* out, int ptr_kind);
 /* the batched causal attention of LlamaModel::forward_batch_impl (the per-(token, head) loop at

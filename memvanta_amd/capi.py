@@ -216,8 +216,8 @@ def _rows(a):
             raise ValueError("host rows must be 2-D, C-contiguous and float32")
         n, width = a.shape
         return a.ctypes.data, n, width, width
-    if a.dtype is not _torch_f32():
-        raise ValueError("device rows must be float32")
+    if a.dtype is not _torch_f32() or not a.is_cuda:
+        raise ValueError("device rows must be float32 in device memory")
     shape = a.shape
     if len(shape) == 1:
         n, width = 1, shape[0]
@@ -375,16 +375,16 @@ class Context:
         torch = sys.modules["torch"]
         shape = logits.shape
         rows, n = (1, shape[0]) if len(shape) == 1 else shape
-        if logits.dtype is not torch.float32 or not logits.is_contiguous():
-            raise ValueError("logits must be contiguous float32 rows")
+        if logits.dtype is not torch.float32 or not logits.is_contiguous() or not logits.is_cuda:
+            raise ValueError("logits must be contiguous float32 rows in device memory")
 
         def at(a, dtype, count, name):
             if a is None:
                 return None
             if isinstance(a, np.ndarray):
                 raise ValueError("mix of host and device buffers in one call")
-            if a.dtype is not dtype or a.numel() < count or not a.is_contiguous():
-                raise ValueError(f"{name} must be {count} contiguous elements of {dtype}")
+            if a.dtype is not dtype or a.numel() < count or not a.is_contiguous() or not a.is_cuda:
+                raise ValueError(f"{name} must be {count} contiguous elements of {dtype} in device memory")
             return a.data_ptr()
 
         f32, i32 = torch.float32, torch.int32
@@ -520,8 +520,8 @@ class Rope:
                 raise ValueError("mix of host and device buffers in one call")
             if len(positions) != n or str(positions.dtype) not in ("int32", "torch.int32"):
                 raise ValueError("positions must be one int32 per row")
-            if not host and not positions.is_contiguous():
-                raise ValueError("positions must be contiguous")
+            if not host and not (positions.is_contiguous() and positions.is_cuda):
+                raise ValueError("positions must be contiguous and in device memory")
             at = _ptr(positions)
         ctx = self.ctx
         ctx._check(ctx.lib.mvh_rope_apply(ctx.h, self.h, x_at, pitch, n, n_head, at, pos, y_at, out_pitch,

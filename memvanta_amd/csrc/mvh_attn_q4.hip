@@ -130,7 +130,9 @@ __device__ __forceinline__ void write_sum(const Q4Args& a, int kh, int row, int 
 // then holds p of 8 consecutive cache rows of one query row: with the cache
 // rows in that order in V's words too, p is the next product's operand as it
 // is.  sum p c and sum p are one more product whose operand rows are the
-// blocks' c, and ones.
+// blocks' c, and ones.  64 query rows on 8 kv heads of 128 at position 1500: 13.1
+// us, 8 rows at 30000: 18.7 (2.1 TB/s); VALU-bound (9 operations unpack 8 codes,
+// 3 scale 2 weights in both parts).
 template <int NB, bool UNI>
 __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4Args a) {
     constexpr int HD = 32 * NB, PITCH = HD + 4;
@@ -824,7 +826,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_q4_narrow_kernel(Q4Args a
 // order of the scales: again the next product's operand, and one 16-byte load
 // of steps or middles.  q lies in LDS for all waves; a step's scales go
 // through LDS too, where 32 lanes read the same ones (from the caches such
-// loads would take as long as the arithmetic).
+// loads would take as long as the arithmetic).  256 tokens at 1700, 32 heads on 8
+// of 128: 28.6 us (16 rows a tile: 39.6), of which 9 start and end; a step of 32
+// x 32 takes a wave 440 VALU operations beside 37 matrix instructions (VALU 44 %,
+// matrix pipe 22 % busy at two waves per SIMD; four waves a workgroup 1.15 times
+// as long).
 constexpr int kRows32 = 32, kWaves32 = 8;
 template <int NB, bool UNI>
 __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a) {
@@ -1163,7 +1169,6 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
     const size_t out_row = static_cast<size_t>(row / a.group) * a.n_head + kh * a.group + row % a.group;
     const size_t at = out_row * n_split + blockIdx.z;
     float* dst = a.part ? a.part + at * HD : a.out + out_row * HD;
-    const float scale = a.part ? 1.0f : __fdiv_rn(1.0f, l);
 #pragma unroll
     for (int i = 0; i < NO / kWaves32; i += 4) {
         const int reg = wave * (NO / kWaves32) + i, b = reg / 16;
@@ -1176,8 +1181,10 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
         }
         // registers 4 q .. of a block: channels 8 q + 4 j2 ..; rows of the output are only known to be 4-byte aligned
         typedef f32x4 f32x4_at4 __attribute__((aligned(4)));
-        *reinterpret_cast<f32x4_at4*>(dst + 32 * b + 2 * (reg % 16) + 4 * j2) =
-            f32x4{(v[0] + c) * scale, (v[1] + c) * scale, (v[2] + c) * scale, (v[3] + c) * scale};
+        f32x4 r;  // divided as the join does it: a row has the same bits whether its call has one split or more
+#pragma unroll
+        for (int x = 0; x < 4; ++x) r[x] = a.part ? v[x] + c : __fdiv_rn(v[x] + c, l);
+        *reinterpret_cast<f32x4_at4*>(dst + 32 * b + 2 * (reg % 16) + 4 * j2) = r;
     }
     if (a.part && wave == 0 && j2 == 0) {
         float* ml = a.part + static_cast<size_t>(a.n_tokens) * a.n_head * n_split * HD + 2 * at;
@@ -1188,7 +1195,8 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
 
 // Head sizes that are not whole blocks (48: a block then belongs to two heads)
 // or have no kernel above: a workgroup per (head, token, split), a thread a row
-// for the scores, a thread a channel for the values, 256 rows at a time.
+// for the scores, a thread a channel for the values, 256 rows at a time.  Bound
+// by the unpacking, done once a head instead of once a kv head.
 constexpr int kAny = 256;
 __global__ __launch_bounds__(kAny) void attn_q4_any_kernel(Q4Args a) {
     extern __shared__ float s_q[];  // [hd] q, then [hd] sums
@@ -1284,8 +1292,8 @@ __global__ __launch_bounds__(kAny) void attn_q4_any_kernel(Q4Args a) {
 }
 
 // The splits of a row joined: weights 2^(m - max) once in LDS, four channels a
-// thread, the splits in turn over the workgroup's groups of hd / 4 threads (a
-// split's turn depends on its index alone).  Latency is all it spends: the first
+// thread, the splits in turn over the workgroup's groups of hd / 4 threads (as
+// many for any number of splits: a row's sums have one order in every chunk).  Latency is all it spends: the first
 // kAhead values of a thread are on their way before the weights are known
 // (one token at 65000: 23.5 us with the kernel before it, 24.4 with a thread a channel and no reads ahead).
 constexpr int kMaxSplit = 256, kJoin = 512, kAhead = 8;
@@ -1483,11 +1491,9 @@ hipError_t launch_attn_q4(const void* const* pt_k, const void* const* pt_v, cons
     }
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     if (splits > 1) {
-        const size_t n4 = hd / 4;  // at least a wave, at most kJoin threads
-        const size_t groups = std::max((splits + kAhead - 1) / kAhead, (63 + n4) / n4);
-        attn_q4_join_kernel<<<static_cast<unsigned>(n_tokens * n_head),
-                              dim3(static_cast<unsigned>(n4), static_cast<unsigned>(std::min(groups, kJoin / n4))), 0, st>>>(
-            a, static_cast<int>(splits));
+        const size_t n4 = hd / 4, groups = std::max(std::min<size_t>(8, kJoin / n4), (63 + n4) / n4);  // a wave at least
+        attn_q4_join_kernel<<<static_cast<unsigned>(n_tokens * n_head), dim3(static_cast<unsigned>(n4), static_cast<unsigned>(groups)),
+                              0, st>>>(a, static_cast<int>(splits));
         return hipGetLastError();
     }
     return hipSuccess;

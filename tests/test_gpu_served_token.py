@@ -269,6 +269,24 @@ def test_model_chunks_join(model_path, mode, batch):
     f.close()
 
 
+@pytest.mark.parametrize("heads,kv_heads,hd", [(8, 2, 128), (16, 4, 64), (4, 4, 96)])
+def test_model_long_chunks_join(tmp_path, heads, kv_heads, hd):
+    """The same past 512 positions, where the attention is split: a token's rows are those of any other chunk."""
+    cfg = synth.ModelConfig("q4kv-long", heads * hd, 2 * heads * hd, 2, heads, kv_heads, 512, 1400, synth.Q4_0, synth.Q4_0, synth.Q4_0)
+    path = str(tmp_path / "m.gguf")
+    synth.write_model(cfg, path, seed=6, device="cuda", digest=False)
+    m = capi.Model(path, act_mode=1, max_batch=256, kv_type=capi.MVH_KV_Q4)
+    for n, batch in ((530, 64), (1050, 64), (1300, 96)):
+        prompt = np.random.default_rng(n).integers(0, 512, n).astype(np.int32)
+        got = m.prefill(prompt, batch).copy()
+        m.reset()
+        for i in range(0, n, batch):
+            want = m.prefill(prompt[i:i + batch], batch)
+        assert np.isfinite(got).all() and (got.view(np.uint32) == want.view(np.uint32)).all(), n
+        m.reset()
+    m.close()
+
+
 @pytest.mark.parametrize("mode", [0, 1])
 def test_model_greedy(model_path, mode):
     """Greedy decoding from captured graphs gives the tokens and logits of single steps."""

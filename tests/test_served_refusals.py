@@ -32,3 +32,14 @@ def test_q4_type_name():
     assert capi.kv_type_name(capi.MVH_KV_Q4) == "q4"
     with pytest.raises(capi.MvhError, match="unknown KV cache type: q4_0"):
         capi.kv_parse_type("q4_0")
+
+
+def test_rows_in_host_tensors():
+    """A tensor in host memory is not taken for device rows."""
+    torch = pytest.importorskip("torch")
+    for rows in (torch.zeros(2, 64), torch.zeros(2, 64, dtype=torch.float16), torch.zeros(64, 2).t()):
+        with pytest.raises(ValueError, match="device"):
+            capi._rows(rows)
+    ctx = object.__new__(capi.Context)  # no device: the check comes before the call
+    with pytest.raises(ValueError, match="device memory"):
+        ctx.logprobs(torch.zeros(2, 64))
