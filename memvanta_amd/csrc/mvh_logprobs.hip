@@ -12,10 +12,10 @@
 // The most probable tokens, a tile of the row (32 elements a lane) at a time:
 // the k-th of the largest elements of 64 groups of lanes is a bound that at
 // least k elements reach, and few more (24 of 32000 random ones for k = 20);
-// what reaches it is set aside in LDS, and one wave sorts that by value,
-// then index, into the best 64 so far.  In later
-// tiles the bound is the k-th best so far.  Where too many are equal (a masked
-// row) every wave sorts its own elements 64 at a time instead.
+// what reaches it is set aside in LDS, sorted by value, then index, by the waves
+// 64 at a time, and merged by one into the best 64 so far.  In later tiles the
+// bound is the k-th best so far.  Where too many are equal (a masked row) every
+// wave sorts its own elements 64 at a time instead.
 #include "mvh_kernels.hpp"
 
 #include <type_traits>
@@ -301,9 +301,14 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(LpArgs a) {
             const int count = s_count[odd];
             if (first && wave == 0) sums();
             if (count <= kSetAside) {
+                auto sorted = [&](int c) { return sort_ascending(c + lane < count ? s_key[c + lane] : u64{0}, lane); };
+                if (count > 64) {  // 64 a wave
+                    for (int c = wave * 64; c < count; c += NT) s_key[c + lane] = sorted(c);
+                    __syncthreads();
+                }
                 if (wave == kKeyWave) {
                     for (int c = 0; c < count; c += 64) {
-                        const u64 more_keys = sort_ascending(c + lane < count ? s_key[c + lane] : u64{0}, lane);
+                        const u64 more_keys = count > 64 ? s_key[c + lane] : sorted(c);
                         best = first && !c ? key_reversed(more_keys, lane) : merge_best(best, more_keys, lane);
                     }
                 }
