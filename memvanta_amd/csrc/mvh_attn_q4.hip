@@ -393,11 +393,11 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
             u32x4 fh, fl;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const half2v s = as_half2(vs[b][i]), t = hi[i] * s;
+                const half2v s = as_half2(EDGE ? vs[b][i] & seen[i] : vs[b][i]), t = hi[i] * s;
                 half2v w = __builtin_elementwise_fma(hi[i], s, -t);
                 w = __builtin_elementwise_fma(lo[i], s, w);
-                fh[i] = EDGE ? as_u32(t) & seen[i] : as_u32(t);
-                fl[i] = EDGE ? as_u32(w) & seen[i] : as_u32(w);
+                fh[i] = as_u32(t);
+                fl[i] = as_u32(w);
             }
             o[b][0] = mfma2(__builtin_bit_cast(u32x4, q4_unpack(vn[b].x, ones)), fh, fl, o[b][0]);
             o[b][1] = mfma2(__builtin_bit_cast(u32x4, q4_unpack(vn[b].y, ones)), fh, fl, o[b][1]);
@@ -750,11 +750,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_q4_narrow_kernel(Q4Args a
                 u32x2 fh, fl;
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    const half2v s = as_half2(k ? vs[h][t].y : vs[h][t].x), x = as_half2(dh[t][k]), z = x * s;
+                    const uint32_t sv = k ? vs[h][t].y : vs[h][t].x;
+                    const half2v s = as_half2(EDGE ? sv & seen[t][k] : sv), x = as_half2(dh[t][k]), z = x * s;
                     half2v w = __builtin_elementwise_fma(x, s, -z);
                     w = __builtin_elementwise_fma(as_half2(dl[t][k]), s, w);
-                    fh[k] = EDGE ? as_u32(z) & seen[t][k] : as_u32(z);
-                    fl[k] = EDGE ? as_u32(w) & seen[t][k] : as_u32(w);
+                    fh[k] = as_u32(z);
+                    fl[k] = as_u32(w);
                 }
                 const half4v ah = __builtin_bit_cast(half4v, fh), al = __builtin_bit_cast(half4v, fl);
                 auto quads = [&](auto g_tag) {
@@ -832,8 +833,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_q4_narrow_kernel(Q4Args a
 // matrix pipe 22 % busy at two waves per SIMD; four waves a workgroup 1.15 times
 // as long).
 constexpr int kRows32 = 32, kWaves32 = 8;
-template <int NB, bool UNI>
+enum class Pages { kSteps, kGroups, kRows };  // pages of whole steps, of whole groups of 8 rows, of any number of rows
+template <int NB, Pages PAGES>
 __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a) {
+    constexpr bool UNI = PAGES == Pages::kSteps;
     constexpr int HD = 32 * NB, NO = 16 * NB, SCALES = NB * 128;  // bytes of a step's scales of K, or of V
     typedef float f32x16 __attribute__((ext_vector_type(16)));
     __shared__ __align__(16) uint8_t s_mem[kWaves32 * NO * 256 + kWaves32 * 6 * 256];
@@ -988,8 +991,12 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
         return *reinterpret_cast<const u32x4*>(s_sc + which * SCALES + (b * 4 + 2 * k + j2) * 32 + 16 * c);
     };
 
-    auto step = [&](auto edge_tag) {
-        constexpr bool EDGE = decltype(edge_tag)::value;
+    // the rows that group vg has on its page: 1 .. 8, or more
+    auto room_of = [&](int vg) { return a.map.page_tokens - (vg - a.map.page_of(vg) * groups) * 8; };
+    // EDGE: rows that some query rows do not see; PAD: pages that end inside a group, whose other slots hold anything: their
+    // scales are cleared on the way into LDS (pages of 20 rows, 256 tokens at 16000: 236 us; with every step an EDGE 354)
+    auto step = [&](auto kind_tag) {
+        constexpr bool EDGE = decltype(kind_tag)::value == 2, PAD = decltype(kind_tag)::value == 1;
         const int nst = after(st);
         u32x4 qv[2][4], ks[2][2];
         auto load_q = [&](int b, u32x4 (&v)[4], u32x4 (&s)[2]) {
@@ -1002,6 +1009,13 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
         };
         // this wave's own memory: its reads of the last step are done, and reads follow writes in order
         bool big_step = false;
+        if constexpr (PAD) {  // their steps and middles: 0
+            const int room = room_of(4 * st + sl_g), first = (sl_p & 8) / 4;  // pairs of rows (0, 4), (1, 5) or (2, 6), (7, 3)
+            const uint32_t x = (first < room ? 0xffffu : 0u) | (first + 4 < room ? 0xffff0000u : 0u);
+            const uint32_t y = first ? (7 < room ? 0xffffu : 0u) | (3 < room ? 0xffff0000u : 0u)
+                                     : (1 < room ? 0xffffu : 0u) | (5 < room ? 0xffff0000u : 0u);
+            ksc.x &= x, ksc.y &= y, vsc.x &= x, vsc.y &= y;
+        }
         if (NB == 4 || lane < 32) {
             *reinterpret_cast<uint2*>(s_sc + (sl_b * 4 + sl_g) * 32 + sl_p) = ksc;
             *reinterpret_cast<uint2*>(s_sc + SCALES + (sl_b * 4 + sl_g) * 32 + sl_p) = vsc;
@@ -1046,6 +1060,16 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
         add(xs[(NB - 1) & 1], ks[(NB - 1) & 1]);
         // rows that a query row does not see: p = 0, whatever is stored there
         uint32_t seen[2][4], seen_c[2][4];
+        if constexpr (PAD) {
+            const int order[8] = {0, 4, 1, 5, 2, 6, 7, 3};
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int room = room_of(4 * st + 2 * k + j2);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (order[i] >= room) sc[8 * k + i] = -INFINITY;
+            }
+        }
         if constexpr (EDGE) {
             const int order[8] = {0, 4, 1, 5, 2, 6, 7, 3};
 #pragma unroll
@@ -1122,11 +1146,11 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
                 u32x4 fh, fl;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const half2v z = as_half2(s[i]), x = as_half2(ph[k][i]), t = x * z;
+                    const half2v z = as_half2(EDGE ? s[i] & seen[k][i] : s[i]), x = as_half2(ph[k][i]), t = x * z;
                     half2v w = __builtin_elementwise_fma(x, z, -t);
                     w = __builtin_elementwise_fma(as_half2(pl[k][i]), z, w);
-                    fh[i] = EDGE ? as_u32(t) & seen[k][i] : as_u32(t);
-                    fl[i] = EDGE ? as_u32(w) & seen[k][i] : as_u32(w);
+                    fh[i] = as_u32(t);
+                    fl[i] = as_u32(w);
                 }
                 const u32x4 w = __builtin_bit_cast(u32x4, q4_unpack(vn[b][k], ones));
                 o[b] = mfma(w, fl, o[b]);
@@ -1138,10 +1162,10 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
         next_v = page_of_step(a.pt_v, after(nst));
         __builtin_amdgcn_wave_barrier();
     };
-    // steps that every query row sees whole; none where pages end inside a group
-    const int full = a.map.page_tokens & 7 ? 0 : (first_lim + 1) / 32;
-    for (; st < min(end, full); st += kWaves32) step(std::false_type{});
-    for (; st < end; st += kWaves32) step(std::true_type{});
+    // steps that every query row sees whole, then the others
+    const int full = min(end, a.map.group_of(first_lim + 1) / 4);
+    for (; st < full; st += kWaves32) step(std::integral_constant<int, PAGES == Pages::kRows ? 1 : 0>{});
+    for (; st < end; st += kWaves32) step(std::integral_constant<int, 2>{});
 
     // the waves joined: every wave's sums by register and lane, then each wave a quarter of the registers
     __syncthreads();
@@ -1466,11 +1490,14 @@ hipError_t launch_attn_q4(const void* const* pt_k, const void* const* pt_v, cons
     }
     case Q4Kind::kTile32: {
         const dim3 grid(static_cast<unsigned>(n_head_kv), static_cast<unsigned>((n_tokens * a.group + kRows32 - 1) / kRows32), z);
-        const bool uni = page_tokens % 32 == 0;
-        if (hd == 128 && uni) attn_q4_tile_kernel<4, true><<<grid, 64 * kWaves32, 0, st>>>(a);
-        else if (hd == 128) attn_q4_tile_kernel<4, false><<<grid, 64 * kWaves32, 0, st>>>(a);
-        else if (uni) attn_q4_tile_kernel<2, true><<<grid, 64 * kWaves32, 0, st>>>(a);
-        else attn_q4_tile_kernel<2, false><<<grid, 64 * kWaves32, 0, st>>>(a);
+        auto launch = [&](auto pages) {
+            constexpr Pages P = decltype(pages)::value;
+            if (hd == 128) attn_q4_tile_kernel<4, P><<<grid, 64 * kWaves32, 0, st>>>(a);
+            else attn_q4_tile_kernel<2, P><<<grid, 64 * kWaves32, 0, st>>>(a);
+        };
+        if (page_tokens % 32 == 0) launch(std::integral_constant<Pages, Pages::kSteps>{});
+        else if (page_tokens % 8 == 0) launch(std::integral_constant<Pages, Pages::kGroups>{});
+        else launch(std::integral_constant<Pages, Pages::kRows>{});
         break;
     }
     case Q4Kind::kTile16: {

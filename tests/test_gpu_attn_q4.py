@@ -149,6 +149,23 @@ def test_rows_past_the_position_do_not_count(ctx, hd, page):
     assert np.isnan(outs[2][20:]).all()
 
 
+@pytest.mark.parametrize("hd,page", [(128, 20), (64, 20), (128, 9), (64, 33)])
+def test_slots_behind_a_page(ctx, hd, page):
+    """Pages that end inside a group of 8: what the group's other slots hold (here memory that held NaN) does not count."""
+    rng = np.random.default_rng(page)
+    n_kv, rows = 2, 1800
+    bad = ctx.kv_cache(1, n_kv * hd, 128, 4 * rows, kv_type=capi.MVH_KV_Q4)
+    x = np.full((4 * rows, n_kv * hd), np.nan, np.float32)
+    bad.write(0, 0, x, x)
+    bad.close()
+    kv, k, v = _case(ctx, rng, n_kv, hd, page, rows)
+    for group, pos, n in ((1, rows - 1, 1), (4, rows - 5, 1), (8, 700, 3), (4, 1500, 200), (4, 1700, 100)):
+        q = rng.standard_normal((n, group * n_kv, hd), dtype=np.float32) * np.float32(1.5)
+        got = kv.attn_batch(0, q.reshape(n, -1), pos, n, group * n_kv, n_kv, hd).reshape(q.shape)
+        _check(got, attend(q, k, v, pos, group), (group, pos, n))
+    kv.close()
+
+
 @pytest.mark.parametrize("hd", [128, 48])
 def test_bad_rows_stay_with_their_head(ctx, hd):
     """A NaN in one kv head's row makes that head's outputs NaN from there on, and no other's (blocks of 32 at hd 48 hold
