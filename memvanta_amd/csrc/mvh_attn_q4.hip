@@ -12,6 +12,7 @@
 #include "mvh_kernels.hpp"
 #include "mvh_kv4.hpp"
 
+#include <numeric>
 #include <type_traits>
 
 namespace mvh {
@@ -133,13 +134,21 @@ __device__ __forceinline__ void write_sum(const Q4Args& a, int kh, int row, int 
 // blocks' c, and ones.  64 query rows on 8 kv heads of 128 at position 1500: 13.1
 // us, 8 rows at 30000: 18.7 (2.1 TB/s); VALU-bound (9 operations unpack 8 codes,
 // 3 scale 2 weights in both parts).
-template <int NB, bool UNI>
+//
+// PART: heads that do not fill NB whole blocks.  A head's channels lie in the
+// blocks from its first one on, with q zero at the others' channels of these
+// (6 heads of 48 at position 1500: 9.4 us, 64 tokens there 12.0; on the kernel
+// for heads of more than 8 blocks 35.5 and 192).
+template <int NB, bool UNI, bool PART>
 __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4Args a) {
     constexpr int HD = 32 * NB, PITCH = HD + 4;
     __shared__ float s_o[kWaves][kTile][PITCH];
     __shared__ float s_c[kWaves][kTile][12];  // [0..NB) sum p c of the blocks, [NB] sum p
     __shared__ float s_m[kWaves][kTile];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, j = lane >> 4;
+    // the head's first block, its first channel there, the blocks it lies in
+    const int hd = PART ? a.hd : HD, b0 = PART ? blockIdx.x * hd / 32 : blockIdx.x * NB, shift = PART ? blockIdx.x * hd % 32 : 0;
+    const int nb = PART ? (shift + hd + 31) / 32 : NB;
     const int kh = blockIdx.x, row0 = blockIdx.y * kTile, rows = a.n_tokens * a.group;
     const int pos = a.d_pos ? *a.d_pos : a.pos;
     const int tile_lim = pos + (min(row0 + kTile, rows) - 1) / a.group, first_lim = pos + row0 / a.group;
@@ -149,14 +158,14 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
 
     const int groups = a.map.groups, last_group = a.map.group_of(tile_lim);
     const size_t sc_off = kv4_scales(a.map.page_tokens, a.kv_dim);
-    const size_t n_head_off = static_cast<size_t>(kh * NB) * groups * 128, s_head_off = sc_off + static_cast<size_t>(kh * NB) * groups * 32;
+    const size_t n_head_off = static_cast<size_t>(b0) * groups * 128, s_head_off = sc_off + static_cast<size_t>(b0) * groups * 32;
     const size_t n_blk = static_cast<size_t>(groups) * 128, s_blk = static_cast<size_t>(groups) * 32;
     const uint32_t kn_lane = (col >> 2) * 128 + (j * 4 + (col & 3)) * 8, vn_lane = j * 128 + col * 8, s_lane = j * 32;
-    const uint32_t vc_lane = static_cast<uint32_t>(min(col, NB - 1)) * static_cast<uint32_t>(s_blk) + j * 32 + 16;
+    const uint32_t vc_lane = static_cast<uint32_t>(min(col, nb - 1)) * static_cast<uint32_t>(s_blk) + j * 32 + 16;
     uint32_t kc_lane[(NB + 3) / 4];
 #pragma unroll
     for (int k = 0; k < (NB + 3) / 4; ++k)
-        kc_lane[k] = static_cast<uint32_t>(min(j + 4 * k, NB - 1)) * static_cast<uint32_t>(s_blk) + (col >> 2) * 32 + 16 + (col & 3) * 4;
+        kc_lane[k] = static_cast<uint32_t>(min(j + 4 * k, nb - 1)) * static_cast<uint32_t>(s_blk) + (col >> 2) * 32 + 16 + (col & 3) * 4;
 
     // the page of group g (of 4) of step st, and the group's index there (UNI: whole steps lie in a page)
     auto locate = [&](const void* const* pt, int st, int g, const uint8_t*& base, int& at) {
@@ -171,11 +180,12 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
     auto load_k = [&](const uint8_t* page, int st) {
         if constexpr (UNI) {
             const int g0 = 4 * st - a.map.page_of(4 * st) * groups;
-            const uint8_t* nb = page + n_head_off + static_cast<size_t>(g0) * 128;
+            const uint8_t* words = page + n_head_off + static_cast<size_t>(g0) * 128;
             const uint8_t* sb = page + s_head_off + static_cast<size_t>(g0) * 32;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                kn[b] = ld8_at(nb + b * n_blk, kn_lane);
+                if (PART && b >= nb) continue;
+                kn[b] = ld8_at(words + b * n_blk, kn_lane);
                 ks[b] = ld16_at(sb + b * s_blk, s_lane);
             }
 #pragma unroll
@@ -187,22 +197,24 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
             locate(a.pt_k, st, j, bs, gs);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
+                if (PART && b >= nb) continue;
                 kn[b] = ld8_at(bn + n_head_off + b * n_blk + static_cast<size_t>(gn) * 128, (j * 4 + (col & 3)) * 8);
                 ks[b] = ld16_at(bs + s_head_off + b * s_blk + static_cast<size_t>(gs) * 32, 0);
             }
 #pragma unroll
             for (int k = 0; k < NQ; ++k)
-                kc[k] = ld4_at(bn + s_head_off + min(j + 4 * k, NB - 1) * s_blk + static_cast<size_t>(gn) * 32, 16 + (col & 3) * 4);
+                kc[k] = ld4_at(bn + s_head_off + min(j + 4 * k, nb - 1) * s_blk + static_cast<size_t>(gn) * 32, 16 + (col & 3) * 4);
         }
     };
     auto load_v = [&](const uint8_t* page, int st) {
         if constexpr (UNI) {
             const int g0 = 4 * st - a.map.page_of(4 * st) * groups;
-            const uint8_t* nb = page + n_head_off + static_cast<size_t>(g0) * 128;
+            const uint8_t* words = page + n_head_off + static_cast<size_t>(g0) * 128;
             const uint8_t* sb = page + s_head_off + static_cast<size_t>(g0) * 32;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                vn[b] = ld8_at(nb + b * n_blk, vn_lane);
+                if (PART && b >= nb) continue;
+                vn[b] = ld8_at(words + b * n_blk, vn_lane);
                 vs[b] = ld16_at(sb + b * s_blk, s_lane);
             }
             vc = ld16_at(sb, vc_lane);
@@ -212,10 +224,11 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
             locate(a.pt_v, st, j, base, g);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
+                if (PART && b >= nb) continue;
                 vn[b] = ld8_at(base + n_head_off + b * n_blk + static_cast<size_t>(g) * 128, col * 8);
                 vs[b] = ld16_at(base + s_head_off + b * s_blk + static_cast<size_t>(g) * 32, 0);
             }
-            vc = ld16_at(base + s_head_off + min(col, NB - 1) * s_blk + static_cast<size_t>(g) * 32, 16);
+            vc = ld16_at(base + s_head_off + min(col, nb - 1) * s_blk + static_cast<size_t>(g) * 32, 16);
         }
     };
     auto page_of_step = [&](const void* const* pt, int st) -> const uint8_t* {
@@ -231,7 +244,7 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
 
     // q: lane (col, j) holds channels 8 j .. of each block of row col; scaled by a power of two to [1, 2)
     const int r = min(row0 + col, rows - 1), lim = pos + r / a.group;
-    const float* qr = a.q + static_cast<size_t>(r / a.group) * a.q_pitch + static_cast<size_t>(kh * a.group + r % a.group) * HD;
+    const float* qr = a.q + static_cast<size_t>(r / a.group) * a.q_pitch + static_cast<size_t>(kh * a.group + r % a.group) * hd - shift;
     // masks and constants that the compiler is not to see: as selects and literals they take more operations
     uint32_t c_mask = col < NB ? 0xffffffffu : 0u, c_fill = col == NB ? 0x3c003c00u : 0u;  // ones: sum p
     float minus1 = -1.0f;
@@ -249,16 +262,18 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
         float f[NB][8], top = 0.0f;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
+            const int c = 32 * b + 8 * j;
+            const bool own = !PART || (c >= shift && c < shift + hd);  // both are multiples of 8
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                f[b][i] = qr[32 * b + 8 * j + i];
+                f[b][i] = own ? qr[c + i] : 0.0f;
                 top = fmaxf(top, fabsf(f[b][i]));
             }
         }
         top = rows_max(top);
         const int e = top > 0.0f && top <= 3.402823466e38f ? max(__builtin_amdgcn_frexp_expf(top) - 1, -120) : 0;
         const float down = ldexpf(1.0f, -e);
-        y_scale = ldexpf(__fdiv_rn(kLog2e, sqrt_rn(static_cast<float>(HD))), e);
+        y_scale = ldexpf(__fdiv_rn(kLog2e, sqrt_rn(static_cast<float>(hd))), e);
         float mine[NQ];
 #pragma unroll
         for (int k = 0; k < NQ; ++k) mine[k] = 0.0f;
@@ -320,6 +335,7 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
         }
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
+            if (PART && b >= nb) continue;
             const f32x4 c0 = mfma2(__builtin_bit_cast(u32x4, q4_unpack(kn[b].x, ones)), qh[b], ql[b], zero);
             const f32x4 c1 = mfma2(__builtin_bit_cast(u32x4, q4_unpack(kn[b].y, ones)), qh[b], ql[b], zero);
 #pragma unroll
@@ -356,7 +372,8 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
         for (int i = 0; i < 4; ++i) {
             uint32_t w = 0;
 #pragma unroll
-            for (int b = 0; b < NB; ++b) w |= vs[b][i];
+            for (int b = 0; b < NB; ++b)
+                if (!PART || b < nb) w |= vs[b][i];
             big |= EDGE ? w & seen[i] : w;
         }
         big &= 0x40004000u;
@@ -389,6 +406,7 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
         oc = mfma2(cf, ph, pl, oc);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
+            if (PART && b >= nb) continue;
             // p s in two parts: hi s rounded, and what that lost plus lo s
             u32x4 fh, fl;
 #pragma unroll
@@ -435,7 +453,7 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
             sum = fmaf(f, s_o[w][c][d] + s_c[w][c][d / 32], sum);
             l = fmaf(f, s_c[w][c][NB], l);
         }
-        write_sum(a, kh, row, d, HD, n_split, sum, l, top);
+        if (!PART || (d >= shift && d < shift + hd)) write_sum(a, kh, row, d - shift, hd, n_split, sum, l, top);
     }
 }
 
@@ -1217,8 +1235,7 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
     }
 }
 
-// Head sizes that are not whole blocks (48: a block then belongs to two heads)
-// or have no kernel above: a workgroup per (head, token, split), a thread a row
+// Heads of more than 8 blocks: a workgroup per (head, token, split), a thread a row
 // for the scores, a thread a channel for the values, 256 rows at a time.  Bound
 // by the unpacking, done once a head instead of once a kv head.
 constexpr int kAny = 256;
@@ -1388,7 +1405,9 @@ __global__ __launch_bounds__(kJoin) void attn_q4_join_kernel(Q4Args a, int n_spl
     }
 }
 
-bool q4_tiles(size_t hd) { return hd % 32 == 0 && (hd <= 128 || hd == 192 || hd == 256); }
+// The most blocks of 32 channels that a head lies in: it starts at any multiple of the greatest common divisor
+size_t q4_cover(size_t hd) { return (hd + 32 - std::gcd(hd, size_t{32}) + 31) / 32; }
+bool q4_tiles(size_t hd) { return q4_cover(hd) <= 8; }
 
 // Which kernel takes a call.  A chunk of fixed splits is to give a token the
 // bits it has in any other chunk: one kernel for all (the tiles of 32 rows, where
@@ -1435,8 +1454,12 @@ size_t q4_splits(size_t max_pos, size_t n_tokens, size_t n_head, size_t n_head_k
 
 template <int NB>
 void q4_launch(const Q4Args& a, dim3 grid, hipStream_t st) {
-    if (a.map.page_tokens % 32 == 0) attn_q4_kernel<NB, true><<<grid, 64 * kWaves, 0, st>>>(a);
-    else attn_q4_kernel<NB, false><<<grid, 64 * kWaves, 0, st>>>(a);
+    auto launch = [&](auto uni) {
+        if (a.hd == 32 * NB) attn_q4_kernel<NB, decltype(uni)::value, false><<<grid, 64 * kWaves, 0, st>>>(a);
+        else attn_q4_kernel<NB, decltype(uni)::value, true><<<grid, 64 * kWaves, 0, st>>>(a);
+    };
+    if (a.map.page_tokens % 32 == 0) launch(std::true_type{});
+    else launch(std::false_type{});
 }
 
 }  // namespace
@@ -1502,11 +1525,12 @@ hipError_t launch_attn_q4(const void* const* pt_k, const void* const* pt_v, cons
     }
     case Q4Kind::kTile16: {
         const dim3 grid(static_cast<unsigned>(n_head_kv), static_cast<unsigned>((n_tokens * a.group + kTile - 1) / kTile), z);
-        switch (hd / 32) {
+        switch (q4_cover(hd)) {
         case 1: q4_launch<1>(a, grid, st); break;
         case 2: q4_launch<2>(a, grid, st); break;
         case 3: q4_launch<3>(a, grid, st); break;
         case 4: q4_launch<4>(a, grid, st); break;
+        case 5:
         case 6: q4_launch<6>(a, grid, st); break;
         default: q4_launch<8>(a, grid, st); break;
         }

@@ -29,11 +29,13 @@ def _check(got, want, what):
     assert abs(got - want).max() <= 40 * REL * max(rms, abs(want).max()), what
 
 
-# head_dims of one block to eight, part blocks (48, 40, 80: blocks shared by heads) and no kernel of their own (160);
+# head_dims of one block to eight, parts of blocks (48, 40, 24 ..: blocks shared by heads), more than eight blocks (288);
 # groups of 1 to 12 heads; pages of 1 row, no whole groups, whole groups, whole steps
 @pytest.mark.parametrize("n_head,n_kv,hd,page", [(8, 1, 64, 128), (4, 4, 128, 128), (2, 2, 32, 7), (6, 2, 96, 64), (6, 6, 48, 16),
                                                  (32, 4, 64, 20), (2, 1, 192, 32), (2, 1, 256, 8), (24, 2, 32, 1),
-                                                 (5, 1, 128, 96), (4, 4, 40, 9), (2, 2, 80, 128), (2, 1, 160, 128)])
+                                                 (5, 1, 128, 96), (4, 4, 40, 9), (2, 2, 80, 128), (2, 1, 160, 128),
+                                                 (8, 8, 24, 128), (8, 4, 72, 20), (2, 2, 112, 32), (4, 4, 56, 16), (4, 4, 8, 128),
+                                                 (4, 2, 16, 5), (1, 1, 224, 128), (2, 1, 288, 128)])
 def test_decode(ctx, n_head, n_kv, hd, page):
     rng = np.random.default_rng(hd + page + n_head)
     kv, k, v = _case(ctx, rng, n_kv, hd, page, 1100)
@@ -45,7 +47,8 @@ def test_decode(ctx, n_head, n_kv, hd, page):
 
 
 @pytest.mark.parametrize("n_head,n_kv,hd,page", [(8, 2, 64, 128), (4, 4, 128, 16), (12, 1, 32, 7), (6, 6, 48, 128),
-                                                 (32, 8, 128, 128), (3, 3, 256, 20), (4, 2, 96, 1)])
+                                                 (32, 8, 128, 128), (3, 3, 256, 20), (4, 2, 96, 1),
+                                                 (8, 8, 24, 16), (16, 4, 72, 128), (4, 4, 56, 20), (2, 1, 160, 128), (2, 1, 288, 16)])
 def test_batch(ctx, n_head, n_kv, hd, page):
     rng = np.random.default_rng(hd + page + n_head + 1)
     kv, k, v = _case(ctx, rng, n_kv, hd, page, 400)
