@@ -40,11 +40,23 @@ struct Q4Args {
 
 constexpr float kLowest = -1.0e12f;  // m before the first row: finite, so that 2^(-inf - m) is 0; scores stay above it
 constexpr float kLog2e = 1.44269504088896340736f;
-// Weights are 2^(y - m + lift), and m follows the maximum only when that is
+// Weights are 2^(y - m + kLift), and m follows the maximum only when that is
 // kSlack ahead (the sums are rescaled seldom, the decision is each row's own): at
-// most 2^(lift + kSlack), so that p s stays clear of both ends of fp16 with lift
-// 10 while every step s seen is below 2, then 2 (s <= 512).
-constexpr float kLift = 10.0f, kLiftBig = 2.0f, kSlack = 4.0f;
+// most 2^14.  fp16 keeps 22 bits of such a weight in two parts down to 2^-12 of
+// the largest, and 2^-35 of the largest below.
+//
+// p s keeps that range only where a block's steps are near 1.  So a block's sums
+// are held times a power of two u, by the largest step that the query row has
+// seen there (unit_of): 1 while that is in [2^-7, 2), else what brings it to [1/2,
+// 1); it falls, and the sums with it, when a step times u reaches 2.  u >= 1
+// scales the steps, exactly; blocks with u < 1 (a step of 2 .. 512) form p s u in
+// 32 bits and split it.  p s u is below 2^15, and off by 2^-22 of itself or 2^-35
+// of the largest weight times the block's largest step, whatever other blocks
+// hold.  A wave's first step looks whether all its blocks start with u = 1; while
+// they stay there, the usual case, steps are taken as they are.
+constexpr float kLift = 10.0f, kSlack = 4.0f;
+constexpr uint32_t kUnitOne = 0x3c00u, kUnitFirst = 30u << 10;  // 1, and 2^15: before any step
+constexpr uint32_t kUsualBits = 0x60006000u, kWideBits = 0x40004000u;  // of a step >= 2^-7, >= 2 (or NaN), in either half
 constexpr int kWaves = 4;
 constexpr int kTile = 16;  // query rows of a workgroup
 
@@ -69,6 +81,32 @@ __device__ __forceinline__ float rows_sum(float v) {
     auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
+
+__device__ __forceinline__ uint32_t rows_max_bits(uint32_t v) {
+    auto a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = max(a[0], a[1]);
+    auto b = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return max(b[0], b[1]);
+}
+
+// u of a block whose largest step has these bits (NaN: as the largest step there is)
+__device__ __forceinline__ uint32_t unit_of(uint32_t step) {
+    const uint32_t e = min(step >> 10, 24u);
+    return e >= 8 && e < 16 ? kUnitOne : (29 - e) << 10;
+}
+// a step times u that is 2 or more, or NaN, shows in bit 14 of its half
+__device__ __forceinline__ uint32_t reaches_2(uint32_t steps, half2v u) { return as_u32(as_half2(steps) * u) & kWideBits; }
+__device__ __forceinline__ half2v both(uint32_t u) { return as_half2(u | (u << 16)); }
+__device__ __forceinline__ bool below_1(half2v u) { return (as_u32(u) & 0xffffu) < kUnitOne; }
+__device__ __forceinline__ float unit_f(half2v u) { return static_cast<float>(u.x); }
+__device__ __forceinline__ float unit_inverse(half2v u) {  // of a power of two
+    return __uint_as_float((254u << 23) - __float_as_uint(unit_f(u)));
+}
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t max_halves(uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+__device__ __forceinline__ uint32_t max_half(uint32_t a) { return max(a & 0xffffu, a >> 16); }
 
 // Loads at a base that is the same in every lane plus a 32-bit offset: the base
 // stays in scalar registers.
@@ -105,6 +143,22 @@ __device__ __forceinline__ f32x4 mfma2(u32x4 a, u32x4 high, u32x4 low, f32x4 c) 
 }
 // p - h (exact where h is p rounded, or 0): the conversion inside the addition
 __device__ __forceinline__ float less(float p, _Float16 h, float minus1) { return fmaf(static_cast<float>(h), minus1, p); }
+
+// Two weights (in two parts each) times their steps, in two parts: the product rounded, and what that lost plus lo s
+__device__ __forceinline__ void times_steps(half2v hi, half2v lo, half2v s, uint32_t& h, uint32_t& l) {
+    const half2v t = hi * s;
+    half2v w = __builtin_elementwise_fma(hi, s, -t);
+    w = __builtin_elementwise_fma(lo, s, w);
+    h = as_u32(t);
+    l = as_u32(w);
+}
+// Two weights times their steps and u in 32 bits, in two parts
+__device__ __forceinline__ void times_steps(float p, float q, half2v s, float u, float minus1, uint32_t& h, uint32_t& l) {
+    const float x = p * static_cast<float>(s.x) * u, y = q * static_cast<float>(s.y) * u;
+    const half2v t = pk_half(x, y);
+    h = as_u32(t);
+    l = as_u32(pk_half(less(x, t.x, minus1), less(y, t.y, minus1)));
+}
 
 // A workgroup's result for channel d of query row `row`: the output, or the split's part of it
 __device__ __forceinline__ void write_sum(const Q4Args& a, int kh, int row, int d, int hd, int n_split, float sum, float l, float top) {
@@ -145,6 +199,7 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
     __shared__ float s_o[kWaves][kTile][PITCH];
     __shared__ float s_c[kWaves][kTile][12];  // [0..NB) sum p c of the blocks, [NB] sum p
     __shared__ float s_m[kWaves][kTile];
+    __shared__ uint32_t s_unit[kWaves][NB][kTile];  // u of the blocks, twice: seldom looked at, so not in registers
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, j = lane >> 4;
     // the head's first block, its first channel there, the blocks it lies in
     const int hd = PART ? a.hd : HD, b0 = PART ? blockIdx.x * hd / 32 : blockIdx.x * NB, shift = PART ? blockIdx.x * hd % 32 : 0;
@@ -304,12 +359,16 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
     f32x4 o[NB][2], oc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int b = 0; b < NB; ++b) o[b][0] = o[b][1] = oc;
-    float m = kLowest, lift = kLift;  // m: of the scores before y_scale
+    float m = kLowest;  // of the scores before y_scale
+    bool uneven = false;  // in the wave: a u that is not 1
+    auto unit = [&](int b) { return uneven ? as_half2(s_unit[wave][b][col]) : both(kUnitOne); };
+    uint32_t wide = 0;    // a u below 1, by block
     const uint32_t c_turn = (col & 3) == 3 ? 16 : 0;  // rows 3 and 7 are stored the other way round
 
     const u32x4 zero_words = {0u, 0u, 0u, 0u};
     auto step = [&](auto edge_tag) {
         constexpr bool EDGE = decltype(edge_tag)::value;
+        const bool fresh = st == begin + wave;
         const uint8_t *next_k = nullptr, *next_v = nullptr;
         const bool more = st + kWaves < end;
         if (more) {
@@ -366,59 +425,131 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
 #pragma unroll
         for (int i = 0; i < 4; ++i) mx = fmaxf(fmaxf(mx, s0[i]), s1[i]);
         mx = rows_max(mx);
-        // a step of 2 and more (fp16 bit 14) among the rows that the query row sees
+        // steps that the query row sees
+        auto steps = [&](int b, int i) { return EDGE ? vs[b][i] & seen[i] : vs[b][i]; };
+        // one that reaches 2 with its block's u
         uint32_t big = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t w = 0;
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-                if (!PART || b < nb) w |= vs[b][i];
-            big |= EDGE ? w & seen[i] : w;
-        }
-        big &= 0x40004000u;
-        if (__any((mx - m) * y_scale > kSlack || (big && lift == kLift))) {
-            const float top = (mx - m) * y_scale > kSlack ? mx : m, down = rows_max(big ? 1.0f : 0.0f) > 0.0f ? kLiftBig : lift;
-            const float f = __builtin_amdgcn_exp2f(fmaf(m - top, y_scale, down - lift));
-            m = top;
-            lift = down;
-            oc *= f;
+        if (uneven) {
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                o[b][0] *= f;
-                o[b][1] *= f;
+                if (PART && b >= nb) continue;
+                const half2v u = unit(b);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) big |= reaches_2(steps(b, i), u);
             }
-        }
-        const float below = fmaf(-m, y_scale, lift);
-        half2v hi[4], lo[4];
-        u32x4 ph, pl, cf;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float p0 = __builtin_amdgcn_exp2f(fmaf(s0[i], y_scale, below)), p1 = __builtin_amdgcn_exp2f(fmaf(s1[i], y_scale, below));
-            uint32_t h, l;
-            part(i < 3 ? p0 : p1, i < 3 ? p1 : p0, h, l);
-            ph[i] = h;
-            pl[i] = l;
-            hi[i] = as_half2(h);
-            lo[i] = as_half2(l);
-            cf[i] = ((EDGE ? vc[i] & seen_c[i] : vc[i]) & c_mask) | c_fill;
-        }
-        oc = mfma2(cf, ph, pl, oc);
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            if (PART && b >= nb) continue;
-            // p s in two parts: hi s rounded, and what that lost plus lo s
-            u32x4 fh, fl;
+        } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const half2v s = as_half2(EDGE ? vs[b][i] & seen[i] : vs[b][i]), t = hi[i] * s;
-                half2v w = __builtin_elementwise_fma(hi[i], s, -t);
-                w = __builtin_elementwise_fma(lo[i], s, w);
-                fh[i] = as_u32(t);
-                fl[i] = as_u32(w);
+                uint32_t w = 0;
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+                    if (!PART || b < nb) w |= vs[b][i];
+                big |= EDGE ? w & seen[i] : w;
             }
-            o[b][0] = mfma2(__builtin_bit_cast(u32x4, q4_unpack(vn[b].x, ones)), fh, fl, o[b][0]);
-            o[b][1] = mfma2(__builtin_bit_cast(u32x4, q4_unpack(vn[b].y, ones)), fh, fl, o[b][1]);
+            big &= kWideBits;
+        }
+        // a row that sees nothing here sees nothing later
+        auto blind = [&] {
+            const int page = a.map.page_of(4 * st);
+            return EDGE && lim < page * a.map.page_tokens + (4 * st - page * groups) * 8;
+        };
+        bool small = false;  // the first step has a block with none of 2^-7 or more
+        if (fresh) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                if (PART && b >= nb) continue;
+                uint64_t rows_with = __ballot(((steps(b, 0) | steps(b, 1) | steps(b, 2) | steps(b, 3)) & kUsualBits) || blind());
+                rows_with |= rows_with >> 32;
+                rows_with |= rows_with >> 16;
+                small = small || (rows_with & 0xffff) != 0xffff;
+            }
+        }
+        const bool ahead = (mx - m) * y_scale > kSlack;
+        if (small || __any(ahead || big)) {
+            const float top = ahead ? mx : m, f = __builtin_amdgcn_exp2f((m - top) * y_scale);
+            m = top;
+            oc *= f;
+            if (small || __any(big)) {
+                wide = 0;
+                uint32_t other = 0;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    if (PART && b >= nb) continue;
+                    uint32_t most = max_half(max_halves(max_halves(steps(b, 0), steps(b, 1)), max_halves(steps(b, 2), steps(b, 3))));
+                    most = rows_max_bits(most);
+                    const half2v was = fresh ? both(blind() ? kUnitOne : kUnitFirst) : unit(b);
+                    const half2v u = reaches_2(most, was) ? both(unit_of(most)) : was;
+                    s_unit[wave][b][col] = as_u32(u);
+                    const float g = f * unit_f(u) * unit_inverse(was);
+                    o[b][0] *= g;
+                    o[b][1] *= g;
+                    other |= (as_u32(u) & 0xffffu) ^ kUnitOne;
+                    if (__any(below_1(u))) wide |= 1u << b;
+                }
+                uneven = __any(other);
+            } else {
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    o[b][0] *= f;
+                    o[b][1] *= f;
+                }
+            }
+        }
+        const float below = fmaf(-m, y_scale, kLift);
+        if (uneven) {
+            float scale = y_scale;
+            asm("" : "+v"(scale));  // or the weights are formed for both here, apart from the products below
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                if (PART && b >= nb) continue;
+                const half2v u = unit(b);
+                if (wide >> b & 1) {
+                    u32x4 fh, fl;
+                    const float uw = below_1(u) ? unit_f(u) : 0.0f;  // the other query rows' below
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float p0 = __builtin_amdgcn_exp2f(fmaf(s0[i], scale, below)), p1 = __builtin_amdgcn_exp2f(fmaf(s1[i], scale, below));
+                        uint32_t h, l;
+                        times_steps(i < 3 ? p0 : p1, i < 3 ? p1 : p0, as_half2(steps(b, i)), uw, minus1, h, l);
+                        fh[i] = h;
+                        fl[i] = l;
+                    }
+                    o[b][0] = mfma2(__builtin_bit_cast(u32x4, q4_unpack(vn[b].x, ones)), fh, fl, o[b][0]);
+                    o[b][1] = mfma2(__builtin_bit_cast(u32x4, q4_unpack(vn[b].y, ones)), fh, fl, o[b][1]);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) vs[b][i] = below_1(u) ? 0u : as_u32(as_half2(steps(b, i)) * u);
+            }
+        }
+        {
+            half2v hi[4], lo[4];
+            u32x4 ph, pl, cf;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(s0[i], y_scale, below)), p1 = __builtin_amdgcn_exp2f(fmaf(s1[i], y_scale, below));
+                uint32_t h, l;
+                part(i < 3 ? p0 : p1, i < 3 ? p1 : p0, h, l);
+                ph[i] = h;
+                pl[i] = l;
+                hi[i] = as_half2(h);
+                lo[i] = as_half2(l);
+                cf[i] = ((EDGE ? vc[i] & seen_c[i] : vc[i]) & c_mask) | c_fill;
+            }
+            oc = mfma2(cf, ph, pl, oc);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                if (PART && b >= nb) continue;
+                u32x4 fh, fl;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t h, l;
+                    times_steps(hi[i], lo[i], as_half2(steps(b, i)), h, l);
+                    fh[i] = h;
+                    fl[i] = l;
+                }
+                o[b][0] = mfma2(__builtin_bit_cast(u32x4, q4_unpack(vn[b].x, ones)), fh, fl, o[b][0]);
+                o[b][1] = mfma2(__builtin_bit_cast(u32x4, q4_unpack(vn[b].y, ones)), fh, fl, o[b][1]);
+            }
         }
         if (more) load_v(next_v, st + kWaves);
     };
@@ -430,16 +561,17 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
     // the waves joined
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
+        const float inverse = unit_inverse(unit(b));
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const f32x4 v = o[b][h];
+            const f32x4 v = o[b][h] * inverse;
             *reinterpret_cast<float4*>(&s_o[wave][col][32 * b + 16 * h + 4 * j]) = make_float4(v[0], v[1], v[2], v[3]);
         }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         if (4 * j + i <= NB) s_c[wave][col][4 * j + i] = oc[i];
-    if (lane < kTile) s_m[wave][lane] = fmaf(m, y_scale, -lift);
+    if (lane < kTile) s_m[wave][lane] = fmaf(m, y_scale, -kLift);
     __syncthreads();
     for (int idx = threadIdx.x; idx < kTile * HD; idx += 64 * kWaves) {
         const int c = idx / HD, d = idx % HD, row = row0 + c;
@@ -634,11 +766,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_q4_narrow_kernel(Q4Args a
     for (int h = 0; h < NH; ++h) oh[h] = ol[h] = zero;
 #pragma unroll
     for (int k = 0; k < NQuad<NB>::value; ++k) oc[k] = zero;
-    float m = kLowest, l = 0.0f, lift = kLift;
+    float m = kLowest, l = 0.0f;
+    half2v unit[NH];  // u, twice, of the lane's block (2 h + half32) for query row `head`
+#pragma unroll
+    for (int h = 0; h < NH; ++h) unit[h] = both(kUnitOne);
+    bool uneven = false;  // in the wave: a u that is not 1
+    uint32_t wide = 0;    // a u below 1, by pair of blocks
 
     auto step = [&](auto edge_tag) {
         constexpr bool EDGE = decltype(edge_tag)::value;
-        const bool more = it + kWaves < it_end;
+        const bool more = it + kWaves < it_end, fresh = it == begin / 2 + wave;
         const uint8_t *next_k = nullptr, *next_v = nullptr;
         if (more) {
             next_k = page_of_it(a.pt_k, it + kWaves);
@@ -705,90 +842,175 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_q4_narrow_kernel(Q4Args a
         mx = fmaxf(mx, dpp_mov<0x124>(mx));  // over the quads: lanes 4 and 8 on, then the 16-lane rows
         mx = fmaxf(mx, dpp_mov<0x128>(mx));
         mx = rows_max(mx);
+        // steps that the query row sees
+        auto steps = [&](int h, int t, int k) {
+            const uint32_t s = k ? vs[h][t].y : vs[h][t].x;
+            return EDGE ? s & seen[t][k] : s;
+        };
+        // one that reaches 2 with its block's u; the first step has a block with none of 2^-7 or more
         uint32_t big = 0;
+        bool small = false;
 #pragma unroll
         for (int h = 0; h < NH; ++h)
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
-                big |= EDGE ? (vs[h][t].x & seen[t][0]) | (vs[h][t].y & seen[t][1]) : vs[h][t].x | vs[h][t].y;
-        big &= 0x40004000u;
-        if (__any((mx - m) * y_scale > kSlack || (big && lift == kLift))) {
-            float any_big = big ? 1.0f : 0.0f;
-            any_big = fmaxf(any_big, dpp_mov<0x124>(any_big));
-            any_big = fmaxf(any_big, dpp_mov<0x128>(any_big));
-            const float top = (mx - m) * y_scale > kSlack ? mx : m, down = rows_max(any_big) > 0.0f ? kLiftBig : lift;
-            const float f = __builtin_amdgcn_exp2f(fmaf(m - top, y_scale, down - lift));
-            m = top;
-            lift = down;
-            l *= f;
+            for (int t = 0; t < 2; ++t) big |= reaches_2(steps(h, t, 0), unit[h]) | reaches_2(steps(h, t, 1), unit[h]);
+        // a row that sees nothing here sees nothing later
+        auto blind = [&] {
+            const int page = a.map.page_of(8 * it);
+            return EDGE && lim < page * a.map.page_tokens + (8 * it - page * groups) * 8;
+        };
+        if (fresh) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float fi = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), i));
-#pragma unroll
-                for (int h = 0; h < NH; ++h) {
-                    oh[h][i] *= fi;
-                    ol[h][i] *= fi;
-                }
-#pragma unroll
-                for (int k = 0; k < NQuad<NB>::value; ++k) oc[k][i] *= fi;
+            for (int h = 0; h < NH; ++h) {
+                uint64_t rows_with = __ballot(((steps(h, 0, 0) | steps(h, 0, 1) | steps(h, 1, 0) | steps(h, 1, 1)) & kUsualBits) || blind());
+                rows_with |= rows_with >> 16;
+                rows_with |= rows_with >> 8;
+                rows_with |= rows_with >> 4;
+                small = small || (rows_with & 0xf0000000full) != 0xf0000000full;
             }
         }
-        const float below = fmaf(-m, y_scale, lift);
-        u32x2 ph, pl;
-        {
-            float p[4];
+        const bool ahead = (mx - m) * y_scale > kSlack;
+        if (small || __any(ahead || big)) {
+            const float top = ahead ? mx : m, f = __builtin_amdgcn_exp2f((m - top) * y_scale);
+            m = top;
+            l *= f;
+            float g[NH];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], y_scale, below));
-            l += (p[0] + p[1]) + (p[2] + p[3]);
-            uint32_t x, y;
-            part(p[0], p[1], x, y);
-            ph[0] = x, pl[0] = y;
-            part(p[2], p[3], x, y);
-            ph[1] = x, pl[1] = y;
-        }
+            for (int h = 0; h < NH; ++h) g[h] = f;
+            if (small || __any(big)) {
+                wide = 0;
+                uint32_t other = 0;
 #pragma unroll
-        for (int k = 0; k < NQuad<NB>::value; ++k) {
-            const u32x2 c = {EDGE ? vc[k].x & seen_c[0] : vc[k].x, EDGE ? vc[k].y & seen_c[1] : vc[k].y};
-            oc[k] = __builtin_amdgcn_mfma_f32_4x4x4f16(__builtin_bit_cast(half4v, pl), __builtin_bit_cast(half4v, c), oc[k], 0, 0, 0);
-            oc[k] = __builtin_amdgcn_mfma_f32_4x4x4f16(__builtin_bit_cast(half4v, ph), __builtin_bit_cast(half4v, c), oc[k], 0, 0, 0);
-        }
-        // rows 0..31 and 32..63 of the step, each in both halves of the wave
-        uint32_t dh[2][2], dl[2][2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const auto x = __builtin_amdgcn_permlane32_swap(ph[k], ph[k], false, false);
-            const auto y = __builtin_amdgcn_permlane32_swap(pl[k], pl[k], false, false);
-            dh[0][k] = x[0], dh[1][k] = x[1];
-            dl[0][k] = y[0], dl[1][k] = y[1];
-        }
-#pragma unroll
-        for (int h = 0; h < NH; ++h) {
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                u32x2 fh, fl;
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const uint32_t sv = k ? vs[h][t].y : vs[h][t].x;
-                    const half2v s = as_half2(EDGE ? sv & seen[t][k] : sv), x = as_half2(dh[t][k]), z = x * s;
-                    half2v w = __builtin_elementwise_fma(x, s, -z);
-                    w = __builtin_elementwise_fma(as_half2(dl[t][k]), s, w);
-                    fh[k] = as_u32(z);
-                    fl[k] = as_u32(w);
+                for (int h = 0; h < NH; ++h) {
+                    uint32_t most = max_half(max_halves(max_halves(steps(h, 0, 0), steps(h, 0, 1)), max_halves(steps(h, 1, 0), steps(h, 1, 1))));
+                    // over the lanes of the block and query row: 4, 8 and 16 on
+                    most = max(most, static_cast<uint32_t>(dpp_mov<0x124>(static_cast<int>(most))));
+                    most = max(most, static_cast<uint32_t>(dpp_mov<0x128>(static_cast<int>(most))));
+                    const auto x = __builtin_amdgcn_permlane16_swap(most, most, false, false);
+                    most = max(x[0], x[1]);
+                    const half2v was = fresh ? both(blind() ? kUnitOne : kUnitFirst) : unit[h];
+                    if (reaches_2(most, was)) unit[h] = both(unit_of(most));
+                    else unit[h] = was;
+                    g[h] = f * unit_f(unit[h]) * unit_inverse(was);
+                    other |= (as_u32(unit[h]) & 0xffffu) ^ kUnitOne;
+                    if (__any(below_1(unit[h]))) wide |= 1u << h;
                 }
-                const half4v ah = __builtin_bit_cast(half4v, fh), al = __builtin_bit_cast(half4v, fl);
-                auto quads = [&](auto g_tag) {
-                    constexpr int G = decltype(g_tag)::value;
-                    const u32x4 w = __builtin_bit_cast(u32x4, q4_unpack(vn[h][4 * t + G], ones));
-                    const half4v w0 = __builtin_bit_cast(half4v, u32x2{w[0], w[1]}), w1 = __builtin_bit_cast(half4v, u32x2{w[2], w[3]});
-                    ol[h] = __builtin_amdgcn_mfma_f32_4x4x4f16(al, w0, ol[h], 3, 2 * G, 0);
-                    oh[h] = __builtin_amdgcn_mfma_f32_4x4x4f16(ah, w0, oh[h], 3, 2 * G, 0);
-                    ol[h] = __builtin_amdgcn_mfma_f32_4x4x4f16(al, w1, ol[h], 3, 2 * G + 1, 0);
-                    oh[h] = __builtin_amdgcn_mfma_f32_4x4x4f16(ah, w1, oh[h], 3, 2 * G + 1, 0);
-                };
-                quads(std::integral_constant<int, 0>{});
-                quads(std::integral_constant<int, 1>{});
-                quads(std::integral_constant<int, 2>{});
-                quads(std::integral_constant<int, 3>{});
+                uneven = __any(other);
+            }
+            // of query row i: the quad's lane i, in the half of the channel's block
+            auto rescale = [&](auto i_tag) {
+                constexpr int I = decltype(i_tag)::value;
+                const float fi = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), I));
+#pragma unroll
+                for (int h = 0; h < NH; ++h) {
+                    const float gi = dpp_mov<I * 0x55>(g[h]);
+                    oh[h][I] *= gi;
+                    ol[h][I] *= gi;
+                }
+#pragma unroll
+                for (int k = 0; k < NQuad<NB>::value; ++k) oc[k][I] *= fi;
+            };
+            rescale(std::integral_constant<int, 0>{});
+            rescale(std::integral_constant<int, 1>{});
+            rescale(std::integral_constant<int, 2>{});
+            rescale(std::integral_constant<int, 3>{});
+        }
+        const float below = fmaf(-m, y_scale, kLift);
+        // 32 rows' p s by the codes of one pair of blocks
+        auto product = [&](int h, int t, u32x2 high, u32x2 low) {
+            const half4v ah = __builtin_bit_cast(half4v, high), al = __builtin_bit_cast(half4v, low);
+            auto quads = [&](auto g_tag) {
+                constexpr int G = decltype(g_tag)::value;
+                const u32x4 w = __builtin_bit_cast(u32x4, q4_unpack(vn[h][4 * t + G], ones));
+                const half4v w0 = __builtin_bit_cast(half4v, u32x2{w[0], w[1]}), w1 = __builtin_bit_cast(half4v, u32x2{w[2], w[3]});
+                ol[h] = __builtin_amdgcn_mfma_f32_4x4x4f16(al, w0, ol[h], 3, 2 * G, 0);
+                oh[h] = __builtin_amdgcn_mfma_f32_4x4x4f16(ah, w0, oh[h], 3, 2 * G, 0);
+                ol[h] = __builtin_amdgcn_mfma_f32_4x4x4f16(al, w1, ol[h], 3, 2 * G + 1, 0);
+                oh[h] = __builtin_amdgcn_mfma_f32_4x4x4f16(ah, w1, oh[h], 3, 2 * G + 1, 0);
+            };
+            quads(std::integral_constant<int, 0>{});
+            quads(std::integral_constant<int, 1>{});
+            quads(std::integral_constant<int, 2>{});
+            quads(std::integral_constant<int, 3>{});
+        };
+        if (uneven) {
+            float scale = y_scale;
+            asm("" : "+v"(scale));  // or the weights are formed for both here, apart from the products below
+#pragma unroll
+            for (int h = 0; h < NH; ++h) {
+                if (wide >> h & 1) {
+                    const float uw = below_1(unit[h]) ? unit_f(unit[h]) : 0.0f;  // the other query rows' and block's below
+                    float p[2][4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t w = __float_as_uint(__builtin_amdgcn_exp2f(fmaf(sc[i], scale, below)));
+                        const auto x = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+                        p[0][i] = __uint_as_float(x[0]);
+                        p[1][i] = __uint_as_float(x[1]);
+                    }
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        u32x2 fh, fl;
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            uint32_t x, y;
+                            times_steps(p[t][2 * k], p[t][2 * k + 1], as_half2(steps(h, t, k)), uw, minus1, x, y);
+                            fh[k] = x;
+                            fl[k] = y;
+                        }
+                        product(h, t, fh, fl);
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const uint32_t x = steps(h, t, 0), y = steps(h, t, 1);
+                    vs[h][t].x = below_1(unit[h]) ? 0u : as_u32(as_half2(x) * unit[h]);
+                    vs[h][t].y = below_1(unit[h]) ? 0u : as_u32(as_half2(y) * unit[h]);
+                }
+            }
+        }
+        {
+            u32x2 ph, pl;
+            {
+                float p[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], y_scale, below));
+                l += (p[0] + p[1]) + (p[2] + p[3]);
+                uint32_t x, y;
+                part(p[0], p[1], x, y);
+                ph[0] = x, pl[0] = y;
+                part(p[2], p[3], x, y);
+                ph[1] = x, pl[1] = y;
+            }
+#pragma unroll
+            for (int k = 0; k < NQuad<NB>::value; ++k) {
+                const u32x2 c = {EDGE ? vc[k].x & seen_c[0] : vc[k].x, EDGE ? vc[k].y & seen_c[1] : vc[k].y};
+                oc[k] = __builtin_amdgcn_mfma_f32_4x4x4f16(__builtin_bit_cast(half4v, pl), __builtin_bit_cast(half4v, c), oc[k], 0, 0, 0);
+                oc[k] = __builtin_amdgcn_mfma_f32_4x4x4f16(__builtin_bit_cast(half4v, ph), __builtin_bit_cast(half4v, c), oc[k], 0, 0, 0);
+            }
+            // rows 0..31 and 32..63 of the step, each in both halves of the wave
+            uint32_t dh[2][2], dl[2][2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const auto x = __builtin_amdgcn_permlane32_swap(ph[k], ph[k], false, false);
+                const auto y = __builtin_amdgcn_permlane32_swap(pl[k], pl[k], false, false);
+                dh[0][k] = x[0], dh[1][k] = x[1];
+                dl[0][k] = y[0], dl[1][k] = y[1];
+            }
+#pragma unroll
+            for (int h = 0; h < NH; ++h) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    u32x2 fh, fl;
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        uint32_t x, y;
+                        times_steps(as_half2(dh[t][k]), as_half2(dl[t][k]), as_half2(steps(h, t, k)), x, y);
+                        fh[k] = x;
+                        fl[k] = y;
+                    }
+                    product(h, t, fh, fl);
+                }
             }
         }
         if (more) load_v(next_v, it + kWaves);
@@ -806,10 +1028,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_q4_narrow_kernel(Q4Args a
     };
     l = over_quads(l);
     const int ch = 32 * half32 + 16 * (lane & 1) + ((lane & 31) >> 1);
+    float inverse[NH][4];
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+        const float x = unit_inverse(unit[h]);
+        inverse[h][0] = dpp_mov<0x00>(x);
+        inverse[h][1] = dpp_mov<0x55>(x);
+        inverse[h][2] = dpp_mov<0xaa>(x);
+        inverse[h][3] = dpp_mov<0xff>(x);
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
-        for (int h = 0; h < NH; ++h) s_o[wave][i][64 * h + ch] = oh[h][i] + ol[h][i];
+        for (int h = 0; h < NH; ++h) s_o[wave][i][64 * h + ch] = (oh[h][i] + ol[h][i]) * inverse[h][i];
 #pragma unroll
         for (int k = 0; k < NQuad<NB>::value; ++k) {
             const float v = over_quads(oc[k][i]);
@@ -817,7 +1048,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_q4_narrow_kernel(Q4Args a
         }
     }
     if (lane < 4) {
-        s_m[wave][lane] = fmaf(m, y_scale, -lift);
+        s_m[wave][lane] = fmaf(m, y_scale, -kLift);
         s_l[wave][lane] = l;
     }
     __syncthreads();
@@ -858,6 +1089,7 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
     constexpr int HD = 32 * NB, NO = 16 * NB, SCALES = NB * 128;  // bytes of a step's scales of K, or of V
     typedef float f32x16 __attribute__((ext_vector_type(16)));
     __shared__ __align__(16) uint8_t s_mem[kWaves32 * NO * 256 + kWaves32 * 6 * 256];
+    __shared__ uint32_t s_unit[kWaves32][NB][kRows32];  // u of the blocks, twice: seldom looked at, so not in registers
     static_assert(kWaves32 * NO * 256 >= NB * 4 * 1024 + kWaves32 * 2 * SCALES);
     u32x4(*s_q)[2][64] = reinterpret_cast<u32x4(*)[2][64]>(s_mem);  // [block * 2 + ks][high, low][lane]
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, j2 = lane >> 5;
@@ -1000,7 +1232,11 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
     oc = zero;
 #pragma unroll
     for (int b = 0; b < NB; ++b) o[b] = zero;
-    float m = kLowest, lift = kLift;
+    float m = kLowest;
+    half2v most_unit = both(kUnitOne);  // of the lane's block of scales: no query row's u is larger
+    bool uneven = false;  // in the wave: a u that is not 1
+    auto unit = [&](int b) { return uneven ? as_half2(s_unit[wave][b][col]) : both(kUnitOne); };
+    uint32_t wide = 0;    // a u below 1, by block
     auto mfma = [](u32x4 x, u32x4 y, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, x), __builtin_bit_cast(half8, y), c, 0, 0, 0);
     };
@@ -1027,17 +1263,33 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
         };
         // this wave's own memory: its reads of the last step are done, and reads follow writes in order
         bool big_step = false;
+        // of the lane's pairs of rows (0, 4), (1, 5) or (2, 6), (7, 3), those below n
+        auto rows_below = [&](int n, uint32_t& x, uint32_t& y) {
+            const int first = (sl_p & 8) / 4;
+            x = (first < n ? 0xffffu : 0u) | (first + 4 < n ? 0xffff0000u : 0u);
+            y = first ? (7 < n ? 0xffffu : 0u) | (3 < n ? 0xffff0000u : 0u) : (1 < n ? 0xffffu : 0u) | (5 < n ? 0xffff0000u : 0u);
+        };
         if constexpr (PAD) {  // their steps and middles: 0
-            const int room = room_of(4 * st + sl_g), first = (sl_p & 8) / 4;  // pairs of rows (0, 4), (1, 5) or (2, 6), (7, 3)
-            const uint32_t x = (first < room ? 0xffffu : 0u) | (first + 4 < room ? 0xffff0000u : 0u);
-            const uint32_t y = first ? (7 < room ? 0xffffu : 0u) | (3 < room ? 0xffff0000u : 0u)
-                                     : (1 < room ? 0xffffu : 0u) | (5 < room ? 0xffff0000u : 0u);
+            uint32_t x, y;
+            rows_below(room_of(4 * st + sl_g), x, y);
             ksc.x &= x, ksc.y &= y, vsc.x &= x, vsc.y &= y;
         }
         if (NB == 4 || lane < 32) {
             *reinterpret_cast<uint2*>(s_sc + (sl_b * 4 + sl_g) * 32 + sl_p) = ksc;
             *reinterpret_cast<uint2*>(s_sc + SCALES + (sl_b * 4 + sl_g) * 32 + sl_p) = vsc;
-            big_step = sl_p < 16 && ((vsc.x | vsc.y) & 0x40004000u);
+            big_step = sl_p < 16 && reaches_2(max_halves(vsc.x, vsc.y), most_unit);
+        }
+        const bool fresh = st == begin + wave;
+        bool small = false;  // the first step has a block with none of 2^-7 or more in the rows that all query rows see
+        if (fresh) {
+            uint32_t x = 0xffffffffu, y = x;
+            if constexpr (EDGE) {
+                const int vg = 4 * st + sl_g, page = a.map.page_of(vg), g = vg - page * groups;
+                rows_below(min(a.map.page_tokens - g * 8, first_lim + 1 - page * a.map.page_tokens - g * 8), x, y);
+            }
+            const uint64_t with = __ballot(sl_p < 16 && (((vsc.x & x) | (vsc.y & y)) & kUsualBits));
+#pragma unroll
+            for (int b = 0; b < NB; ++b) small = small || !(with >> (16 * b) & 0xffff);
         }
         __builtin_amdgcn_wave_barrier();
         const uint16_t* c = reinterpret_cast<const uint16_t*>(s_sc + (j2 * 4 + kg) * 32 + 16) + kr;
@@ -1116,63 +1368,118 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
             const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
             mx = fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
         }
-        uint32_t big = __any(big_step);
-        if (EDGE && big) {  // of the rows that the query row sees
-            big = 0;
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
+        const bool ahead = (mx - m) * y_scale > kSlack;
+        if (small || __any(ahead || big_step)) {
+            const float top = ahead ? mx : m, f = __builtin_amdgcn_exp2f((m - top) * y_scale);
+            m = top;
+            oc *= f;
+            if (small || __any(big_step)) {
+                half2v start = both(kUnitFirst);
+                if constexpr (EDGE) {  // a row that sees nothing here sees nothing later
+                    const int page = a.map.page_of(4 * st);
+                    if (lim < page * a.map.page_tokens + (4 * st - page * groups) * 8) start = both(kUnitOne);
+                    if (fresh) most_unit = both(kUnitFirst);
+                }
+                wide = 0;
+                uint32_t other = 0;
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    const u32x4 s = scales(1, b, k, 0);
+                    uint32_t most = 0;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) big |= s[i] & seen[k][i] & 0x40004000u;
+                    for (int k = 0; k < 2; ++k) {
+                        const u32x4 s = scales(1, b, k, 0);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) most = max_halves(most, EDGE ? s[i] & seen[k][i] : s[i]);
+                    }
+                    most = max_half(most);
+                    const auto t = __builtin_amdgcn_permlane32_swap(most, most, false, false);
+                    most = max(t[0], t[1]);
+                    const half2v was = fresh ? start : unit(b), u = reaches_2(most, was) ? both(unit_of(most)) : was;
+                    s_unit[wave][b][col] = as_u32(u);
+                    o[b] *= f * unit_f(u) * unit_inverse(was);
+                    other |= (as_u32(u) & 0xffffu) ^ kUnitOne;
+                    if (__any(below_1(u))) wide |= 1u << b;
+                    if (!EDGE && sl_b == b) most_unit = u;  // one for all query rows
                 }
-        }
-        if (__any((mx - m) * y_scale > kSlack || (big && lift == kLift))) {
-            const auto t = __builtin_amdgcn_permlane32_swap(big, big, false, false);
-            const float top = (mx - m) * y_scale > kSlack ? mx : m, down = (t[0] | t[1]) ? kLiftBig : lift;
-            const float f = __builtin_amdgcn_exp2f(fmaf(m - top, y_scale, down - lift));
-            m = top;
-            lift = down;
-            oc *= f;
+                uneven = __any(other);
+            } else {
 #pragma unroll
-            for (int b = 0; b < NB; ++b) o[b] *= f;
-        }
-        const float below = fmaf(-m, y_scale, lift);
-        u32x4 ph[2], pl[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint32_t h, l;
-                part(__builtin_amdgcn_exp2f(fmaf(sc[8 * k + 2 * i], y_scale, below)),
-                     __builtin_amdgcn_exp2f(fmaf(sc[8 * k + 2 * i + 1], y_scale, below)), h, l);
-                ph[k][i] = h;
-                pl[k][i] = l;
+                for (int b = 0; b < NB; ++b) o[b] *= f;
             }
-            u32x4 c = *reinterpret_cast<const u32x4*>(s_sc + SCALES + (min(col, NB - 1) * 4 + 2 * k + j2) * 32 + 16);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) c[i] = ((EDGE ? c[i] & seen_c[k][i] : c[i]) & c_mask) | c_fill;
-            oc = mfma(c, pl[k], oc);
-            oc = mfma(c, ph[k], oc);
         }
+        const float below = fmaf(-m, y_scale, kLift);
+        if (uneven) {
+            float scale = y_scale;
+            asm("" : "+v"(scale));  // or the weights are formed for both here, apart from the products below
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
+            for (int b = 0; b < NB; ++b) {
+                if (!(wide >> b & 1)) continue;
+                const half2v u = unit(b);
+                const float uw = below_1(u) ? unit_f(u) : 0.0f;  // the other query rows' below
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const u32x4 s = scales(1, b, k, 0);
+                    u32x4 fh, fl;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t h, l;
+                        times_steps(__builtin_amdgcn_exp2f(fmaf(sc[8 * k + 2 * i], scale, below)),
+                                    __builtin_amdgcn_exp2f(fmaf(sc[8 * k + 2 * i + 1], scale, below)),
+                                    as_half2(EDGE ? s[i] & seen[k][i] : s[i]), uw, minus1, h, l);
+                        fh[i] = h;
+                        fl[i] = l;
+                    }
+                    const u32x4 w = __builtin_bit_cast(u32x4, q4_unpack(vn[b][k], ones));
+                    o[b] = mfma(w, fl, o[b]);
+                    o[b] = mfma(w, fh, o[b]);
+                }
+            }
+            if (!EDGE && sl_p < 16 && (NB == 4 || lane < 32)) {  // where rows differ in what they see, each takes its own below
+                uint2* const s = reinterpret_cast<uint2*>(s_sc + SCALES + (sl_b * 4 + sl_g) * 32 + sl_p);
+                *s = below_1(most_unit) ? make_uint2(0u, 0u)
+                                        : make_uint2(as_u32(as_half2(s->x) * most_unit), as_u32(as_half2(s->y) * most_unit));
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+        {
+            u32x4 ph[2], pl[2];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const u32x4 s = scales(1, b, k, 0);
-                u32x4 fh, fl;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const half2v z = as_half2(EDGE ? s[i] & seen[k][i] : s[i]), x = as_half2(ph[k][i]), t = x * z;
-                    half2v w = __builtin_elementwise_fma(x, z, -t);
-                    w = __builtin_elementwise_fma(as_half2(pl[k][i]), z, w);
-                    fh[i] = as_u32(t);
-                    fl[i] = as_u32(w);
+                    uint32_t h, l;
+                    part(__builtin_amdgcn_exp2f(fmaf(sc[8 * k + 2 * i], y_scale, below)),
+                         __builtin_amdgcn_exp2f(fmaf(sc[8 * k + 2 * i + 1], y_scale, below)), h, l);
+                    ph[k][i] = h;
+                    pl[k][i] = l;
                 }
-                const u32x4 w = __builtin_bit_cast(u32x4, q4_unpack(vn[b][k], ones));
-                o[b] = mfma(w, fl, o[b]);
-                o[b] = mfma(w, fh, o[b]);
+                u32x4 c = *reinterpret_cast<const u32x4*>(s_sc + SCALES + (min(col, NB - 1) * 4 + 2 * k + j2) * 32 + 16);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) c[i] = ((EDGE ? c[i] & seen_c[k][i] : c[i]) & c_mask) | c_fill;
+                oc = mfma(c, pl[k], oc);
+                oc = mfma(c, ph[k], oc);
+            }
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                half2v u = {};
+                if constexpr (EDGE) u = unit(b);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const u32x4 s = scales(1, b, k, 0);
+                    u32x4 fh, fl;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        half2v z = as_half2(s[i]);
+                        if constexpr (EDGE) z = as_half2(below_1(u) ? 0u : as_u32(as_half2(s[i] & seen[k][i]) * u));
+                        uint32_t h, l;
+                        times_steps(as_half2(ph[k][i]), as_half2(pl[k][i]), z, h, l);
+                        fh[i] = h;
+                        fl[i] = l;
+                    }
+                    const u32x4 w = __builtin_bit_cast(u32x4, q4_unpack(vn[b][k], ones));
+                    o[b] = mfma(w, fl, o[b]);
+                    o[b] = mfma(w, fh, o[b]);
+                }
             }
         }
         load(a.pt_v, next_v, nst, vn, false);
@@ -1185,17 +1492,20 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
     for (; st < full; st += kWaves32) step(std::integral_constant<int, PAGES == Pages::kRows ? 1 : 0>{});
     for (; st < end; st += kWaves32) step(std::integral_constant<int, 2>{});
 
-    // the waves joined: every wave's sums by register and lane, then each wave a quarter of the registers
+    // the waves joined: every wave's sums by register and lane, then each wave an eighth of the registers
     __syncthreads();
     float(*s_o)[NO][64] = reinterpret_cast<float(*)[NO][64]>(s_mem);
     float(*s_x)[6][64] = reinterpret_cast<float(*)[6][64]>(s_mem + kWaves32 * NO * 256);  // sums of p c and p (rows 0..7), m
+    float inverse[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) inverse[b] = unit_inverse(unit(b));
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s_o[wave][16 * b + i][lane] = o[b][i];
+        for (int i = 0; i < 16; ++i) s_o[wave][16 * b + i][lane] = o[b][i] * inverse[b];
 #pragma unroll
     for (int i = 0; i < 4; ++i) s_x[wave][i][lane] = oc[i];
-    s_x[wave][4][lane] = fmaf(m, y_scale, -lift);
+    s_x[wave][4][lane] = fmaf(m, y_scale, -kLift);
     __syncthreads();
     float w[kWaves32], top = s_x[0][4][lane], l = 0.0f;
 #pragma unroll
