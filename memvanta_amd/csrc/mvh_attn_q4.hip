@@ -7,8 +7,8 @@
 //   q.K_t       = sum_b s_tb (sum_i q_i (n_ti - 8)) + c_tb sum_i q_i,
 //   sum p_t V_t = sum_t (p_t s_tb) (n_t - 8) + sum_t p_t c_tb :
 // n - 8 is exact in fp16, so the products run on the fp16 matrix pipe with the
-// codes as they are; q and p s are split into two fp16 (22 bits: 2^-22 of
-// the largest, where one fp16 would leave 2^-11), sums are fp32.
+// codes as they are; q and p s are split into two fp16 (22 bits, where one fp16
+// would leave 11), sums are fp32.
 #include "mvh_kernels.hpp"
 #include "mvh_kv4.hpp"
 
@@ -140,6 +140,12 @@ __device__ __forceinline__ f32x4 mfma2(u32x4 a, u32x4 high, u32x4 low, f32x4 c) 
     const half8 m = __builtin_bit_cast(half8, a);
     c = __builtin_amdgcn_mfma_f32_16x16x32_f16(m, __builtin_bit_cast(half8, low), c, 0, 0, 0);
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(m, __builtin_bit_cast(half8, high), c, 0, 0, 0);
+}
+// The power of two that brings a query row's largest element to [2^9, 2^10): its
+// elements keep 22 bits in two fp16 down to 2^-13 of that one and 2^-35 of it below
+// (so a small one counts on a wide key channel), and a block's sum, below 2^15, fits too
+__device__ __forceinline__ int query_exponent(float top) {
+    return (top > 0.0f && top <= 3.402823466e38f ? max(__builtin_amdgcn_frexp_expf(top) - 1, -110) : 0) - 9;
 }
 // p - h (exact where h is p rounded, or 0): the conversion inside the addition
 __device__ __forceinline__ float less(float p, _Float16 h, float minus1) { return fmaf(static_cast<float>(h), minus1, p); }
@@ -297,7 +303,7 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
         load_v(page_of_step(a.pt_v, st), st);
     }
 
-    // q: lane (col, j) holds channels 8 j .. of each block of row col; scaled by a power of two to [1, 2)
+    // q: lane (col, j) holds channels 8 j .. of each block of row col; scaled by a power of two
     const int r = min(row0 + col, rows - 1), lim = pos + r / a.group;
     const float* qr = a.q + static_cast<size_t>(r / a.group) * a.q_pitch + static_cast<size_t>(kh * a.group + r % a.group) * hd - shift;
     // masks and constants that the compiler is not to see: as selects and literals they take more operations
@@ -326,7 +332,7 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
             }
         }
         top = rows_max(top);
-        const int e = top > 0.0f && top <= 3.402823466e38f ? max(__builtin_amdgcn_frexp_expf(top) - 1, -120) : 0;
+        const int e = query_exponent(top);
         const float down = ldexpf(1.0f, -e);
         y_scale = ldexpf(__fdiv_rn(kLog2e, sqrt_rn(static_cast<float>(hd))), e);
         float mine[NQ];
@@ -735,7 +741,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_q4_narrow_kernel(Q4Args a
             for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(f[R][i]));
         }
         top = rows_max(top);
-        const int e = top > 0.0f && top <= 3.402823466e38f ? max(__builtin_amdgcn_frexp_expf(top) - 1, -120) : 0;
+        const int e = query_exponent(top);
         const float down = ldexpf(1.0f, -e);
         y_scale = ldexpf(__fdiv_rn(kLog2e, sqrt_rn(static_cast<float>(HD))), e);
 #pragma unroll
@@ -1168,7 +1174,7 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
         lo = as_u32(pk_half(less(x, h.x, minus1), less(y, h.y, minus1)));
     };
     // q: pieces of 16 channels, half of a block, a wave's own one (lane (col, j2): channels 8 j2 .. of row col); the row's
-    // maximum and the block sums go through LDS.  Scaled by a power of two to [1, 2)
+    // maximum and the block sums go through LDS.  Scaled by a power of two
     const int r = min(row0 + col, rows - 1), lim = pos + r / a.group;
     uint32_t qch, qcl;  // block sums of blocks j2 and j2 + 2, in two parts: the operand that meets the c of K
     float y_scale;
@@ -1198,7 +1204,7 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < 2 * NB; ++k) top = fmaxf(top, fmaxf(s_top[k][col], s_top[k][col + 32]));
-        const int e = top > 0.0f && top <= 3.402823466e38f ? max(__builtin_amdgcn_frexp_expf(top) - 1, -120) : 0;
+        const int e = query_exponent(top);
         const float down = ldexpf(1.0f, -e);
         y_scale = ldexpf(__fdiv_rn(kLog2e, sqrt_rn(static_cast<float>(HD))), e);
         if (wave < 2 * NB) {

@@ -1,5 +1,5 @@
-"""Attention over a 4-bit cache where its numbers are far apart: blocks of values of different size, rows that outweigh
-others; against attention in 64 bits over the values that the cache holds, block by block."""
+"""Attention over a 4-bit cache where its numbers are far apart: blocks of values of different size, small query elements on
+wide key channels; against attention in 64 bits over the values that the cache holds, block by block."""
 import numpy as np
 import pytest
 
@@ -80,3 +80,19 @@ def test_first_row_takes_the_weight(ctx, heads, n_kv, hd, pos, n):
     k[0] = np.float32(8.0 / np.sqrt(hd))
     got, want, _ = _run(ctx, q, k, v, heads, n_kv, hd, pos, n)
     _by_block(got, want, hd, REL + 5.3e-6, "")
+
+
+@pytest.mark.parametrize("heads,n_kv,hd,pos,n", CALLS)
+def test_small_queries_on_wide_keys(ctx, heads, n_kv, hd, pos, n):
+    """Blocks of q a thousand times smaller than others, on keys as much wider: each block gives its share of the score."""
+    rng = np.random.default_rng(hd + pos + 3)
+    k, v = (rng.standard_normal((pos + n, n_kv * hd), dtype=np.float32) for _ in range(2))
+    q = rng.standard_normal((n, heads, hd), dtype=np.float32) * np.float32(1.5)
+    if hd % 32:  # blocks that heads share: a size per head's middle
+        width = np.where(np.arange(n_kv * hd) // 32 % 2 == 0, np.float32(1000.0), np.float32(1.0))
+    else:
+        width = np.tile(np.float32([1000.0, 1.0, 30.0, 1.0, 200.0, 1.0, 1.0, 1000.0, 5.0])[: hd // 32].repeat(32), n_kv)
+    k *= width
+    q /= width.reshape(n_kv, hd).repeat(heads // n_kv, axis=0)
+    got, want, _ = _run(ctx, q, k, v, heads, n_kv, hd, pos, n)
+    _by_block(got, want, hd, REL, "")
