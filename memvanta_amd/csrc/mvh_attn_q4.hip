@@ -38,7 +38,7 @@ struct Q4Args {
     Kv4Map map;
 };
 
-constexpr float kLowest = -1.0e12f;  // m before the first row: finite, so that 2^(-inf - m) is 0; scores stay above it
+constexpr float kLowest = -1.0e12f;  // m before the first row, below any score of a scaled query: finite, so that 2^(-inf - m) is 0
 constexpr float kLog2e = 1.44269504088896340736f;
 // Weights are 2^(y - m + kLift), and m follows the maximum only when that is
 // kSlack ahead (the sums are rescaled seldom, the decision is each row's own): at
@@ -54,7 +54,12 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // of the largest weight times the block's largest step, whatever other blocks
 // hold.  A wave's first step looks whether all its blocks start with u = 1; while
 // they stay there, the usual case, steps are taken as they are.
-constexpr float kLift = 10.0f, kSlack = 4.0f;
+//
+// The exponent of a weight is y_scale s - y_scale m + kLift, the second product
+// rounded once for all of a step's rows (and for the join); where it is beyond
+// kFar, and that rounding a large factor, m is taken off the scores first.  So is
+// the m of a query row that has seen nothing yet.
+constexpr float kLift = 10.0f, kSlack = 4.0f, kFar = 1048576.0f;
 constexpr uint32_t kUnitOne = 0x3c00u, kUnitFirst = 30u << 10;  // 1, and 2^15: before any step
 constexpr uint32_t kUsualBits = 0x60006000u, kWideBits = 0x40004000u;  // of a step >= 2^-7, >= 2 (or NaN), in either half
 constexpr int kWaves = 4;
@@ -501,7 +506,13 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
                 }
             }
         }
-        const float below = fmaf(-m, y_scale, kLift);
+        const bool far = fabsf(m * y_scale) > kFar;
+        if (__any(far)) {
+            const float base = far ? m : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s0[i] -= base, s1[i] -= base;
+        }
+        const float below = far ? kLift : fmaf(-m, y_scale, kLift);
         if (uneven) {
             float scale = y_scale;
             asm("" : "+v"(scale));  // or the weights are formed for both here, apart from the products below
@@ -921,7 +932,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_q4_narrow_kernel(Q4Args a
             rescale(std::integral_constant<int, 2>{});
             rescale(std::integral_constant<int, 3>{});
         }
-        const float below = fmaf(-m, y_scale, kLift);
+        const bool far = fabsf(m * y_scale) > kFar;
+        if (__any(far)) {
+            const float base = far ? m : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[i] -= base;
+        }
+        const float below = far ? kLift : fmaf(-m, y_scale, kLift);
         // 32 rows' p s by the codes of one pair of blocks
         auto product = [&](int h, int t, u32x2 high, u32x2 low) {
             const half4v ah = __builtin_bit_cast(half4v, high), al = __builtin_bit_cast(half4v, low);
@@ -1413,7 +1430,13 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
                 for (int b = 0; b < NB; ++b) o[b] *= f;
             }
         }
-        const float below = fmaf(-m, y_scale, kLift);
+        const bool far = fabsf(m * y_scale) > kFar;
+        if (__any(far)) {
+            const float base = far ? m : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sc[i] -= base;
+        }
+        const float below = far ? kLift : fmaf(-m, y_scale, kLift);
         if (uneven) {
             float scale = y_scale;
             asm("" : "+v"(scale));  // or the weights are formed for both here, apart from the products below
@@ -1573,7 +1596,7 @@ __global__ __launch_bounds__(kAny) void attn_q4_any_kernel(Q4Args a) {
     const int e0 = h / a.group * hd;  // the head's first element of a row
     const size_t sc_off = kv4_scales(a.map.page_tokens, a.kv_dim);
     const float y_scale = __fdiv_rn(kLog2e, sqrt_rn(static_cast<float>(hd)));
-    float m = kLowest, l = 0.0f;
+    float m = -INFINITY, l = 0.0f;  // the first 256 rows hold one that the token sees
     for (int g0 = begin; g0 < end; g0 += kAny / 8) {
         const int vg = min(g0 + tid / 8, end - 1), i = tid & 7;
         const int page = a.map.page_of(vg), g = vg - page * a.map.groups;
@@ -1678,7 +1701,7 @@ __global__ __launch_bounds__(kJoin) void attn_q4_join_kernel(Q4Args a, int n_spl
     const int chunk = split_chunk(a, pos, n_split);
     const int used = (steps_of(a.map, lim) + chunk - 1) / chunk;
     if (tid < 64) {
-        float top = kLowest, sum = 0.0f;
+        float top = -INFINITY, sum = 0.0f;
 #pragma unroll
         for (int k = 0; k < kMaxSplit / 64; ++k)
             if (tid + 64 * k < used) top = fmaxf(top, in[k].x);

@@ -1,5 +1,5 @@
 """Attention over a 4-bit cache where its numbers are far apart: blocks of values of different size, small query elements on
-wide key channels; against attention in 64 bits over the values that the cache holds, block by block."""
+wide key channels, large queries; against attention in 64 bits over the values that the cache holds, block by block."""
 import numpy as np
 import pytest
 
@@ -96,3 +96,30 @@ def test_small_queries_on_wide_keys(ctx, heads, n_kv, hd, pos, n):
     q /= width.reshape(n_kv, hd).repeat(heads // n_kv, axis=0)
     got, want, _ = _run(ctx, q, k, v, heads, n_kv, hd, pos, n)
     _by_block(got, want, hd, REL, "")
+
+
+@pytest.mark.parametrize("heads,n_kv,hd,pos,n", CALLS + [(1, 1, 128, 1022, 4), (1, 1, 64, 1021, 4), (8, 2, 128, 20, 40), (4, 2, 128, 0, 300)])
+@pytest.mark.parametrize("size,low", [(1e9, False), (1e28, False), (1e34, False), (1e14, True), (1e20, True)])
+def test_large_queries(ctx, heads, n_kv, hd, pos, n, size, low):
+    """Queries whose scores are far from 0 (from 1e9 on, all of them below -1e12 or not) and finite: one row takes all the
+    weight."""
+    rng = np.random.default_rng(hd + pos + 4)
+    k, v = (rng.standard_normal((pos + n, n_kv * hd), dtype=np.float32) for _ in range(2))
+    q = rng.standard_normal((n, heads, hd), dtype=np.float32)
+    if low:
+        k -= np.float32(3.0)
+        q = abs(q) + np.float32(0.5)
+    q *= np.float32(size)
+    got, want, k = _run(ctx, q, k, v, heads, n_kv, hd, pos, n)
+    assert np.isfinite(got).all()
+    # where the two best scores are clear of each other (2^-20 of the score's terms), the output is the best row's values
+    clear = 0
+    for t in range(n):
+        for h in range(heads):
+            s = np.sort((k[: pos + t + 1, h // (heads // n_kv)].astype(np.float64) @ q[t, h].astype(np.float64)))
+            if len(s) > 1 and s[-1] - s[-2] < 2.0 ** -20 * hd * 6 * size:
+                continue
+            g, w = got[t].reshape(heads, hd)[h], want[t].reshape(heads, hd)[h]
+            assert abs(g - w).max() <= 2.0 ** -20 * abs(w).max(), (t, h)
+            clear += 1
+    assert clear >= n * heads // 2
