@@ -540,6 +540,9 @@ hipError_t append_q4(const RotArgs& a, const int* d_pos, hipStream_t st) {
 
 RopeView no_rope() { return RopeView{}; }
 
+constexpr size_t kMostTokens = size_t{1} << 22;  // of a launch of rotate_kernel
+constexpr size_t kMostQuads = size_t{1} << 31;   // of a launch of kv_read_kernel, a thread each
+
 }  // namespace
 
 hipError_t launch_rope(const RopeView& rope, const float* x, size_t x_pitch, float* out, size_t out_pitch,
@@ -547,15 +550,19 @@ hipError_t launch_rope(const RopeView& rope, const float* x, size_t x_pitch, flo
     if (!n_tokens || !n_head) return hipSuccess;
     RotArgs a{};
     a.rope = rope;
-    a.q = x;
-    a.q_out = out;
     a.q_pitch = x_pitch;
     a.out_pitch = out_pitch;
-    a.positions = positions;
-    a.pos = static_cast<int>(pos);
-    a.n_tokens = static_cast<int>(n_tokens);
     a.n_head = static_cast<int>(n_head);
-    return rotate_typed<kNoPages>(a, st);
+    // a workgroup a token at worst: launches of 2^22 tokens stay below the 2^32 threads a grid may have
+    for (size_t t = 0; t < n_tokens; t += kMostTokens) {
+        a.q = x + t * x_pitch;
+        a.q_out = out + t * out_pitch;
+        a.positions = positions ? positions + t : nullptr;
+        a.pos = static_cast<int>(pos + t);
+        a.n_tokens = static_cast<int>(std::min(n_tokens - t, kMostTokens));
+        if (hipError_t e = rotate_typed<kNoPages>(a, st); e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 hipError_t launch_kv_append(int kv_type, const RopeView& rope, void* const* pt_k, void* const* pt_v, const float* q,
@@ -627,18 +634,23 @@ hipError_t launch_kv4_write(void* const* pt_k, void* const* pt_v, const float* k
 
 hipError_t launch_kv_read(int kv_type, const void* const* pt_k, const void* const* pt_v, size_t pos, size_t n_tokens,
                           size_t kv_dim, size_t page_tokens, float* k, float* v, hipStream_t st) {
-    if (!n_tokens) return hipSuccess;
-    const dim3 grid(static_cast<unsigned>((n_tokens * (kv_dim / 4) + 255) / 256), 2);
-    const int p = static_cast<int>(pos), n = static_cast<int>(n_tokens), kd = static_cast<int>(kv_dim),
-              pt = static_cast<int>(page_tokens);
-    switch (kv_type) {
-    case kKvF32: kv_read_kernel<kKvF32><<<grid, 256, 0, st>>>(pt_k, pt_v, p, n, kd, pt, k, v); break;
-    case kKvF16: kv_read_kernel<kKvF16><<<grid, 256, 0, st>>>(pt_k, pt_v, p, n, kd, pt, k, v); break;
-    case kKvQ8: kv_read_kernel<kKvQ8><<<grid, 256, 0, st>>>(pt_k, pt_v, p, n, kd, pt, k, v); break;
-    case kKvQ4: kv_read_kernel<kKvQ4><<<grid, 256, 0, st>>>(pt_k, pt_v, p, n, kd, pt, k, v); break;
-    default: return hipErrorInvalidValue;
+    const size_t quads = kv_dim / 4, most = std::max<size_t>(1, kMostQuads / quads);
+    for (size_t t = 0; t < n_tokens; t += most) {
+        const size_t rows = std::min(n_tokens - t, most);
+        const dim3 grid(static_cast<unsigned>((rows * quads + 255) / 256), 2);
+        const int p = static_cast<int>(pos + t), n = static_cast<int>(rows), kd = static_cast<int>(kv_dim),
+                  pt = static_cast<int>(page_tokens);
+        float *kt = k ? k + t * kv_dim : nullptr, *vt = v ? v + t * kv_dim : nullptr;
+        switch (kv_type) {
+        case kKvF32: kv_read_kernel<kKvF32><<<grid, 256, 0, st>>>(pt_k, pt_v, p, n, kd, pt, kt, vt); break;
+        case kKvF16: kv_read_kernel<kKvF16><<<grid, 256, 0, st>>>(pt_k, pt_v, p, n, kd, pt, kt, vt); break;
+        case kKvQ8: kv_read_kernel<kKvQ8><<<grid, 256, 0, st>>>(pt_k, pt_v, p, n, kd, pt, kt, vt); break;
+        case kKvQ4: kv_read_kernel<kKvQ4><<<grid, 256, 0, st>>>(pt_k, pt_v, p, n, kd, pt, kt, vt); break;
+        default: return hipErrorInvalidValue;
+        }
+        if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     }
-    return hipGetLastError();
+    return hipSuccess;
 }
 
 }  // namespace mvh
