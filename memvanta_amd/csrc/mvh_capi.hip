@@ -340,8 +340,6 @@ int check_kv(const mvh_kv_cache* kv, size_t layer) {
     return MVH_OK;
 }
 
-constexpr size_t kMaxKv4Tokens = size_t{1} << 20, kMaxKv4Dim = size_t{1} << 16;
-
 // The cache is on the context's device, and layer is one of its layers.
 int check_kv_on(const mvh_context* c, const mvh_kv_cache* kv, size_t layer) {
     if (int rc = check_kv(kv, layer)) return rc;
@@ -1024,9 +1022,9 @@ int mvh_kv_create(mvh_context* c, size_t n_layer, size_t kv_dim, size_t page_tok
     if (kv_dim % 8) return fail(MVH_E_SHAPE, "kv_dim must be a multiple of 8");
     if (kv_type == MVH_KV_Q4) {
         if (kv_dim % 32) return fail(MVH_E_SHAPE, "kv_dim of a 4-bit KV cache must be a multiple of 32");
-        if (kv_dim > kMaxKv4Dim) return fail(MVH_E_RANGE, "kv_dim above %zu is not supported", kMaxKv4Dim);
-        if (max_tokens > kMaxKv4Tokens || page_tokens > kMaxKv4Tokens)
-            return fail(MVH_E_RANGE, "max_tokens and page_tokens above %zu are not supported", kMaxKv4Tokens);
+        if (kv_dim > mvh::kMaxKv4Dim) return fail(MVH_E_RANGE, "kv_dim above %zu is not supported", mvh::kMaxKv4Dim);
+        if (max_tokens > mvh::kMaxKv4Tokens || page_tokens > mvh::kMaxKv4Tokens)
+            return fail(MVH_E_RANGE, "max_tokens and page_tokens above %zu are not supported", mvh::kMaxKv4Tokens);
     } else if (max_tokens > 16000) {
         return fail(MVH_E_RANGE, "max_tokens above 16000 is not supported");
     }

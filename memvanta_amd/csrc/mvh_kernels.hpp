@@ -132,6 +132,9 @@ hipError_t launch_attn_decode(int kv_type, const void* const* pt_k, const void* 
                               float* scores, float* out, size_t pos, size_t n_head, size_t n_head_kv, size_t hd,
                               size_t kv_dim, size_t page_tokens, hipStream_t st);
 
+// what positions, pages and rows of 4-bit pages are limited to (their divisions go by reciprocals)
+constexpr size_t kMaxKv4Tokens = size_t{1} << 20, kMaxKv4Dim = size_t{1} << 16;
+
 // ---- 4-bit pages: attention (mvh_attn_q4.hip) ----
 // The attention of launch_attn over kKvQ4 pages, any hd % 8 == 0, kv_dim % 32
 // == 0: n_tokens query tokens at positions pos.. (*d_pos when d_pos != null),

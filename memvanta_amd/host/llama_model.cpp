@@ -86,6 +86,9 @@ LlamaModel::LlamaModel(const std::string& path, int device, std::size_t ctx_over
         throw std::runtime_error("device path needs n_embd, n_ff % 32 == 0 and head_dim % 8 == 0");
     if (kv_type_ == mvh::kKvQ4 && c_.kv_dim() % 32)
         throw std::runtime_error("kv_dim of a 4-bit KV cache must be a multiple of 32");
+    if (kv_type_ == mvh::kKvQ4 && (c_.n_ctx > mvh::kMaxKv4Tokens || page_tokens_ > mvh::kMaxKv4Tokens || c_.kv_dim() > mvh::kMaxKv4Dim))
+        throw std::runtime_error("a 4-bit KV cache takes up to " + std::to_string(mvh::kMaxKv4Tokens) + " tokens and tokens a page, and a kv_dim up to " +
+                                 std::to_string(mvh::kMaxKv4Dim));
 
     check(hipSetDevice(device_), "hipSetDevice");
     check(hipStreamCreateWithFlags(&lanes_[0].st, hipStreamNonBlocking), "hipStreamCreate");
