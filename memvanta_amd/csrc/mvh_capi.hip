@@ -1028,6 +1028,8 @@ int mvh_kv_create(mvh_context* c, size_t n_layer, size_t kv_dim, size_t page_tok
     } else if (max_tokens > 16000) {
         return fail(MVH_E_RANGE, "max_tokens above 16000 is not supported");
     }
+    if (kv_dim > 0x7fffffff || page_tokens > 0x7fffffff)  // the kernels' int
+        return fail(MVH_E_RANGE, "kv_dim and page_tokens above 2147483647 are not supported");
     const size_t max_pages = (max_tokens - 1) / page_tokens + 1;
     if (n_layer > (size_t{1} << 31) / max_pages)
         return fail(MVH_E_RANGE, "KV cache of more than 2147483648 pages");
@@ -1321,6 +1323,7 @@ int mvh_kv_append(mvh_context* c, mvh_kv_cache* kv, size_t layer, size_t pos, si
     const size_t hd = static_cast<size_t>(r->view.head_dim), kv_dim = kv->kv_dim;
     if (hd % 8 || kv_dim % hd) return fail(MVH_E_SHAPE, "kv_dim must be whole heads of a multiple of 8 elements");
     if (k_pitch < kv_dim || v_pitch < kv_dim) return fail(MVH_E_SHAPE, "row pitch below kv_dim");
+    if (kv_dim > (size_t{1} << 24)) return fail(MVH_E_RANGE, "rows above 16777216 elements");
     if (kv->type == MVH_KV_Q8 && kv_dim > 16384) return fail(MVH_E_SHAPE, "kv_dim of Q8 rows above 16384 is not supported");
     if (!n_tokens) return MVH_OK;
     if (!k || !v) return fail(MVH_E_INVALID, "null k/v");

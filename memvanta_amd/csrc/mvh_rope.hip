@@ -510,7 +510,7 @@ hipError_t rotate_typed(const RotArgs& a, hipStream_t st) {
     const int units = heads * (hd / (vec ? 8 : 2));
     // several tokens a workgroup while they fit 256 threads (and 32 KB of turns); else a token's units in shares
     const int T = std::max(1, std::min({256 / units, a.n_tokens, 4096 / std::max(1, rot / 2)}));
-    const int share = T > 1 ? units : std::min(units, a.n_tokens >= 512 ? 512 : 256);
+    const int share = T > 1 ? units : std::max(std::min(units, a.n_tokens >= 512 ? 512 : 256), (units + 65534) / 65535);
     const dim3 grid(static_cast<unsigned>((a.n_tokens + T - 1) / T), static_cast<unsigned>((units + share - 1) / share));
     const size_t lds = static_cast<size_t>(T) * (rot / 2) * sizeof(float2);
     if (vec) rotate_kernel<KT, 4><<<grid, 256, lds, st>>>(a, T, share);
