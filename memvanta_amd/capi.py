@@ -208,6 +208,14 @@ def _host_rows(a):
     return a[None] if a.ndim == 1 else a
 
 
+def _host_int32(a, name: str):
+    """Host integers as int32; what does not fit is refused, not wrapped."""
+    a = np.asarray(a)
+    if a.size and not ((a >= -2 ** 31) & (a < 2 ** 31)).all():
+        raise ValueError(f"{name} must be 32-bit integers")
+    return np.ascontiguousarray(a, np.int32)
+
+
 def _rows(a):
     """(address, rows, elements of a row, elements from one row to the next) of float32 rows: a host array from
     _host_rows, or a device tensor, which may be a view with a row stride."""
@@ -363,7 +371,7 @@ class Context:
             rows, n = logits.shape
             out = {"entropy": np.empty(rows, np.float32)}
             if targets is not None:
-                targets = np.ascontiguousarray(targets, np.int32).reshape(rows)
+                targets = _host_int32(targets, "targets").reshape(rows)
                 out["logprob"] = np.empty(rows, np.float32)
             if top_k:
                 out["top_ids"] = np.empty((rows, top_k), np.int32)
@@ -505,7 +513,7 @@ class Rope:
             x = _host_rows(x)
             out = np.empty((x.shape[0], n_head * self.head_dim), np.float32) if out is None else out
             if positions is not None:
-                positions = np.ascontiguousarray(positions, np.int32)
+                positions = _host_int32(positions, "positions")
         elif out is None:
             raise ValueError("device rows need an out")
         if isinstance(out, np.ndarray) != host:
