@@ -240,7 +240,7 @@ typedef struct mvh_rope_config {
     int layout;        /* MVH_ROPE_HALF or MVH_ROPE_INTERLEAVED */
     int scaling;       /* MVH_ROPE_SCALE_* */
     double base;       /* > 1 */
-    double factor;     /* > 0; read unless scaling is NONE */
+    double factor;     /* 2^-20 or more; read unless scaling is NONE */
     double orig_ctx;   /* trained context, TURNS and INDEX: > 0 */
     double low, high;  /* turns, TURNS and INDEX: 0 < low < high */
     double attn_scale; /* > 0; 1 leaves lengths as they are */

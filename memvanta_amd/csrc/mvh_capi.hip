@@ -1200,6 +1200,8 @@ int mvh_rope_create(mvh_context* c, const mvh_rope_config* cfg, mvh_rope** out) 
     const bool blend = cfg->scaling == MVH_ROPE_SCALE_TURNS || cfg->scaling == MVH_ROPE_SCALE_INDEX;
     if (cfg->scaling != MVH_ROPE_SCALE_NONE && !positive(cfg->factor))
         return fail(MVH_E_INVALID, "rope factor must be positive");
+    // an angle is pos f: 31 bits of position and 20 more leave it and its reduction a meaning in 64
+    if (cfg->scaling != MVH_ROPE_SCALE_NONE && cfg->factor < 0x1p-20) return fail(MVH_E_RANGE, "rope factor below 2^-20");
     if (blend && (!positive(cfg->orig_ctx) || !positive(cfg->low) || !positive(cfg->high) || cfg->low >= cfg->high))
         return fail(MVH_E_INVALID, "rope scaling needs orig_ctx > 0 and 0 < low < high");
     auto* r = new (std::nothrow) mvh_rope;

@@ -21,9 +21,10 @@ struct RopeView {
 };
 
 // sin and cos of an angle: the nearest multiple k of pi/2 taken off with pi/2
-// in two doubles (k < 2^31: the fused products keep the rest exact to 1e-16),
-// then the Taylor series on |y| <= pi/4, cut where the next term is below
-// 2^-45 -- 2^-21 of half an fp32 step.
+// in two doubles (k < 2^51, of 2^31 positions and factors of 2^-20: the fused
+// products keep the rest exact to 1e-16), then the Taylor series on |y| <= pi/4,
+// cut where the next term is below 2^-45 -- 2^-21 of half an fp32 step (1.1,
+// where k from 2^49 on is off by one: 2^-38).
 __device__ __forceinline__ void sin_cos(double a, double& s, double& c) {
     const double k = rint(a * 0.63661977236758134308);
     double y = fma(-k, 1.57079632679489655800, a);
