@@ -50,10 +50,13 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // seen there (unit_of): 1 while that is in [2^-7, 2), else what brings it to [1/2,
 // 1); it falls, and the sums with it, when a step times u reaches 2.  u >= 1
 // scales the steps, exactly; blocks with u < 1 (a step of 2 .. 512) form p s u in
-// 32 bits and split it.  p s u is below 2^15, and off by 2^-22 of itself or 2^-35
-// of the largest weight times the block's largest step, whatever other blocks
-// hold.  A wave's first step looks whether all its blocks start with u = 1; while
-// they stay there, the usual case, steps are taken as they are.
+// 32 bits and split it.  p s u is below 2^15, and p s off by 2^-22 of itself or
+// 2^-28 of the largest weight times the block's largest step (2^-35 where that is
+// not in [2^-7, 1)), whatever other blocks hold.  A wave's first step looks whether
+// all its blocks start with u = 1; while they stay there, the usual case, steps
+// are taken as they are.  256 tokens at
+// 16000, 8 kv heads of 128: 180 us, with values of size 0.01 191, with a row of 200 in
+// one block of each head 195; one u for the head was 177.
 //
 // The exponent of a weight is y_scale s - y_scale m + kLift, the second product
 // rounded once for all of a step's rows (and for the join); where it is beyond
@@ -196,14 +199,15 @@ __device__ __forceinline__ void write_sum(const Q4Args& a, int kh, int row, int 
 // then holds p of 8 consecutive cache rows of one query row: with the cache
 // rows in that order in V's words too, p is the next product's operand as it
 // is.  sum p c and sum p are one more product whose operand rows are the
-// blocks' c, and ones.  64 query rows on 8 kv heads of 128 at position 1500: 13.1
-// us, 8 rows at 30000: 18.7 (2.1 TB/s); VALU-bound (9 operations unpack 8 codes,
-// 3 scale 2 weights in both parts).
+// blocks' c, and ones.  64 query rows on 8 kv heads of 128 at position 1500: 13.5
+// us, 8 rows at 30000: 19.0 (2.1 TB/s).  Neither pipe is a bound (VALU 20 and 40 %
+// busy, matrix pipe 3 and 11 %): two waves per SIMD wait for their loads and for
+// each other's turns, at the start most of all (a token at 100: 5.8 us).
 //
 // PART: heads that do not fill NB whole blocks.  A head's channels lie in the
 // blocks from its first one on, with q zero at the others' channels of these
-// (6 heads of 48 at position 1500: 9.4 us, 64 tokens there 12.0; on the kernel
-// for heads of more than 8 blocks 35.5 and 192).
+// (6 heads of 48 at position 1500: 9.6 us, 64 tokens there 12.1; on the kernel
+// for heads of more than 8 blocks 35.3 and 192).
 template <int NB, bool UNI, bool PART>
 __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4Args a) {
     constexpr int HD = 32 * NB, PITCH = HD + 4;
@@ -618,7 +622,9 @@ __global__ __launch_bounds__(64 * kWaves, NB > 4 ? 1 : 2) void attn_q4_kernel(Q4
 // The scores leave a lane with four cache rows of one query row, which is the
 // operand that the values take.  Rows of a group go in the order of the scales
 // (0 4 1 5, 2 6 7 3), as the words unpack.  65000 rows of 8 kv heads of 128, 4
-// heads each: 21.4 us (3.9 TB/s), with the kernel above 26.5.
+// heads each: 24.0 us with the join (alone 21.6 traced, 3.9 TB/s), with the kernel
+// above 26.5.  Of its wave cycles 31 % wait, with two waves per SIMD (204
+// registers) that load one step ahead; VALU 48 %, matrix pipe 16 % busy.
 template <int NB, bool UNI>
 __global__ __launch_bounds__(64 * kWaves, 2) void attn_q4_narrow_kernel(Q4Args a) {
     constexpr int HD = 32 * NB, NH = NB / 2, NR = 2 * NB;  // 64-channel halves; q registers (of four channel steps)
@@ -1100,10 +1106,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_q4_narrow_kernel(Q4Args a
 // of steps or middles.  q lies in LDS for all waves; a step's scales go
 // through LDS too, where 32 lanes read the same ones (from the caches such
 // loads would take as long as the arithmetic).  256 tokens at 1700, 32 heads on 8
-// of 128: 28.6 us (16 rows a tile: 39.6), of which 9 start and end; a step of 32
-// x 32 takes a wave 440 VALU operations beside 37 matrix instructions (VALU 44 %,
-// matrix pipe 22 % busy at two waves per SIMD; four waves a workgroup 1.15 times
-// as long).
+// of 128: 29.5 us (16 rows a tile: 38.5), of which 9 start and end; at 16000: 180.
+// A step of 32 x 32 takes a wave 460 VALU operations beside 37 matrix
+// instructions, which run in turn (VALU 44 %, matrix pipe 21 % busy at 1700, 52 and
+// 31 % at 16000): 256 registers, with 21 .. 22 spilled around the loops of heads of
+// 128 and none in the one of whole steps, and 147 KB of LDS leave two waves per
+// SIMD and a workgroup a CU (four waves a workgroup: 1.15 times as long).
 constexpr int kRows32 = 32, kWaves32 = 8;
 enum class Pages { kSteps, kGroups, kRows };  // pages of whole steps, of whole groups of 8 rows, of any number of rows
 template <int NB, Pages PAGES>
@@ -1271,7 +1279,7 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
     // the rows that group vg has on its page: 1 .. 8, or more
     auto room_of = [&](int vg) { return a.map.page_tokens - (vg - a.map.page_of(vg) * groups) * 8; };
     // EDGE: rows that some query rows do not see; PAD: pages that end inside a group, whose other slots hold anything: their
-    // scales are cleared on the way into LDS (pages of 20 rows, 256 tokens at 16000: 236 us; with every step an EDGE 354)
+    // scales are cleared on the way into LDS (pages of 20 rows, 256 tokens at 16000: 246 us; with every step an EDGE 406)
     auto step = [&](auto kind_tag) {
         constexpr bool EDGE = decltype(kind_tag)::value == 2, PAD = decltype(kind_tag)::value == 1;
         const int nst = after(st);
@@ -1437,6 +1445,9 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
             for (int i = 0; i < 16; ++i) sc[i] -= base;
         }
         const float below = far ? kLift : fmaf(-m, y_scale, kLift);
+        half2v times[NB];  // where rows differ in what they see, each query row's own; 0: formed here
+#pragma unroll
+        for (int b = 0; b < NB; ++b) times[b] = both(kUnitOne);
         if (uneven) {
             float scale = y_scale;
             asm("" : "+v"(scale));  // or the weights are formed for both here, apart from the products below
@@ -1463,7 +1474,11 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
                     o[b] = mfma(w, fh, o[b]);
                 }
             }
-            if (!EDGE && sl_p < 16 && (NB == 4 || lane < 32)) {  // where rows differ in what they see, each takes its own below
+            if constexpr (EDGE) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b) times[b] = as_half2(below_1(unit(b)) ? 0u : as_u32(unit(b)));
+            }
+            if (!EDGE && sl_p < 16 && (NB == 4 || lane < 32)) {
                 uint2* const s = reinterpret_cast<uint2*>(s_sc + SCALES + (sl_b * 4 + sl_g) * 32 + sl_p);
                 *s = below_1(most_unit) ? make_uint2(0u, 0u)
                                         : make_uint2(as_u32(as_half2(s->x) * most_unit), as_u32(as_half2(s->y) * most_unit));
@@ -1490,8 +1505,6 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
             }
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                half2v u = {};
-                if constexpr (EDGE) u = unit(b);
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     const u32x4 s = scales(1, b, k, 0);
@@ -1499,7 +1512,7 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         half2v z = as_half2(s[i]);
-                        if constexpr (EDGE) z = as_half2(below_1(u) ? 0u : as_u32(as_half2(s[i] & seen[k][i]) * u));
+                        if constexpr (EDGE) z = as_half2(s[i] & seen[k][i]) * times[b];
                         uint32_t h, l;
                         times_steps(as_half2(ph[k][i]), as_half2(pl[k][i]), z, h, l);
                         fh[i] = h;
@@ -1675,7 +1688,7 @@ __global__ __launch_bounds__(kAny) void attn_q4_any_kernel(Q4Args a) {
 // thread, the splits in turn over the workgroup's groups of hd / 4 threads (as
 // many for any number of splits: a row's sums have one order in every chunk).  Latency is all it spends: the first
 // kAhead values of a thread are on their way before the weights are known
-// (one token at 65000: 23.5 us with the kernel before it, 24.4 with a thread a channel and no reads ahead).
+// (one token at 65000: 24.0 us with the kernel before it; a thread a channel and no reads ahead take 0.9 more).
 constexpr int kMaxSplit = 256, kJoin = 512, kAhead = 8;
 __global__ __launch_bounds__(kJoin) void attn_q4_join_kernel(Q4Args a, int n_split) {
     __shared__ float s_w[kMaxSplit];
@@ -1752,15 +1765,15 @@ bool q4_tiles(size_t hd) { return q4_cover(hd) <= 8; }
 // bits it has in any other chunk: one kernel for all (the tiles of 32 rows, where
 // they take the head).  Else, by query rows of a kv head and steps of 32 cache rows:
 //   up to 4 rows, from 32 steps on, the 4 x 4 products.  8 kv heads of 128,
-//     1 / 4 rows, against the tiles of 16: position 1500 9.1 / 10.3 us against
-//     9.5 / 10.3, 30000 15.0 / 17.2 against 16.6 / 17.6; below, fewer of the waves
-//     have a step: position 100 5.5 / 6.4 against 5.0 / 5.5;
+//     1 / 4 rows, against the tiles of 16: position 1500 9.7 / 10.6 us against
+//     10.3 / 10.8, 30000 15.2 / 17.3 against 17.4 / 18.1; below, fewer of the waves
+//     have a step: position 100 5.7 / 6.7 against 5.4 / 5.9;
 //   the tiles of 32 rows from 16 rows and 32768 rows x steps x kv heads on (they
 //     unpack a step for twice the rows, but start and end slower): position 1500,
-//     64 / 256 rows 14.4 / 19.0 us against 13.1 / 21.5; 16000, 8 / 16 / 32 rows
-//     15.1 / 15.5 / 16.4 against 14.5 / 16.9 / 20.8; 100, 256 / 1024 rows 10.1 /
-//     12.1 against 8.9 / 13.7; 4 kv heads of 64, 16000, 16 / 32 rows 11.4 / 11.5
-//     against 10.5 / 12.6.
+//     64 / 256 rows 15.9 / 21.0 us against 13.5 / 23.3; 16000, 8 / 16 / 32 rows
+//     15.5 / 16.3 / 17.3 against 14.8 / 17.9 / 21.7; 100, 256 / 1024 rows 11.4 /
+//     12.8 against 9.2 / 14.2; 4 kv heads of 64, 16000, 16 / 32 rows 12.4 / 12.0
+//     against 10.7 / 12.5.
 enum class Q4Kind { kNarrow, kTile16, kTile32, kAny };
 Q4Kind q4_kind(size_t hd, size_t rows, size_t steps, size_t n_head_kv, size_t chunk) {
     if (!q4_tiles(hd)) return Q4Kind::kAny;

@@ -14,8 +14,11 @@
 // least k elements reach, and few more (24 of 32000 random ones for k = 20);
 // what reaches it is set aside in LDS, sorted by value, then index, by the waves
 // 64 at a time, and merged by one into the best 64 so far.  In later tiles the
-// bound is the k-th best so far.  Where too many are equal (a masked row) every
-// wave sorts its own elements 64 at a time instead.
+// bound is the k-th best so far.  Where too many are equal (a row with fewer
+// unmasked tokens than k, or than there are groups that hold one) every wave
+// sorts its own elements 64 at a time instead, three to four times as long (one row
+// of 32000 with 64 tops 12.3 us, 42 with 32 tokens left; 768 rows with 20 tops 29
+// and 114).
 #include "mvh_kernels.hpp"
 
 #include <type_traits>
@@ -399,6 +402,8 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(LpArgs a) {
 // workgroup a CU without top tokens, two with (the search for them waits more).
 // 32000 logits, 256 / 400 rows without: 6.5 / 12.2 us against 7.5 / 11.1 with 256
 // threads; with 20 top tokens 1 / 512 / 768 rows: 8.6 / 22.8 / 32.4 against 17.5 / 25.0 / 29.4.
+// The wide forms take 73 registers with top tokens (one workgroup a CU, where 64
+// would let in two) and 128 with 11 spilled without.
 bool lp_wide(size_t n, size_t rows, size_t k) { return n > 256 * kPer && rows <= (k ? 512 : 256); }
 size_t lp_parts(size_t n, size_t rows, size_t k) {
     if (!lp_wide(n, rows, k) || n <= 2 * 1024 * kPer) return 1;
