@@ -1478,6 +1478,7 @@ __global__ __launch_bounds__(64 * kWaves32, 2) void attn_q4_tile_kernel(Q4Args a
 #pragma unroll
                 for (int b = 0; b < NB; ++b) times[b] = as_half2(below_1(unit(b)) ? 0u : as_u32(unit(b)));
             }
+            __builtin_amdgcn_wave_barrier();  // the steps above are read before other lanes change them
             if (!EDGE && sl_p < 16 && (NB == 4 || lane < 32)) {
                 uint2* const s = reinterpret_cast<uint2*>(s_sc + SCALES + (sl_b * 4 + sl_g) * 32 + sl_p);
                 *s = below_1(most_unit) ? make_uint2(0u, 0u)
