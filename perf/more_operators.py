@@ -188,12 +188,14 @@ def prepare(case, seed):
 # ---- the operators in their plain form ------------------------------------------------------------------------
 
 def _eight_bits(x):
-    """x [rows][cols] as it is in e4m3 with a scale per 128 columns: the largest |x| / 448, codes by ties to even."""
+    """x [rows][cols] as it is in e4m3 with a scale s per 128 columns: s = the largest |x| / 448, codes x (1 / s), ties to
+    even; a block whose scale is no normal number is held as zeros."""
     rows, cols = x.shape
     b = torch.nn.functional.pad(x, (0, -cols % 128)).reshape(rows, -1, 128)
     top = b.abs().amax(dim=2, keepdim=True)
     scale = top / torch.full_like(top, TOP)
-    z = torch.where(scale > 0, b / scale, torch.zeros_like(b)).clamp(-TOP, TOP)
+    scale = torch.where(scale < 2.0 ** -126, torch.zeros_like(scale), scale)
+    z = torch.where(scale > 0, b * (torch.ones_like(scale) / scale), torch.zeros_like(b))
     exponent = (torch.frexp(z)[1] - 1).clamp(min=-6)  # 3 bits after the leading one; steps of 2^-9 below 2^-6
     z = torch.ldexp(torch.round(torch.ldexp(z, 3 - exponent)), exponent - 3)
     return (z * scale).reshape(rows, -1)[:, :cols]
@@ -285,7 +287,9 @@ def _quantised(x):
     for block in x.split(128, dim=1):
         largest = torch.linalg.vector_norm(block, ord=math.inf, dim=1, keepdim=True)
         scale = torch.div(largest, torch.full_like(largest, 448))
-        parts.append(torch.div(block, scale).nan_to_num(0.0).to(torch.float8_e4m3fn).double() * scale.double())
+        inverse = torch.reciprocal(scale.double()).float()
+        code = torch.mul(block, inverse).to(torch.float8_e4m3fn).double() * scale.double()
+        parts.append(torch.where(scale.double() < 2.0 ** -126, torch.zeros_like(code), code))
     return torch.cat(parts, dim=1)
 
 
