@@ -107,6 +107,15 @@ extern "C" {
 #define MVH_TYPE_NATIVE_Q4_0 0x1002
 #define MVH_TYPE_NATIVE_Q8_0 0x1008
 
+/* No counterpart in the reference: 8-bit floating point (e4m3: 4 bits of exponent, 3 of mantissa, no infinities, largest
+ * value 448) with a float scale per 128 x 128 elements: codes [ne1][ne0], then scales [ceil(ne1/128)][ceil(ne0/128)].
+ * ne0 % 16 == 0.  Only mvh_matmul_fp8 and mvh_gated_ffn_fp8 accept it. */
+#define MVH_TYPE_FP8_B128 0x1010
+
+/* the activation of mvh_gated_ffn_fp8 */
+#define MVH_GATE_SILU 0 /* g / (1 + e^-g) */
+#define MVH_GATE_GELU 1 /* g (1 + erf(g / sqrt(2))) / 2 */
+
 typedef struct mvh_context mvh_context;
 typedef struct mvh_tensor mvh_tensor;
 typedef struct mvh_kv_cache mvh_kv_cache;
@@ -201,6 +210,24 @@ int mvh_matmul_q4_0_batch(mvh_context* ctx, const mvh_tensor* a, const float* x,
 /* matvec_q4_0 / matvec_q8_0: y[r] = dot_q4_0 / dot_q8_0(row r, x), fp32 activations */
 int mvh_matvec_q4_0(mvh_context* ctx, const mvh_tensor* a, const float* x, float* y, int ptr_kind);
 int mvh_matvec_q8_0(mvh_context* ctx, const mvh_tensor* a, const float* x, float* y, int ptr_kind);
+
+/* ---- 8-bit floating point weights (no counterpart in the reference) ---- */
+/* x [rows][cols] (cols % 16 == 0) to e4m3 codes [rows][cols] and scales [ceil(rows/block_rows)][ceil(cols/128)], one per
+ * block_rows (1 or 128) rows and 128 columns: scale = max |x| / 448, code = x times the scale's inverse, each rounded to 32
+ * bits, then to e4m3, ties to even.  A block whose scale would be below 2^-126 is held as zeros (scale 0); one with a NaN or
+ * an infinity has such a scale and reads as NaN.  block_rows 128 with scales behind the codes are the bytes of a
+ * MVH_TYPE_FP8_B128 tensor.  Device x must be 16-byte aligned, codes and scales 4-byte. */
+int mvh_quantize_fp8(mvh_context* ctx, const float* x, size_t rows, size_t cols, size_t block_rows, uint8_t* codes,
+                     float* scales, int ptr_kind);
+/* y [batch][ne1] = x [batch][ne0] times the MVH_TYPE_FP8_B128 tensor w; x is quantised as mvh_quantize_fp8 does it with
+ * block_rows 1, products of codes and their sums over 128 are the matrix pipe's, scales and sums of blocks fp32.  A token's bits may depend on
+ * the batch's size, whose kernels add in different orders.  Uses the context's workspace: see mvh_attn_decode for calls
+ * captured into graphs. */
+int mvh_matmul_fp8(mvh_context* ctx, const mvh_tensor* w, const float* x, float* y, size_t batch, int ptr_kind);
+/* The gated feed-forward block before its last product: y [batch][ne1] = act(x gate^T) * (x up^T), both tensors
+ * MVH_TYPE_FP8_B128 of one shape, act MVH_GATE_*; x and the products as in mvh_matmul_fp8, act and the product fp32. */
+int mvh_gated_ffn_fp8(mvh_context* ctx, const mvh_tensor* gate, const mvh_tensor* up, int act, const float* x, float* y,
+                      size_t batch, int ptr_kind);
 
 /* ---- paged KV cache (F32 / F16 / Q8 / Q4 pages): all layers of one model on one device ---- */
 /* parse_kv_cache_type: "f32", "f16", "q8" or "q8_0", and "q4"; anything else fails with

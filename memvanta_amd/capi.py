@@ -24,6 +24,8 @@ MVH_KV_Q4 = 3  # 4-bit codes, a step and a middle per block of 32
 MVH_ROPE_HALF, MVH_ROPE_INTERLEAVED = 0, 1
 MVH_ROPE_SCALE_NONE, MVH_ROPE_SCALE_LINEAR, MVH_ROPE_SCALE_TURNS, MVH_ROPE_SCALE_INDEX = 0, 1, 2, 3
 MVH_TYPE_NATIVE_Q4_0, MVH_TYPE_NATIVE_Q8_0 = 0x1002, 0x1008  # BlockQ4_0 (20 B) / BlockQ8_0 (36 B) of quant.hpp
+MVH_TYPE_FP8_B128 = 0x1010  # e4m3 codes, a float scale per 128 x 128
+MVH_GATE_SILU, MVH_GATE_GELU = 0, 1
 KV_DTYPE = {MVH_KV_F32: np.float32, MVH_KV_F16: np.uint16, MVH_KV_Q8: np.int8,
             MVH_KV_Q4: np.float32}
 STATUS = {0: "MVH_OK", 1: "MVH_E_INVALID", 2: "MVH_E_SHAPE", 3: "MVH_E_TYPE", 4: "MVH_E_DEVICE",
@@ -87,6 +89,9 @@ _SIGS = {
     "mvh_rope_apply": (_int, [_vp, _vp, _vp, _sz, _sz, _sz, _vp, _sz, _vp, _sz, _int]),
     "mvh_kv_append": (_int, [_vp, _vp, _sz, _sz, _sz, _vp, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _int]),
     "mvh_logprobs": (_int, [_vp, _vp, _sz, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _int]),
+    "mvh_quantize_fp8": (_int, [_vp, _vp, _sz, _sz, _sz, _vp, _vp, _int]),
+    "mvh_matmul_fp8": (_int, [_vp, _vp, _vp, _vp, _sz, _int]),
+    "mvh_gated_ffn_fp8": (_int, [_vp, _vp, _vp, _int, _vp, _vp, _sz, _int]),
     "mvh_model_open": (_int, [C.c_char_p, _int, _sz, _sz, _int, _int, _sz, C.POINTER(_vp)]),
     "mvh_model_kv_type": (_int, [_vp, C.POINTER(_int)]),
     "mvh_model_close": (_int, [_vp]),
@@ -239,6 +244,18 @@ def _rows(a):
     if stride[-1] != 1 and width > 1:
         raise ValueError("a row's elements must be consecutive")
     return a.data_ptr(), n, width, stride[0] if n > 1 else width
+
+
+def _flat(a, dtype: str, count: int, host: bool, name: str) -> int:
+    """Address of a contiguous array of at least count elements, on the side that the call is on."""
+    if isinstance(a, np.ndarray):
+        good = host and a.dtype == dtype and a.size >= count and a.flags["C_CONTIGUOUS"]
+    else:
+        good = (not host and a is not None and str(a.dtype) == "torch." + dtype and a.numel() >= count
+                and a.is_contiguous() and a.is_cuda)
+    if not good:
+        raise ValueError(f"{name} must be {count} contiguous elements of {dtype} in {'host' if host else 'device'} memory")
+    return _ptr(a)
 
 
 class Context:
@@ -456,6 +473,58 @@ class Context:
             x = np.ascontiguousarray(x, np.float32)
             y = np.empty(a.ne1, np.float32)
         self._check(fn(self.h, a.h, _ptr(x), _ptr(y), _kind(x, y)))
+        return y
+
+    # -- 8-bit floating point weights --
+    def quantize_fp8(self, x, block_rows: int = 1, codes=None, scales=None):
+        """mvh_quantize_fp8 of rows x: (codes uint8 [rows][cols], scales float32 [ceil(rows/block_rows)][ceil(cols/128)]);
+        device rows need both outputs."""
+        host = isinstance(x, np.ndarray)
+        if host:
+            x = _host_rows(x)
+        at, n, cols, pitch = _rows(x)
+        if pitch != cols:
+            raise ValueError("x must be contiguous rows")
+        shape = ((n + block_rows - 1) // max(1, block_rows), (cols + 127) // 128)
+        if host and codes is None and scales is None:
+            codes, scales = np.empty((n, cols), np.uint8), np.empty(shape, np.float32)
+        c_at = _flat(codes, "uint8", n * cols, host, "codes")
+        s_at = _flat(scales, "float32", shape[0] * shape[1], host, "scales")
+        self._check(self.lib.mvh_quantize_fp8(self.h, at, n, cols, block_rows, c_at, s_at, MVH_HOST if host else MVH_DEVICE))
+        return codes, scales
+
+    def upload_fp8(self, name: str, w: np.ndarray) -> "Tensor":
+        """A host matrix [rows][cols] as a MVH_TYPE_FP8_B128 tensor."""
+        codes, scales = self.quantize_fp8(w, 128)
+        return self.upload(name, MVH_TYPE_FP8_B128, codes.shape[1], codes.shape[0],
+                           np.concatenate([codes.ravel(), scales.ravel().view(np.uint8)]))
+
+    def _fp8_rows(self, w: "Tensor", x, y):
+        """(x, y, addresses, rows) of a product with w."""
+        host = isinstance(x, np.ndarray)
+        if host:
+            x = _host_rows(x)
+            y = np.empty((x.shape[0], w.ne1), np.float32) if y is None else y
+        elif y is None:
+            raise ValueError("device rows need a y")
+        if isinstance(y, np.ndarray) != host:
+            raise ValueError("mix of host and device buffers in one call")
+        x_at, n, width, pitch = _rows(x)
+        y_at, y_n, y_width, y_pitch = _rows(y)
+        if width != w.ne0 or y_width != w.ne1 or y_n != n or pitch != width or y_pitch != y_width:
+            raise ValueError("x must be contiguous rows of ne0 elements and y as many of ne1")
+        return y, x_at, y_at, n, MVH_HOST if host else MVH_DEVICE
+
+    def matmul_fp8(self, w: "Tensor", x, y=None):
+        """mvh_matmul_fp8: rows x [batch][ne0] times the FP8 tensor w."""
+        y, x_at, y_at, n, kind = self._fp8_rows(w, x, y)
+        self._check(self.lib.mvh_matmul_fp8(self.h, w.h, x_at, y_at, n, kind))
+        return y
+
+    def gated_ffn_fp8(self, gate: "Tensor", up: "Tensor", x, act: int = MVH_GATE_SILU, y=None):
+        """mvh_gated_ffn_fp8: act(x gate^T) * (x up^T)."""
+        y, x_at, y_at, n, kind = self._fp8_rows(gate, x, y)
+        self._check(self.lib.mvh_gated_ffn_fp8(self.h, gate.h, up.h, act, x_at, y_at, n, kind))
         return y
 
     def kv_cache(self, n_layer: int, kv_dim: int, page_tokens: int = 128, max_tokens: int = 2048,

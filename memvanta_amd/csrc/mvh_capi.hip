@@ -110,13 +110,17 @@ const char* type_name(uint32_t t) {
         case MVH_TYPE_Q6_K: return "Q6_K";
         case MVH_TYPE_NATIVE_Q4_0: return "native Q4_0";
         case MVH_TYPE_NATIVE_Q8_0: return "native Q8_0";
+        case MVH_TYPE_FP8_B128: return "FP8";
     }
     return "type-?";
 }
 
 // ggml_tensor_nbytes (src/gguf.cpp:82-105) for the accepted types; 0 = invalid
-uint64_t tensor_nbytes(uint32_t t, uint64_t n) {
+uint64_t tensor_nbytes(uint32_t t, uint64_t ne0, uint64_t ne1) {
+    const uint64_t n = ne0 * ne1;
     switch (t) {
+        case MVH_TYPE_FP8_B128:  // sides up to the kernels' int: the product stays below 2^62
+            return ne0 % 16 || ne0 > 0x7fffffff || ne1 > 0x7fffffff ? 0 : n + (ne1 + 127) / 128 * ((ne0 + 127) / 128) * 4;
         case MVH_TYPE_F32: return n * 4;
         case MVH_TYPE_F16: return n * 2;
         case MVH_TYPE_Q4_0: return n % 32 ? 0 : n / 32 * 18;
@@ -281,7 +285,8 @@ namespace prof = memvanta::hip::prof;
 // records the stop event before the output copy and waits for it.
 class ProfSpan {
 public:
-    ProfSpan(mvh_context* c, const mvh_tensor* w, size_t batch) : name_(w->name), batch_(batch) {
+    ProfSpan(mvh_context* c, const mvh_tensor* w, size_t batch) : ProfSpan(c, w->name, batch) {}
+    ProfSpan(mvh_context* c, std::string name, size_t batch) : name_(std::move(name)), batch_(batch) {
         if (!prof::enabled()) return;
         rec_.emplace(c->stream);
         if (rec_->start() != hipSuccess) rec_.reset();
@@ -518,9 +523,10 @@ static int make_tensor(mvh_context* c, const char* name, uint32_t type, uint64_t
                        mvh_tensor** out) {
     if (!out) return fail(MVH_E_INVALID, "null out");
     *out = nullptr;
-    const uint64_t want = tensor_nbytes(type, ne0 * ne1);
+    const uint64_t want = tensor_nbytes(type, ne0, ne1);
     if (type != MVH_TYPE_F32 && type != MVH_TYPE_F16 && type != MVH_TYPE_Q4_0 && type != MVH_TYPE_Q8_0 &&
-        type != MVH_TYPE_Q6_K && type != MVH_TYPE_NATIVE_Q4_0 && type != MVH_TYPE_NATIVE_Q8_0)
+        type != MVH_TYPE_Q6_K && type != MVH_TYPE_NATIVE_Q4_0 && type != MVH_TYPE_NATIVE_Q8_0 &&
+        type != MVH_TYPE_FP8_B128)
         return fail(MVH_E_TYPE, "unsupported GGML type %u: %s", type, name ? name : "");
     if (!want || want != nbytes)
         return fail(MVH_E_SHAPE, "tensor byte size %llu does not match %s [%llu x %llu]: %s",
@@ -614,8 +620,9 @@ int mvh_quantize_q8(mvh_context* c, const float* x, size_t batch, size_t cols, i
     return MVH_OK;
 }
 
+// a type that only calls of its own accept
 static bool is_native(const mvh_tensor* w) {
-    return w->type == MVH_TYPE_NATIVE_Q4_0 || w->type == MVH_TYPE_NATIVE_Q8_0;
+    return w->type == MVH_TYPE_NATIVE_Q4_0 || w->type == MVH_TYPE_NATIVE_Q8_0 || w->type == MVH_TYPE_FP8_B128;
 }
 
 int mvh_matvec(mvh_context* c, const mvh_tensor* w, const float* x, float* y, int kind) {
@@ -987,6 +994,99 @@ int mvh_matvec_q4_0(mvh_context* c, const mvh_tensor* w, const float* x, float* 
 
 int mvh_matvec_q8_0(mvh_context* c, const mvh_tensor* w, const float* x, float* y, int kind) {
     return native_f32act(c, w, MVH_TYPE_NATIVE_Q8_0, "matvec_q8_0", "q8_0 cols must be multiple of 32", x, y, 1, kind);
+}
+
+// ---- 8-bit floating point weights ----
+
+int mvh_quantize_fp8(mvh_context* c, const float* x, size_t rows, size_t cols, size_t block_rows, uint8_t* codes,
+                     float* scales, int kind) {
+    CHECK_CTX(c);
+    if (kind != MVH_HOST && kind != MVH_DEVICE) return fail(MVH_E_INVALID, "ptr_kind must be MVH_HOST or MVH_DEVICE");
+    if (block_rows != 1 && block_rows != 128) return fail(MVH_E_INVALID, "block_rows must be 1 or 128");
+    if (cols % 16) return fail(MVH_E_SHAPE, "fp8 columns must be a multiple of 16");
+    if (cols > 0x7fffff00 || rows > 0x7fffffff) return fail(MVH_E_RANGE, "fp8 rows or columns above 2147483392");
+    if (!rows || !cols) return MVH_OK;
+    if (!x || !codes || !scales) return fail(MVH_E_INVALID, "null argument");
+    const size_t blocks = (cols + 127) / 128, n_scale = (rows + block_rows - 1) / block_rows * blocks;
+    // a launch's grid has fewer than 2^32 threads: 32 lanes a block of a row, 256 a block of 128 rows
+    if (n_scale > (block_rows == 1 ? size_t{1} << 26 : size_t{1} << 23)) return fail(MVH_E_RANGE, "fp8 matrix too large");
+    if (kind == MVH_DEVICE && ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(scales)) & 3))
+        return fail(MVH_E_INVALID, "device codes and scales must be 4-byte aligned");
+    const void* xd = nullptr;
+    if (int rc = stage_in_act(c, c->xin, x, rows * cols * 4, kind, &xd)) return rc;
+    uint8_t* cd = codes;
+    float* sd = scales;
+    if (kind == MVH_HOST) {
+        if (int rc = grow(c, c->yout, rows * cols + n_scale * 4)) return rc;
+        cd = static_cast<uint8_t*>(c->yout.p);
+        sd = reinterpret_cast<float*>(cd + rows * cols);
+    }
+    MVH_HIP(mvh::launch_quantize_fp8(static_cast<const float*>(xd), rows, cols, block_rows, cd, sd, c->stream));
+    if (kind == MVH_HOST) {
+        MVH_HIP(hipMemcpyAsync(codes, cd, rows * cols, hipMemcpyDeviceToHost, c->stream));
+        MVH_HIP(hipMemcpyAsync(scales, sd, n_scale * 4, hipMemcpyDeviceToHost, c->stream));
+        MVH_HIP(hipStreamSynchronize(c->stream));
+    }
+    return MVH_OK;
+}
+
+static int need_fp8(const mvh_context* c, const mvh_tensor* w, const char* fn) {
+    if (!w) return fail(MVH_E_INVALID, "null tensor");
+    if (w->type != MVH_TYPE_FP8_B128)
+        return fail(MVH_E_TYPE, "%s needs a FP8 tensor, got %s: %s", fn, type_name(w->type), w->name.c_str());
+    if (w->device != c->device)
+        return fail(MVH_E_INVALID, "tensor of device %d used with a context of device %d: %s", w->device, c->device,
+                    w->name.c_str());
+    return MVH_OK;
+}
+
+// mvh_matmul_fp8, or with up mvh_gated_ffn_fp8, past the tensors' checks
+static int fp8_call(mvh_context* c, const mvh_tensor* w, const mvh_tensor* up, int act, const float* x, float* y, size_t batch,
+                    int kind) {
+    if (kind != MVH_HOST && kind != MVH_DEVICE) return fail(MVH_E_INVALID, "ptr_kind must be MVH_HOST or MVH_DEVICE");
+    const size_t cols = w->ne0, rows = w->ne1;
+    if (batch > (size_t{1} << 20)) return fail(MVH_E_RANGE, "more than 1048576 tokens");
+    const size_t blocks = (cols + 127) / 128;
+    if (batch * blocks > (size_t{1} << 26) || (rows + 15) / 16 > (size_t{1} << 22))
+        return fail(MVH_E_RANGE, "fp8 product too large");
+    if (!batch) return MVH_OK;
+    if (!x || !y) return fail(MVH_E_INVALID, "null x/y");
+    const void* xd = nullptr;
+    if (int rc = stage_in_act(c, c->xin, x, batch * cols * 4, kind, &xd)) return rc;
+    float* yd = y;
+    if (kind == MVH_HOST) {
+        if (int rc = grow(c, c->yout, batch * rows * 4)) return rc;
+        yd = static_cast<float*>(c->yout.p);
+    }
+    if (int rc = grow_kept(c, c->work, mvh::fp8_scratch(cols, batch))) return rc;
+    std::string name;
+    try {
+        name = up ? w->name + "+" + up->name : w->name;
+    } catch (const std::bad_alloc&) {
+        return fail(MVH_E_NOMEM, "host allocation failed");
+    }
+    ProfSpan span(c, std::move(name), batch);
+    MVH_HIP(mvh::launch_fp8(static_cast<const uint8_t*>(w->d), up ? static_cast<const uint8_t*>(up->d) : nullptr, act,
+                            static_cast<const float*>(xd), yd, rows, cols, batch, c->work.p, c->stream));
+    if (int rc = span.end()) return rc;
+    return finish_out(c, y, yd, batch * rows * 4, kind);
+}
+
+int mvh_matmul_fp8(mvh_context* c, const mvh_tensor* w, const float* x, float* y, size_t batch, int kind) {
+    CHECK_CTX(c);
+    if (int rc = need_fp8(c, w, "matmul_fp8")) return rc;
+    return fp8_call(c, w, nullptr, 0, x, y, batch, kind);
+}
+
+int mvh_gated_ffn_fp8(mvh_context* c, const mvh_tensor* gate, const mvh_tensor* up, int act, const float* x, float* y,
+                      size_t batch, int kind) {
+    CHECK_CTX(c);
+    if (int rc = need_fp8(c, gate, "gated_ffn_fp8")) return rc;
+    if (int rc = need_fp8(c, up, "gated_ffn_fp8")) return rc;
+    if (gate->ne0 != up->ne0 || gate->ne1 != up->ne1)
+        return fail(MVH_E_SHAPE, "gate and up differ in shape: %s, %s", gate->name.c_str(), up->name.c_str());
+    if (act != MVH_GATE_SILU && act != MVH_GATE_GELU) return fail(MVH_E_INVALID, "bad gate activation %d", act);
+    return fp8_call(c, gate, up, act, x, y, batch, kind);
 }
 
 int mvh_kv_parse_type(const char* s, int* type) {

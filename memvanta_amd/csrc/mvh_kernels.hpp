@@ -175,6 +175,19 @@ size_t logprobs_scratch(size_t n, size_t rows, size_t k);
 hipError_t launch_logprobs(const float* logits, size_t pitch, size_t n, size_t rows, const int* targets, size_t k,
                            float* logprob, float* entropy, int* top_ids, float* top_lp, void* scratch, hipStream_t st);
 
+// ---- 8-bit floating point weights (mvh_fp8.hip) ----
+enum : int { kGateSilu = 0, kGateGelu = 1 };
+// x [rows][cols], cols % 16 == 0, to e4m3 codes [rows][cols] and scales
+// [ceil(rows / block_rows)][ceil(cols / 128)]; block_rows 1 or 128
+hipError_t launch_quantize_fp8(const float* x, size_t rows, size_t cols, size_t block_rows, uint8_t* codes, float* scales,
+                               hipStream_t st);
+// y [M][N] = x [M][K] w^T, or, with w2, act(x w^T) * (x w2^T) (gate: kGate*).
+// w: codes [N][K] (K % 16 == 0, 16-byte aligned), then scales
+// [ceil(N / 128)][ceil(K / 128)].  scratch: fp8_scratch(K, M) bytes, 16-byte aligned.
+size_t fp8_scratch(size_t K, size_t M);
+hipError_t launch_fp8(const uint8_t* w, const uint8_t* w2, int gate, const float* x, float* y, size_t N, size_t K, size_t M,
+                      void* scratch, hipStream_t st);
+
 // ---- measurement probe (mvh_probe.hip) ----
 // reads bytes (a multiple of 16) of buf once; sink holds sink_words words (at
 // least 256 x the grid: 8 workgroups per CU)
