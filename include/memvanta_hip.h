@@ -301,6 +301,20 @@ int mvh_attn_decode(mvh_context* ctx, const mvh_kv_cache* kv, size_t layer, cons
 int mvh_attn_batch(mvh_context* ctx, const mvh_kv_cache* kv, size_t layer, const float* q, size_t pos,
                    size_t n_tokens, size_t n_head, size_t n_head_kv, size_t head_dim, float* out, int ptr_kind);
 
+/* No counterpart in the reference: attention of a batch of sequences that share a prefix, whose rows are read once for
+ * all of them.  Sequence i has n_tokens[i] query tokens (n_tokens NULL: one each; 0: none) at positions pos[i]..; token b
+ * of it sees rows 0..prefix_len-1 of the cache `prefix` and rows prefix_len..pos[i]+b of its own cache kvs[i], which holds
+ * them at their positions (mvh_kv_write / mvh_kv_append with pos >= prefix_len; the pages below stay unallocated).  pos[i] >=
+ * prefix_len; prefix may be NULL when prefix_len is 0.  F16 and Q8 caches of one type and kv_dim, the sequences' of one
+ * page size; a cache may stand for several sequences, or be the prefix too.  head_dim up to 256.  q and out are rows of
+ * n_head*head_dim, the tokens of sequence 0, then of 1, ...; kvs, pos and n_tokens are host arrays, read during the call.
+ * A token's bits may depend on the batch, which decides how rows are cut and joined.  A NaN or an infinity in a row makes
+ * what a token that sees it gets from it NaN or infinite, and leaves other tokens alone.  For the context's workspace and
+ * calls captured into graphs see mvh_attn_decode. */
+int mvh_attn_shared(mvh_context* ctx, const mvh_kv_cache* prefix, size_t prefix_len, const mvh_kv_cache* const* kvs,
+                    const size_t* pos, const size_t* n_tokens, size_t n_seq, size_t layer, const float* q, size_t n_head,
+                    size_t n_head_kv, size_t head_dim, float* out, int ptr_kind);
+
 /* ---- kernel profiler: enable_kernel_profiling, reset_kernel_profile, kernel_profile_snapshot,
  * kernel_profile_kind_name (include/memvanta/gguf_kernels.hpp:11-23, src/gguf_kernels.cpp:34-73,:219-222) ----
  * While enabled, every mvh_matvec / mvh_matvec_q8 / mvh_matmul_batch / mvh_matmul_batch_v06 call, and

@@ -92,6 +92,7 @@ _SIGS = {
     "mvh_quantize_fp8": (_int, [_vp, _vp, _sz, _sz, _sz, _vp, _vp, _int]),
     "mvh_matmul_fp8": (_int, [_vp, _vp, _vp, _vp, _sz, _int]),
     "mvh_gated_ffn_fp8": (_int, [_vp, _vp, _vp, _int, _vp, _vp, _sz, _int]),
+    "mvh_attn_shared": (_int, [_vp, _vp, _sz, _vp, _vp, _vp, _sz, _sz, _vp, _sz, _sz, _sz, _vp, _int]),
     "mvh_model_open": (_int, [C.c_char_p, _int, _sz, _sz, _int, _int, _sz, C.POINTER(_vp)]),
     "mvh_model_kv_type": (_int, [_vp, C.POINTER(_int)]),
     "mvh_model_close": (_int, [_vp]),
@@ -526,6 +527,31 @@ class Context:
         y, x_at, y_at, n, kind = self._fp8_rows(gate, x, y)
         self._check(self.lib.mvh_gated_ffn_fp8(self.h, gate.h, up.h, act, x_at, y_at, n, kind))
         return y
+
+    def attn_shared(self, kvs, layer: int, q, pos, n_head: int, n_head_kv: int, head_dim: int, out=None, prefix=None,
+                    prefix_len: int = 0, n_tokens=None):
+        """mvh_attn_shared: the tokens of sequence i (n_tokens[i] of them, one by default, at positions pos[i]..) see
+        rows 0 .. prefix_len-1 of the cache prefix and their own cache kvs[i]'s from there on.  q and out: rows of
+        n_head*head_dim, the sequences' tokens in turn."""
+        n_seq = len(kvs)
+        count = n_seq if n_tokens is None else int(sum(n_tokens))
+        if len(pos) != n_seq or (n_tokens is not None and len(n_tokens) != n_seq):
+            raise ValueError("pos and n_tokens must have one entry per sequence")
+        if any(p < 0 for p in pos) or (n_tokens is not None and any(n < 0 for n in n_tokens)):
+            raise ValueError("pos and n_tokens must not be negative")
+        host = isinstance(q, np.ndarray)
+        if host:
+            q = _host_rows(q)
+            out = np.empty_like(q) if out is None else out
+        q_at = _flat(q, "float32", count * n_head * head_dim, host, "q")
+        o_at = _flat(out, "float32", count * n_head * head_dim, host, "out")
+        handles = (_vp * n_seq)(*[kv.h for kv in kvs])
+        at = (_sz * n_seq)(*pos)
+        counts = None if n_tokens is None else (_sz * n_seq)(*n_tokens)
+        self._check(self.lib.mvh_attn_shared(self.h, None if prefix is None else prefix.h, prefix_len, handles, at, counts,
+                                             n_seq, layer, q_at, n_head, n_head_kv, head_dim, o_at,
+                                             MVH_HOST if host else MVH_DEVICE))
+        return out
 
     def kv_cache(self, n_layer: int, kv_dim: int, page_tokens: int = 128, max_tokens: int = 2048,
                  kv_type: int = MVH_KV_F16) -> "KVCache":

@@ -76,20 +76,6 @@ __device__ __forceinline__ int split_chunk(const Q4Args& a, int pos, int n_split
     return (per + 2 * kWaves - 1) / (2 * kWaves) * (2 * kWaves);
 }
 
-// max over the four 16-lane rows of a wave, in every lane
-__device__ __forceinline__ float rows_max(float v) {
-    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ __forceinline__ float rows_sum(float v) {
-    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
 __device__ __forceinline__ uint32_t rows_max_bits(uint32_t v) {
     auto a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
     v = max(a[0], a[1]);
@@ -137,23 +123,11 @@ __device__ __forceinline__ const uint8_t* page_at(const void* const* pt, int pag
     return reinterpret_cast<const uint8_t*>(*reinterpret_cast<entry>(reinterpret_cast<uintptr_t>(pt + page)));
 }
 
-// Two floats as fp16, rounded to nearest
-__device__ __forceinline__ half2v pk_half(float a, float b) {
-    typedef float f32x2 __attribute__((ext_vector_type(2)));
-    const f32x2 v = {a, b};
-    return __builtin_convertvector(v, half2v);
-}
 // a times (high + low) + c, the low parts first
 __device__ __forceinline__ f32x4 mfma2(u32x4 a, u32x4 high, u32x4 low, f32x4 c) {
     const half8 m = __builtin_bit_cast(half8, a);
     c = __builtin_amdgcn_mfma_f32_16x16x32_f16(m, __builtin_bit_cast(half8, low), c, 0, 0, 0);
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(m, __builtin_bit_cast(half8, high), c, 0, 0, 0);
-}
-// The power of two that brings a query row's largest element to [2^9, 2^10): its
-// elements keep 22 bits in two fp16 down to 2^-13 of that one and 2^-35 of it below
-// (so a small one counts on a wide key channel), and a block's sum, below 2^15, fits too
-__device__ __forceinline__ int query_exponent(float top) {
-    return (top > 0.0f && top <= 3.402823466e38f ? max(__builtin_amdgcn_frexp_expf(top) - 1, -110) : 0) - 9;
 }
 // p - h (exact where h is p rounded, or 0): the conversion inside the addition
 __device__ __forceinline__ float less(float p, _Float16 h, float minus1) { return fmaf(static_cast<float>(h), minus1, p); }

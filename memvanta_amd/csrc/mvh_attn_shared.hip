@@ -1,0 +1,629 @@
+// mvh_attn_shared.hip -- attention of a batch of sequences that share a prefix:
+// every query token sees rows 0 .. prefix_len - 1 of the prefix cache and its own
+// sequence's rows prefix_len .. its position (F16 and Q8 pages).
+//
+//   y_t = log2(e) / sqrt(hd) * q.K_t,  out = sum_t 2^(y_t - m) V_t / sum_t 2^(y_t - m)
+// over both, in parts (a range of rows each) with a running m, joined at the end.
+// The prefix's parts take the query rows of all sequences as the columns of one
+// product, so its pages are read once per tile of rows and not once per sequence.
+//
+// The products run on the fp16 matrix pipe: stored fp16 values and int8 codes
+// enter exactly; q and the weights are split into two fp16 (22 bits, where one
+// would leave 11); sums are fp32.  A Q8 row's scale multiplies its score, and its
+// weight before that is split.
+#include "mvh_kernels.hpp"
+
+namespace mvh {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.44269504088896340736f;
+// Weights are 2^(y - m + kLift), and m follows the maximum only when that is kSlack
+// ahead: at most 2^14, and in two fp16 they keep 22 bits down to 2^-12 of the
+// largest, 2^-35 of it below.
+constexpr float kLift = 10.0f, kSlack = 4.0f;
+constexpr int kPages = 514;    // page addresses that a part holds: of up to 512 whole pages
+constexpr int kBatch = 128;    // sequences of a launch: their places are kernel arguments
+
+struct SharedSeq {
+    const void* const* pt_k;
+    const void* const* pt_v;
+    int pos, row0;  // of the first query token, and its place among the tokens
+};
+struct SharedArgs {
+    const void* const* pt_k;  // the prefix
+    const void* const* pt_v;
+    const float* q;
+    float* out;
+    float* part;  // [row][slot][hd], then [row][slot][2]: sums and (m, l); null with one part
+    int prefix_len, n_tokens, n_head, group, kv_heads, kv_dim, hd, slots;
+    int p_page, s_page;  // rows of a page
+    uint32_t p_magic, s_magic;
+    int p_tiles, p_splits, p_chunk, p_items, s_tiles, s_splits, s_chunk;
+    SharedSeq seq[kBatch + 1];  // row0 of the last: n_tokens
+};
+
+// A part: rows t0 .. t1 - 1 of one cache for query rows r0 .. r0 + n - 1 (row = token
+// of the call * group + head of the kv head)
+struct Part {
+    const void* const* pt_k;
+    const void* const* pt_v;
+    int page;
+    uint32_t magic;
+    int t0, t1, r0, n, kh, slot;
+    int lim0, lim_row;  // row r sees rows up to lim0 + (r - lim_row) / group
+};
+
+// t / page size, t < 2^14: magic = ceil(2^31 / that), 0 where one page holds all
+__device__ __forceinline__ int page_of(int t, uint32_t magic) { return static_cast<int>(__umulhi(2 * static_cast<uint32_t>(t), magic)); }
+
+// The order of a row's 16-byte chunks in LDS, so that the 16 rows of a K operand,
+// and the 16 rows x 32 bytes of a transposed V operand, lie in different banks
+template <int CPR>
+__device__ __forceinline__ int k_turn(int row) { return CPR >= 16 ? row & 15 : (row >> 1) & 7; }
+template <int CPR>
+__device__ __forceinline__ int v_turn(int row) { return CPR >= 16 ? (row & 7) * 2 : ((row >> 1) & 3) * 2; }
+
+// RW waves along the query rows with RT tiles of 16 each, TW along the T rows of a step
+template <int RW_, int RT_, int TW_, int T_>
+struct Shape {
+    static constexpr int RW = RW_, RT = RT_, TW = TW_, T = T_, ROWS = 16 * RW_ * RT_;
+    static_assert(RW_ * TW_ == 4 && T_ / TW_ % 32 == 0);
+};
+template <int NB, class S>
+constexpr size_t tile_bytes() {
+    const size_t kv = 2 * static_cast<size_t>(S::T) * NB * 64, join = S::TW > 1 ? 4 * S::RT * 16 * (32 * NB + 4) * 4 : 0;
+    return kv > join ? kv : join;
+}
+
+// Eight int8 as fp16: a byte plus 128, in the low bits of 1024, less 1152
+__device__ __forceinline__ uint4 half_of_int8(uint2 w) {
+    const uint32_t a = w.x ^ 0x80808080u, b = w.y ^ 0x80808080u, one = 0x64646464u;
+    const half2v off = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
+    return make_uint4(as_u32(as_half2(__builtin_amdgcn_perm(one, a, 0x04010400u)) + off),
+                      as_u32(as_half2(__builtin_amdgcn_perm(one, a, 0x04030402u)) + off),
+                      as_u32(as_half2(__builtin_amdgcn_perm(one, b, 0x04010400u)) + off),
+                      as_u32(as_half2(__builtin_amdgcn_perm(one, b, 0x04030402u)) + off));
+}
+__device__ __forceinline__ bool unbounded(_Float16 h) {  // an infinity or NaN
+    return (__builtin_bit_cast(uint16_t, h) & 0x7c00u) == 0x7c00u;
+}
+
+template <int KT, int NB, class S>
+__device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8_t* tile, uint64_t* s_pk, uint64_t* s_pv, float* s_sc,
+                                       float (*s_ml)[2 * S::RT][16]) {
+    constexpr int RW = S::RW, RT = S::RT, TW = S::TW, T = S::T, CPR = 4 * NB, HDP = 32 * NB, ITEMS = T * CPR / 256, ND = 2 * NB;
+    constexpr bool Q8 = KT == kKvQ8;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, j = lane >> 4;
+    const int rw = wave % RW, tw = wave / RW, hd = a.hd;
+    uint8_t* const s_k = tile;
+    uint8_t* const s_v = tile + T * HDP * 2;
+
+    // page addresses of the part
+    const int page0 = page_of(p.t0, p.magic), pages = page_of(p.t1 - 1, p.magic) - page0 + 1;
+    for (int i = tid; i < pages; i += 256) {
+        s_pk[i] = reinterpret_cast<uint64_t>(p.pt_k[page0 + i]);
+        s_pv[i] = reinterpret_cast<uint64_t>(p.pt_v[page0 + i]);
+    }
+    __syncthreads();
+
+    const size_t sc_off = kv_scale_offset(p.page, a.kv_dim);
+    typename std::conditional<Q8, uint2, uint4>::type kr[ITEMS], vr[ITEMS];
+    float scale = 0.0f;
+    auto row_at = [&](const uint64_t* s_p, int t, int& slot) {  // rows behind the part: its first one again, masked
+        const int tc = t < p.t1 ? t : p.t0, pg = page_of(tc, p.magic);
+        slot = tc - pg * p.page;
+        return reinterpret_cast<const uint8_t*>(s_p[pg - page0]);
+    };
+    auto load = [&](int base) {
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const int at = i * 256 + tid, row = at / CPR, kc = (at % CPR) ^ k_turn<CPR>(row), vc = (at % CPR) ^ v_turn<CPR>(row);
+            int slot;
+            const uint8_t* pk = row_at(s_pk, base + row, slot);
+            const uint8_t* pv = row_at(s_pv, base + row, slot);
+            const size_t off = static_cast<size_t>(slot) * a.kv_dim + p.kh * hd;
+            if constexpr (Q8) {
+                kr[i] = vr[i] = make_uint2(0u, 0u);
+                if (kc * 8 < hd) kr[i] = ld_global8(pk + off + kc * 8);
+                if (vc * 8 < hd) vr[i] = ld_global8(pv + off + vc * 8);
+            } else {
+                kr[i] = vr[i] = make_uint4(0u, 0u, 0u, 0u);
+                if (kc * 8 < hd) kr[i] = ld_global16(pk + 2 * (off + kc * 8));
+                if (vc * 8 < hd) vr[i] = ld_global16(pv + 2 * (off + vc * 8));
+            }
+        }
+        if (Q8 && tid < 2 * T) {
+            int slot;
+            const uint8_t* page = row_at(tid < T ? s_pk : s_pv, base + (tid & (T - 1)), slot);
+            scale = *(const __attribute__((address_space(1))) float*)(reinterpret_cast<uintptr_t>(page + sc_off + 4 * static_cast<size_t>(slot)));
+        }
+    };
+    auto store = [&] {
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const int at = (i * 256 + tid) * 16;
+            if constexpr (Q8) {
+                *reinterpret_cast<uint4*>(s_k + at) = half_of_int8(kr[i]);
+                *reinterpret_cast<uint4*>(s_v + at) = half_of_int8(vr[i]);
+            } else {
+                *reinterpret_cast<uint4*>(s_k + at) = kr[i];
+                *reinterpret_cast<uint4*>(s_v + at) = vr[i];
+            }
+        }
+        if (Q8 && tid < 2 * T) s_sc[tid] = scale;
+    };
+    load(p.t0);
+
+    // q of the wave's rows: lane (n, j) holds channels 8 j .. of each block of 32
+    half8 qh[RT][NB], ql[RT][NB];
+    float y_scale[RT];
+    int lim[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int r = p.r0 + min((rw * RT + rt) * 16 + n, p.n - 1);
+        lim[rt] = p.lim0 + (r - p.lim_row) / a.group;
+        const float* qr = a.q + (static_cast<size_t>(r / a.group) * a.n_head + p.kh * a.group + r % a.group) * hd;
+        float f[NB][8], top = 0.0f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                f[b][i] = 32 * b + 8 * j < hd ? qr[32 * b + 8 * j + i] : 0.0f;
+                top = fmaxf(top, fabsf(f[b][i]));
+            }
+        const int e = query_exponent(rows_max(top));
+        const float down = ldexpf(1.0f, -e);
+        y_scale[rt] = ldexpf(__fdiv_rn(kLog2e, sqrt_rn(static_cast<float>(hd))), e);
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float x = f[b][i] * down;
+                qh[rt][b][i] = static_cast<_Float16>(x);
+                ql[rt][b][i] = static_cast<_Float16>(x - static_cast<float>(qh[rt][b][i]));
+            }
+    }
+    const int first_lim = p.lim0 + (p.r0 - p.lim_row) / a.group, seen_by_all = min(p.t1, first_lim + 1);
+
+    f32x4 o[RT][ND];
+    float m[RT], l[RT];
+    int unit[RT];  // Q8: sums are held times 2^-unit, the exponent of the largest scale seen
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        m[rt] = -__builtin_inff();
+        l[rt] = 0.0f;
+        unit[rt] = -126;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[rt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    auto block = [&](int tg, int tb) {  // rows tg .. tg + 31, at tb of the tile
+        const bool edge = tg + 32 > seen_by_all;
+        f32x4 s[RT][2];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) s[rt][0] = s[rt][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int row = tb + 16 * h + n;
+                const half8 k = *reinterpret_cast<const half8*>(s_k + (row * CPR + ((4 * b + j) ^ k_turn<CPR>(row))) * 16);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    s[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[rt][b], s[rt][h], 0, 0, 0);
+                    s[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[rt][b], s[rt][h], 0, 0, 0);
+                }
+            }
+        f32x4 ks[2], vs[2];
+        if constexpr (Q8)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                ks[h] = *reinterpret_cast<const f32x4*>(s_sc + tb + 16 * h + 4 * j);
+                vs[h] = *reinterpret_cast<const f32x4*>(s_sc + T + tb + 16 * h + 4 * j);
+            }
+        half8 ph[RT], pl[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            bool seen[2][4];
+            float y[2][4], top = -__builtin_inff();
+            int widest = -126;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int t = tg + 16 * h + 4 * j + i;
+                    seen[h][i] = !edge || (t < p.t1 && t <= lim[rt]);
+                    float v = s[rt][h][i];
+                    if constexpr (Q8) v *= ks[h][i];
+                    v *= y_scale[rt];
+                    y[h][i] = seen[h][i] ? v : -__builtin_inff();
+                    top = fmaxf(top, y[h][i]);
+                    if constexpr (Q8) {
+                        const int e = static_cast<int>((__float_as_uint(vs[h][i]) >> 23) & 255u) - 127;
+                        if (seen[h][i] && e < 128) widest = max(widest, e);
+                    }
+                }
+            top = rows_max(top);
+            const bool ahead = top > m[rt] + kSlack;
+            if constexpr (Q8) {
+                auto x = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(widest + 126), static_cast<uint32_t>(widest + 126), false, false);
+                uint32_t w = max(x[0], x[1]);
+                auto z = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+                widest = static_cast<int>(max(z[0], z[1])) - 126;
+            }
+            const bool wider = Q8 && widest > unit[rt];
+            if (__any(ahead || wider)) {
+                float down = 1.0f;
+                if (ahead) {
+                    down = m[rt] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m[rt] - top);
+                    m[rt] = top;
+                }
+                l[rt] *= down;
+                if (wider) {
+                    down = ldexpf(down, max(unit[rt] - widest, -250));
+                    unit[rt] = widest;
+                }
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[rt][d][i] *= down;
+            }
+            const float from = (m[rt] == -__builtin_inff() ? 0.0f : m[rt]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float w = __builtin_amdgcn_exp2f((y[h][i] - from) + kLift);
+                    l[rt] += w;
+                    if constexpr (Q8) w = seen[h][i] ? w * ldexpf(vs[h][i], -unit[rt]) : 0.0f;
+                    ph[rt][4 * h + i] = static_cast<_Float16>(w);
+                    pl[rt][4 * h + i] = static_cast<_Float16>(w - static_cast<float>(ph[rt][4 * h + i]));
+                }
+        }
+        bool odd = false;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+            union {
+                s16x4 w[2];
+                half8 h;
+            } v;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int row = tb + 16 * h + 4 * j + (n >> 2), chunk = (2 * d + ((n >> 1) & 1)) ^ v_turn<CPR>(row);
+                typedef __attribute__((address_space(3))) s16x4 lds_t;
+                v.w[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(s_v + (row * CPR + chunk) * 16 + (n & 1) * 8));
+            }
+            if (!Q8 && edge) {
+                // a row that some do not see: what is no number there must not meet their weight of 0
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (unbounded(v.h[i])) {
+                        odd = true;
+                        v.h[i] = static_cast<_Float16>(0.0f);
+                    }
+            }
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v.h, pl[rt], o[rt][d], 0, 0, 0);
+                o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v.h, ph[rt], o[rt][d], 0, 0, 0);
+            }
+        }
+        if (!Q8 && __any(odd)) {  // the products left out, for the rows that see them
+            for (int t = 0; t < 32; ++t) {
+                const int row = tb + t, from_lane = n + 16 * ((t >> 2) & 3), at = 4 * (t >> 4) + (t & 3);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    float w = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (i == at) w = static_cast<float>(ph[rt][i]) + static_cast<float>(pl[rt][i]);
+                    w = __shfl(w, from_lane);
+                    if (tg + t >= p.t1 || tg + t > lim[rt]) continue;
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int ch = 16 * d + 4 * j + i;
+                            const _Float16 v = *reinterpret_cast<const _Float16*>(
+                                s_v + (row * CPR + ((ch >> 3) ^ v_turn<CPR>(row))) * 16 + (ch & 7) * 2);
+                            if (unbounded(v)) o[rt][d][i] = fmaf(w, static_cast<float>(v), o[rt][d][i]);
+                        }
+                }
+            }
+        }
+    };
+
+    for (int base = p.t0; base < p.t1; base += T) {
+        __syncthreads();
+        store();
+        __syncthreads();
+        if (base + T < p.t1) load(base + T);
+#pragma unroll 1
+        for (int u = 0; u < T / TW / 32; ++u) {
+            const int tb = tw * (T / TW) + 32 * u;
+            if (base + tb < p.t1) block(base + tb, tb);
+        }
+    }
+
+    // the result: of the wave, or of the TW waves that shared the rows
+    const size_t gs = static_cast<size_t>(a.n_tokens) * a.n_head;
+    auto put = [&](int row, int d, f32x4 v, float top, float sum) {
+        const int r = p.r0 + row;
+        const size_t g = static_cast<size_t>(r / a.group) * a.n_head + p.kh * a.group + r % a.group;
+        if (!a.part) {
+            *reinterpret_cast<f32x4*>(a.out + g * hd + d) =
+                f32x4{__fdiv_rn(v[0], sum), __fdiv_rn(v[1], sum), __fdiv_rn(v[2], sum), __fdiv_rn(v[3], sum)};
+            return;
+        }
+        const size_t at = g * a.slots + p.slot;
+        *reinterpret_cast<f32x4*>(a.part + at * hd + d) = v;
+        if (d == 0) {
+            float* ml = a.part + gs * a.slots * hd + 2 * at;
+            ml[0] = top;
+            ml[1] = sum;
+        }
+    };
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        l[rt] = rows_sum(l[rt]);
+        if constexpr (Q8)
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[rt][d][i] = ldexpf(o[rt][d][i], unit[rt]);
+    }
+    if constexpr (TW == 1) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const int row = (rw * RT + rt) * 16 + n;
+            if (row >= p.n) continue;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+                if (16 * d + 4 * j < hd) put(row, 16 * d + 4 * j, o[rt][d], m[rt], l[rt]);
+        }
+    } else {
+        float* s_o = reinterpret_cast<float*>(tile);  // [wave][rt][16][HDP + 4]
+        __syncthreads();
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+                *reinterpret_cast<f32x4*>(s_o + ((wave * RT + rt) * 16 + n) * (HDP + 4) + 16 * d + 4 * j) = o[rt][d];
+            if (j == 0) {
+                s_ml[wave][rt][n] = m[rt];
+                s_ml[wave][RT + rt][n] = l[rt];
+            }
+        }
+        __syncthreads();
+        for (int e = tid; e < S::ROWS * (HDP / 4); e += 256) {
+            const int row = e / (HDP / 4), d = e % (HDP / 4) * 4, w0 = row / (16 * RT), rt = row / 16 % RT, c = row % 16;
+            if (row >= p.n || d >= hd) continue;
+            float top = s_ml[w0][rt][c];
+#pragma unroll
+            for (int k = 1; k < TW; ++k) top = fmaxf(top, s_ml[w0 + k * RW][rt][c]);
+            f32x4 v = {0.f, 0.f, 0.f, 0.f};
+            float sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < TW; ++k) {
+                const int w = w0 + k * RW;
+                const float mine = s_ml[w][rt][c], f = mine == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mine - top);
+                if (s_ml[w][RT + rt][c] == 0.0f) continue;
+                const f32x4 x = *reinterpret_cast<const f32x4*>(s_o + ((w * RT + rt) * 16 + c) * (HDP + 4) + d);
+                sum = fmaf(f, s_ml[w][RT + rt][c], sum);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = fmaf(f, x[i], v[i]);
+            }
+            put(row, d, v, top, sum);
+        }
+    }
+}
+
+// A workgroup: a part of the prefix for a tile of all query rows, or, behind those,
+// a part of one sequence's own rows.
+template <int KT, int NB, class P, class S>
+__global__ __launch_bounds__(256, 2) void attn_shared_kernel(SharedArgs a) {
+    constexpr size_t kP = tile_bytes<NB, P>(), kS = tile_bytes<NB, S>();
+    __shared__ __align__(16) uint8_t tile[kP > kS ? kP : kS];
+    __shared__ uint64_t s_pk[kPages], s_pv[kPages];
+    __shared__ __align__(16) float s_sc[2 * (P::T > S::T ? P::T : S::T)];
+    __shared__ float s_ml[4 * 2 * (P::RT > S::RT ? P::RT : S::RT) * 16];
+    const int item = blockIdx.x;
+    Part p;
+    if (item < a.p_items) {
+        // the tiles of a range of rows on one XCD (workgroups go to the eight in turn), whose L2 then holds it for all of them
+        const int pair = item / (8 * a.p_tiles) * 8 + item % 8, tile_at = item / 8 % a.p_tiles;
+        if (pair >= a.kv_heads * a.p_splits) return;
+        p.kh = pair % a.kv_heads;
+        p.slot = pair / a.kv_heads;
+        p.pt_k = a.pt_k, p.pt_v = a.pt_v, p.page = a.p_page, p.magic = a.p_magic;
+        p.t0 = p.slot * a.p_chunk;
+        p.t1 = min(p.t0 + a.p_chunk, a.prefix_len);
+        p.r0 = tile_at * P::ROWS;
+        p.n = min(P::ROWS, a.n_tokens * a.group - p.r0);
+        p.lim0 = 0x3fffffff, p.lim_row = p.r0;  // all rows see all
+        attend<KT, NB, P>(a, p, tile, s_pk, s_pv, s_sc, reinterpret_cast<float(*)[2 * P::RT][16]>(s_ml));
+        return;
+    }
+    int at = item - a.p_items;
+    p.kh = at % a.kv_heads;
+    at /= a.kv_heads;
+    const int tile_at = at % a.s_tiles;
+    at /= a.s_tiles;
+    const int split = at % a.s_splits, i = at / a.s_splits;
+    const int rows = (a.seq[i + 1].row0 - a.seq[i].row0) * a.group, first = tile_at * S::ROWS;
+    if (first >= rows) return;
+    p.slot = a.p_splits + split;
+    p.pt_k = a.seq[i].pt_k, p.pt_v = a.seq[i].pt_v, p.page = a.s_page, p.magic = a.s_magic;
+    p.lim0 = a.seq[i].pos, p.lim_row = a.seq[i].row0 * a.group;
+    p.r0 = p.lim_row + first;
+    p.n = min(S::ROWS, rows - first);
+    p.t0 = a.prefix_len + split * a.s_chunk;
+    p.t1 = min(p.t0 + a.s_chunk, p.lim0 + (first + p.n - 1) / a.group + 1);
+    if (p.t0 >= p.t1) {  // behind the last row that is seen: a part of no weight
+        for (int r = threadIdx.x; r < p.n; r += 256) {
+            const size_t g = static_cast<size_t>((p.r0 + r) / a.group) * a.n_head + p.kh * a.group + (p.r0 + r) % a.group;
+            float* ml = a.part + static_cast<size_t>(a.n_tokens) * a.n_head * a.slots * a.hd + 2 * (g * a.slots + p.slot);
+            ml[0] = -__builtin_inff();
+            ml[1] = 0.0f;
+        }
+        return;
+    }
+    attend<KT, NB, S>(a, p, tile, s_pk, s_pv, s_sc, reinterpret_cast<float(*)[2 * S::RT][16]>(s_ml));
+}
+
+// out row = sum over its parts, four channels a thread
+__global__ __launch_bounds__(256) void attn_shared_join(const float* __restrict__ part, float* __restrict__ out, size_t rows,
+                                                        int slots, int hd) {
+    const int per = hd / 4, in = threadIdx.x / per, d = threadIdx.x % per * 4;
+    const size_t row = static_cast<size_t>(blockIdx.x) * (256 / per) + in;
+    if (in >= 256 / per || row >= rows) return;
+    const float* ml = part + rows * slots * hd + 2 * row * slots;
+    float top = -__builtin_inff();
+    for (int k = 0; k < slots; ++k) top = fmaxf(top, ml[2 * k]);
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    float sum = 0.0f;
+    for (int k = 0; k < slots; ++k) {
+        if (ml[2 * k + 1] == 0.0f) continue;  // no row seen
+        const float f = ml[2 * k] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ml[2 * k] - top);
+        const f32x4 x = *reinterpret_cast<const f32x4*>(part + (row * slots + k) * hd + d);
+        sum = fmaf(f, ml[2 * k + 1], sum);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = fmaf(f, x[i], v[i]);
+    }
+    *reinterpret_cast<f32x4*>(out + row * hd + d) =
+        f32x4{__fdiv_rn(v[0], sum), __fdiv_rn(v[1], sum), __fdiv_rn(v[2], sum), __fdiv_rn(v[3], sum)};
+}
+
+uint32_t magic_of(size_t page_tokens) {
+    return page_tokens >= 16384 || !page_tokens ? 0 : static_cast<uint32_t>(((uint64_t{1} << 31) + page_tokens - 1) / page_tokens);
+}
+
+// How a launch is cut.  Parts of the prefix and of the sequences' own rows are so
+// many that there are about 512 workgroups of each (two a CU).
+struct Cut {
+    bool chunks;  // own rows in tiles of many query rows
+    int p_shape;  // 0, 1, 2: tiles of up to 16, 32, more query rows
+    size_t p_tiles, p_splits, p_chunk, s_tiles, s_splits, s_chunk;
+    size_t slots() const { return p_splits + s_splits; }
+};
+constexpr int kWide = 4;  // blocks of 32 channels up to which a wave takes two tiles of query rows
+size_t rows_of(int shape, int nb) { return shape == 0 && nb <= kWide ? 16 : shape <= 1 ? 32 : nb <= kWide ? 128 : 64; }
+int blocks_of(size_t hd) { return hd <= 64 ? 2 : hd <= 128 ? 4 : 8; }
+
+Cut cut_of(const SharedCall& c) {
+    Cut k{};
+    const int nb = blocks_of(c.head_dim);
+    const size_t group = c.n_head / c.n_head_kv;
+    size_t most = 0, own = 0, tokens = 0;
+    for (size_t i = 0; i < c.n_seq; ++i) {
+        if (!c.n_tokens[i]) continue;
+        tokens += c.n_tokens[i];
+        most = std::max(most, c.n_tokens[i] * group);
+        own = std::max(own, c.pos[i] + c.n_tokens[i] - c.prefix_len);
+    }
+    const size_t rows = tokens * group;
+    k.chunks = most > 32;
+    k.p_shape = k.chunks || rows > 32 ? 2 : rows > 16 ? 1 : 0;
+    auto split = [](size_t len, size_t others, size_t page, size_t& splits, size_t& chunk) {
+        if (!len) return void(splits = chunk = 0);
+        const size_t most_rows = 512 * page;
+        splits = std::min((len + 127) / 128, (512 + others - 1) / others);
+        chunk = std::min(((len + splits - 1) / splits + 127) / 128 * 128, most_rows);
+        splits = (len + chunk - 1) / chunk;
+    };
+    const size_t p_rows = rows_of(k.p_shape, nb), s_rows = rows_of(k.chunks ? 2 : 0, nb);
+    k.p_tiles = (rows + p_rows - 1) / p_rows;
+    k.s_tiles = (most + s_rows - 1) / s_rows;
+    split(c.prefix_len, k.p_tiles * c.n_head_kv, c.p_page, k.p_splits, k.p_chunk);
+    split(own, c.n_seq * c.n_head_kv * k.s_tiles, c.s_page, k.s_splits, k.s_chunk);
+    return k;
+}
+
+template <int KT, int NB>
+hipError_t run_shapes(const Cut& k, const SharedArgs& a, unsigned grid, hipStream_t st) {
+    constexpr bool W = NB <= kWide;
+    using A = typename std::conditional<W, Shape<1, 1, 4, 128>, Shape<2, 1, 2, 64>>::type;
+    using B = Shape<2, 1, 2, 64>;
+    using C = typename std::conditional<W, Shape<4, 2, 1, 64>, Shape<4, 1, 1, 64>>::type;
+    if (k.chunks) attn_shared_kernel<KT, NB, C, C><<<grid, 256, 0, st>>>(a);
+    else if (k.p_shape == 2) attn_shared_kernel<KT, NB, C, A><<<grid, 256, 0, st>>>(a);
+    else if (k.p_shape == 1) attn_shared_kernel<KT, NB, B, A><<<grid, 256, 0, st>>>(a);
+    else attn_shared_kernel<KT, NB, A, A><<<grid, 256, 0, st>>>(a);
+    return hipGetLastError();
+}
+template <int KT>
+hipError_t run_type(int nb, const Cut& k, const SharedArgs& a, unsigned grid, hipStream_t st) {
+    return nb == 2 ? run_shapes<KT, 2>(k, a, grid, st) : nb == 4 ? run_shapes<KT, 4>(k, a, grid, st) : run_shapes<KT, 8>(k, a, grid, st);
+}
+
+// Sequences first .. first + n - 1 as a call of their own
+SharedCall some(const SharedCall& c, size_t first, size_t n) {
+    SharedCall s = c;
+    s.seq += first, s.pos += first, s.n_tokens += first;
+    s.n_seq = n;
+    for (size_t i = 0; i < first; ++i) {
+        s.q += c.n_tokens[i] * c.n_head * c.head_dim;
+        s.out += c.n_tokens[i] * c.n_head * c.head_dim;
+    }
+    return s;
+}
+size_t tokens_of(const SharedCall& c) {
+    size_t n = 0;
+    for (size_t i = 0; i < c.n_seq; ++i) n += c.n_tokens[i];
+    return n;
+}
+
+}  // namespace
+
+size_t attn_shared_scratch(const SharedCall& c) {
+    size_t most = 0;
+    for (size_t at = 0; at < c.n_seq; at += kBatch) {
+        const SharedCall s = some(c, at, std::min<size_t>(kBatch, c.n_seq - at));
+        const Cut k = cut_of(s);
+        if (k.slots() > 1) most = std::max(most, tokens_of(s) * c.n_head * k.slots() * (c.head_dim + 2) * 4);
+    }
+    return most;
+}
+
+hipError_t launch_attn_shared(const SharedCall& call, void* scratch, hipStream_t st) {
+    for (size_t first = 0; first < call.n_seq; first += kBatch) {
+        const SharedCall c = some(call, first, std::min<size_t>(kBatch, call.n_seq - first));
+        const size_t tokens = tokens_of(c);
+        if (!tokens) continue;
+        const Cut k = cut_of(c);
+        SharedArgs a{};
+        a.pt_k = c.prefix_k, a.pt_v = c.prefix_v, a.q = c.q, a.out = c.out;
+        a.part = k.slots() > 1 ? static_cast<float*>(scratch) : nullptr;
+        a.prefix_len = static_cast<int>(c.prefix_len), a.n_tokens = static_cast<int>(tokens);
+        a.n_head = static_cast<int>(c.n_head), a.kv_heads = static_cast<int>(c.n_head_kv), a.group = a.n_head / a.kv_heads;
+        a.kv_dim = static_cast<int>(c.kv_dim), a.hd = static_cast<int>(c.head_dim), a.slots = static_cast<int>(k.slots());
+        a.p_page = static_cast<int>(c.p_page), a.s_page = static_cast<int>(c.s_page);
+        a.p_magic = magic_of(c.p_page), a.s_magic = magic_of(c.s_page);
+        a.p_tiles = static_cast<int>(k.p_tiles), a.p_splits = static_cast<int>(k.p_splits), a.p_chunk = static_cast<int>(k.p_chunk);
+        a.s_tiles = static_cast<int>(k.s_tiles), a.s_splits = static_cast<int>(k.s_splits), a.s_chunk = static_cast<int>(k.s_chunk);
+        a.p_items = static_cast<int>((k.p_splits * c.n_head_kv + 7) / 8 * 8 * k.p_tiles);
+        int row = 0;
+        for (size_t i = 0; i < c.n_seq; ++i) {
+            a.seq[i] = {c.seq[i].pt_k, c.seq[i].pt_v, static_cast<int>(c.pos[i]), row};
+            row += static_cast<int>(c.n_tokens[i]);
+        }
+        a.seq[c.n_seq].row0 = row;
+        const size_t grid = a.p_items + c.n_seq * c.n_head_kv * k.s_tiles * k.s_splits;
+        if (grid > 0xffffff) return hipErrorInvalidValue;  // a launch has fewer than 2^32 threads
+        const int nb = blocks_of(c.head_dim);
+        const hipError_t e = c.kv_type == kKvQ8 ? run_type<kKvQ8>(nb, k, a, static_cast<unsigned>(grid), st)
+                                                : run_type<kKvF16>(nb, k, a, static_cast<unsigned>(grid), st);
+        if (e != hipSuccess) return e;
+        if (a.part) {
+            const size_t rows = tokens * c.n_head, per = 256 / (c.head_dim / 4);
+            attn_shared_join<<<dim3(static_cast<unsigned>((rows + per - 1) / per)), 256, 0, st>>>(a.part, c.out, rows, a.slots, a.hd);
+            if (const hipError_t j = hipGetLastError(); j != hipSuccess) return j;
+        }
+    }
+    return hipSuccess;
+}
+
+}  // namespace mvh

@@ -1603,6 +1603,88 @@ int mvh_attn_batch(mvh_context* c, const mvh_kv_cache* kv, size_t layer, const f
     return finish_out(c, out, od, qn * 4, kind);
 }
 
+int mvh_attn_shared(mvh_context* c, const mvh_kv_cache* prefix, size_t prefix_len, const mvh_kv_cache* const* kvs,
+                    const size_t* pos, const size_t* n_tokens, size_t n_seq, size_t layer, const float* q, size_t n_head,
+                    size_t n_head_kv, size_t head_dim, float* out, int kind) {
+    CHECK_CTX(c);
+    if (kind != MVH_HOST && kind != MVH_DEVICE) return fail(MVH_E_INVALID, "ptr_kind must be MVH_HOST or MVH_DEVICE");
+    if (!n_head || !n_head_kv || n_head % n_head_kv || !head_dim)
+        return fail(MVH_E_SHAPE, "invalid Llama head configuration");
+    if (head_dim % 8 || head_dim > 256) return fail(MVH_E_SHAPE, "head_dim must be a multiple of 8 up to 256");
+    if (n_head > (size_t{1} << 16)) return fail(MVH_E_RANGE, "n_head above 65536");
+    if (!n_seq) return MVH_OK;
+    if (!kvs || !pos) return fail(MVH_E_INVALID, "null kvs/pos");
+    if (n_seq > (size_t{1} << 16)) return fail(MVH_E_RANGE, "more than 65536 sequences");
+    const mvh_kv_cache* one = nullptr;  // what all caches have to be like
+    auto check = [&](const mvh_kv_cache* kv, size_t first, size_t end) {
+        if (int rc = check_kv_on(c, kv, layer)) return rc;
+        if (kv->type != MVH_KV_F16 && kv->type != MVH_KV_Q8)
+            return fail(MVH_E_TYPE, "attention behind a shared prefix takes F16 and Q8 caches, got %s", mvh_kv_type_name(kv->type));
+        if (!one) one = kv;
+        if (kv->type != one->type || kv->kv_dim != one->kv_dim) return fail(MVH_E_SHAPE, "KV caches of different types or kv_dim");
+        if (end > kv->max_tokens) return fail(MVH_E_RANGE, "context exhausted");
+        return first < end ? check_pages(kv, layer, first, end - 1) : MVH_OK;
+    };
+    if (prefix_len || prefix)
+        if (int rc = check(prefix, 0, prefix_len)) return rc;
+    size_t tokens = 0;
+    for (size_t i = 0; i < n_seq; ++i) {
+        const size_t n = n_tokens ? n_tokens[i] : 1;
+        if (!n) continue;
+        if (pos[i] < prefix_len) return fail(MVH_E_RANGE, "position %zu of sequence %zu lies in the prefix", pos[i], i);
+        if (n > 16000 || pos[i] > 16000) return fail(MVH_E_RANGE, "context exhausted");
+        if (int rc = check(kvs[i], prefix_len, pos[i] + n)) return rc;
+        tokens += n;
+    }
+    if (!tokens) return MVH_OK;
+    if (n_head_kv * head_dim > one->kv_dim) return fail(MVH_E_SHAPE, "n_head_kv*head_dim must be <= kv_dim");
+    if (!q || !out) return fail(MVH_E_INVALID, "null q/out");
+    if (tokens * n_head > (size_t{1} << 24)) return fail(MVH_E_RANGE, "more than 16777216 query rows");
+    if (kind == MVH_DEVICE && ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15))
+        return fail(MVH_E_INVALID, "device q and out must be 16-byte aligned");
+    std::vector<mvh::SharedCall::Pages> seq;
+    std::vector<size_t> at, count;
+    size_t s_page = 0;
+    try {
+        seq.reserve(n_seq), at.reserve(n_seq), count.reserve(n_seq);
+    } catch (const std::bad_alloc&) {
+        return fail(MVH_E_NOMEM, "host allocation failed");
+    }
+    for (size_t i = 0; i < n_seq; ++i) {  // sequences without a token are left out
+        const size_t n = n_tokens ? n_tokens[i] : 1;
+        if (!n) continue;
+        if (!s_page) s_page = kvs[i]->page_tokens;
+        if (kvs[i]->page_tokens != s_page) return fail(MVH_E_SHAPE, "KV caches of different page sizes");
+        const size_t base = layer * kvs[i]->max_pages;
+        seq.push_back({kvs[i]->dk + base, kvs[i]->dv + base});
+        at.push_back(pos[i]);
+        count.push_back(n);
+    }
+    mvh::SharedCall call{};
+    call.kv_type = one->type;
+    if (prefix_len) {
+        call.prefix_k = prefix->dk + layer * prefix->max_pages;
+        call.prefix_v = prefix->dv + layer * prefix->max_pages;
+        call.p_page = prefix->page_tokens;
+    }
+    call.prefix_len = prefix_len;
+    call.seq = seq.data(), call.pos = at.data(), call.n_tokens = count.data();
+    call.n_seq = seq.size(), call.s_page = s_page;
+    call.n_head = n_head, call.n_head_kv = n_head_kv, call.head_dim = head_dim, call.kv_dim = one->kv_dim;
+    const size_t qn = tokens * n_head * head_dim;
+    const void* qd = nullptr;
+    if (int rc = stage_in(c, c->xin, q, qn * 4, kind, &qd)) return rc;
+    float* od = out;
+    if (kind == MVH_HOST) {
+        if (int rc = grow(c, c->yout, qn * 4)) return rc;
+        od = static_cast<float*>(c->yout.p);
+    }
+    call.q = static_cast<const float*>(qd), call.out = od;
+    if (int rc = grow_kept(c, c->work, mvh::attn_shared_scratch(call))) return rc;
+    MVH_HIP(mvh::launch_attn_shared(call, c->work.p, c->stream));
+    return finish_out(c, out, od, qn * 4, kind);
+}
+
 }  // extern "C"
 
 namespace {

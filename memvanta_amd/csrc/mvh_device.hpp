@@ -164,6 +164,39 @@ __device__ __forceinline__ half8 as_half8(uint4 w) {
     return __builtin_bit_cast(half8, v);
 }
 
+// ---- attention on the fp16 matrix pipe -----------------------------------------
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ half2v as_half2(uint32_t w) { return __builtin_bit_cast(half2v, w); }
+__device__ __forceinline__ uint32_t as_u32(half2v h) { return __builtin_bit_cast(uint32_t, h); }
+
+// max over the four 16-lane rows of a wave, in every lane
+__device__ __forceinline__ float rows_max(float v) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float rows_sum(float v) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// Two floats as fp16, rounded to nearest
+__device__ __forceinline__ half2v pk_half(float a, float b) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    const f32x2 v = {a, b};
+    return __builtin_convertvector(v, half2v);
+}
+
+// The power of two that brings a query row's largest element to [2^9, 2^10): its
+// elements keep 22 bits in two fp16 down to 2^-13 of that one and 2^-35 of it below
+// (so a small one counts on a wide key channel), and a block's sum, below 2^15, fits too
+__device__ __forceinline__ int query_exponent(float top) {
+    return (top > 0.0f && top <= 3.402823466e38f ? max(__builtin_amdgcn_frexp_expf(top) - 1, -110) : 0) - 9;
+}
+
 // 16-byte load through a pointer that is known to address global memory but
 // was itself loaded from memory (a page table): the address-space cast makes
 // it a global_load instead of a flat_load, whose LDS/VMEM counter coupling

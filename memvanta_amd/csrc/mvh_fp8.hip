@@ -14,7 +14,6 @@ namespace mvh {
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 
 constexpr int kBlk = 128;
 constexpr float kTop = 448.0f;            // largest e4m3 value

@@ -148,6 +148,30 @@ hipError_t launch_attn_q4(const void* const* pt_k, const void* const* pt_v, cons
                           float* out, const int* d_pos, size_t pos, size_t max_pos, size_t n_tokens, size_t n_head,
                           size_t n_head_kv, size_t hd, size_t kv_dim, size_t page_tokens, size_t chunk, hipStream_t st);
 
+// ---- attention behind a shared prefix (mvh_attn_shared.hip) ----
+// Sequence i's n_tokens[i] query tokens at positions pos[i].. see rows 0 ..
+// prefix_len - 1 of the prefix's pages and their own sequence's rows from
+// prefix_len up to their position; F16 or Q8 pages, positions below 2^14, head_dim
+// a multiple of 8 up to 256.  q and out: the tokens of all sequences in turn.
+struct SharedCall {
+    struct Pages {
+        const void* const* pt_k;
+        const void* const* pt_v;
+    };
+    int kv_type;
+    const void* const* prefix_k;
+    const void* const* prefix_v;
+    size_t prefix_len, p_page;  // p_page, s_page: rows of a page of the prefix, of the sequences
+    const Pages* seq;
+    const size_t* pos;
+    const size_t* n_tokens;
+    size_t n_seq, s_page, n_head, n_head_kv, head_dim, kv_dim;
+    const float* q;
+    float* out;
+};
+size_t attn_shared_scratch(const SharedCall& c);  // bytes
+hipError_t launch_attn_shared(const SharedCall& c, void* scratch, hipStream_t st);
+
 // ---- rotary positions and rotated appends (mvh_rope.hip) ----
 // out row t = x row t (n_head heads) rotated by position positions[t], or pos +
 // t when positions == null; out == x with equal pitches is allowed

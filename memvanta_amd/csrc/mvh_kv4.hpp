@@ -39,10 +39,6 @@ __host__ __device__ constexpr size_t kv4_scales(size_t page_tokens, size_t kv_di
 __host__ __device__ constexpr int kv4_k_word(int row, int kq) { return (kq * 4 + (row & 3)) * 2 + (row >> 2); }
 __host__ __device__ constexpr int kv4_v_word(int ch) { return (ch & 15) * 2 + (ch >> 4); }
 
-typedef _Float16 half2v __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ half2v as_half2(uint32_t w) { return __builtin_bit_cast(half2v, w); }
-__device__ __forceinline__ uint32_t as_u32(half2v h) { return __builtin_bit_cast(uint32_t, h); }
-
 // natural word (nibble j at bits 4j..) <-> stored word
 __host__ __device__ constexpr uint32_t kv4_store(uint32_t nat) { return (nat << 6) | (nat >> 26); }
 __host__ __device__ constexpr uint32_t kv4_nat(uint32_t w) { return (w >> 6) | (w << 26); }

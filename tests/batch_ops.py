@@ -75,3 +75,26 @@ def gated(x, wg, wu, act):
     # act itself: a handful of roundings of it, and of g where 1 + erf cancels
     ea = 1.13 * eg + 8 * STEP * np.abs(a) + 4 * STEP * np.abs(g)
     return a * u, ea * np.abs(u) + np.abs(a) * eu + ea * eu + STEP * np.abs(a * u)
+
+
+def attend_shared(q, prefix, own, pos, n_tokens, heads, kv_heads):
+    """Attention in 64 bits: prefix (k, v) [rows][kv_heads * hd], own the same per sequence (rows from the prefix's end on);
+    also the sum of the magnitudes that an output adds up."""
+    hd = q.shape[1] // heads
+    cut = lambda x: x.astype(np.float64).reshape(len(x), kv_heads, hd)
+    q = q.astype(np.float64).reshape(len(q), heads, hd)
+    out, size = np.empty_like(q), np.empty_like(q)
+    row, (pk, pv) = 0, map(cut, prefix)
+    for (k, v), p, n in zip(own, pos, n_tokens):
+        k, v = np.concatenate([pk, cut(k)]), np.concatenate([pv, cut(v)])
+        for t in range(n):
+            end = p + t + 1
+            for h in range(heads):
+                g = h // (heads // kv_heads)
+                s = k[:end, g] @ q[row, h] / math.sqrt(hd)
+                w = np.exp(s - s.max())
+                w /= w.sum()
+                with np.errstate(invalid="ignore"):
+                    out[row, h], size[row, h] = w @ v[:end, g], w @ np.abs(v[:end, g])
+            row += 1
+    return out.reshape(len(q), -1), size.reshape(len(q), -1)
