@@ -192,6 +192,151 @@ __global__ __launch_bounds__(64 * W) void fp8_rows_kernel(Fp8Args a) {
     }
 }
 
+// TM tokens x TN rows of the weights (with two matrices TN / 2 of each), four
+// waves of half the tokens and half the rows each; a step is one block of 128
+// columns.  The codes go from memory to LDS as they are, one step ahead, and are
+// widened behind it: as fp16 they would take twice the LDS reads, which at 64 x 64
+// a wave are half of the matrix pipe's time already.
+typedef __attribute__((address_space(3))) void lds_void;
+typedef const __attribute__((address_space(1))) void global_void;
+
+template <int TM, int TN>
+struct Step {  // rows of 128 bytes, their 16-byte chunks turned by the row: 16 rows' reads fall in different banks
+    uint8_t x[TM * kBlk], w[TN * kBlk];
+};
+__device__ __forceinline__ int turn(int row) { return (row >> 1) & 7; }
+__device__ __forceinline__ Codes32 codes_at(const uint8_t* rows, int row, int j) {
+    const uint8_t* r = rows + row * kBlk;
+    return widen(*reinterpret_cast<const uint4*>(r + ((j ^ turn(row)) * 16)), *reinterpret_cast<const uint4*>(r + (((j + 4) ^ turn(row)) * 16)));
+}
+
+template <int MATS, int TM, int TN>
+__global__ __launch_bounds__(256, 2) void fp8_tile_kernel(Fp8Args a) {
+    constexpr int WM = TM / 2, WN = TN / 2, XT = WM / 16, WT = WN / 16, PER = TN / MATS;  // PER: rows of a matrix
+    __shared__ __align__(16) Step<TM, TN> s0, s1;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, j = lane >> 4;
+    const int wm = wave & 1, wn = wave >> 1;
+    // tiles in eight runs, one per XCD (workgroups go to them in turn), tokens first: an XCD's L2 then holds few rows of the weights at a time
+    const int tiles_m = (a.M + TM - 1) / TM, tiles = tiles_m * ((a.N + PER - 1) / PER);
+    const int id = blockIdx.x, share = tiles / 8, more = tiles % 8, xcd = id & 7;
+    const int tile = xcd * share + min(xcd, more) + (id >> 3);
+    const int t0 = tile % tiles_m * TM, r0 = tile / tiles_m * PER;
+    const size_t pitch = static_cast<size_t>(a.blocks) * kBlk;
+    const uint32_t last = static_cast<uint32_t>(a.K - 16);
+
+    // eight rows of 128 bytes an instruction
+    constexpr int XI = TM / 32, WI = TN / 32;
+    uint32_t xo[XI], wo[WI];
+    const int in = lane >> 3, c = lane & 7;
+    const uint8_t* const xb = a.xq + static_cast<size_t>(t0) * pitch;
+#pragma unroll
+    for (int i = 0; i < XI; ++i) {
+        const int row = (i * 4 + wave) * 8 + in;
+        xo[i] = static_cast<uint32_t>(min(row, a.M - 1 - t0)) * static_cast<uint32_t>(pitch) + ((c ^ turn(row)) * 16);
+    }
+    uint32_t wc[WI];
+#pragma unroll
+    for (int i = 0; i < WI; ++i) {
+        const int row = (i * 4 + wave) * 8 + in;
+        wo[i] = static_cast<uint32_t>(min(row % PER, a.N - 1 - r0)) * static_cast<uint32_t>(a.K);
+        wc[i] = (c ^ turn(row)) * 16;
+    }
+    auto load = [&](Step<TM, TN>& s, int kb) {
+#pragma unroll
+        for (int i = 0; i < XI; ++i)
+            __builtin_amdgcn_global_load_lds((global_void*)(xb + (xo[i] + static_cast<uint32_t>(kb) * kBlk)),
+                                             (lds_void*)(s.x + (i * 4 + wave) * 1024), 16, 0, 0);
+#pragma unroll
+        for (int i = 0; i < WI; ++i) {
+            const int m = MATS == 2 ? (i * 4 + wave) * 8 / PER : 0;
+            const uint8_t* const wb = (m ? a.w[1] : a.w[0]) + static_cast<size_t>(r0) * a.K;
+            // a last block that is short: columns of the row again, against zeros
+            __builtin_amdgcn_global_load_lds((global_void*)(wb + (wo[i] + min(static_cast<uint32_t>(kb) * kBlk + wc[i], last))),
+                                             (lds_void*)(s.w + (i * 4 + wave) * 1024), 16, 0, 0);
+        }
+    };
+    const float* xs[XT];
+#pragma unroll
+    for (int t = 0; t < XT; ++t) xs[t] = a.xs + min(t0 + wm * WM + 16 * t + n, a.M - 1);
+    float xn[XT], wsn[MATS];
+    auto scales = [&](int kb) {
+#pragma unroll
+        for (int t = 0; t < XT; ++t) xn[t] = xs[t][static_cast<size_t>(kb) * a.M];
+#pragma unroll
+        for (int m = 0; m < MATS; ++m) wsn[m] = a.ws[m][static_cast<size_t>(r0 / kBlk) * a.blocks + kb];
+    };
+
+    f32x4 acc[WT][XT];
+#pragma unroll
+    for (int w = 0; w < WT; ++w)
+#pragma unroll
+        for (int t = 0; t < XT; ++t) acc[w][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto step = [&](const Step<TM, TN>& s, Step<TM, TN>& next, int kb) {
+        float sc[MATS][XT];
+#pragma unroll
+        for (int m = 0; m < MATS; ++m)
+#pragma unroll
+            for (int t = 0; t < XT; ++t) sc[m][t] = xn[t] * wsn[m];
+        __syncthreads();
+        if (kb + 1 < a.blocks) {
+            load(next, kb + 1);
+            scales(kb + 1);
+        }
+        Codes32 x[XT];
+#pragma unroll
+        for (int t = 0; t < XT; ++t) x[t] = codes_at(s.x, wm * WM + 16 * t + n, j);
+#pragma unroll
+        for (int w = 0; w < WT; ++w) {
+            const int m = MATS == 2 ? w / (WT / 2) : 0;
+            const int row = MATS == 2 ? m * PER + wn * (WN / 2) + 16 * (w % (WT / 2)) : wn * WN + 16 * w;
+            const Codes32 v = codes_at(s.w, row + n, j);
+#pragma unroll
+            for (int t = 0; t < XT; ++t) {
+                const f32x4 d = dot128(v, x[t]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[w][t][i] = fmaf(sc[m][t], d[i], acc[w][t][i]);
+            }
+        }
+    };
+    load(s0, 0);
+    scales(0);
+    for (int kb = 0; kb < a.blocks; kb += 2) {
+        step(s0, s1, kb);
+        if (kb + 1 < a.blocks) step(s1, s0, kb + 1);
+    }
+
+    const bool vec = a.N % 4 == 0;
+#pragma unroll
+    for (int t = 0; t < XT; ++t) {
+        const int token = t0 + wm * WM + 16 * t + n;
+        if (token >= a.M) continue;
+#pragma unroll
+        for (int w = 0; w < WT / MATS; ++w) {
+            const int r = r0 + wn * (WN / MATS) + 16 * w + 4 * j;
+            f32x4 v = acc[w][t];
+            if constexpr (MATS == 2)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = gated(v[i], acc[w + WT / 2][t][i], a.gate);
+            float* y = a.y + static_cast<size_t>(token) * a.N + r;
+            if (vec && r + 3 < a.N) *reinterpret_cast<f32x4*>(y) = v;
+            else
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (r + i < a.N) y[i] = v[i];
+        }
+    }
+}
+
+template <int MATS>
+void launch_tile(const Fp8Args& a, hipStream_t st) {
+    const int big = ((a.M + 127) / 128) * ((a.N * MATS + 127) / 128);
+    if (big >= 200) {
+        fp8_tile_kernel<MATS, 128, 128><<<dim3(static_cast<unsigned>((a.M + 127) / 128) * ((a.N + 128 / MATS - 1) / (128 / MATS))), 256, 0, st>>>(a);
+    } else {
+        fp8_tile_kernel<MATS, 64, 64><<<dim3(static_cast<unsigned>((a.M + 63) / 64) * ((a.N + 64 / MATS - 1) / (64 / MATS))), 256, 0, st>>>(a);
+    }
+}
+
 }  // namespace
 
 size_t fp8_scratch(size_t K, size_t M) {
@@ -228,6 +373,11 @@ hipError_t launch_fp8(const uint8_t* w, const uint8_t* w2, int gate, const float
     a.xq = xq, a.xs = xs, a.y = y;
     quantize_rows_kernel<<<dim3(static_cast<unsigned>((items + 7) / 8)), 256, 0, st>>>(
         x, a.K, a.blocks, items, xq, blocks * kBlk, xs, 1, M);
+    if (M > 64) {
+        if (w2) launch_tile<2>(a, st);
+        else launch_tile<1>(a, st);
+        return hipGetLastError();
+    }
     const dim3 grid(static_cast<unsigned>((N + 15) / 16), static_cast<unsigned>((M + 15) / 16));
     if (w2) fp8_rows_kernel<2, 1, 4><<<grid, 256, 0, st>>>(a);
     else fp8_rows_kernel<1, 1, 4><<<grid, 256, 0, st>>>(a);
