@@ -1045,11 +1045,12 @@ static int fp8_call(mvh_context* c, const mvh_tensor* w, const mvh_tensor* up, i
                     int kind) {
     if (kind != MVH_HOST && kind != MVH_DEVICE) return fail(MVH_E_INVALID, "ptr_kind must be MVH_HOST or MVH_DEVICE");
     const size_t cols = w->ne0, rows = w->ne1;
+    // offsets of 32 bits within a tile's rows; fewer than 2^32 threads a launch
     if (batch > (size_t{1} << 20)) return fail(MVH_E_RANGE, "more than 1048576 tokens");
-    const size_t blocks = (cols + 127) / 128;
-    if (batch * blocks > (size_t{1} << 26) || (rows + 15) / 16 > (size_t{1} << 22))
+    if (cols > (size_t{1} << 23) || batch * ((cols + 127) / 128) > (size_t{1} << 26) ||
+        ((batch + 63) / 64) * ((rows + 31) / 32) * 8 > (size_t{1} << 24))
         return fail(MVH_E_RANGE, "fp8 product too large");
-    if (!batch) return MVH_OK;
+    if (!batch || !rows || !cols) return MVH_OK;
     if (!x || !y) return fail(MVH_E_INVALID, "null x/y");
     const void* xd = nullptr;
     if (int rc = stage_in_act(c, c->xin, x, batch * cols * 4, kind, &xd)) return rc;
@@ -1058,7 +1059,7 @@ static int fp8_call(mvh_context* c, const mvh_tensor* w, const mvh_tensor* up, i
         if (int rc = grow(c, c->yout, batch * rows * 4)) return rc;
         yd = static_cast<float*>(c->yout.p);
     }
-    if (int rc = grow_kept(c, c->work, mvh::fp8_scratch(cols, batch))) return rc;
+    if (int rc = grow_kept(c, c->work, mvh::fp8_scratch(rows, cols, batch, up != nullptr))) return rc;
     std::string name;
     try {
         name = up ? w->name + "+" + up->name : w->name;

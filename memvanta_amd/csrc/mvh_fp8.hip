@@ -10,6 +10,8 @@
 // themselves against 64 bits, 40 times what they are here.
 #include "mvh_kernels.hpp"
 
+#include <cmath>
+
 namespace mvh {
 namespace {
 
@@ -18,6 +20,8 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr int kBlk = 128;
 constexpr float kTop = 448.0f;            // largest e4m3 value
 constexpr float kLeast = 0x1p-126f;       // scales below are no normal numbers: the block is held as zeros
+
+size_t up16(size_t n) { return (n + 15) & ~size_t{15}; }
 
 // 32 codes as fp16
 struct Codes32 {
@@ -114,156 +118,283 @@ __global__ __launch_bounds__(256) void quantize_tiles_kernel(const float* __rest
 struct Fp8Args {
     const uint8_t* w[2];   // codes [N][K]
     const float* ws[2];    // scales [ceil(N / 128)][blocks]
-    const uint8_t* xq;     // codes [M][128 blocks], zeros behind column K
-    const float* xs;       // scales [blocks][M]
+    const float* x;        // [M][K]
+    const uint8_t* xq;     // codes [M][128 blocks], zeros behind column K; or operands (quantize_operand_kernel)
+    const float* xs;       // scales [blocks][M], or [blocks][x_rows]
     float* y;              // [M][N]
-    int N, K, M, blocks, gate;
+    float* part;           // sums of the splits of K, [split][matrix][M][n4]; null without splits
+    int N, K, M, blocks, gate, x_rows, n4, per;  // per: blocks of a split
 };
+
+// A float at an address that is the same in every lane, through the scalar cache
+__device__ __forceinline__ float load_const(const float* p) {
+    typedef const __attribute__((address_space(4))) float* entry;
+    return *reinterpret_cast<entry>(reinterpret_cast<uintptr_t>(p));
+}
 
 __device__ __forceinline__ float gated(float g, float u, int gate) {
     const float a = gate == kGateSilu ? __fdiv_rn(g, 1.0f + expf(-g)) : 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
     return a * u;
 }
 
-// One workgroup: 16 rows of the weights, 16 TT tokens, its waves the blocks of K
-// in turn.
-template <int MATS, int TT, int W>
+// ---- up to 64 tokens: bound by the weights' bytes -------------------------------
+
+// x as codes in the operand's order for tiles of 16 tokens: [tile][block][half][lane],
+// the 16 codes that the lane (token, j) holds of each half of the block; scales
+// [block][16 tiles].  32 lanes a block of a token, four codes each; tokens behind the
+// last are the last one.
+__global__ __launch_bounds__(256) void quantize_operand_kernel(const float* __restrict__ x, int cols, int blocks, int M, int items,
+                                                               uint8_t* __restrict__ op, float* __restrict__ scales) {
+    const int lane = threadIdx.x & 31, item = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (item >= items) return;
+    const int row = item / blocks, kb = item - row * blocks, at = kb * kBlk + lane * 4;
+    const float4 v = at < cols ? *reinterpret_cast<const float4*>(x + static_cast<size_t>(min(row, M - 1)) * cols + at) : make_float4(0.f, 0.f, 0.f, 0.f);
+    const float s = scale_of(half_max(top4(v)));
+    const size_t to = ((static_cast<size_t>(row >> 4) * blocks + kb) * 2 + (lane >> 4)) * 1024 + (((lane >> 2) & 3) * 16 + (row & 15)) * 16 + (lane & 3) * 4;
+    *reinterpret_cast<uint32_t*>(op + to) = codes4(v, inverse_of(s));
+    if (lane == 0) scales[static_cast<size_t>(kb) * (items / blocks) + row] = s;
+}
+
+// A workgroup: 16 rows of the weights (of both matrices) after another, 16 TT
+// tokens; its W waves take the blocks of K in turn, U at a time with the next U on
+// their way, and join through LDS.  QIN: x is quantised here, by every workgroup
+// for itself, while the first weights come; else it comes as operands.
+template <int MATS, int TT, int W, int U, bool QIN>
 __global__ __launch_bounds__(64 * W) void fp8_rows_kernel(Fp8Args a) {
+    extern __shared__ __align__(16) uint8_t s_x[];  // QIN: codes [M][128 blocks + 16], scales [blocks][M]
     __shared__ float s_y[W][MATS][TT][16][17];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, j = lane >> 4;
-    const int r0 = blockIdx.x * 16, t0 = blockIdx.y * 16 * TT, last16 = a.K / 16 - 1;
-    const size_t pitch = static_cast<size_t>(a.blocks) * kBlk;
-    const uint8_t* wp[MATS];
-    const float* sp[MATS];
+    const int t0 = blockIdx.y * 16 * TT, last16 = a.K / 16 - 1, tiles = (a.N + 15) / 16;
+    const int pitch = a.blocks * kBlk + 16;
+    float* const s_xs = reinterpret_cast<float*>(s_x + a.M * pitch);
+    int from[TT];  // lanes of tokens behind the last read what the last one's does: fewer lines
 #pragma unroll
-    for (int m = 0; m < MATS; ++m) {
-        wp[m] = a.w[m] + static_cast<size_t>(min(r0 + n, a.N - 1)) * a.K;
-        sp[m] = a.ws[m] + static_cast<size_t>(r0 / kBlk) * a.blocks;
-    }
-    f32x4 acc[MATS][TT];
+    for (int t = 0; t < TT; ++t) from[t] = j * 16 + min(n, max(a.M - 1 - t0 - 16 * t, 0));
+    struct Group {
+        uint4 w[U][MATS][2];
+    };
+    auto load = [&](Group& g, int tile, int first) {  // blocks behind the last: the last one again, left out of the sums
+        const int row = min(tile * 16 + n, a.N - 1);
 #pragma unroll
-    for (int m = 0; m < MATS; ++m)
-#pragma unroll
-        for (int t = 0; t < TT; ++t) acc[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int kb = wave; kb < a.blocks; kb += W) {
-        // a last block that is short: columns of the row again, against zeros
-        const size_t c0 = 16 * static_cast<size_t>(min(kb * 8 + j, last16)), c1 = 16 * static_cast<size_t>(min(kb * 8 + 4 + j, last16));
-        Codes32 w[MATS];
-        float ws[MATS];
-#pragma unroll
-        for (int m = 0; m < MATS; ++m) {
-            w[m] = widen(ld_global16(wp[m] + c0), ld_global16(wp[m] + c1));
-            ws[m] = sp[m][kb];
-        }
-#pragma unroll
-        for (int t = 0; t < TT; ++t) {
-            const int tok = min(t0 + 16 * t + n, a.M - 1);
-            const uint8_t* xp = a.xq + tok * pitch + kb * kBlk + 16 * j;
-            const Codes32 x = widen(ld_global16(xp), ld_global16(xp + 64));
-            const float xs = a.xs[static_cast<size_t>(kb) * a.M + tok];
+        for (int u = 0; u < U; ++u) {
+            const int kb = min(first + u * W, a.blocks - 1);
+            // a last block that is short: columns of the row again, against zeros
+            const size_t c0 = 16 * static_cast<size_t>(min(kb * 8 + j, last16)), c1 = 16 * static_cast<size_t>(min(kb * 8 + 4 + j, last16));
 #pragma unroll
             for (int m = 0; m < MATS; ++m) {
-                const f32x4 c = dot128(w[m], x);
-                const float s = xs * ws[m];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[m][t][i] = fmaf(s, c[i], acc[m][t][i]);
+                const uint8_t* w = a.w[m] + static_cast<size_t>(row) * a.K;
+                g.w[u][m][0] = ld_stream16(w + c0);
+                g.w[u][m][1] = ld_stream16(w + c1);
             }
         }
-    }
+    };
+    Group now;
+    load(now, blockIdx.x, wave);
+    if constexpr (QIN) {
+        // four blocks of a half wave at a time: one trip to memory
+        const int lane32 = threadIdx.x & 31, items = a.M * a.blocks;
+        for (int first = threadIdx.x >> 5; first < items; first += 8 * W) {
+            float4 v[4];
 #pragma unroll
-    for (int m = 0; m < MATS; ++m)
+            for (int u = 0; u < 4; ++u) {
+                const int item = min(first + 2 * W * u, items - 1), tok = item / a.blocks, at = (item - tok * a.blocks) * kBlk + lane32 * 4;
+                v[u] = at < a.K ? *reinterpret_cast<const float4*>(a.x + static_cast<size_t>(tok) * a.K + at) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
 #pragma unroll
-        for (int t = 0; t < TT; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s_y[wave][m][t][n][4 * j + i] = acc[m][t][i];
-    __syncthreads();
-    for (int e = threadIdx.x; e < 256 * TT; e += 64 * W) {
-        const int t = e >> 8, tok = (e >> 4) & 15, r = e & 15;
-        float v[MATS];
-#pragma unroll
-        for (int m = 0; m < MATS; ++m) {
-            v[m] = s_y[0][m][t][tok][r];
-#pragma unroll
-            for (int k = 1; k < W; ++k) v[m] += s_y[k][m][t][tok][r];
+            for (int u = 0; u < 4; ++u) {
+                const int item = first + 2 * W * u, tok = item / a.blocks, kb = item - tok * a.blocks;
+                const float s = scale_of(half_max(top4(v[u])));
+                if (item >= items) break;
+                *reinterpret_cast<uint32_t*>(s_x + tok * pitch + kb * kBlk + lane32 * 4) = codes4(v[u], inverse_of(s));
+                if (lane32 == 0) s_xs[kb * a.M + tok] = s;
+            }
         }
-        const int token = t0 + 16 * t + tok;
-        if (token < a.M && r0 + r < a.N)
-            a.y[static_cast<size_t>(token) * a.N + r0 + r] = MATS == 2 ? gated(v[0], v[MATS - 1], a.gate) : v[0];
+        __syncthreads();
+    }
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        f32x4 acc[MATS][TT];
+#pragma unroll
+        for (int m = 0; m < MATS; ++m)
+#pragma unroll
+            for (int t = 0; t < TT; ++t) acc[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const size_t srow = static_cast<size_t>(tile * 16 / kBlk) * a.blocks;
+        for (int first = wave; first < a.blocks; first += U * W) {
+            Group next;
+            if (first + U * W < a.blocks) load(next, tile, first + U * W);
+            else if (tile + static_cast<int>(gridDim.x) < tiles) load(next, tile + gridDim.x, wave);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int kb = first + u * W;
+                if (kb >= a.blocks) break;
+                Codes32 w[MATS];
+                float ws[MATS];
+#pragma unroll
+                for (int m = 0; m < MATS; ++m) {
+                    w[m] = widen(now.w[u][m][0], now.w[u][m][1]);
+                    ws[m] = load_const(a.ws[m] + srow + kb);
+                }
+#pragma unroll
+                for (int t = 0; t < TT; ++t) {
+                    Codes32 x;
+                    float xs;
+                    if constexpr (QIN) {
+                        const int tok = min(n, a.M - 1);
+                        const uint8_t* p = s_x + tok * pitch + kb * kBlk + 16 * j;
+                        x = widen(*reinterpret_cast<const uint4*>(p), *reinterpret_cast<const uint4*>(p + 64));
+                        xs = s_xs[kb * a.M + tok];
+                    } else {
+                        const uint4* p = reinterpret_cast<const uint4*>(a.xq) + (static_cast<size_t>(t0 / 16 + t) * a.blocks + kb) * 128 + from[t];
+                        x = widen(p[0], p[64]);
+                        xs = a.xs[static_cast<size_t>(kb) * a.x_rows + t0 + 16 * t + n];
+                    }
+#pragma unroll
+                    for (int m = 0; m < MATS; ++m) {
+                        const f32x4 c = dot128(w[m], x);
+                        const float s = xs * ws[m];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[m][t][i] = fmaf(s, c[i], acc[m][t][i]);
+                    }
+                }
+            }
+            now = next;
+        }
+#pragma unroll
+        for (int m = 0; m < MATS; ++m)
+#pragma unroll
+            for (int t = 0; t < TT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s_y[wave][m][t][n][4 * j + i] = acc[m][t][i];
+        __syncthreads();
+        for (int e = threadIdx.x; e < 256 * TT; e += 64 * W) {
+            const int t = e >> 8, tok = (e >> 4) & 15, r = e & 15;
+            float v[MATS];
+#pragma unroll
+            for (int m = 0; m < MATS; ++m) {
+                v[m] = s_y[0][m][t][tok][r];
+#pragma unroll
+                for (int k = 1; k < W; ++k) v[m] += s_y[k][m][t][tok][r];
+            }
+            const int token = t0 + 16 * t + tok, row = tile * 16 + r;
+            if (token < a.M && row < a.N)
+                a.y[static_cast<size_t>(token) * a.N + row] = MATS == 2 ? gated(v[0], v[MATS - 1], a.gate) : v[0];
+        }
+        __syncthreads();
     }
 }
 
-// TM tokens x TN rows of the weights (with two matrices TN / 2 of each), four
-// waves of half the tokens and half the rows each; a step is one block of 128
-// columns.  The codes go from memory to LDS as they are, one step ahead, and are
-// widened behind it: as fp16 they would take twice the LDS reads, which at 64 x 64
-// a wave are half of the matrix pipe's time already.
-typedef __attribute__((address_space(3))) void lds_void;
-typedef const __attribute__((address_space(1))) void global_void;
+// ---- more tokens: tiles through LDS ----------------------------------------------
+
 
 template <int TM, int TN>
 struct Step {  // rows of 128 bytes, their 16-byte chunks turned by the row: 16 rows' reads fall in different banks
     uint8_t x[TM * kBlk], w[TN * kBlk];
+    float xs[TM < 64 ? 64 : TM];
 };
 __device__ __forceinline__ int turn(int row) { return (row >> 1) & 7; }
-__device__ __forceinline__ Codes32 codes_at(const uint8_t* rows, int row, int j) {
+struct Raw32 {
+    uint4 a, b;
+};
+__device__ __forceinline__ Raw32 raw_at(const uint8_t* rows, int row, int j) {
     const uint8_t* r = rows + row * kBlk;
-    return widen(*reinterpret_cast<const uint4*>(r + ((j ^ turn(row)) * 16)), *reinterpret_cast<const uint4*>(r + (((j + 4) ^ turn(row)) * 16)));
+    return {*reinterpret_cast<const uint4*>(r + ((j ^ turn(row)) * 16)), *reinterpret_cast<const uint4*>(r + (((j + 4) ^ turn(row)) * 16))};
+}
+__device__ __forceinline__ Codes32 widen(const Raw32& r) { return widen(r.a, r.b); }
+
+// Waits for this wave's loads and LDS reads, then for the other waves.  (s_waitcnt: vmcnt in bits 0 - 3 and 14 - 15,
+// expcnt, left alone, in 4 - 6, lgkmcnt in 8 - 11.)
+__device__ __forceinline__ void arrive() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(7 << 4);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+// Memory from p on, for loads that go to LDS: offsets of 32 bits, what lies `bytes` or more behind p reads as 0.  (The
+// host's pass over this file has not the device's buffer type.)
+#ifdef __HIP_DEVICE_COMPILE__
+typedef __amdgpu_buffer_rsrc_t buffer_t;
+#else
+typedef uint4 buffer_t;
+#endif
+__device__ __forceinline__ buffer_t buffer_of(const void* p, size_t bytes) {
+#ifdef __HIP_DEVICE_COMPILE__
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, static_cast<int>(bytes < 0xfffffff0u ? bytes : 0xfffffff0u), 0x00020000);
+#else
+    return {};
+#endif
+}
+// B bytes a lane from `at` + `more` of the buffer to consecutive places of LDS
+template <int B>
+__device__ __forceinline__ void load_lds(buffer_t b, void* to, uint32_t at, int more) {
+#ifdef __HIP_DEVICE_COMPILE__
+    auto* const lds = (__attribute__((address_space(3))) void*)to;
+    if constexpr (B == 16) __builtin_amdgcn_raw_ptr_buffer_load_lds(b, lds, 16, static_cast<int>(at), more, 0, 0);
+    else __builtin_amdgcn_raw_ptr_buffer_load_lds(b, lds, 4, static_cast<int>(at), more, 0, 0);
+#endif
 }
 
-template <int MATS, int TM, int TN>
-__global__ __launch_bounds__(256, 2) void fp8_tile_kernel(Fp8Args a) {
-    constexpr int WM = TM / 2, WN = TN / 2, XT = WM / 16, WT = WN / 16, PER = TN / MATS;  // PER: rows of a matrix
+// TM tokens x TN rows of the weights (with two matrices TN / 2 of each), G times PM
+// x PN waves, which take every G-th block of columns; a step is one block of 128 columns.  The codes go from memory to LDS as
+// they are, D - 1 steps ahead, and are widened behind it: as fp16 they would take
+// twice the LDS reads, which at 64 x 64 a wave are half of the matrix pipe's time
+// already.
+template <int MATS, int TM, int TN, int PM, int PN>
+__global__ __launch_bounds__(64 * PM * PN, 2) void fp8_tile_kernel(Fp8Args a) {
+    constexpr int W = PM * PN, WM = TM / PM, WN = TN / PN, XT = WM / 16, WT = WN / 16, PER = TN / MATS;  // PER: rows of a matrix
+    constexpr int XI = TM / 8 / W, WI = TN / 8 / W, SI = TM > 64 * W ? TM / (64 * W) : 1;
+    static_assert(TM % (8 * W) == 0 && TN % (8 * W) == 0 && WT % MATS == 0 && PER % 8 == 0 && 128 % (WN / MATS) == 0 );
     __shared__ __align__(16) Step<TM, TN> s0, s1;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, j = lane >> 4;
-    const int wm = wave & 1, wn = wave >> 1;
-    // tiles in eight runs, one per XCD (workgroups go to them in turn), tokens first: an XCD's L2 then holds few rows of the weights at a time
+    const int wm = wave % PM, wn = wave / PM;
+    // tiles in eight runs, one per XCD (workgroups go to them in turn)
     const int tiles_m = (a.M + TM - 1) / TM, tiles = tiles_m * ((a.N + PER - 1) / PER);
     const int id = blockIdx.x, share = tiles / 8, more = tiles % 8, xcd = id & 7;
     const int tile = xcd * share + min(xcd, more) + (id >> 3);
-    const int t0 = tile % tiles_m * TM, r0 = tile / tiles_m * PER;
+    // groups of four tiles along the rows, then the tokens
+    const int tiles_n = tiles / tiles_m, group = tile / (4 * tiles_m), wide = min(4, tiles_n - 4 * group), at = tile - 4 * group * tiles_m;
+    const int t0 = at / wide * TM, r0 = (4 * group + at % wide) * PER;
+    const int k0 = blockIdx.y * a.per, k1 = min(k0 + a.per, a.blocks);
     const size_t pitch = static_cast<size_t>(a.blocks) * kBlk;
     const uint32_t last = static_cast<uint32_t>(a.K - 16);
 
     // eight rows of 128 bytes an instruction
-    constexpr int XI = TM / 32, WI = TN / 32;
-    uint32_t xo[XI], wo[WI];
+    uint32_t xo[XI], wo[WI], wc[WI];
     const int in = lane >> 3, c = lane & 7;
-    const uint8_t* const xb = a.xq + static_cast<size_t>(t0) * pitch;
+    const buffer_t xb = buffer_of(a.xq + static_cast<size_t>(t0) * pitch, static_cast<size_t>(a.M - t0) * pitch);
+    const buffer_t sb = buffer_of(a.xs, static_cast<size_t>(a.blocks) * a.M * 4);
+    buffer_t wb[MATS];
+#pragma unroll
+    for (int m = 0; m < MATS; ++m) wb[m] = buffer_of(a.w[m] + static_cast<size_t>(r0) * a.K, static_cast<size_t>(a.N - r0) * a.K);
 #pragma unroll
     for (int i = 0; i < XI; ++i) {
-        const int row = (i * 4 + wave) * 8 + in;
+        const int row = (i * W + wave) * 8 + in;
         xo[i] = static_cast<uint32_t>(min(row, a.M - 1 - t0)) * static_cast<uint32_t>(pitch) + ((c ^ turn(row)) * 16);
     }
-    uint32_t wc[WI];
 #pragma unroll
     for (int i = 0; i < WI; ++i) {
-        const int row = (i * 4 + wave) * 8 + in;
+        const int row = (i * W + wave) * 8 + in;
         wo[i] = static_cast<uint32_t>(min(row % PER, a.N - 1 - r0)) * static_cast<uint32_t>(a.K);
         wc[i] = (c ^ turn(row)) * 16;
     }
-    auto load = [&](Step<TM, TN>& s, int kb) {
+    uint32_t so[SI];  // scales, 64 tokens an instruction; waves beyond them load some again, so that all waves count alike
+#pragma unroll
+    for (int i = 0; i < SI; ++i) so[i] = static_cast<uint32_t>(min(t0 + ((i * W + wave) * 64) % TM + lane % TM, a.M - 1));
+    const size_t srow = static_cast<size_t>(min(r0 + wn * (WN / MATS), a.N - 1) / kBlk) * a.blocks;  // of the wave's rows
+    // Behind the last block the last one again, so that the waits' counts hold
+    auto load = [&](Step<TM, TN>& s, int step) {
+        const int kb = min(k0 + step, k1 - 1);
 #pragma unroll
         for (int i = 0; i < XI; ++i)
-            __builtin_amdgcn_global_load_lds((global_void*)(xb + (xo[i] + static_cast<uint32_t>(kb) * kBlk)),
-                                             (lds_void*)(s.x + (i * 4 + wave) * 1024), 16, 0, 0);
+            load_lds<16>(xb, s.x + (i * W + wave) * 1024, xo[i], kb * kBlk);
 #pragma unroll
         for (int i = 0; i < WI; ++i) {
-            const int m = MATS == 2 ? (i * 4 + wave) * 8 / PER : 0;
-            const uint8_t* const wb = (m ? a.w[1] : a.w[0]) + static_cast<size_t>(r0) * a.K;
+            const int m = MATS == 2 ? (i * W + wave) * 8 / PER : 0;
             // a last block that is short: columns of the row again, against zeros
-            __builtin_amdgcn_global_load_lds((global_void*)(wb + (wo[i] + min(static_cast<uint32_t>(kb) * kBlk + wc[i], last))),
-                                             (lds_void*)(s.w + (i * 4 + wave) * 1024), 16, 0, 0);
+            const uint32_t at = wo[i] + min(static_cast<uint32_t>(kb) * kBlk + wc[i], last);
+            load_lds<16>(m ? wb[MATS - 1] : wb[0], s.w + (i * W + wave) * 1024, at, 0);
         }
-    };
-    const float* xs[XT];
 #pragma unroll
-    for (int t = 0; t < XT; ++t) xs[t] = a.xs + min(t0 + wm * WM + 16 * t + n, a.M - 1);
-    float xn[XT], wsn[MATS];
-    auto scales = [&](int kb) {
-#pragma unroll
-        for (int t = 0; t < XT; ++t) xn[t] = xs[t][static_cast<size_t>(kb) * a.M];
-#pragma unroll
-        for (int m = 0; m < MATS; ++m) wsn[m] = a.ws[m][static_cast<size_t>(r0 / kBlk) * a.blocks + kb];
+        for (int i = 0; i < SI; ++i)
+            load_lds<4>(sb, s.xs + ((i * W + wave) * 64) % TM, so[i] * 4, kb * a.M * 4);
     };
 
     f32x4 acc[WT][XT];
@@ -271,25 +402,27 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel(Fp8Args a) {
     for (int w = 0; w < WT; ++w)
 #pragma unroll
         for (int t = 0; t < XT; ++t) acc[w][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto step = [&](const Step<TM, TN>& s, Step<TM, TN>& next, int kb) {
+    auto step = [&](const Step<TM, TN>& s, Step<TM, TN>& next, int k) {
+        float ws[MATS];
+#pragma unroll
+        for (int m = 0; m < MATS; ++m) ws[m] = load_const(a.ws[m] + srow + k0 + k);
+        arrive();  // this step's codes are there, and nobody reads the last step's any more
+        load(next, k + 1);
         float sc[MATS][XT];
 #pragma unroll
-        for (int m = 0; m < MATS; ++m)
+        for (int t = 0; t < XT; ++t) {
+            const float xs = s.xs[wm * WM + 16 * t + n];
 #pragma unroll
-            for (int t = 0; t < XT; ++t) sc[m][t] = xn[t] * wsn[m];
-        __syncthreads();
-        if (kb + 1 < a.blocks) {
-            load(next, kb + 1);
-            scales(kb + 1);
+            for (int m = 0; m < MATS; ++m) sc[m][t] = xs * ws[m];
         }
         Codes32 x[XT];
 #pragma unroll
-        for (int t = 0; t < XT; ++t) x[t] = codes_at(s.x, wm * WM + 16 * t + n, j);
+        for (int t = 0; t < XT; ++t) x[t] = widen(raw_at(s.x, wm * WM + 16 * t + n, j));
 #pragma unroll
         for (int w = 0; w < WT; ++w) {
             const int m = MATS == 2 ? w / (WT / 2) : 0;
             const int row = MATS == 2 ? m * PER + wn * (WN / 2) + 16 * (w % (WT / 2)) : wn * WN + 16 * w;
-            const Codes32 v = codes_at(s.w, row + n, j);
+            const Codes32 v = widen(raw_at(s.w, row + n, j));
 #pragma unroll
             for (int t = 0; t < XT; ++t) {
                 const f32x4 d = dot128(v, x[t]);
@@ -298,18 +431,28 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel(Fp8Args a) {
             }
         }
     };
+    const int steps = k1 - k0;
     load(s0, 0);
-    scales(0);
-    for (int kb = 0; kb < a.blocks; kb += 2) {
-        step(s0, s1, kb);
-        if (kb + 1 < a.blocks) step(s1, s0, kb + 1);
+    for (int k = 0; k < steps; k += 2) {
+        step(s0, s1, k);
+        if (k + 1 < steps) step(s1, s0, k + 1);
     }
+    arrive();  // no load into LDS outlives the workgroup
 
     const bool vec = a.N % 4 == 0;
 #pragma unroll
     for (int t = 0; t < XT; ++t) {
         const int token = t0 + wm * WM + 16 * t + n;
         if (token >= a.M) continue;
+        if (a.part) {
+#pragma unroll
+            for (int w = 0; w < WT; ++w) {
+                const int m = w / (WT / MATS), r = r0 + wn * (WN / MATS) + 16 * (w % (WT / MATS)) + 4 * j;
+                if (r < a.N)
+                    *reinterpret_cast<f32x4*>(a.part + ((static_cast<size_t>(blockIdx.y) * MATS + m) * a.M + token) * a.n4 + r) = acc[w][t];
+            }
+            continue;
+        }
 #pragma unroll
         for (int w = 0; w < WT / MATS; ++w) {
             const int r = r0 + wn * (WN / MATS) + 16 * w + 4 * j;
@@ -327,21 +470,134 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel(Fp8Args a) {
     }
 }
 
+// y from the sums of the splits, four rows of the weights a thread
 template <int MATS>
-void launch_tile(const Fp8Args& a, hipStream_t st) {
-    const int big = ((a.M + 127) / 128) * ((a.N * MATS + 127) / 128);
-    if (big >= 200) {
-        fp8_tile_kernel<MATS, 128, 128><<<dim3(static_cast<unsigned>((a.M + 127) / 128) * ((a.N + 128 / MATS - 1) / (128 / MATS))), 256, 0, st>>>(a);
-    } else {
-        fp8_tile_kernel<MATS, 64, 64><<<dim3(static_cast<unsigned>((a.M + 63) / 64) * ((a.N + 64 / MATS - 1) / (64 / MATS))), 256, 0, st>>>(a);
+__global__ __launch_bounds__(256) void fp8_join_kernel(Fp8Args a, int splits) {
+    const size_t at = (static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x) * 4, all = static_cast<size_t>(a.M) * a.n4;
+    if (at >= all) return;
+    f32x4 v[MATS];
+#pragma unroll
+    for (int m = 0; m < MATS; ++m) v[m] = *reinterpret_cast<const f32x4*>(a.part + m * all + at);
+    for (int k = 1; k < splits; ++k)
+#pragma unroll
+        for (int m = 0; m < MATS; ++m) v[m] += *reinterpret_cast<const f32x4*>(a.part + (static_cast<size_t>(k) * MATS + m) * all + at);
+    if constexpr (MATS == 2)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[0][i] = gated(v[0][i], v[1][i], a.gate);
+    const size_t token = at / a.n4;
+    const int r = static_cast<int>(at - token * a.n4);
+    float* y = a.y + token * a.N + r;
+    if (a.N % 4 == 0) *reinterpret_cast<f32x4*>(y) = v[0];
+    else
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (r + i < a.N) y[i] = v[0][i];
+}
+
+constexpr int kCus = 256;
+
+// Which kernel a product takes, and how it is cut.
+struct Plan {
+    enum { kRowsQuantizing, kRows, kTile64, kTile64x128, kTile128 } kind;
+    int splits;
+};
+struct TileCost {
+    int kind, tm, tn;
+    double alone, each;  // us of a step of a workgroup alone on its CU, and of each of several
+};
+// Weights' bytes bound up to 16 tokens, and up to 64 where they are few: there every
+// workgroup reads all of x, and at 32 tokens and 131 MB (N 32000, K 4096) takes 45 us
+// where tiles take 37, at 48 and 45 MB 24 and 19, at 64 and 11 MB 10.5 and 12.2.
+// x is quantised within the kernel while that costs less than a launch (4 tokens, K
+// 4096: 7.9 and 8.4 us; K 11008: 18.9 and 16.5).
+//
+// Of the tiles the one with the least time by this model: steps of 128 columns that
+// cost `alone` while a CU has one workgroup, and `each` a workgroup where that is
+// more; a split of K adds a launch and two passes over its sums.  Measured (us) and
+// modelled less 4 for the launches, 333 tokens, K 11008 -> 4096: 64 x 64 whole 58 / 57,
+// in two 48 / 52; 64 x 128 in two 50 / 52, in four 45 / 47; 128 x 128 in two 53 / 51.
+Plan plan_of(size_t N, size_t K, size_t M, int mats) {
+    const double mb = static_cast<double>(N) * K * mats * 1e-6;
+    if (M <= 16 || (M <= 32 && mb <= 100) || (M <= 64 && mb <= 20)) {
+        const size_t blocks = (K + kBlk - 1) / kBlk;
+        const bool here = M <= 4 && M * K <= 32768 && M * (blocks * (kBlk + 4) + 16) <= 40 << 10;
+        return {here ? Plan::kRowsQuantizing : Plan::kRows, 1};
     }
+    static constexpr TileCost kTiles[] = {{Plan::kTile64, 64, 64, 0.47, 0.33}, {Plan::kTile64x128, 64, 128, 0.66, 0.5}, {Plan::kTile128, 128, 128, 0.97, 0.85}};
+    const int blocks = static_cast<int>((K + kBlk - 1) / kBlk);
+    Plan best{Plan::kTile64, 1};
+    double least = 1e300;
+    for (const TileCost& t : kTiles) {
+        const double tiles = static_cast<double>((M + t.tm - 1) / t.tm) * static_cast<double>((N * mats + t.tn - 1) / t.tn);
+        for (int splits = 1; splits <= 8 && blocks / splits >= 4; splits *= 2) {
+            const double join = splits > 1 ? 2.0 + 8e-6 / 4 * splits * M * N * mats : 0.0;
+            const double us = (blocks + splits - 1) / splits * std::max(t.alone, std::ceil(tiles * splits / kCus) * t.each) + join;
+            if (us < least) least = us, best = {static_cast<decltype(Plan::kind)>(t.kind), splits};
+        }
+    }
+    return best;
+}
+
+template <int MATS, int TM, int TN, int PM, int PN>
+void run_tile(Fp8Args& a, int splits, hipStream_t st) {
+    const unsigned grid = static_cast<unsigned>((a.M + TM - 1) / TM) * ((a.N + TN / MATS - 1) / (TN / MATS));
+    a.per = (a.blocks + splits - 1) / splits;
+    splits = (a.blocks + a.per - 1) / a.per;
+    if (splits == 1) a.part = nullptr;
+    fp8_tile_kernel<MATS, TM, TN, PM, PN><<<dim3(grid, static_cast<unsigned>(splits)), 64 * PM * PN, 0, st>>>(a);
+    if (splits > 1)
+        fp8_join_kernel<MATS><<<dim3(static_cast<unsigned>((static_cast<size_t>(a.M) * a.n4 / 4 + 255) / 256)), 256, 0, st>>>(a, splits);
+}
+template <int MATS, int TT, int W, bool QIN>
+void run_rows(const Fp8Args& a, int wgs, size_t lds, hipStream_t st) {
+    fp8_rows_kernel<MATS, TT, W, 1, QIN><<<dim3(static_cast<unsigned>(std::min((a.N + 15) / 16, wgs))), 64 * W, lds, st>>>(a);
+}
+
+template <int MATS>
+hipError_t run(Fp8Args& a, const Plan& p, void* scratch, hipStream_t st) {
+    // waves of a workgroup: 16 where all rows of the weights are on the chip at once (K 11008 -> 4096, one token: 13.5 us, with 8 15.2)
+    const bool few = (a.N + 15) / 16 <= kCus;
+    if (p.kind == Plan::kRowsQuantizing) {
+        const size_t lds = static_cast<size_t>(a.M) * (a.blocks * (kBlk + 4) + 16);
+        if (few) run_rows<MATS, 1, 16, true>(a, 2 * kCus, lds, st);
+        else run_rows<MATS, 1, 8, true>(a, 2 * kCus, lds, st);
+        return hipGetLastError();
+    }
+    auto* xq = static_cast<uint8_t*>(scratch);
+    a.xq = xq;
+    if (p.kind == Plan::kRows) {
+        a.x_rows = (a.M + 15) / 16 * 16;
+        const int items = a.x_rows * a.blocks;
+        auto* xs = reinterpret_cast<float*>(xq + static_cast<size_t>(items) * kBlk);
+        a.xs = xs;
+        quantize_operand_kernel<<<dim3(static_cast<unsigned>((items + 7) / 8)), 256, 0, st>>>(a.x, a.K, a.blocks, a.M, items, xq, xs);
+        if (a.M <= 16 && few) run_rows<MATS, 1, 16, false>(a, 4 * kCus, 0, st);
+        else if (a.M <= 16) run_rows<MATS, 1, 8, false>(a, 4 * kCus, 0, st);
+        else if (a.M <= 32) run_rows<MATS, 2, 8, false>(a, 4 * kCus, 0, st);
+        else if (a.M <= 48) run_rows<MATS, 3, 4, false>(a, 4 * kCus, 0, st);
+        else run_rows<MATS, 4, 4, false>(a, 4 * kCus, 0, st);
+        return hipGetLastError();
+    }
+    const size_t items = static_cast<size_t>(a.M) * a.blocks;
+    auto* xs = reinterpret_cast<float*>(xq + items * kBlk);
+    a.xs = xs;
+    a.part = reinterpret_cast<float*>(xq + up16(items * (kBlk + 4)));
+    quantize_rows_kernel<<<dim3(static_cast<unsigned>((items + 7) / 8)), 256, 0, st>>>(
+        a.x, a.K, a.blocks, items, xq, static_cast<size_t>(a.blocks) * kBlk, xs, 1, a.M);
+    if (p.kind == Plan::kTile128) run_tile<MATS, 128, 128, 2, 2>(a, p.splits, st);
+    else if (p.kind == Plan::kTile64x128) run_tile<MATS, 64, 128, 2, 2>(a, p.splits, st);
+    else run_tile<MATS, 64, 64, 2, 2>(a, p.splits, st);
+    return hipGetLastError();
 }
 
 }  // namespace
 
-size_t fp8_scratch(size_t K, size_t M) {
-    const size_t blocks = (K + kBlk - 1) / kBlk;
-    return M * blocks * (kBlk + 4);
+size_t fp8_scratch(size_t N, size_t K, size_t M, bool gated) {
+    const size_t blocks = (K + kBlk - 1) / kBlk, mats = gated ? 2 : 1;
+    const Plan p = plan_of(N, K, M, gated ? 2 : 1);
+    if (p.kind == Plan::kRowsQuantizing) return 0;
+    const size_t x = up16((p.kind == Plan::kRows ? (M + 15) / 16 * 16 : M) * blocks * (kBlk + 4));
+    return x + (p.splits > 1 ? p.splits * mats * M * ((N + 3) / 4 * 4) * 4 : 0);
 }
 
 hipError_t launch_quantize_fp8(const float* x, size_t rows, size_t cols, size_t block_rows, uint8_t* codes, float* scales,
@@ -361,27 +617,17 @@ hipError_t launch_quantize_fp8(const float* x, size_t rows, size_t cols, size_t 
 
 hipError_t launch_fp8(const uint8_t* w, const uint8_t* w2, int gate, const float* x, float* y, size_t N, size_t K, size_t M,
                       void* scratch, hipStream_t st) {
-    const size_t blocks = (K + kBlk - 1) / kBlk, items = M * blocks;
     Fp8Args a{};
-    a.N = static_cast<int>(N), a.K = static_cast<int>(K), a.M = static_cast<int>(M), a.blocks = static_cast<int>(blocks);
+    a.N = static_cast<int>(N), a.K = static_cast<int>(K), a.M = static_cast<int>(M);
+    a.blocks = static_cast<int>((K + kBlk - 1) / kBlk);
+    a.n4 = static_cast<int>((N + 3) / 4 * 4);
     a.gate = gate;
     a.w[0] = w, a.w[1] = w2;
     a.ws[0] = reinterpret_cast<const float*>(w + N * K);
     a.ws[1] = w2 ? reinterpret_cast<const float*>(w2 + N * K) : nullptr;
-    auto* xq = static_cast<uint8_t*>(scratch);
-    auto* xs = reinterpret_cast<float*>(xq + M * blocks * kBlk);
-    a.xq = xq, a.xs = xs, a.y = y;
-    quantize_rows_kernel<<<dim3(static_cast<unsigned>((items + 7) / 8)), 256, 0, st>>>(
-        x, a.K, a.blocks, items, xq, blocks * kBlk, xs, 1, M);
-    if (M > 64) {
-        if (w2) launch_tile<2>(a, st);
-        else launch_tile<1>(a, st);
-        return hipGetLastError();
-    }
-    const dim3 grid(static_cast<unsigned>((N + 15) / 16), static_cast<unsigned>((M + 15) / 16));
-    if (w2) fp8_rows_kernel<2, 1, 4><<<grid, 256, 0, st>>>(a);
-    else fp8_rows_kernel<1, 1, 4><<<grid, 256, 0, st>>>(a);
-    return hipGetLastError();
+    a.x = x, a.y = y;
+    const Plan p = plan_of(N, K, M, w2 ? 2 : 1);
+    return w2 ? run<2>(a, p, scratch, st) : run<1>(a, p, scratch, st);
 }
 
 }  // namespace mvh

@@ -207,8 +207,9 @@ hipError_t launch_quantize_fp8(const float* x, size_t rows, size_t cols, size_t 
                                hipStream_t st);
 // y [M][N] = x [M][K] w^T, or, with w2, act(x w^T) * (x w2^T) (gate: kGate*).
 // w: codes [N][K] (K % 16 == 0, 16-byte aligned), then scales
-// [ceil(N / 128)][ceil(K / 128)].  scratch: fp8_scratch(K, M) bytes, 16-byte aligned.
-size_t fp8_scratch(size_t K, size_t M);
+// [ceil(N / 128)][ceil(K / 128)].  scratch: fp8_scratch(...) bytes, 16-byte aligned.
+// M >= 1, N >= 1, 16 <= K <= 2^23, M ceil(K / 128) <= 2^26, fewer than 2^24 tiles of 64 x 64.
+size_t fp8_scratch(size_t N, size_t K, size_t M, bool gated);
 hipError_t launch_fp8(const uint8_t* w, const uint8_t* w2, int gate, const float* x, float* y, size_t N, size_t K, size_t M,
                       void* scratch, hipStream_t st);
 

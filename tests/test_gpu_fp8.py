@@ -79,7 +79,8 @@ def test_quantize_extremes(ctx):
 
 
 SHAPES = [(1, 16, 1), (1, 128, 17), (2, 144, 16), (7, 48, 129), (8, 4096, 64), (16, 272, 127), (17, 1024, 300), (33, 400, 33),
-          (64, 288, 768), (65, 128, 128), (129, 656, 257), (130, 2048, 15), (300, 144, 515), (513, 384, 640)]
+          (64, 288, 768), (65, 128, 128), (129, 656, 257), (130, 2048, 15), (300, 144, 515), (513, 384, 640),
+          (3, 2064, 50), (2, 11008, 40), (40, 5632, 130), (60, 1040, 2100), (70, 8192, 90), (200, 4112, 1030), (700, 1040, 1030)]
 
 
 @pytest.mark.parametrize("batch,k,n", SHAPES)
@@ -103,7 +104,7 @@ def test_gated_ffn(ctx, batch, k, n, act):
 
 
 @pytest.mark.parametrize("batch,k,n", [(1, 11008, 4096), (8, 2048, 32000), (20, 5632, 2048), (64, 4096, 11008),
-                                       (333, 2048, 2560)])
+                                       (333, 2048, 2560), (24, 4096, 32000), (129, 11008, 4097), (1100, 1024, 9000)])
 def test_large(ctx, batch, k, n):
     """Sizes of the models, against 64 bits on the GPU's own double products."""
     rng = np.random.default_rng(n)
