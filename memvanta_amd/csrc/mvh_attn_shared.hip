@@ -72,9 +72,10 @@ struct Shape {
     static constexpr int RW = RW_, RT = RT_, TW = TW_, T = T_, ROWS = 16 * RW_ * RT_;
     static_assert(RW_ * TW_ == 4 && T_ / TW_ % 32 == 0);
 };
+// Bytes of each of a workgroup's two tiles: a step's K or V, or, loaded directly, both; and two waves' results
 template <int NB, class S>
 constexpr size_t tile_bytes() {
-    const size_t kv = 2 * static_cast<size_t>(S::T) * NB * 64, join = S::TW > 1 ? 4 * S::RT * 16 * (32 * NB + 4) * 4 : 0;
+    const size_t kv = static_cast<size_t>(S::T) * NB * 64 * (S::TW == 1 ? 2 : 1), join = S::TW > 1 ? 2 * S::RT * 16 * (32 * NB + 4) * 4 : 0;
     return kv > join ? kv : join;
 }
 
@@ -91,15 +92,17 @@ __device__ __forceinline__ bool unbounded(_Float16 h) {  // an infinity or NaN
     return (__builtin_bit_cast(uint16_t, h) & 0x7c00u) == 0x7c00u;
 }
 
-template <int KT, int NB, class S>
-__device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8_t* tile, uint64_t* s_pk, uint64_t* s_pv, float* s_sc,
-                                       float (*s_ml)[2 * S::RT][16]) {
+// The part of a workgroup.  A step's T rows go to LDS as fp16: of F16 pages in shapes
+// whose waves share them (TW = 1) straight from memory, into one tile while the other
+// is in use; else through registers, loaded a step ahead, K to one tile and V to the
+// other.  CAUSAL: rows may be seen by some of the tokens only.
+template <int KT, int NB, class S, bool CAUSAL>
+__device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8_t* tile0, uint8_t* tile1, uint64_t* s_pk, uint64_t* s_pv,
+                                       float* s_sc, float (*s_ml)[2 * S::RT][16]) {
     constexpr int RW = S::RW, RT = S::RT, TW = S::TW, T = S::T, CPR = 4 * NB, HDP = 32 * NB, ITEMS = T * CPR / 256, ND = 2 * NB;
-    constexpr bool Q8 = KT == kKvQ8;
+    constexpr bool Q8 = KT == kKvQ8, DIRECT = !Q8 && TW == 1;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, j = lane >> 4;
     const int rw = wave % RW, tw = wave / RW, hd = a.hd;
-    uint8_t* const s_k = tile;
-    uint8_t* const s_v = tile + T * HDP * 2;
 
     // page addresses of the part
     const int page0 = page_of(p.t0, p.magic), pages = page_of(p.t1 - 1, p.magic) - page0 + 1;
@@ -107,17 +110,22 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
         s_pk[i] = reinterpret_cast<uint64_t>(p.pt_k[page0 + i]);
         s_pv[i] = reinterpret_cast<uint64_t>(p.pt_v[page0 + i]);
     }
+    if (DIRECT && hd < HDP)  // channels behind the head: no load writes them
+        for (int i = tid; i < 2 * T * CPR; i += 256) {
+            *reinterpret_cast<uint4*>(tile0 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+            *reinterpret_cast<uint4*>(tile1 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+        }
     __syncthreads();
 
     const size_t sc_off = kv_scale_offset(p.page, a.kv_dim);
-    typename std::conditional<Q8, uint2, uint4>::type kr[ITEMS], vr[ITEMS];
+    typename std::conditional<Q8, uint2, uint4>::type kr[DIRECT ? 1 : ITEMS], vr[DIRECT ? 1 : ITEMS];
     float scale = 0.0f;
     auto row_at = [&](const uint64_t* s_p, int t, int& slot) {  // rows behind the part: its first one again, masked
         const int tc = t < p.t1 ? t : p.t0, pg = page_of(tc, p.magic);
         slot = tc - pg * p.page;
         return reinterpret_cast<const uint8_t*>(s_p[pg - page0]);
     };
-    auto load = [&](int base) {
+    auto load = [&](int base, uint8_t* tile) {
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
             const int at = i * 256 + tid, row = at / CPR, kc = (at % CPR) ^ k_turn<CPR>(row), vc = (at % CPR) ^ v_turn<CPR>(row);
@@ -125,7 +133,13 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
             const uint8_t* pk = row_at(s_pk, base + row, slot);
             const uint8_t* pv = row_at(s_pv, base + row, slot);
             const size_t off = static_cast<size_t>(slot) * a.kv_dim + p.kh * hd;
-            if constexpr (Q8) {
+            if constexpr (DIRECT) {
+                typedef const __attribute__((address_space(1))) void from_t;
+                typedef __attribute__((address_space(3))) void to_t;
+                uint8_t* const to = tile + (i * 256 + wave * 64) * 16;
+                if (kc * 8 < hd) __builtin_amdgcn_global_load_lds((from_t*)(pk + 2 * (off + kc * 8)), (to_t*)to, 16, 0, 0);
+                if (vc * 8 < hd) __builtin_amdgcn_global_load_lds((from_t*)(pv + 2 * (off + vc * 8)), (to_t*)(to + T * HDP * 2), 16, 0, 0);
+            } else if constexpr (Q8) {
                 kr[i] = vr[i] = make_uint2(0u, 0u);
                 if (kc * 8 < hd) kr[i] = ld_global8(pk + off + kc * 8);
                 if (vc * 8 < hd) vr[i] = ld_global8(pv + off + vc * 8);
@@ -146,61 +160,78 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
         for (int i = 0; i < ITEMS; ++i) {
             const int at = (i * 256 + tid) * 16;
             if constexpr (Q8) {
-                *reinterpret_cast<uint4*>(s_k + at) = half_of_int8(kr[i]);
-                *reinterpret_cast<uint4*>(s_v + at) = half_of_int8(vr[i]);
+                *reinterpret_cast<uint4*>(tile0 + at) = half_of_int8(kr[i]);
+                *reinterpret_cast<uint4*>(tile1 + at) = half_of_int8(vr[i]);
             } else {
-                *reinterpret_cast<uint4*>(s_k + at) = kr[i];
-                *reinterpret_cast<uint4*>(s_v + at) = vr[i];
+                *reinterpret_cast<uint4*>(tile0 + at) = kr[i];
+                *reinterpret_cast<uint4*>(tile1 + at) = vr[i];
             }
         }
         if (Q8 && tid < 2 * T) s_sc[tid] = scale;
     };
-    load(p.t0);
+    load(p.t0, tile0);
 
-    // q of the wave's rows: lane (n, j) holds channels 8 j .. of each block of 32
+    // q of the wave's rows times log2(e) / sqrt(hd): lane (n, j) holds channels 8 j .. of each block of 32, in two parts
+    // of q 2^-e; scores s stand for y = s 2^e, exactly
     half8 qh[RT][NB], ql[RT][NB];
-    float y_scale[RT];
+    float y_scale[RT], slack[RT];
     int lim[RT];
+    float minus1 = -1.0f;  // a constant that the compiler is not to see: the subtraction takes a conversion in
+    asm("" : "+v"(minus1));
+    auto part2 = [&](float x, float y, half2v& h, half2v& l) {
+        h = pk_half(x, y);
+        l = pk_half(fmaf(static_cast<float>(h.x), minus1, x), fmaf(static_cast<float>(h.y), minus1, y));
+    };
+    const float factor = __fdiv_rn(kLog2e, sqrt_rn(static_cast<float>(hd)));
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         const int r = p.r0 + min((rw * RT + rt) * 16 + n, p.n - 1);
-        lim[rt] = p.lim0 + (r - p.lim_row) / a.group;
+        lim[rt] = CAUSAL ? p.lim0 + (r - p.lim_row) / a.group : 0;
         const float* qr = a.q + (static_cast<size_t>(r / a.group) * a.n_head + p.kh * a.group + r % a.group) * hd;
         float f[NB][8], top = 0.0f;
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+        for (int b = 0; b < NB; ++b) {
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+            if (32 * b + 8 * j < hd) {
+                x = *reinterpret_cast<const float4*>(qr + 32 * b + 8 * j);
+                y = *reinterpret_cast<const float4*>(qr + 32 * b + 8 * j + 4);
+            }
+            const float all[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                f[b][i] = 32 * b + 8 * j < hd ? qr[32 * b + 8 * j + i] : 0.0f;
-                top = fmaxf(top, fabsf(f[b][i]));
+                f[b][i] = all[i];
+                top = fmaxf(top, fabsf(all[i]));
             }
+        }
         const int e = query_exponent(rows_max(top));
         const float down = ldexpf(1.0f, -e);
-        y_scale[rt] = ldexpf(__fdiv_rn(kLog2e, sqrt_rn(static_cast<float>(hd))), e);
+        y_scale[rt] = ldexpf(1.0f, e);
+        slack[rt] = kSlack * down;
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float x = f[b][i] * down;
-                qh[rt][b][i] = static_cast<_Float16>(x);
-                ql[rt][b][i] = static_cast<_Float16>(x - static_cast<float>(qh[rt][b][i]));
+            for (int i = 0; i < 8; i += 2) {
+                half2v h, l;
+                part2(f[b][i] * down * factor, f[b][i + 1] * down * factor, h, l);
+                qh[rt][b][i] = h.x, qh[rt][b][i + 1] = h.y;
+                ql[rt][b][i] = l.x, ql[rt][b][i + 1] = l.y;
             }
     }
-    const int first_lim = p.lim0 + (p.r0 - p.lim_row) / a.group, seen_by_all = min(p.t1, first_lim + 1);
+    const int seen_by_all = CAUSAL ? min(p.t1, p.lim0 + (p.r0 - p.lim_row) / a.group + 1) : p.t1;
 
     f32x4 o[RT][ND];
-    float m[RT], l[RT];
-    int unit[RT];  // Q8: sums are held times 2^-unit, the exponent of the largest scale seen
+    float m[RT], base_y[RT], l[RT];  // the largest s (within kSlack), what is taken off y, the sum of weights
+    int unit[RT];                    // Q8: sums are held times 2^-unit, the exponent of the largest scale seen
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         m[rt] = -__builtin_inff();
-        l[rt] = 0.0f;
+        base_y[rt] = l[rt] = 0.0f;
         unit[rt] = -126;
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[rt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
-    auto block = [&](int tg, int tb) {  // rows tg .. tg + 31, at tb of the tile
+    auto block = [&](const uint8_t* s_k, const uint8_t* s_v, int tg, int tb) {  // rows tg .. tg + 31, at tb of the tile
         const bool edge = tg + 32 > seen_by_all;
         f32x4 s[RT][2];
 #pragma unroll
@@ -212,10 +243,9 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
                 const int row = tb + 16 * h + n;
                 const half8 k = *reinterpret_cast<const half8*>(s_k + (row * CPR + ((4 * b + j) ^ k_turn<CPR>(row))) * 16);
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    s[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[rt][b], s[rt][h], 0, 0, 0);
-                    s[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[rt][b], s[rt][h], 0, 0, 0);
-                }
+                for (int rt = 0; rt < RT; ++rt) s[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[rt][b], s[rt][h], 0, 0, 0);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) s[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[rt][b], s[rt][h], 0, 0, 0);
             }
         f32x4 ks[2], vs[2];
         if constexpr (Q8)
@@ -227,27 +257,35 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
         half8 ph[RT], pl[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            bool seen[2][4];
-            float y[2][4], top = -__builtin_inff();
+            auto seen = [&](int h, int i) {
+                const int t = tg + 16 * h + 4 * j + i;
+                return t < p.t1 && (!CAUSAL || t <= lim[rt]);
+            };
+            float top = -__builtin_inff();
             int widest = -126;
+            if constexpr (Q8)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[rt][h][i] *= ks[h][i];
+            if (edge) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[rt][h][i] = seen(h, i) ? s[rt][h][i] : -__builtin_inff();
+            }
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int t = tg + 16 * h + 4 * j + i;
-                    seen[h][i] = !edge || (t < p.t1 && t <= lim[rt]);
-                    float v = s[rt][h][i];
-                    if constexpr (Q8) v *= ks[h][i];
-                    v *= y_scale[rt];
-                    y[h][i] = seen[h][i] ? v : -__builtin_inff();
-                    top = fmaxf(top, y[h][i]);
+                    top = fmaxf(top, s[rt][h][i]);
                     if constexpr (Q8) {
                         const int e = static_cast<int>((__float_as_uint(vs[h][i]) >> 23) & 255u) - 127;
-                        if (seen[h][i] && e < 128) widest = max(widest, e);
+                        if (e < 128 && (!edge || seen(h, i))) widest = max(widest, e);
                     }
                 }
             top = rows_max(top);
-            const bool ahead = top > m[rt] + kSlack;
+            const bool ahead = top > m[rt] + slack[rt];
             if constexpr (Q8) {
                 auto x = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(widest + 126), static_cast<uint32_t>(widest + 126), false, false);
                 uint32_t w = max(x[0], x[1]);
@@ -258,8 +296,10 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
             if (__any(ahead || wider)) {
                 float down = 1.0f;
                 if (ahead) {
-                    down = m[rt] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m[rt] - top);
+                    const float next = fmaf(top, y_scale[rt], -kLift);
+                    down = m[rt] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(base_y[rt] - next);
                     m[rt] = top;
+                    base_y[rt] = next;
                 }
                 l[rt] *= down;
                 if (wider) {
@@ -271,17 +311,23 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
 #pragma unroll
                     for (int i = 0; i < 4; ++i) o[rt][d][i] *= down;
             }
-            const float from = (m[rt] == -__builtin_inff() ? 0.0f : m[rt]);
+            float w[8], more = 0.0f;
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int i = 0; i < 8; ++i) {
+                w[i] = __builtin_amdgcn_exp2f(fmaf(s[rt][i >> 2][i & 3], y_scale[rt], -base_y[rt]));
+                more += w[i];
+            }
+            l[rt] += more;
+            if constexpr (Q8)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float w = __builtin_amdgcn_exp2f((y[h][i] - from) + kLift);
-                    l[rt] += w;
-                    if constexpr (Q8) w = seen[h][i] ? w * ldexpf(vs[h][i], -unit[rt]) : 0.0f;
-                    ph[rt][4 * h + i] = static_cast<_Float16>(w);
-                    pl[rt][4 * h + i] = static_cast<_Float16>(w - static_cast<float>(ph[rt][4 * h + i]));
-                }
+                for (int i = 0; i < 8; ++i) w[i] = !edge || seen(i >> 2, i & 3) ? w[i] * ldexpf(vs[i >> 2][i & 3], -unit[rt]) : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                half2v h, l2;
+                part2(w[i], w[i + 1], h, l2);
+                ph[rt][i] = h.x, ph[rt][i + 1] = h.y;
+                pl[rt][i] = l2.x, pl[rt][i + 1] = l2.y;
+            }
         }
         bool odd = false;
 #pragma unroll
@@ -296,7 +342,7 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
                 typedef __attribute__((address_space(3))) s16x4 lds_t;
                 v.w[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(s_v + (row * CPR + chunk) * 16 + (n & 1) * 8));
             }
-            if (!Q8 && edge) {
+            if (CAUSAL && !Q8 && edge) {
                 // a row that some do not see: what is no number there must not meet their weight of 0
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
@@ -306,12 +352,12 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
                     }
             }
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v.h, pl[rt], o[rt][d], 0, 0, 0);
-                o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v.h, ph[rt], o[rt][d], 0, 0, 0);
-            }
+            for (int rt = 0; rt < RT; ++rt) o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v.h, pl[rt], o[rt][d], 0, 0, 0);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v.h, ph[rt], o[rt][d], 0, 0, 0);
         }
-        if (!Q8 && __any(odd)) {  // the products left out, for the rows that see them
+        if (CAUSAL && !Q8 && __any(odd)) {  // the products left out, for the rows that see them
+#pragma unroll 1
             for (int t = 0; t < 32; ++t) {
                 const int row = tb + t, from_lane = n + 16 * ((t >> 2) & 3), at = 4 * (t >> 4) + (t & 3);
 #pragma unroll
@@ -336,15 +382,29 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
         }
     };
 
-    for (int base = p.t0; base < p.t1; base += T) {
-        __syncthreads();
-        store();
-        __syncthreads();
-        if (base + T < p.t1) load(base + T);
+    if constexpr (DIRECT) {
+        auto step = [&](int base, const uint8_t* tile, uint8_t* other) {
+            __syncthreads();  // this tile's rows are there, and nobody reads the other any more
+            if (base + T < p.t1) load(base + T, other);
 #pragma unroll 1
-        for (int u = 0; u < T / TW / 32; ++u) {
-            const int tb = tw * (T / TW) + 32 * u;
-            if (base + tb < p.t1) block(base + tb, tb);
+            for (int u = 0; u < T / 32; ++u)
+                if (base + 32 * u < p.t1) block(tile, tile + T * HDP * 2, base + 32 * u, 32 * u);
+        };
+        for (int base = p.t0; base < p.t1; base += 2 * T) {
+            step(base, tile0, tile1);
+            if (base + T < p.t1) step(base + T, tile1, tile0);
+        }
+    } else {
+        for (int base = p.t0; base < p.t1; base += T) {
+            __syncthreads();
+            store();
+            __syncthreads();
+            if (base + T < p.t1) load(base + T, tile0);
+#pragma unroll 1
+            for (int u = 0; u < T / TW / 32; ++u) {
+                const int tb = tw * (T / TW) + 32 * u;
+                if (base + tb < p.t1) block(tile0, tile1, base + tb, tb);
+            }
         }
     }
 
@@ -369,6 +429,7 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         l[rt] = rows_sum(l[rt]);
+        if (m[rt] == -__builtin_inff()) base_y[rt] = m[rt];  // nothing seen
         if constexpr (Q8)
 #pragma unroll
             for (int d = 0; d < ND; ++d)
@@ -382,18 +443,19 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
             if (row >= p.n) continue;
 #pragma unroll
             for (int d = 0; d < ND; ++d)
-                if (16 * d + 4 * j < hd) put(row, 16 * d + 4 * j, o[rt][d], m[rt], l[rt]);
+                if (16 * d + 4 * j < hd) put(row, 16 * d + 4 * j, o[rt][d], base_y[rt], l[rt]);
         }
     } else {
-        float* s_o = reinterpret_cast<float*>(tile);  // [wave][rt][16][HDP + 4]
+        auto sums = [&](int w, int rt, int row) {  // [rt][16][HDP + 4] of wave w, two waves a tile
+            return reinterpret_cast<float*>(w < 2 ? tile0 : tile1) + (((w & 1) * RT + rt) * 16 + row) * (HDP + 4);
+        };
         __syncthreads();
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
-            for (int d = 0; d < ND; ++d)
-                *reinterpret_cast<f32x4*>(s_o + ((wave * RT + rt) * 16 + n) * (HDP + 4) + 16 * d + 4 * j) = o[rt][d];
+            for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4*>(sums(wave, rt, n) + 16 * d + 4 * j) = o[rt][d];
             if (j == 0) {
-                s_ml[wave][rt][n] = m[rt];
+                s_ml[wave][rt][n] = base_y[rt];
                 s_ml[wave][RT + rt][n] = l[rt];
             }
         }
@@ -411,7 +473,7 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
                 const int w = w0 + k * RW;
                 const float mine = s_ml[w][rt][c], f = mine == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mine - top);
                 if (s_ml[w][RT + rt][c] == 0.0f) continue;
-                const f32x4 x = *reinterpret_cast<const f32x4*>(s_o + ((w * RT + rt) * 16 + c) * (HDP + 4) + d);
+                const f32x4 x = *reinterpret_cast<const f32x4*>(sums(w, rt, c) + d);
                 sum = fmaf(f, s_ml[w][RT + rt][c], sum);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) v[i] = fmaf(f, x[i], v[i]);
@@ -424,9 +486,9 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
 // A workgroup: a part of the prefix for a tile of all query rows, or, behind those,
 // a part of one sequence's own rows.
 template <int KT, int NB, class P, class S>
-__global__ __launch_bounds__(256, 2) void attn_shared_kernel(SharedArgs a) {
+__global__ __launch_bounds__(256, NB > 4 ? 1 : 2) void attn_shared_kernel(SharedArgs a) {
     constexpr size_t kP = tile_bytes<NB, P>(), kS = tile_bytes<NB, S>();
-    __shared__ __align__(16) uint8_t tile[kP > kS ? kP : kS];
+    __shared__ __align__(16) uint8_t tile0[kP > kS ? kP : kS], tile1[kP > kS ? kP : kS];
     __shared__ uint64_t s_pk[kPages], s_pv[kPages];
     __shared__ __align__(16) float s_sc[2 * (P::T > S::T ? P::T : S::T)];
     __shared__ float s_ml[4 * 2 * (P::RT > S::RT ? P::RT : S::RT) * 16];
@@ -443,8 +505,8 @@ __global__ __launch_bounds__(256, 2) void attn_shared_kernel(SharedArgs a) {
         p.t1 = min(p.t0 + a.p_chunk, a.prefix_len);
         p.r0 = tile_at * P::ROWS;
         p.n = min(P::ROWS, a.n_tokens * a.group - p.r0);
-        p.lim0 = 0x3fffffff, p.lim_row = p.r0;  // all rows see all
-        attend<KT, NB, P>(a, p, tile, s_pk, s_pv, s_sc, reinterpret_cast<float(*)[2 * P::RT][16]>(s_ml));
+        p.lim0 = p.lim_row = 0;
+        attend<KT, NB, P, false>(a, p, tile0, tile1, s_pk, s_pv, s_sc, reinterpret_cast<float(*)[2 * P::RT][16]>(s_ml));
         return;
     }
     int at = item - a.p_items;
@@ -471,29 +533,84 @@ __global__ __launch_bounds__(256, 2) void attn_shared_kernel(SharedArgs a) {
         }
         return;
     }
-    attend<KT, NB, S>(a, p, tile, s_pk, s_pv, s_sc, reinterpret_cast<float(*)[2 * S::RT][16]>(s_ml));
+    attend<KT, NB, S, true>(a, p, tile0, tile1, s_pk, s_pv, s_sc, reinterpret_cast<float(*)[2 * S::RT][16]>(s_ml));
 }
 
-// out row = sum over its parts, four channels a thread
-__global__ __launch_bounds__(256) void attn_shared_join(const float* __restrict__ part, float* __restrict__ out, size_t rows,
-                                                        int slots, int hd) {
-    const int per = hd / 4, in = threadIdx.x / per, d = threadIdx.x % per * 4;
-    const size_t row = static_cast<size_t>(blockIdx.x) * (256 / per) + in;
-    if (in >= 256 / per || row >= rows) return;
-    const float* ml = part + rows * slots * hd + 2 * row * slots;
-    float top = -__builtin_inff();
-    for (int k = 0; k < slots; ++k) top = fmaxf(top, ml[2 * k]);
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    float sum = 0.0f;
-    for (int k = 0; k < slots; ++k) {
-        if (ml[2 * k + 1] == 0.0f) continue;  // no row seen
-        const float f = ml[2 * k] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ml[2 * k] - top);
-        const f32x4 x = *reinterpret_cast<const f32x4*>(part + (row * slots + k) * hd + d);
-        sum = fmaf(f, ml[2 * k + 1], sum);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = fmaf(f, x[i], v[i]);
+// out row = sum over its parts.  `per` = hd / 4 threads hold a row's channels, four
+// each; `ways` such groups share the parts of a row, and 256 / per / ways rows a
+// workgroup.  A part without a seen row (l = 0) has no sums.
+constexpr int kSlots = 256;
+__global__ __launch_bounds__(256) void attn_shared_join(const float* __restrict__ part, float* __restrict__ out, int rows,
+                                                        int slots, int hd, int per, int ways) {
+    __shared__ float s_f[kSlots * 8];   // [row of the workgroup][slot]: the part's weight
+    __shared__ float s_sum[256];        // of a row
+    __shared__ f32x4 s_v[256];
+    const int many = 256 / per / ways, group = threadIdx.x / per, d = threadIdx.x % per * 4, in = group / ways, way = group % ways;
+    const int row0 = blockIdx.x * many;
+    const float* ml = part + static_cast<size_t>(rows) * slots * hd;
+    // 256 / many threads a row find its maximum and turn m and l into weights
+    {
+        const int lanes = 256 / many, r = threadIdx.x / lanes, lane = threadIdx.x % lanes;
+        const float* mine = ml + static_cast<size_t>(min(row0 + r, rows - 1)) * 2 * slots;
+        const bool on = r < many && row0 + r < rows;
+        float top = -__builtin_inff();
+        if (on)
+            for (int k = lane; k < slots; k += lanes) {
+                const float m = mine[2 * k];
+                s_f[r * slots + k] = m;
+                top = fmaxf(top, m);
+            }
+        if (r < many) s_sum[threadIdx.x] = top;
+        __syncthreads();
+        if (on)
+            for (int k = 0; k < lanes; ++k) top = fmaxf(top, s_sum[r * lanes + k]);
+        __syncthreads();
+        float sum = 0.0f;
+        if (on)
+            for (int k = lane; k < slots; k += lanes) {
+                const float m = s_f[r * slots + k], l = mine[2 * k + 1];
+                const float f = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+                s_f[r * slots + k] = l == 0.0f ? -1.0f : f;
+                if (l != 0.0f) sum = fmaf(f, l, sum);
+            }
+        if (r < many) s_sum[threadIdx.x] = sum;
+        __syncthreads();
+        sum = 0.0f;
+        if (on)
+            for (int k = 0; k < lanes; ++k) sum += s_sum[r * lanes + k];
+        __syncthreads();
+        if (on && lane == 0) s_sum[r] = sum;
+        __syncthreads();
     }
-    *reinterpret_cast<f32x4*>(out + row * hd + d) =
+    const int row = row0 + in;
+    const bool on = in < many && row < rows;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (on) {
+        const float* x = part + static_cast<size_t>(row) * slots * hd + d;
+        for (int k = way; k < slots; k += 4 * ways) {
+            f32x4 a[4];
+            float f[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int at = k + u * ways;
+                f[u] = at < slots ? s_f[in * slots + at] : -1.0f;
+                a[u] = f[u] >= 0.0f || f[u] != f[u] ? *reinterpret_cast<const f32x4*>(x + static_cast<size_t>(at) * hd) : f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = fmaf(f[u] == -1.0f ? 0.0f : f[u], a[u][i], v[i]);
+        }
+    }
+    if (ways > 1) {
+        s_v[threadIdx.x] = v;
+        __syncthreads();
+        if (!on || way) return;
+        for (int w = 1; w < ways; ++w) v += s_v[threadIdx.x + w * per];
+    }
+    if (!on) return;
+    const float sum = s_sum[in];
+    *reinterpret_cast<f32x4*>(out + static_cast<size_t>(row) * hd + d) =
         f32x4{__fdiv_rn(v[0], sum), __fdiv_rn(v[1], sum), __fdiv_rn(v[2], sum), __fdiv_rn(v[3], sum)};
 }
 
@@ -618,8 +735,13 @@ hipError_t launch_attn_shared(const SharedCall& call, void* scratch, hipStream_t
                                                 : run_type<kKvF16>(nb, k, a, static_cast<unsigned>(grid), st);
         if (e != hipSuccess) return e;
         if (a.part) {
-            const size_t rows = tokens * c.n_head, per = 256 / (c.head_dim / 4);
-            attn_shared_join<<<dim3(static_cast<unsigned>((rows + per - 1) / per)), 256, 0, st>>>(a.part, c.out, rows, a.slots, a.hd);
+            // the groups share a row's parts while each has two or more, or there are few rows; at most 8 rows (kSlots)
+            const int rows = static_cast<int>(tokens * c.n_head), per = a.hd / 4, groups = 256 / per;
+            int ways = 1;
+            while (2 * ways <= groups && (2 * ways * 2 <= a.slots || groups / ways > 8)) ways *= 2;
+            const int many = groups / ways;
+            attn_shared_join<<<dim3(static_cast<unsigned>((rows + many - 1) / many)), 256, 0, st>>>(a.part, c.out, rows, a.slots, a.hd,
+                                                                                                    per, ways);
             if (const hipError_t j = hipGetLastError(); j != hipSuccess) return j;
         }
     }
