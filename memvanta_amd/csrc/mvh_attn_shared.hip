@@ -24,7 +24,7 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // ahead: at most 2^14, and in two fp16 they keep 22 bits down to 2^-12 of the
 // largest, 2^-35 of it below.
 constexpr float kLift = 10.0f, kSlack = 4.0f;
-constexpr int kPages = 514;    // page addresses that a part holds: of up to 512 whole pages
+constexpr int kAhead = 256;    // rows whose addresses are formed at a time, one a thread
 constexpr int kBatch = 128;    // sequences of a launch: their places are kernel arguments
 
 struct SharedSeq {
@@ -97,19 +97,40 @@ __device__ __forceinline__ bool unbounded(_Float16 h) {  // an infinity or NaN
 // is in use; else through registers, loaded a step ahead, K to one tile and V to the
 // other.  CAUSAL: rows may be seen by some of the tokens only.
 template <int KT, int NB, class S, bool CAUSAL>
-__device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8_t* tile0, uint8_t* tile1, uint64_t* s_pk, uint64_t* s_pv,
-                                       float* s_sc, float (*s_ml)[2 * S::RT][16]) {
+__device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8_t* tile0, uint8_t* tile1, ulonglong2* s_row, float* s_sc,
+                                        float (*s_ml)[2 * S::RT][16]) {
     constexpr int RW = S::RW, RT = S::RT, TW = S::TW, T = S::T, CPR = 4 * NB, HDP = 32 * NB, ITEMS = T * CPR / 256, ND = 2 * NB;
     constexpr bool Q8 = KT == kKvQ8, DIRECT = !Q8 && TW == 1;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, j = lane >> 4;
     const int rw = wave % RW, tw = wave / RW, hd = a.hd;
 
-    // page addresses of the part
-    const int page0 = page_of(p.t0, p.magic), pages = page_of(p.t1 - 1, p.magic) - page0 + 1;
-    for (int i = tid; i < pages; i += 256) {
-        s_pk[i] = reinterpret_cast<uint64_t>(p.pt_k[page0 + i]);
-        s_pv[i] = reinterpret_cast<uint64_t>(p.pt_v[page0 + i]);
-    }
+    // Addresses of the part's rows, 256 ahead of those in use: s_row[row % 512], and for Q8 pages their scales in s_sc.
+    // Rows behind the part are its first one again, masked.
+    const uint8_t *next_k = nullptr, *next_v = nullptr;  // the pages of this thread's next row
+    int next_slot = 0;
+    auto pages_of = [&](int first) {
+        const int t = p.t0 + first + tid, tc = t < p.t1 ? t : p.t0, pg = page_of(tc, p.magic);
+        next_k = static_cast<const uint8_t*>(p.pt_k[pg]);
+        next_v = static_cast<const uint8_t*>(p.pt_v[pg]);
+        next_slot = tc - pg * p.page;
+    };
+    constexpr int EB = Q8 ? 1 : 2;  // bytes of an element
+    auto rows_of_pages = [&](int first) {
+        const size_t off = EB * (static_cast<size_t>(next_slot) * a.kv_dim + p.kh * hd);
+        s_row[(first + tid) & (2 * kAhead - 1)] = make_ulonglong2(reinterpret_cast<uint64_t>(next_k) + off, reinterpret_cast<uint64_t>(next_v) + off);
+    };
+    const size_t sc_off = kv_scale_offset(p.page, a.kv_dim);
+    auto scales_of_pages = [&](int first) {
+        if constexpr (Q8) {
+            typedef const __attribute__((address_space(1))) float* from_t;
+            const size_t off = sc_off + 4 * static_cast<size_t>(next_slot);
+            s_sc[(first + tid) & (2 * kAhead - 1)] = *(from_t)(reinterpret_cast<uintptr_t>(next_k) + off);
+            s_sc[2 * kAhead + ((first + tid) & (2 * kAhead - 1))] = *(from_t)(reinterpret_cast<uintptr_t>(next_v) + off);
+        }
+    };
+    pages_of(0);
+    rows_of_pages(0);
+    scales_of_pages(0);
     if (DIRECT && hd < HDP)  // channels behind the head: no load writes them
         for (int i = tid; i < 2 * T * CPR; i += 256) {
             *reinterpret_cast<uint4*>(tile0 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
@@ -117,42 +138,29 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
         }
     __syncthreads();
 
-    const size_t sc_off = kv_scale_offset(p.page, a.kv_dim);
     typename std::conditional<Q8, uint2, uint4>::type kr[DIRECT ? 1 : ITEMS], vr[DIRECT ? 1 : ITEMS];
-    float scale = 0.0f;
-    auto row_at = [&](const uint64_t* s_p, int t, int& slot) {  // rows behind the part: its first one again, masked
-        const int tc = t < p.t1 ? t : p.t0, pg = page_of(tc, p.magic);
-        slot = tc - pg * p.page;
-        return reinterpret_cast<const uint8_t*>(s_p[pg - page0]);
-    };
-    auto load = [&](int base, uint8_t* tile) {
+    auto load = [&](int rel, uint8_t* tile) {  // rows t0 + rel ..
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
             const int at = i * 256 + tid, row = at / CPR, kc = (at % CPR) ^ k_turn<CPR>(row), vc = (at % CPR) ^ v_turn<CPR>(row);
-            int slot;
-            const uint8_t* pk = row_at(s_pk, base + row, slot);
-            const uint8_t* pv = row_at(s_pv, base + row, slot);
-            const size_t off = static_cast<size_t>(slot) * a.kv_dim + p.kh * hd;
+            const ulonglong2 from = s_row[(rel + row) & (2 * kAhead - 1)];
+            const auto* pk = reinterpret_cast<const uint8_t*>(from.x + EB * 8 * kc);
+            const auto* pv = reinterpret_cast<const uint8_t*>(from.y + EB * 8 * vc);
             if constexpr (DIRECT) {
                 typedef const __attribute__((address_space(1))) void from_t;
                 typedef __attribute__((address_space(3))) void to_t;
                 uint8_t* const to = tile + (i * 256 + wave * 64) * 16;
-                if (kc * 8 < hd) __builtin_amdgcn_global_load_lds((from_t*)(pk + 2 * (off + kc * 8)), (to_t*)to, 16, 0, 0);
-                if (vc * 8 < hd) __builtin_amdgcn_global_load_lds((from_t*)(pv + 2 * (off + vc * 8)), (to_t*)(to + T * HDP * 2), 16, 0, 0);
+                if (kc * 8 < hd) __builtin_amdgcn_global_load_lds((from_t*)pk, (to_t*)to, 16, 0, 0);
+                if (vc * 8 < hd) __builtin_amdgcn_global_load_lds((from_t*)pv, (to_t*)(to + T * HDP * 2), 16, 0, 0);
             } else if constexpr (Q8) {
                 kr[i] = vr[i] = make_uint2(0u, 0u);
-                if (kc * 8 < hd) kr[i] = ld_global8(pk + off + kc * 8);
-                if (vc * 8 < hd) vr[i] = ld_global8(pv + off + vc * 8);
+                if (kc * 8 < hd) kr[i] = ld_global8(pk);
+                if (vc * 8 < hd) vr[i] = ld_global8(pv);
             } else {
                 kr[i] = vr[i] = make_uint4(0u, 0u, 0u, 0u);
-                if (kc * 8 < hd) kr[i] = ld_global16(pk + 2 * (off + kc * 8));
-                if (vc * 8 < hd) vr[i] = ld_global16(pv + 2 * (off + vc * 8));
+                if (kc * 8 < hd) kr[i] = ld_global16(pk);
+                if (vc * 8 < hd) vr[i] = ld_global16(pv);
             }
-        }
-        if (Q8 && tid < 2 * T) {
-            int slot;
-            const uint8_t* page = row_at(tid < T ? s_pk : s_pv, base + (tid & (T - 1)), slot);
-            scale = *(const __attribute__((address_space(1))) float*)(reinterpret_cast<uintptr_t>(page + sc_off + 4 * static_cast<size_t>(slot)));
         }
     };
     auto store = [&] {
@@ -167,9 +175,8 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
                 *reinterpret_cast<uint4*>(tile1 + at) = vr[i];
             }
         }
-        if (Q8 && tid < 2 * T) s_sc[tid] = scale;
     };
-    load(p.t0, tile0);
+    load(0, tile0);
 
     // q of the wave's rows times log2(e) / sqrt(hd): lane (n, j) holds channels 8 j .. of each block of 32, in two parts
     // of q 2^-e; scores s stand for y = s 2^e, exactly
@@ -251,8 +258,9 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
         if constexpr (Q8)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                ks[h] = *reinterpret_cast<const f32x4*>(s_sc + tb + 16 * h + 4 * j);
-                vs[h] = *reinterpret_cast<const f32x4*>(s_sc + T + tb + 16 * h + 4 * j);
+                const int at = (tg - p.t0 + 16 * h + 4 * j) & (2 * kAhead - 1);
+                ks[h] = *reinterpret_cast<const f32x4*>(s_sc + at);
+                vs[h] = *reinterpret_cast<const f32x4*>(s_sc + 2 * kAhead + at);
             }
         half8 ph[RT], pl[RT];
 #pragma unroll
@@ -382,29 +390,44 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
         }
     };
 
+    const int count = p.t1 - p.t0;
+    // the next 256 rows: their pages in a turn of 256 rows' first step, addresses at its end, scales in the second step
+    auto look_ahead = [&](int rel) {
+        if (rel % kAhead == 0 && rel + kAhead < count) pages_of(rel + kAhead);
+    };
+    auto note_ahead = [&](int rel) {
+        const int first = rel - rel % kAhead + kAhead;
+        if (first >= count) return;
+        if (rel % kAhead == 0) rows_of_pages(first);
+        if (rel % kAhead == T) scales_of_pages(first);
+    };
     if constexpr (DIRECT) {
-        auto step = [&](int base, const uint8_t* tile, uint8_t* other) {
+        auto step = [&](int rel, const uint8_t* tile, uint8_t* other) {
             __syncthreads();  // this tile's rows are there, and nobody reads the other any more
-            if (base + T < p.t1) load(base + T, other);
+            if (rel + T < count) load(rel + T, other);
+            look_ahead(rel);
 #pragma unroll 1
             for (int u = 0; u < T / 32; ++u)
-                if (base + 32 * u < p.t1) block(tile, tile + T * HDP * 2, base + 32 * u, 32 * u);
+                if (rel + 32 * u < count) block(tile, tile + T * HDP * 2, p.t0 + rel + 32 * u, 32 * u);
+            note_ahead(rel);
         };
-        for (int base = p.t0; base < p.t1; base += 2 * T) {
-            step(base, tile0, tile1);
-            if (base + T < p.t1) step(base + T, tile1, tile0);
+        for (int rel = 0; rel < count; rel += 2 * T) {
+            step(rel, tile0, tile1);
+            if (rel + T < count) step(rel + T, tile1, tile0);
         }
     } else {
-        for (int base = p.t0; base < p.t1; base += T) {
+        for (int rel = 0; rel < count; rel += T) {
             __syncthreads();
             store();
             __syncthreads();
-            if (base + T < p.t1) load(base + T, tile0);
+            if (rel + T < count) load(rel + T, tile0);
+            look_ahead(rel);
 #pragma unroll 1
             for (int u = 0; u < T / TW / 32; ++u) {
                 const int tb = tw * (T / TW) + 32 * u;
-                if (base + tb < p.t1) block(tile0, tile1, base + tb, tb);
+                if (rel + tb < count) block(tile0, tile1, p.t0 + rel + tb, tb);
             }
+            note_ahead(rel);
         }
     }
 
@@ -489,8 +512,8 @@ template <int KT, int NB, class P, class S>
 __global__ __launch_bounds__(256, NB > 4 ? 1 : 2) void attn_shared_kernel(SharedArgs a) {
     constexpr size_t kP = tile_bytes<NB, P>(), kS = tile_bytes<NB, S>();
     __shared__ __align__(16) uint8_t tile0[kP > kS ? kP : kS], tile1[kP > kS ? kP : kS];
-    __shared__ uint64_t s_pk[kPages], s_pv[kPages];
-    __shared__ __align__(16) float s_sc[2 * (P::T > S::T ? P::T : S::T)];
+    __shared__ ulonglong2 s_row[2 * kAhead];
+    __shared__ __align__(16) float s_sc[KT == kKvQ8 ? 4 * kAhead : 4];
     __shared__ float s_ml[4 * 2 * (P::RT > S::RT ? P::RT : S::RT) * 16];
     const int item = blockIdx.x;
     Part p;
@@ -506,7 +529,7 @@ __global__ __launch_bounds__(256, NB > 4 ? 1 : 2) void attn_shared_kernel(Shared
         p.r0 = tile_at * P::ROWS;
         p.n = min(P::ROWS, a.n_tokens * a.group - p.r0);
         p.lim0 = p.lim_row = 0;
-        attend<KT, NB, P, false>(a, p, tile0, tile1, s_pk, s_pv, s_sc, reinterpret_cast<float(*)[2 * P::RT][16]>(s_ml));
+        attend<KT, NB, P, false>(a, p, tile0, tile1, s_row, s_sc, reinterpret_cast<float(*)[2 * P::RT][16]>(s_ml));
         return;
     }
     int at = item - a.p_items;
@@ -533,73 +556,47 @@ __global__ __launch_bounds__(256, NB > 4 ? 1 : 2) void attn_shared_kernel(Shared
         }
         return;
     }
-    attend<KT, NB, S, true>(a, p, tile0, tile1, s_pk, s_pv, s_sc, reinterpret_cast<float(*)[2 * S::RT][16]>(s_ml));
+    attend<KT, NB, S, true>(a, p, tile0, tile1, s_row, s_sc, reinterpret_cast<float(*)[2 * S::RT][16]>(s_ml));
 }
 
 // out row = sum over its parts.  `per` = hd / 4 threads hold a row's channels, four
 // each; `ways` such groups share the parts of a row, and 256 / per / ways rows a
 // workgroup.  A part without a seen row (l = 0) has no sums.
-constexpr int kSlots = 256;
+constexpr int kSlots = 256, kJoined = 8;  // parts of a row, rows of a workgroup
 __global__ __launch_bounds__(256) void attn_shared_join(const float* __restrict__ part, float* __restrict__ out, int rows,
                                                         int slots, int hd, int per, int ways) {
-    __shared__ float s_f[kSlots * 8];   // [row of the workgroup][slot]: the part's weight
-    __shared__ float s_sum[256];        // of a row
+    __shared__ float2 s_ml[kSlots * kJoined];
     __shared__ f32x4 s_v[256];
     const int many = 256 / per / ways, group = threadIdx.x / per, d = threadIdx.x % per * 4, in = group / ways, way = group % ways;
-    const int row0 = blockIdx.x * many;
-    const float* ml = part + static_cast<size_t>(rows) * slots * hd;
-    // 256 / many threads a row find its maximum and turn m and l into weights
-    {
-        const int lanes = 256 / many, r = threadIdx.x / lanes, lane = threadIdx.x % lanes;
-        const float* mine = ml + static_cast<size_t>(min(row0 + r, rows - 1)) * 2 * slots;
-        const bool on = r < many && row0 + r < rows;
-        float top = -__builtin_inff();
-        if (on)
-            for (int k = lane; k < slots; k += lanes) {
-                const float m = mine[2 * k];
-                s_f[r * slots + k] = m;
-                top = fmaxf(top, m);
-            }
-        if (r < many) s_sum[threadIdx.x] = top;
-        __syncthreads();
-        if (on)
-            for (int k = 0; k < lanes; ++k) top = fmaxf(top, s_sum[r * lanes + k]);
-        __syncthreads();
-        float sum = 0.0f;
-        if (on)
-            for (int k = lane; k < slots; k += lanes) {
-                const float m = s_f[r * slots + k], l = mine[2 * k + 1];
-                const float f = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-                s_f[r * slots + k] = l == 0.0f ? -1.0f : f;
-                if (l != 0.0f) sum = fmaf(f, l, sum);
-            }
-        if (r < many) s_sum[threadIdx.x] = sum;
-        __syncthreads();
-        sum = 0.0f;
-        if (on)
-            for (int k = 0; k < lanes; ++k) sum += s_sum[r * lanes + k];
-        __syncthreads();
-        if (on && lane == 0) s_sum[r] = sum;
-        __syncthreads();
-    }
-    const int row = row0 + in;
-    const bool on = in < many && row < rows;
+    const int row0 = blockIdx.x * many, here = min(many, rows - row0);
+    const float2* ml = reinterpret_cast<const float2*>(part + static_cast<size_t>(rows) * slots * hd) + static_cast<size_t>(row0) * slots;
+    for (int i = threadIdx.x; i < here * slots; i += 256) s_ml[i] = ml[i];
+    __syncthreads();
+    const bool on = in < here;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    float sum = 0.0f;
     if (on) {
-        const float* x = part + static_cast<size_t>(row) * slots * hd + d;
+        const float2* mine = s_ml + in * slots;
+        float top = -__builtin_inff();
+        for (int k = 0; k < slots; ++k) top = fmaxf(top, mine[k].x);
+        auto weight = [&](float2 p) { return p.x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(p.x - top); };
+        for (int k = 0; k < slots; ++k)
+            if (mine[k].y != 0.0f) sum = fmaf(weight(mine[k]), mine[k].y, sum);
+        const float* x = part + static_cast<size_t>(row0 + in) * slots * hd + d;
         for (int k = way; k < slots; k += 4 * ways) {
             f32x4 a[4];
             float f[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const int at = k + u * ways;
-                f[u] = at < slots ? s_f[in * slots + at] : -1.0f;
-                a[u] = f[u] >= 0.0f || f[u] != f[u] ? *reinterpret_cast<const f32x4*>(x + static_cast<size_t>(at) * hd) : f32x4{0.f, 0.f, 0.f, 0.f};
+                const bool some = at < slots && mine[min(at, slots - 1)].y != 0.0f;
+                f[u] = some ? weight(mine[at]) : 0.0f;
+                a[u] = some ? *reinterpret_cast<const f32x4*>(x + static_cast<size_t>(at) * hd) : f32x4{0.f, 0.f, 0.f, 0.f};
             }
 #pragma unroll
             for (int u = 0; u < 4; ++u)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = fmaf(f[u] == -1.0f ? 0.0f : f[u], a[u][i], v[i]);
+                for (int i = 0; i < 4; ++i) v[i] = fmaf(f[u], a[u][i], v[i]);
         }
     }
     if (ways > 1) {
@@ -609,8 +606,7 @@ __global__ __launch_bounds__(256) void attn_shared_join(const float* __restrict_
         for (int w = 1; w < ways; ++w) v += s_v[threadIdx.x + w * per];
     }
     if (!on) return;
-    const float sum = s_sum[in];
-    *reinterpret_cast<f32x4*>(out + static_cast<size_t>(row) * hd + d) =
+    *reinterpret_cast<f32x4*>(out + static_cast<size_t>(row0 + in) * hd + d) =
         f32x4{__fdiv_rn(v[0], sum), __fdiv_rn(v[1], sum), __fdiv_rn(v[2], sum), __fdiv_rn(v[3], sum)};
 }
 
@@ -644,18 +640,23 @@ Cut cut_of(const SharedCall& c) {
     const size_t rows = tokens * group;
     k.chunks = most > 32;
     k.p_shape = k.chunks || rows > 32 ? 2 : rows > 16 ? 1 : 0;
-    auto split = [](size_t len, size_t others, size_t page, size_t& splits, size_t& chunk) {
+    auto split = [](size_t target, size_t len, size_t others, size_t& splits, size_t& chunk) {
         if (!len) return void(splits = chunk = 0);
-        const size_t most_rows = 512 * page;
-        splits = std::min((len + 127) / 128, (512 + others - 1) / others);
-        chunk = std::min(((len + splits - 1) / splits + 127) / 128 * 128, most_rows);
+        splits = std::min((len + 127) / 128, (target + others - 1) / others);
+        chunk = ((len + splits - 1) / splits + 127) / 128 * 128;
         splits = (len + chunk - 1) / chunk;
     };
     const size_t p_rows = rows_of(k.p_shape, nb), s_rows = rows_of(k.chunks ? 2 : 0, nb);
     k.p_tiles = (rows + p_rows - 1) / p_rows;
     k.s_tiles = (most + s_rows - 1) / s_rows;
-    split(c.prefix_len, k.p_tiles * c.n_head_kv, c.p_page, k.p_splits, k.p_chunk);
-    split(own, c.n_seq * c.n_head_kv * k.s_tiles, c.s_page, k.s_splits, k.s_chunk);
+#ifndef PT
+#define PT 256
+#endif
+#ifndef ST
+#define ST 512
+#endif
+    split(PT, c.prefix_len, k.p_tiles * c.n_head_kv, k.p_splits, k.p_chunk);
+    split(ST, own, c.n_seq * c.n_head_kv * k.s_tiles, k.s_splits, k.s_chunk);
     return k;
 }
 
@@ -735,10 +736,10 @@ hipError_t launch_attn_shared(const SharedCall& call, void* scratch, hipStream_t
                                                 : run_type<kKvF16>(nb, k, a, static_cast<unsigned>(grid), st);
         if (e != hipSuccess) return e;
         if (a.part) {
-            // the groups share a row's parts while each has two or more, or there are few rows; at most 8 rows (kSlots)
+            // the groups share a row's parts while each has two or more, and are at most kJoined rows
             const int rows = static_cast<int>(tokens * c.n_head), per = a.hd / 4, groups = 256 / per;
             int ways = 1;
-            while (2 * ways <= groups && (2 * ways * 2 <= a.slots || groups / ways > 8)) ways *= 2;
+            while (2 * ways <= groups && (2 * ways * 2 <= a.slots || groups / ways > kJoined)) ways *= 2;
             const int many = groups / ways;
             attn_shared_join<<<dim3(static_cast<unsigned>((rows + many - 1) / many)), 256, 0, st>>>(a.part, c.out, rows, a.slots, a.hd,
                                                                                                     per, ways);
