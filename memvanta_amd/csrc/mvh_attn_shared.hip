@@ -24,6 +24,7 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // ahead: at most 2^14, and in two fp16 they keep 22 bits down to 2^-12 of the
 // largest, 2^-35 of it below.
 constexpr float kLift = 10.0f, kSlack = 4.0f;
+constexpr float kLeastUnit = 0x1p-126f;
 constexpr int kAhead = 256;    // rows whose addresses are formed at a time, one a thread
 constexpr int kBatch = 128;    // sequences of a launch: their places are kernel arguments
 
@@ -70,12 +71,13 @@ __device__ __forceinline__ int v_turn(int row) { return CPR >= 16 ? (row & 7) * 
 template <int RW_, int RT_, int TW_, int T_>
 struct Shape {
     static constexpr int RW = RW_, RT = RT_, TW = TW_, T = T_, ROWS = 16 * RW_ * RT_;
+    static constexpr bool kShared = TW_ == 1;  // all waves take all rows of a step
     static_assert(RW_ * TW_ == 4 && T_ / TW_ % 32 == 0);
 };
 // Bytes of each of a workgroup's two tiles: a step's K or V, or, loaded directly, both; and two waves' results
 template <int NB, class S>
 constexpr size_t tile_bytes() {
-    const size_t kv = static_cast<size_t>(S::T) * NB * 64 * (S::TW == 1 ? 2 : 1), join = S::TW > 1 ? 2 * S::RT * 16 * (32 * NB + 4) * 4 : 0;
+    const size_t kv = static_cast<size_t>(S::T) * NB * 64 * (S::kShared ? 2 : 1), join = S::TW > 1 ? 2 * S::RT * 16 * (32 * NB + 4) * 4 : 0;
     return kv > join ? kv : join;
 }
 
@@ -93,16 +95,16 @@ __device__ __forceinline__ bool unbounded(_Float16 h) {  // an infinity or NaN
 }
 
 // The part of a workgroup.  A step's T rows go to LDS as fp16: of F16 pages in shapes
-// whose waves share them (TW = 1) straight from memory, into one tile while the other
+// whose waves share them straight from memory, into one tile while the other
 // is in use; else through registers, loaded a step ahead, K to one tile and V to the
 // other.  CAUSAL: rows may be seen by some of the tokens only.
 template <int KT, int NB, class S, bool CAUSAL>
 __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8_t* tile0, uint8_t* tile1, ulonglong2* s_row, float* s_sc,
                                         float (*s_ml)[2 * S::RT][16]) {
     constexpr int RW = S::RW, RT = S::RT, TW = S::TW, T = S::T, CPR = 4 * NB, HDP = 32 * NB, ITEMS = T * CPR / 256, ND = 2 * NB;
-    constexpr bool Q8 = KT == kKvQ8, DIRECT = !Q8 && TW == 1;
+    constexpr bool Q8 = KT == kKvQ8, DIRECT = !Q8 && S::kShared;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, j = lane >> 4;
-    const int rw = wave % RW, tw = wave / RW, hd = a.hd;
+    const int rw = wave % RW, tw = wave / RW, hd = a.hd, kh = p.kh;
 
     // Addresses of the part's rows, 256 ahead of those in use: s_row[row % 512], and for Q8 pages their scales in s_sc.
     // Rows behind the part are its first one again, masked.
@@ -194,7 +196,7 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
     for (int rt = 0; rt < RT; ++rt) {
         const int r = p.r0 + min((rw * RT + rt) * 16 + n, p.n - 1);
         lim[rt] = CAUSAL ? p.lim0 + (r - p.lim_row) / a.group : 0;
-        const float* qr = a.q + (static_cast<size_t>(r / a.group) * a.n_head + p.kh * a.group + r % a.group) * hd;
+        const float* qr = a.q + (static_cast<size_t>(r / a.group) * a.n_head + kh * a.group + r % a.group) * hd;
         float f[NB][8], top = 0.0f;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -228,80 +230,113 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
 
     f32x4 o[RT][ND];
     float m[RT], base_y[RT], l[RT];  // the largest s (within kSlack), what is taken off y, the sum of weights
-    int unit[RT];                    // Q8: sums are held times 2^-unit, the exponent of the largest scale seen
+    float unit[RT], per_unit[RT];    // Q8: sums are held in units, the power of two at the largest V scale seen, and 1 / unit
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         m[rt] = -__builtin_inff();
         base_y[rt] = l[rt] = 0.0f;
-        unit[rt] = -126;
+        unit[rt] = kLeastUnit, per_unit[rt] = 1.0f / kLeastUnit;
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[rt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
-    auto block = [&](const uint8_t* s_k, const uint8_t* s_v, int tg, int tb) {  // rows tg .. tg + 31, at tb of the tile
-        const bool edge = tg + 32 > seen_by_all;
-        f32x4 s[RT][2];
+    constexpr int U = 1;
+    // A lane's first LDS reads; those of other blocks of channels differ in bits of the chunk, those of other rows by whole rows
+    const int k_first = (n * CPR + (j ^ k_turn<CPR>(n))) * 16;
+    const int v_row = 4 * j + (n >> 2), v_first = (v_row * CPR + (((n >> 1) & 1) ^ v_turn<CPR>(v_row))) * 16 + (n & 1) * 8;
+    auto block = [&](const uint8_t* s_k, const uint8_t* s_v, int tg, int tb) {  // rows tg .., at tb of the tile
+        const bool edge = tg + 32 * U > seen_by_all;
+        f32x4 s[RT][2 * U];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) s[rt][0] = s[rt][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+            for (int h = 0; h < 2 * U; ++h) s[rt][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+        // LDS reads ahead of their use, held there: else each is waited for alone
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            half8 k[NB][2];
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    k[b][h] = *reinterpret_cast<const half8*>(s_k + ((tb * CPR * 16 + k_first) ^ (b * 64)) + (32 * u + 16 * h) * CPR * 16);
+                }
+            if (u == 0) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int part = 0; part < 2; ++part)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt)
+                            s[rt][2 * u + h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[b][h], part ? qh[rt][b] : ql[rt][b], s[rt][2 * u + h], 0, 0, 0);
+        }
+        auto value = [&](int u, int d) {  // rows of V as columns: lane (n, j) gets channel 16 d + n of rows 4 j .. and 16 + 4 j ..
+            union {
+                s16x4 w[2];
+                half8 h;
+            } v;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int row = tb + 16 * h + n;
-                const half8 k = *reinterpret_cast<const half8*>(s_k + (row * CPR + ((4 * b + j) ^ k_turn<CPR>(row))) * 16);
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) s[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[rt][b], s[rt][h], 0, 0, 0);
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) s[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[rt][b], s[rt][h], 0, 0, 0);
+                typedef __attribute__((address_space(3))) s16x4 lds_t;
+                v.w[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (lds_t*)(s_v + ((tb * CPR * 16 + v_first) ^ (d * 32)) + (32 * u + 16 * h) * CPR * 16));
             }
-        f32x4 ks[2], vs[2];
+            return v.h;
+        };
+        constexpr int DV = ND < 4 ? ND : 4, BATCHES = U * ND / DV;  // V comes in batches of DV operands, one ahead
+        half8 v[2][DV];
+        auto fetch = [&](int i) {
+#pragma unroll
+            for (int d = 0; d < DV; ++d) v[i & 1][d] = value(i * DV / ND, i * DV % ND + d);
+        };
+        fetch(0);
+        __builtin_amdgcn_sched_barrier(0);
+        f32x4 ks[2 * U], vs[2 * U];
         if constexpr (Q8)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < 2 * U; ++h) {
                 const int at = (tg - p.t0 + 16 * h + 4 * j) & (2 * kAhead - 1);
                 ks[h] = *reinterpret_cast<const f32x4*>(s_sc + at);
                 vs[h] = *reinterpret_cast<const f32x4*>(s_sc + 2 * kAhead + at);
             }
-        half8 ph[RT], pl[RT];
+        half8 ph[RT][U], pl[RT][U];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             auto seen = [&](int h, int i) {
                 const int t = tg + 16 * h + 4 * j + i;
                 return t < p.t1 && (!CAUSAL || t <= lim[rt]);
             };
-            float top = -__builtin_inff();
-            int widest = -126;
+            float top = -__builtin_inff(), widest = 0.0f;
             if constexpr (Q8)
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                for (int h = 0; h < 2 * U; ++h)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) s[rt][h][i] *= ks[h][i];
             if (edge) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                for (int h = 0; h < 2 * U; ++h)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s[rt][h][i] = seen(h, i) ? s[rt][h][i] : -__builtin_inff();
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    top = fmaxf(top, s[rt][h][i]);
-                    if constexpr (Q8) {
-                        const int e = static_cast<int>((__float_as_uint(vs[h][i]) >> 23) & 255u) - 127;
-                        if (e < 128 && (!edge || seen(h, i))) widest = max(widest, e);
+                    for (int i = 0; i < 4; ++i) {
+                        s[rt][h][i] = seen(h, i) ? s[rt][h][i] : -__builtin_inff();
+                        if constexpr (Q8) widest = fmaxf(widest, seen(h, i) ? vs[h][i] : 0.0f);
                     }
-                }
-            top = rows_max(top);
-            const bool ahead = top > m[rt] + slack[rt];
-            if constexpr (Q8) {
-                auto x = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(widest + 126), static_cast<uint32_t>(widest + 126), false, false);
-                uint32_t w = max(x[0], x[1]);
-                auto z = __builtin_amdgcn_permlane16_swap(w, w, false, false);
-                widest = static_cast<int>(max(z[0], z[1])) - 126;
+            } else if constexpr (Q8) {
+#pragma unroll
+                for (int h = 0; h < 2 * U; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) widest = fmaxf(widest, vs[h][i]);
             }
-            const bool wider = Q8 && widest > unit[rt];
-            if (__any(ahead || wider)) {
+#pragma unroll
+            for (int h = 0; h < 2 * U; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top = fmaxf(top, s[rt][h][i]);
+            // seldom so for any row: its maximum over the lanes is formed only then
+            if (__any(top > m[rt] + slack[rt] || (Q8 && widest >= 2.0f * unit[rt]))) {
+                top = rows_max(top);
+                if constexpr (Q8) widest = rows_max(widest);
+                const bool ahead = top > m[rt] + slack[rt], wider = Q8 && widest >= 2.0f * unit[rt];
                 float down = 1.0f;
                 if (ahead) {
                     const float next = fmaf(top, y_scale[rt], -kLift);
@@ -310,70 +345,77 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
                     base_y[rt] = next;
                 }
                 l[rt] *= down;
-                if (wider) {
-                    down = ldexpf(down, max(unit[rt] - widest, -250));
-                    unit[rt] = widest;
+                if (wider) {  // the exponent of the widest, of an infinity's the largest there is
+                    const float next = __uint_as_float(min(__float_as_uint(widest) & 0x7f800000u, 0x7e800000u));
+                    down *= unit[rt] / next;
+                    unit[rt] = next;
+                    per_unit[rt] = 1.0f / next;
                 }
 #pragma unroll
                 for (int d = 0; d < ND; ++d)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) o[rt][d][i] *= down;
             }
-            float w[8], more = 0.0f;
+            float more = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                w[i] = __builtin_amdgcn_exp2f(fmaf(s[rt][i >> 2][i & 3], y_scale[rt], -base_y[rt]));
-                more += w[i];
+            for (int u = 0; u < U; ++u) {
+                float w[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    w[i] = __builtin_amdgcn_exp2f(fmaf(s[rt][2 * u + (i >> 2)][i & 3], y_scale[rt], -base_y[rt]));
+                    more += w[i];
+                }
+                if constexpr (Q8)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        w[i] = !edge || seen(2 * u + (i >> 2), i & 3) ? w[i] * (vs[2 * u + (i >> 2)][i & 3] * per_unit[rt]) : 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    half2v h, l2;
+                    part2(w[i], w[i + 1], h, l2);
+                    ph[rt][u][i] = h.x, ph[rt][u][i + 1] = h.y;
+                    pl[rt][u][i] = l2.x, pl[rt][u][i + 1] = l2.y;
+                }
             }
             l[rt] += more;
-            if constexpr (Q8)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) w[i] = !edge || seen(i >> 2, i & 3) ? w[i] * ldexpf(vs[i >> 2][i & 3], -unit[rt]) : 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                half2v h, l2;
-                part2(w[i], w[i + 1], h, l2);
-                ph[rt][i] = h.x, ph[rt][i + 1] = h.y;
-                pl[rt][i] = l2.x, pl[rt][i + 1] = l2.y;
-            }
         }
         bool odd = false;
 #pragma unroll
-        for (int d = 0; d < ND; ++d) {
-            union {
-                s16x4 w[2];
-                half8 h;
-            } v;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int row = tb + 16 * h + 4 * j + (n >> 2), chunk = (2 * d + ((n >> 1) & 1)) ^ v_turn<CPR>(row);
-                typedef __attribute__((address_space(3))) s16x4 lds_t;
-                v.w[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(s_v + (row * CPR + chunk) * 16 + (n & 1) * 8));
-            }
+        for (int i = 0; i < BATCHES; ++i) {
+            const int u = i * DV / ND, d0 = i * DV % ND;
+            if (i + 1 < BATCHES) fetch(i + 1);
+            __builtin_amdgcn_sched_barrier(0);
             if (CAUSAL && !Q8 && edge) {
                 // a row that some do not see: what is no number there must not meet their weight of 0
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (unbounded(v.h[i])) {
-                        odd = true;
-                        v.h[i] = static_cast<_Float16>(0.0f);
-                    }
+                for (int d = 0; d < DV; ++d)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (unbounded(v[i & 1][d][e])) {
+                            odd = true;
+                            v[i & 1][d][e] = static_cast<_Float16>(0.0f);
+                        }
             }
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v.h, pl[rt], o[rt][d], 0, 0, 0);
+            for (int part = 0; part < 2; ++part)
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v.h, ph[rt], o[rt][d], 0, 0, 0);
+                for (int d = 0; d < DV; ++d)
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt)
+                        o[rt][d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[i & 1][d], part ? ph[rt][u] : pl[rt][u], o[rt][d0 + d], 0, 0, 0);
         }
         if (CAUSAL && !Q8 && __any(odd)) {  // the products left out, for the rows that see them
 #pragma unroll 1
-            for (int t = 0; t < 32; ++t) {
-                const int row = tb + t, from_lane = n + 16 * ((t >> 2) & 3), at = 4 * (t >> 4) + (t & 3);
+            for (int t = 0; t < 32 * U; ++t) {
+                const int row = tb + t, from_lane = n + 16 * ((t >> 2) & 3), at = 4 * ((t >> 4) & 1) + (t & 3);
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
                     float w = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (i == at) w = static_cast<float>(ph[rt][i]) + static_cast<float>(pl[rt][i]);
+                    for (int u = 0; u < U; ++u)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (i == at && u == t >> 5) w = static_cast<float>(ph[rt][u][i]) + static_cast<float>(pl[rt][u][i]);
                     w = __shfl(w, from_lane);
                     if (tg + t >= p.t1 || tg + t > lim[rt]) continue;
 #pragma unroll
@@ -381,9 +423,9 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const int ch = 16 * d + 4 * j + i;
-                            const _Float16 v = *reinterpret_cast<const _Float16*>(
+                            const _Float16 x = *reinterpret_cast<const _Float16*>(
                                 s_v + (row * CPR + ((ch >> 3) ^ v_turn<CPR>(row))) * 16 + (ch & 7) * 2);
-                            if (unbounded(v)) o[rt][d][i] = fmaf(w, static_cast<float>(v), o[rt][d][i]);
+                            if (unbounded(x)) o[rt][d][i] = fmaf(w, static_cast<float>(x), o[rt][d][i]);
                         }
                 }
             }
@@ -435,7 +477,7 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
     const size_t gs = static_cast<size_t>(a.n_tokens) * a.n_head;
     auto put = [&](int row, int d, f32x4 v, float top, float sum) {
         const int r = p.r0 + row;
-        const size_t g = static_cast<size_t>(r / a.group) * a.n_head + p.kh * a.group + r % a.group;
+        const size_t g = static_cast<size_t>(r / a.group) * a.n_head + kh * a.group + r % a.group;
         if (!a.part) {
             *reinterpret_cast<f32x4*>(a.out + g * hd + d) =
                 f32x4{__fdiv_rn(v[0], sum), __fdiv_rn(v[1], sum), __fdiv_rn(v[2], sum), __fdiv_rn(v[3], sum)};
@@ -457,7 +499,7 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
 #pragma unroll
             for (int d = 0; d < ND; ++d)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[rt][d][i] = ldexpf(o[rt][d][i], unit[rt]);
+                for (int i = 0; i < 4; ++i) o[rt][d][i] *= unit[rt];
     }
     if constexpr (TW == 1) {
 #pragma unroll
@@ -626,6 +668,15 @@ constexpr int kWide = 4;  // blocks of 32 channels up to which a wave takes two 
 size_t rows_of(int shape, int nb) { return shape == 0 && nb <= kWide ? 16 : shape <= 1 ? 32 : nb <= kWide ? 128 : 64; }
 int blocks_of(size_t hd) { return hd <= 64 ? 2 : hd <= 128 ? 4 : 8; }
 
+#ifndef CT
+#define CT 512
+#endif
+#ifndef ST
+#define ST 512
+#endif
+#ifndef PT
+#define PT 256
+#endif
 Cut cut_of(const SharedCall& c) {
     Cut k{};
     const int nb = blocks_of(c.head_dim);
@@ -640,23 +691,20 @@ Cut cut_of(const SharedCall& c) {
     const size_t rows = tokens * group;
     k.chunks = most > 32;
     k.p_shape = k.chunks || rows > 32 ? 2 : rows > 16 ? 1 : 0;
-    auto split = [](size_t target, size_t len, size_t others, size_t& splits, size_t& chunk) {
+    // parts of whole 128 rows
+    auto split = [](size_t len, size_t most, size_t& splits, size_t& chunk) {
         if (!len) return void(splits = chunk = 0);
-        splits = std::min((len + 127) / 128, (target + others - 1) / others);
+        splits = std::min((len + 127) / 128, std::max<size_t>(most, 1));
         chunk = ((len + splits - 1) / splits + 127) / 128 * 128;
         splits = (len + chunk - 1) / chunk;
     };
     const size_t p_rows = rows_of(k.p_shape, nb), s_rows = rows_of(k.chunks ? 2 : 0, nb);
     k.p_tiles = (rows + p_rows - 1) / p_rows;
     k.s_tiles = (most + s_rows - 1) / s_rows;
-#ifndef PT
-#define PT 256
-#endif
-#ifndef ST
-#define ST 512
-#endif
-    split(PT, c.prefix_len, k.p_tiles * c.n_head_kv, k.p_splits, k.p_chunk);
-    split(ST, own, c.n_seq * c.n_head_kv * k.s_tiles, k.s_splits, k.s_chunk);
+    const size_t p_others = k.p_tiles * c.n_head_kv;
+    const size_t s_others = c.n_seq * c.n_head_kv * k.s_tiles;
+    split(c.prefix_len, k.chunks ? CT / p_others : (PT + p_others - 1) / p_others, k.p_splits, k.p_chunk);
+    split(own, (ST + s_others - 1) / s_others, k.s_splits, k.s_chunk);
     return k;
 }
 
