@@ -240,39 +240,34 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
         for (int d = 0; d < ND; ++d) o[rt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
-    constexpr int U = 1;
     // A lane's first LDS reads; those of other blocks of channels differ in bits of the chunk, those of other rows by whole rows
     const int k_first = (n * CPR + (j ^ k_turn<CPR>(n))) * 16;
     const int v_row = 4 * j + (n >> 2), v_first = (v_row * CPR + (((n >> 1) & 1) ^ v_turn<CPR>(v_row))) * 16 + (n & 1) * 8;
-    auto block = [&](const uint8_t* s_k, const uint8_t* s_v, int tg, int tb) {  // rows tg .., at tb of the tile
-        const bool edge = tg + 32 * U > seen_by_all;
-        f32x4 s[RT][2 * U];
+    auto block = [&](const uint8_t* s_k, const uint8_t* s_v, int tg, int tb) {  // rows tg .. tg + 31, at tb of the tile
+        const bool edge = tg + 32 > seen_by_all;
+        f32x4 s[RT][2];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-            for (int h = 0; h < 2 * U; ++h) s[rt][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int h = 0; h < 2; ++h) s[rt][h] = f32x4{0.f, 0.f, 0.f, 0.f};
         // LDS reads ahead of their use, held there: else each is waited for alone
+        half8 k[NB][2];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            half8 k[NB][2];
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+            for (int h = 0; h < 2; ++h)
+                k[b][h] = *reinterpret_cast<const half8*>(s_k + ((tb * CPR * 16 + k_first) ^ (b * 64)) + h * CPR * 256);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    k[b][h] = *reinterpret_cast<const half8*>(s_k + ((tb * CPR * 16 + k_first) ^ (b * 64)) + (32 * u + 16 * h) * CPR * 16);
-                }
-            if (u == 0) __builtin_amdgcn_sched_barrier(0);
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+            for (int part = 0; part < 2; ++part)
 #pragma unroll
-                for (int part = 0; part < 2; ++part)
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int rt = 0; rt < RT; ++rt)
-                            s[rt][2 * u + h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[b][h], part ? qh[rt][b] : ql[rt][b], s[rt][2 * u + h], 0, 0, 0);
-        }
-        auto value = [&](int u, int d) {  // rows of V as columns: lane (n, j) gets channel 16 d + n of rows 4 j .. and 16 + 4 j ..
+                    for (int rt = 0; rt < RT; ++rt)
+                        s[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[b][h], part ? qh[rt][b] : ql[rt][b], s[rt][h], 0, 0, 0);
+        auto value = [&](int d) {  // rows of V as columns: lane (n, j) gets channel 16 d + n of rows 4 j .. and 16 + 4 j ..
             union {
                 s16x4 w[2];
                 half8 h;
@@ -281,27 +276,27 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
             for (int h = 0; h < 2; ++h) {
                 typedef __attribute__((address_space(3))) s16x4 lds_t;
                 v.w[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (lds_t*)(s_v + ((tb * CPR * 16 + v_first) ^ (d * 32)) + (32 * u + 16 * h) * CPR * 16));
+                    (lds_t*)(s_v + ((tb * CPR * 16 + v_first) ^ (d * 32)) + h * CPR * 256));
             }
             return v.h;
         };
-        constexpr int DV = ND < 4 ? ND : 4, BATCHES = U * ND / DV;  // V comes in batches of DV operands, one ahead
+        constexpr int DV = 4, BATCHES = ND / DV;  // V comes in batches of DV operands, one ahead
         half8 v[2][DV];
         auto fetch = [&](int i) {
 #pragma unroll
-            for (int d = 0; d < DV; ++d) v[i & 1][d] = value(i * DV / ND, i * DV % ND + d);
+            for (int d = 0; d < DV; ++d) v[i & 1][d] = value(i * DV + d);
         };
         fetch(0);
         __builtin_amdgcn_sched_barrier(0);
-        f32x4 ks[2 * U], vs[2 * U];
+        f32x4 ks[2], vs[2];
         if constexpr (Q8)
 #pragma unroll
-            for (int h = 0; h < 2 * U; ++h) {
+            for (int h = 0; h < 2; ++h) {
                 const int at = (tg - p.t0 + 16 * h + 4 * j) & (2 * kAhead - 1);
                 ks[h] = *reinterpret_cast<const f32x4*>(s_sc + at);
                 vs[h] = *reinterpret_cast<const f32x4*>(s_sc + 2 * kAhead + at);
             }
-        half8 ph[RT][U], pl[RT][U];
+        half8 ph[RT], pl[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             auto seen = [&](int h, int i) {
@@ -311,12 +306,12 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
             float top = -__builtin_inff(), widest = 0.0f;
             if constexpr (Q8)
 #pragma unroll
-                for (int h = 0; h < 2 * U; ++h)
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) s[rt][h][i] *= ks[h][i];
             if (edge) {
 #pragma unroll
-                for (int h = 0; h < 2 * U; ++h)
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         s[rt][h][i] = seen(h, i) ? s[rt][h][i] : -__builtin_inff();
@@ -324,12 +319,12 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
                     }
             } else if constexpr (Q8) {
 #pragma unroll
-                for (int h = 0; h < 2 * U; ++h)
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) widest = fmaxf(widest, vs[h][i]);
             }
 #pragma unroll
-            for (int h = 0; h < 2 * U; ++h)
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) top = fmaxf(top, s[rt][h][i]);
             // seldom so for any row: its maximum over the lanes is formed only then
@@ -356,33 +351,27 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
 #pragma unroll
                     for (int i = 0; i < 4; ++i) o[rt][d][i] *= down;
             }
-            float more = 0.0f;
+            float w[8], more = 0.0f;
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                float w[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    w[i] = __builtin_amdgcn_exp2f(fmaf(s[rt][2 * u + (i >> 2)][i & 3], y_scale[rt], -base_y[rt]));
-                    more += w[i];
-                }
-                if constexpr (Q8)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        w[i] = !edge || seen(2 * u + (i >> 2), i & 3) ? w[i] * (vs[2 * u + (i >> 2)][i & 3] * per_unit[rt]) : 0.0f;
-#pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    half2v h, l2;
-                    part2(w[i], w[i + 1], h, l2);
-                    ph[rt][u][i] = h.x, ph[rt][u][i + 1] = h.y;
-                    pl[rt][u][i] = l2.x, pl[rt][u][i + 1] = l2.y;
-                }
+            for (int i = 0; i < 8; ++i) {
+                w[i] = __builtin_amdgcn_exp2f(fmaf(s[rt][i >> 2][i & 3], y_scale[rt], -base_y[rt]));
+                more += w[i];
             }
             l[rt] += more;
+            if constexpr (Q8)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) w[i] = !edge || seen(i >> 2, i & 3) ? w[i] * (vs[i >> 2][i & 3] * per_unit[rt]) : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                half2v h, l2;
+                part2(w[i], w[i + 1], h, l2);
+                ph[rt][i] = h.x, ph[rt][i + 1] = h.y;
+                pl[rt][i] = l2.x, pl[rt][i + 1] = l2.y;
+            }
         }
         bool odd = false;
 #pragma unroll
         for (int i = 0; i < BATCHES; ++i) {
-            const int u = i * DV / ND, d0 = i * DV % ND;
             if (i + 1 < BATCHES) fetch(i + 1);
             __builtin_amdgcn_sched_barrier(0);
             if (CAUSAL && !Q8 && edge) {
@@ -402,20 +391,18 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
                 for (int d = 0; d < DV; ++d)
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt)
-                        o[rt][d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[i & 1][d], part ? ph[rt][u] : pl[rt][u], o[rt][d0 + d], 0, 0, 0);
+                        o[rt][i * DV + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[i & 1][d], part ? ph[rt] : pl[rt], o[rt][i * DV + d], 0, 0, 0);
         }
         if (CAUSAL && !Q8 && __any(odd)) {  // the products left out, for the rows that see them
 #pragma unroll 1
-            for (int t = 0; t < 32 * U; ++t) {
-                const int row = tb + t, from_lane = n + 16 * ((t >> 2) & 3), at = 4 * ((t >> 4) & 1) + (t & 3);
+            for (int t = 0; t < 32; ++t) {
+                const int row = tb + t, from_lane = n + 16 * ((t >> 2) & 3), at = 4 * (t >> 4) + (t & 3);
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
                     float w = 0.0f;
 #pragma unroll
-                    for (int u = 0; u < U; ++u)
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (i == at && u == t >> 5) w = static_cast<float>(ph[rt][u][i]) + static_cast<float>(pl[rt][u][i]);
+                    for (int i = 0; i < 8; ++i)
+                        if (i == at) w = static_cast<float>(ph[rt][i]) + static_cast<float>(pl[rt][i]);
                     w = __shfl(w, from_lane);
                     if (tg + t >= p.t1 || tg + t > lim[rt]) continue;
 #pragma unroll
@@ -656,27 +643,21 @@ uint32_t magic_of(size_t page_tokens) {
     return page_tokens >= 16384 || !page_tokens ? 0 : static_cast<uint32_t>(((uint64_t{1} << 31) + page_tokens - 1) / page_tokens);
 }
 
-// How a launch is cut.  Parts of the prefix and of the sequences' own rows are so
-// many that there are about 512 workgroups of each (two a CU).
+// How a launch is cut.  A CU holds two workgroups.  Tokens one by one: the prefix in
+// about a workgroup a CU, whose parts beside them are the sequences' own rows (64
+// sequences behind 8000 rows: 50 us, with two a CU 65, their parts' sums to be
+// joined being twice as many).  Chunks, which have few own rows: at most two a CU.
 struct Cut {
     bool chunks;  // own rows in tiles of many query rows
     int p_shape;  // 0, 1, 2: tiles of up to 16, 32, more query rows
     size_t p_tiles, p_splits, p_chunk, s_tiles, s_splits, s_chunk;
     size_t slots() const { return p_splits + s_splits; }
 };
+constexpr int kCus = 256;
 constexpr int kWide = 4;  // blocks of 32 channels up to which a wave takes two tiles of query rows
 size_t rows_of(int shape, int nb) { return shape == 0 && nb <= kWide ? 16 : shape <= 1 ? 32 : nb <= kWide ? 128 : 64; }
 int blocks_of(size_t hd) { return hd <= 64 ? 2 : hd <= 128 ? 4 : 8; }
 
-#ifndef CT
-#define CT 512
-#endif
-#ifndef ST
-#define ST 512
-#endif
-#ifndef PT
-#define PT 256
-#endif
 Cut cut_of(const SharedCall& c) {
     Cut k{};
     const int nb = blocks_of(c.head_dim);
@@ -703,8 +684,8 @@ Cut cut_of(const SharedCall& c) {
     k.s_tiles = (most + s_rows - 1) / s_rows;
     const size_t p_others = k.p_tiles * c.n_head_kv;
     const size_t s_others = c.n_seq * c.n_head_kv * k.s_tiles;
-    split(c.prefix_len, k.chunks ? CT / p_others : (PT + p_others - 1) / p_others, k.p_splits, k.p_chunk);
-    split(own, (ST + s_others - 1) / s_others, k.s_splits, k.s_chunk);
+    split(c.prefix_len, k.chunks ? 2 * kCus / p_others : (kCus + p_others - 1) / p_others, k.p_splits, k.p_chunk);
+    split(own, (2 * kCus + s_others - 1) / s_others, k.s_splits, k.s_chunk);
     return k;
 }
 
