@@ -24,6 +24,8 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // ahead: at most 2^14, and in two fp16 they keep 22 bits down to 2^-12 of the
 // largest, 2^-35 of it below.
 constexpr float kLift = 10.0f, kSlack = 4.0f;
+// From kCoarse on the base is y itself, exactly: a rounded difference could be off by more than weights may grow.
+constexpr float kCoarse = 0x1p20f;
 constexpr float kLeastUnit = 0x1p-126f;
 constexpr int kAhead = 256;    // rows whose addresses are formed at a time, one a thread
 constexpr int kBatch = 128;    // sequences of a launch: their places are kernel arguments
@@ -334,7 +336,7 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
                 const bool ahead = top > m[rt] + slack[rt], wider = Q8 && widest >= 2.0f * unit[rt];
                 float down = 1.0f;
                 if (ahead) {
-                    const float next = fmaf(top, y_scale[rt], -kLift);
+                    const float y = top * y_scale[rt], next = fabsf(y) < kCoarse ? y - kLift : y;
                     down = m[rt] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(base_y[rt] - next);
                     m[rt] = top;
                     base_y[rt] = next;

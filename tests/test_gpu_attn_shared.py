@@ -180,6 +180,24 @@ def test_large_scores(ctx):
         b.close()
 
 
+@pytest.mark.parametrize("kv_type", [F16, Q8])
+@pytest.mark.parametrize("power", range(20, 34, 2))
+def test_scores_coarser_than_weights(ctx, kv_type, power):
+    """Scores whose last bit stands for a factor of 2^-2 to 2^12 of a weight: still one row that takes all."""
+    rng = np.random.default_rng(17)
+    for seed in range(4):
+        b = _Batch(ctx, rng, kv_type, 64, [99], [1], 2, 2, 64)
+        q = b.q.copy()
+        q[:, 3] = F(2.0 ** power * rng.uniform(1, 2))
+        got = b.run(q)
+        k, v = (np.concatenate([b.held[i], b.own[0][i]]).reshape(-1, 2, 64)[:, 0] for i in range(2))
+        s = (k.astype(np.float64) * q[0, :64]).sum(1) / 8
+        best = s.argmax()
+        if s[best] - np.sort(s)[-2] > 2.0 ** -20 * s[best] + 50:  # beyond what fp32 sums leave in doubt
+            assert abs(got[0, :64] - v[best]).max() <= 2.0 ** -20 * abs(v[best]).max()
+        b.close()
+
+
 def test_rows_of_different_sizes_q8(ctx):
     """Rows whose scales differ by powers of ten, the wide ones late."""
     rng = np.random.default_rng(11)
