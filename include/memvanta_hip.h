@@ -216,13 +216,13 @@ int mvh_matvec_q8_0(mvh_context* ctx, const mvh_tensor* a, const float* x, float
  * block_rows (1 or 128) rows and 128 columns: scale = max |x| / 448, code = x times the scale's inverse, each rounded to 32
  * bits, then to e4m3, ties to even.  A block whose scale would be below 2^-126 is held as zeros (scale 0); one with a NaN or
  * an infinity has such a scale and reads as NaN.  block_rows 128 with scales behind the codes are the bytes of a
- * MVH_TYPE_FP8_B128 tensor.  Device x must be 16-byte aligned, codes and scales 4-byte. */
+ * MVH_TYPE_FP8_B128 tensor.  Device x must be 16-byte aligned, codes and scales 4-byte, and none may overlap another. */
 int mvh_quantize_fp8(mvh_context* ctx, const float* x, size_t rows, size_t cols, size_t block_rows, uint8_t* codes,
                      float* scales, int ptr_kind);
 /* y [batch][ne1] = x [batch][ne0] times the MVH_TYPE_FP8_B128 tensor w; x is quantised as mvh_quantize_fp8 does it with
- * block_rows 1, products of codes and their sums over 128 are the matrix pipe's, scales and sums of blocks fp32.  A token's bits may depend on
- * the batch's size, whose kernels add in different orders.  Uses the context's workspace: see mvh_attn_decode for calls
- * captured into graphs. */
+ * block_rows 1, products of codes and their sums over 128 are the matrix pipe's, scales and sums of blocks fp32.  A token's
+ * bits may depend on the batch's size, whose kernels add in different orders.  Up to 2^20 tokens and 2^23 columns; device x
+ * and y must not overlap.  Uses the context's workspace: see mvh_attn_decode for calls captured into graphs. */
 int mvh_matmul_fp8(mvh_context* ctx, const mvh_tensor* w, const float* x, float* y, size_t batch, int ptr_kind);
 /* The gated feed-forward block before its last product: y [batch][ne1] = act(x gate^T) * (x up^T), both tensors
  * MVH_TYPE_FP8_B128 of one shape, act MVH_GATE_*; x and the products as in mvh_matmul_fp8, act and the product fp32. */
@@ -307,7 +307,8 @@ int mvh_attn_batch(mvh_context* ctx, const mvh_kv_cache* kv, size_t layer, const
  * them at their positions (mvh_kv_write / mvh_kv_append with pos >= prefix_len; the pages below stay unallocated).  pos[i] >=
  * prefix_len; prefix may be NULL when prefix_len is 0.  F16 and Q8 caches of one type and kv_dim, the sequences' of one
  * page size; a cache may stand for several sequences, or be the prefix too.  head_dim up to 256.  q and out are rows of
- * n_head*head_dim, the tokens of sequence 0, then of 1, ...; kvs, pos and n_tokens are host arrays, read during the call.
+ * n_head*head_dim, the tokens of sequence 0, then of 1, ..., up to 2^24 rows of a head; device q and out must be 16-byte
+ * aligned and must not overlap.  kvs, pos and n_tokens are host arrays, read during the call.
  * A token's bits may depend on the batch, which decides how rows are cut and joined.  A NaN or an infinity in a row makes
  * what a token that sees it gets from it NaN or infinite, and leaves other tokens alone.  For the context's workspace and
  * calls captured into graphs see mvh_attn_decode. */

@@ -996,6 +996,12 @@ int mvh_matvec_q8_0(mvh_context* c, const mvh_tensor* w, const float* x, float* 
     return native_f32act(c, w, MVH_TYPE_NATIVE_Q8_0, "matvec_q8_0", "q8_0 cols must be multiple of 32", x, y, 1, kind);
 }
 
+// of device ranges that one workgroup writes and others read
+static bool overlap(const void* a, size_t an, const void* b, size_t bn) {
+    const auto x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + bn && y < x + an;
+}
+
 // ---- 8-bit floating point weights ----
 
 int mvh_quantize_fp8(mvh_context* c, const float* x, size_t rows, size_t cols, size_t block_rows, uint8_t* codes,
@@ -1012,6 +1018,9 @@ int mvh_quantize_fp8(mvh_context* c, const float* x, size_t rows, size_t cols, s
     if (n_scale > (block_rows == 1 ? size_t{1} << 26 : size_t{1} << 23)) return fail(MVH_E_RANGE, "fp8 matrix too large");
     if (kind == MVH_DEVICE && ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(scales)) & 3))
         return fail(MVH_E_INVALID, "device codes and scales must be 4-byte aligned");
+    if (kind == MVH_DEVICE && (overlap(codes, rows * cols, x, rows * cols * 4) || overlap(scales, n_scale * 4, x, rows * cols * 4) ||
+                               overlap(codes, rows * cols, scales, n_scale * 4)))
+        return fail(MVH_E_INVALID, "x, codes and scales must not overlap");
     const void* xd = nullptr;
     if (int rc = stage_in_act(c, c->xin, x, rows * cols * 4, kind, &xd)) return rc;
     uint8_t* cd = codes;
@@ -1052,6 +1061,7 @@ static int fp8_call(mvh_context* c, const mvh_tensor* w, const mvh_tensor* up, i
         return fail(MVH_E_RANGE, "fp8 product too large");
     if (!batch || !rows || !cols) return MVH_OK;
     if (!x || !y) return fail(MVH_E_INVALID, "null x/y");
+    if (kind == MVH_DEVICE && overlap(x, batch * cols * 4, y, batch * rows * 4)) return fail(MVH_E_INVALID, "x and y must not overlap");
     const void* xd = nullptr;
     if (int rc = stage_in_act(c, c->xin, x, batch * cols * 4, kind, &xd)) return rc;
     float* yd = y;
@@ -1673,6 +1683,7 @@ int mvh_attn_shared(mvh_context* c, const mvh_kv_cache* prefix, size_t prefix_le
     call.n_seq = seq.size(), call.s_page = s_page;
     call.n_head = n_head, call.n_head_kv = n_head_kv, call.head_dim = head_dim, call.kv_dim = one->kv_dim;
     const size_t qn = tokens * n_head * head_dim;
+    if (kind == MVH_DEVICE && overlap(q, qn * 4, out, qn * 4)) return fail(MVH_E_INVALID, "q and out must not overlap");
     const void* qd = nullptr;
     if (int rc = stage_in(c, c->xin, q, qn * 4, kind, &qd)) return rc;
     float* od = out;

@@ -124,6 +124,7 @@ struct Fp8Args {
     float* y;              // [M][N]
     float* part;           // sums of the splits of K, [split][matrix][M][n4]; null without splits
     int N, K, M, blocks, gate, x_rows, n4, per;  // per: blocks of a split
+    bool vec;              // rows of y are 16-byte aligned
 };
 
 // A float at an address that is the same in every lane, through the scalar cache
@@ -155,37 +156,33 @@ __global__ __launch_bounds__(256) void quantize_operand_kernel(const float* __re
     if (lane == 0) scales[static_cast<size_t>(kb) * (items / blocks) + row] = s;
 }
 
-// A workgroup: 16 rows of the weights (of both matrices) after another, 16 TT
-// tokens; its W waves take the blocks of K in turn, U at a time with the next U on
+// A workgroup: 16 rows of the weights (of both matrices) after another, all (up to
+// 16 TT) tokens; its W waves take the blocks of K in turn, the next one's weights on
 // their way, and join through LDS.  QIN: x is quantised here, by every workgroup
 // for itself, while the first weights come; else it comes as operands.
-template <int MATS, int TT, int W, int U, bool QIN>
+template <int MATS, int TT, int W, bool QIN>
 __global__ __launch_bounds__(64 * W) void fp8_rows_kernel(Fp8Args a) {
     extern __shared__ __align__(16) uint8_t s_x[];  // QIN: codes [M][128 blocks + 16], scales [blocks][M]
     __shared__ float s_y[W][MATS][TT][16][17];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, j = lane >> 4;
-    const int t0 = blockIdx.y * 16 * TT, last16 = a.K / 16 - 1, tiles = (a.N + 15) / 16;
+    const int last16 = a.K / 16 - 1, tiles = (a.N + 15) / 16;
     const int pitch = a.blocks * kBlk + 16;
     float* const s_xs = reinterpret_cast<float*>(s_x + a.M * pitch);
     int from[TT];  // lanes of tokens behind the last read what the last one's does: fewer lines
 #pragma unroll
-    for (int t = 0; t < TT; ++t) from[t] = j * 16 + min(n, max(a.M - 1 - t0 - 16 * t, 0));
+    for (int t = 0; t < TT; ++t) from[t] = j * 16 + min(n, max(a.M - 1 - 16 * t, 0));
     struct Group {
-        uint4 w[U][MATS][2];
+        uint4 w[MATS][2];
     };
-    auto load = [&](Group& g, int tile, int first) {  // blocks behind the last: the last one again, left out of the sums
+    auto load = [&](Group& g, int tile, int kb) {
         const int row = min(tile * 16 + n, a.N - 1);
+        // a last block that is short: columns of the row again, against zeros
+        const size_t c0 = 16 * static_cast<size_t>(min(kb * 8 + j, last16)), c1 = 16 * static_cast<size_t>(min(kb * 8 + 4 + j, last16));
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int kb = min(first + u * W, a.blocks - 1);
-            // a last block that is short: columns of the row again, against zeros
-            const size_t c0 = 16 * static_cast<size_t>(min(kb * 8 + j, last16)), c1 = 16 * static_cast<size_t>(min(kb * 8 + 4 + j, last16));
-#pragma unroll
-            for (int m = 0; m < MATS; ++m) {
-                const uint8_t* w = a.w[m] + static_cast<size_t>(row) * a.K;
-                g.w[u][m][0] = ld_stream16(w + c0);
-                g.w[u][m][1] = ld_stream16(w + c1);
-            }
+        for (int m = 0; m < MATS; ++m) {
+            const uint8_t* w = a.w[m] + static_cast<size_t>(row) * a.K;
+            g.w[m][0] = ld_stream16(w + c0);
+            g.w[m][1] = ld_stream16(w + c1);
         }
     };
     Group now;
@@ -218,42 +215,37 @@ __global__ __launch_bounds__(64 * W) void fp8_rows_kernel(Fp8Args a) {
 #pragma unroll
             for (int t = 0; t < TT; ++t) acc[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
         const size_t srow = static_cast<size_t>(tile * 16 / kBlk) * a.blocks;
-        for (int first = wave; first < a.blocks; first += U * W) {
+        for (int kb = wave; kb < a.blocks; kb += W) {
             Group next;
-            if (first + U * W < a.blocks) load(next, tile, first + U * W);
+            if (kb + W < a.blocks) load(next, tile, kb + W);
             else if (tile + static_cast<int>(gridDim.x) < tiles) load(next, tile + gridDim.x, wave);
+            Codes32 w[MATS];
+            float ws[MATS];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int kb = first + u * W;
-                if (kb >= a.blocks) break;
-                Codes32 w[MATS];
-                float ws[MATS];
+            for (int m = 0; m < MATS; ++m) {
+                w[m] = widen(now.w[m][0], now.w[m][1]);
+                ws[m] = load_const(a.ws[m] + srow + kb);
+            }
 #pragma unroll
-                for (int m = 0; m < MATS; ++m) {
-                    w[m] = widen(now.w[u][m][0], now.w[u][m][1]);
-                    ws[m] = load_const(a.ws[m] + srow + kb);
+            for (int t = 0; t < TT; ++t) {
+                Codes32 x;
+                float xs;
+                if constexpr (QIN) {
+                    const int tok = min(n, a.M - 1);
+                    const uint8_t* p = s_x + tok * pitch + kb * kBlk + 16 * j;
+                    x = widen(*reinterpret_cast<const uint4*>(p), *reinterpret_cast<const uint4*>(p + 64));
+                    xs = s_xs[kb * a.M + tok];
+                } else {
+                    const uint4* p = reinterpret_cast<const uint4*>(a.xq) + (static_cast<size_t>(t) * a.blocks + kb) * 128 + from[t];
+                    x = widen(p[0], p[64]);
+                    xs = a.xs[static_cast<size_t>(kb) * a.x_rows + 16 * t + n];
                 }
 #pragma unroll
-                for (int t = 0; t < TT; ++t) {
-                    Codes32 x;
-                    float xs;
-                    if constexpr (QIN) {
-                        const int tok = min(n, a.M - 1);
-                        const uint8_t* p = s_x + tok * pitch + kb * kBlk + 16 * j;
-                        x = widen(*reinterpret_cast<const uint4*>(p), *reinterpret_cast<const uint4*>(p + 64));
-                        xs = s_xs[kb * a.M + tok];
-                    } else {
-                        const uint4* p = reinterpret_cast<const uint4*>(a.xq) + (static_cast<size_t>(t0 / 16 + t) * a.blocks + kb) * 128 + from[t];
-                        x = widen(p[0], p[64]);
-                        xs = a.xs[static_cast<size_t>(kb) * a.x_rows + t0 + 16 * t + n];
-                    }
+                for (int m = 0; m < MATS; ++m) {
+                    const f32x4 c = dot128(w[m], x);
+                    const float s = xs * ws[m];
 #pragma unroll
-                    for (int m = 0; m < MATS; ++m) {
-                        const f32x4 c = dot128(w[m], x);
-                        const float s = xs * ws[m];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[m][t][i] = fmaf(s, c[i], acc[m][t][i]);
-                    }
+                    for (int i = 0; i < 4; ++i) acc[m][t][i] = fmaf(s, c[i], acc[m][t][i]);
                 }
             }
             now = next;
@@ -274,7 +266,7 @@ __global__ __launch_bounds__(64 * W) void fp8_rows_kernel(Fp8Args a) {
 #pragma unroll
                 for (int k = 1; k < W; ++k) v[m] += s_y[k][m][t][tok][r];
             }
-            const int token = t0 + 16 * t + tok, row = tile * 16 + r;
+            const int token = 16 * t + tok, row = tile * 16 + r;
             if (token < a.M && row < a.N)
                 a.y[static_cast<size_t>(token) * a.N + row] = MATS == 2 ? gated(v[0], v[MATS - 1], a.gate) : v[0];
         }
@@ -283,7 +275,6 @@ __global__ __launch_bounds__(64 * W) void fp8_rows_kernel(Fp8Args a) {
 }
 
 // ---- more tokens: tiles through LDS ----------------------------------------------
-
 
 template <int TM, int TN>
 struct Step {  // rows of 128 bytes, their 16-byte chunks turned by the row: 16 rows' reads fall in different banks
@@ -332,16 +323,16 @@ __device__ __forceinline__ void load_lds(buffer_t b, void* to, uint32_t at, int 
 #endif
 }
 
-// TM tokens x TN rows of the weights (with two matrices TN / 2 of each), G times PM
-// x PN waves, which take every G-th block of columns; a step is one block of 128 columns.  The codes go from memory to LDS as
-// they are, D - 1 steps ahead, and are widened behind it: as fp16 they would take
+// TM tokens x TN rows of the weights (with two matrices TN / 2 of each) and PM x PN
+// waves; a step is one block of 128 columns.  The codes go from memory to LDS as
+// they are, a step ahead, and are widened behind it: as fp16 they would take
 // twice the LDS reads, which at 64 x 64 a wave are half of the matrix pipe's time
 // already.
 template <int MATS, int TM, int TN, int PM, int PN>
 __global__ __launch_bounds__(64 * PM * PN, 2) void fp8_tile_kernel(Fp8Args a) {
     constexpr int W = PM * PN, WM = TM / PM, WN = TN / PN, XT = WM / 16, WT = WN / 16, PER = TN / MATS;  // PER: rows of a matrix
     constexpr int XI = TM / 8 / W, WI = TN / 8 / W, SI = TM > 64 * W ? TM / (64 * W) : 1;
-    static_assert(TM % (8 * W) == 0 && TN % (8 * W) == 0 && WT % MATS == 0 && PER % 8 == 0 && 128 % (WN / MATS) == 0 );
+    static_assert(TM % (8 * W) == 0 && TN % (8 * W) == 0 && WT % MATS == 0 && PER % 8 == 0 && 128 % (WN / MATS) == 0);
     __shared__ __align__(16) Step<TM, TN> s0, s1;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, j = lane >> 4;
     const int wm = wave % PM, wn = wave / PM;
@@ -439,7 +430,6 @@ __global__ __launch_bounds__(64 * PM * PN, 2) void fp8_tile_kernel(Fp8Args a) {
     }
     arrive();  // no load into LDS outlives the workgroup
 
-    const bool vec = a.N % 4 == 0;
 #pragma unroll
     for (int t = 0; t < XT; ++t) {
         const int token = t0 + wm * WM + 16 * t + n;
@@ -461,7 +451,7 @@ __global__ __launch_bounds__(64 * PM * PN, 2) void fp8_tile_kernel(Fp8Args a) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) v[i] = gated(v[i], acc[w + WT / 2][t][i], a.gate);
             float* y = a.y + static_cast<size_t>(token) * a.N + r;
-            if (vec && r + 3 < a.N) *reinterpret_cast<f32x4*>(y) = v;
+            if (a.vec && r + 3 < a.N) *reinterpret_cast<f32x4*>(y) = v;
             else
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
@@ -487,7 +477,7 @@ __global__ __launch_bounds__(256) void fp8_join_kernel(Fp8Args a, int splits) {
     const size_t token = at / a.n4;
     const int r = static_cast<int>(at - token * a.n4);
     float* y = a.y + token * a.N + r;
-    if (a.N % 4 == 0) *reinterpret_cast<f32x4*>(y) = v[0];
+    if (a.vec) *reinterpret_cast<f32x4*>(y) = v[0];
     else
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -550,7 +540,7 @@ void run_tile(Fp8Args& a, int splits, hipStream_t st) {
 }
 template <int MATS, int TT, int W, bool QIN>
 void run_rows(const Fp8Args& a, int wgs, size_t lds, hipStream_t st) {
-    fp8_rows_kernel<MATS, TT, W, 1, QIN><<<dim3(static_cast<unsigned>(std::min((a.N + 15) / 16, wgs))), 64 * W, lds, st>>>(a);
+    fp8_rows_kernel<MATS, TT, W, QIN><<<dim3(static_cast<unsigned>(std::min((a.N + 15) / 16, wgs))), 64 * W, lds, st>>>(a);
 }
 
 template <int MATS>
@@ -622,6 +612,7 @@ hipError_t launch_fp8(const uint8_t* w, const uint8_t* w2, int gate, const float
     a.blocks = static_cast<int>((K + kBlk - 1) / kBlk);
     a.n4 = static_cast<int>((N + 3) / 4 * 4);
     a.gate = gate;
+    a.vec = N % 4 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
     a.w[0] = w, a.w[1] = w2;
     a.ws[0] = reinterpret_cast<const float*>(w + N * K);
     a.ws[1] = w2 ? reinterpret_cast<const float*>(w2 + N * K) : nullptr;

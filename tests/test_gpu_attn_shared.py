@@ -331,6 +331,9 @@ def test_refusals(ctx):
     flat = torch.zeros(2 * 256 + 1, device="cuda")
     with pytest.raises(capi.MvhError, match="16-byte aligned"):
         go(q=flat[1:].reshape(2, 256), out=torch.zeros((2, 256), device="cuda"))
+    flat = torch.zeros(1024, device="cuda")
+    with pytest.raises(capi.MvhError, match="must not overlap"):
+        go(q=flat[:512].reshape(2, 256), out=flat[508:1020].reshape(2, 256))
     for kv in (*other.values(), empty):
         kv.close()
     b.close()

@@ -159,6 +159,33 @@ def test_device_rows_and_what_lies_around(ctx):
         t.free()
 
 
+@pytest.mark.parametrize("batch,k,n", [(4, 8192, 100), (3, 10912, 1000), (4, 8192, 4100)])
+def test_most_rows_quantised_in_the_kernel(ctx, batch, k, n):
+    """Up to 32768 elements of x are held in LDS beside the waves' sums."""
+    rng = np.random.default_rng(n)
+    wg, wu, x = _weights(rng, n, k), _weights(rng, n, k), _rows(rng, batch, k)
+    tg, tu = _tensor(ctx, *wg), _tensor(ctx, *wu)
+    _check(ctx.gated_ffn_fp8(tg, tu, x, 0), *gated(x, wg, wu, 0))
+    tg.free()
+    tu.free()
+
+
+@pytest.mark.parametrize("batch,k,n", [(3, 128, 64), (20, 256, 64), (70, 128, 260), (70, 8192, 256), (200, 2048, 512)])
+def test_results_at_any_float(ctx, batch, k, n):
+    """y needs a float's alignment only, also where rows of it are stored 16 bytes at a time."""
+    rng = np.random.default_rng(n)
+    w, x = _weights(rng, n, k), _rows(rng, batch, k)
+    t = _tensor(ctx, *w)
+    xd, flat = torch.from_numpy(x).cuda(), torch.full((batch * n + 8,), 7.0, device="cuda")
+    torch.cuda.synchronize()
+    ctx.matmul_fp8(t, xd, flat[3:-5].reshape(batch, n))
+    ctx.synchronize()
+    got = flat.cpu().numpy()
+    assert (got[:3] == 7).all() and (got[-5:] == 7).all()
+    assert (got[3:-5].reshape(batch, n) == ctx.matmul_fp8(t, x)).all()
+    t.free()
+
+
 def test_empty(ctx):
     t = _tensor(ctx, *_weights(np.random.default_rng(0), 20, 32))
     assert ctx.matmul_fp8(t, np.zeros((0, 32), F)).shape == (0, 20)
@@ -238,5 +265,12 @@ def test_refusals(ctx):
     xd = torch.zeros(4 * 32 + 4, device="cuda")
     with pytest.raises(capi.MvhError, match="16-byte aligned"):
         ctx.matmul_fp8(t, xd[1:65].reshape(2, 32), torch.zeros((2, 20), device="cuda"))
+    flat = torch.zeros(256, device="cuda")
+    with pytest.raises(capi.MvhError, match="must not overlap"):
+        ctx.matmul_fp8(t, flat[:64].reshape(2, 32), flat[60:100].reshape(2, 20))
+    raw = flat.view(torch.uint8)
+    for codes, scales in ((raw[:64], flat[128:130]), (raw[512:576], flat[1:3]), (raw[512:576], flat[129:131])):
+        with pytest.raises(capi.MvhError, match="must not overlap"):
+            ctx.quantize_fp8(flat[:64].reshape(2, 32), 1, codes, scales)
     for a in (t, t2, q4):
         a.free()
