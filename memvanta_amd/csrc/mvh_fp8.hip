@@ -16,6 +16,7 @@ namespace mvh {
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kBlk = 128;
 constexpr float kTop = 448.0f;            // largest e4m3 value
@@ -282,15 +283,23 @@ struct Step {  // rows of 128 bytes, their 16-byte chunks turned by the row: 16 
     float xs[TM < 64 ? 64 : TM];
 };
 __device__ __forceinline__ int turn(int row) { return (row >> 1) & 7; }
-struct Raw32 {
-    uint4 a, b;
+// 64 codes as fp16: lane (n, j) of 32 x 2 holds every other chunk of row n's block
+struct Codes64 {
+    half8 h[8];
 };
-__device__ __forceinline__ Raw32 raw_at(const uint8_t* rows, int row, int j) {
+__device__ __forceinline__ Codes64 codes_at(const uint8_t* rows, int row, int j) {
     const uint8_t* r = rows + row * kBlk;
-    return {*reinterpret_cast<const uint4*>(r + ((j ^ turn(row)) * 16)), *reinterpret_cast<const uint4*>(r + (((j + 4) ^ turn(row)) * 16))};
+    uint4 c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = *reinterpret_cast<const uint4*>(r + (((2 * i + j) ^ turn(row)) * 16));
+    Codes64 out;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        out.h[2 * i] = to_half8(c[i].x, c[i].y);
+        out.h[2 * i + 1] = to_half8(c[i].z, c[i].w);
+    }
+    return out;
 }
-__device__ __forceinline__ Codes32 widen(const Raw32& r) { return widen(r.a, r.b); }
-
 // Waits for this wave's loads and LDS reads, then for the other waves.  (s_waitcnt: vmcnt in bits 0 - 3 and 14 - 15,
 // expcnt, left alone, in 4 - 6, lgkmcnt in 8 - 11.)
 __device__ __forceinline__ void arrive() {
@@ -330,11 +339,11 @@ __device__ __forceinline__ void load_lds(buffer_t b, void* to, uint32_t at, int 
 // already.
 template <int MATS, int TM, int TN, int PM, int PN>
 __global__ __launch_bounds__(64 * PM * PN, 2) void fp8_tile_kernel(Fp8Args a) {
-    constexpr int W = PM * PN, WM = TM / PM, WN = TN / PN, XT = WM / 16, WT = WN / 16, PER = TN / MATS;  // PER: rows of a matrix
+    constexpr int W = PM * PN, WM = TM / PM, WN = TN / PN, XT = WM / 32, WT = WN / 32, PER = TN / MATS;  // PER: rows of a matrix
     constexpr int XI = TM / 8 / W, WI = TN / 8 / W, SI = TM > 64 * W ? TM / (64 * W) : 1;
-    static_assert(TM % (8 * W) == 0 && TN % (8 * W) == 0 && WT % MATS == 0 && PER % 8 == 0 && 128 % (WN / MATS) == 0);
+    static_assert(TM % (8 * W) == 0 && TN % (8 * W) == 0 && WM % 32 == 0 && WN % 32 == 0 && PER % 8 == 0 && 128 % (WN / MATS) == 0);
     __shared__ __align__(16) Step<TM, TN> s0, s1;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, j = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 31, j = lane >> 5;
     const int wm = wave % PM, wn = wave / PM;
     // tiles in eight runs, one per XCD (workgroups go to them in turn)
     const int tiles_m = (a.M + TM - 1) / TM, tiles = tiles_m * ((a.N + PER - 1) / PER);
@@ -388,11 +397,13 @@ __global__ __launch_bounds__(64 * PM * PN, 2) void fp8_tile_kernel(Fp8Args a) {
             load_lds<4>(sb, s.xs + ((i * W + wave) * 64) % TM, so[i] * 4, kb * a.M * 4);
     };
 
-    f32x4 acc[WT][XT];
+    // of two matrices a tile of 32 rows takes 16 each
+    const int w_row = MATS == 2 ? (n >> 4) * PER + wn * (WN / 2) + (n & 15) : wn * WN + n;
+    f32x16 acc[WT][XT];
 #pragma unroll
     for (int w = 0; w < WT; ++w)
 #pragma unroll
-        for (int t = 0; t < XT; ++t) acc[w][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < XT; ++t) acc[w][t] = f32x16{};
     auto step = [&](const Step<TM, TN>& s, Step<TM, TN>& next, int k) {
         float ws[MATS];
 #pragma unroll
@@ -402,24 +413,25 @@ __global__ __launch_bounds__(64 * PM * PN, 2) void fp8_tile_kernel(Fp8Args a) {
         float sc[MATS][XT];
 #pragma unroll
         for (int t = 0; t < XT; ++t) {
-            const float xs = s.xs[wm * WM + 16 * t + n];
+            const float xs = s.xs[wm * WM + 32 * t + n];
 #pragma unroll
             for (int m = 0; m < MATS; ++m) sc[m][t] = xs * ws[m];
         }
-        Codes32 x[XT];
+        Codes64 x[XT];
 #pragma unroll
-        for (int t = 0; t < XT; ++t) x[t] = widen(raw_at(s.x, wm * WM + 16 * t + n, j));
+        for (int t = 0; t < XT; ++t) x[t] = codes_at(s.x, wm * WM + 32 * t + n, j);
 #pragma unroll
         for (int w = 0; w < WT; ++w) {
-            const int m = MATS == 2 ? w / (WT / 2) : 0;
-            const int row = MATS == 2 ? m * PER + wn * (WN / 2) + 16 * (w % (WT / 2)) : wn * WN + 16 * w;
-            const Codes32 v = widen(raw_at(s.w, row + n, j));
+            const Codes64 v = codes_at(s.w, w_row + 32 / MATS * w, j);
+            f32x16 d[XT] = {};  // 32 x 32 sums of 128 products: lane (n, j) gets column n of rows 8 g + 4 j .. in values 4 g ..
 #pragma unroll
-            for (int t = 0; t < XT; ++t) {
-                const f32x4 d = dot128(v, x[t]);
+            for (int i = 0; i < 8; ++i)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[w][t][i] = fmaf(sc[m][t], d[i], acc[w][t][i]);
-            }
+                for (int t = 0; t < XT; ++t) d[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v.h[i], x[t].h[i], d[t], 0, 0, 0);
+#pragma unroll
+            for (int t = 0; t < XT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[w][t][i] = fmaf(sc[i * MATS / 16][t], d[t][i], acc[w][t][i]);
         }
     };
     const int steps = k1 - k0;
@@ -432,31 +444,35 @@ __global__ __launch_bounds__(64 * PM * PN, 2) void fp8_tile_kernel(Fp8Args a) {
 
 #pragma unroll
     for (int t = 0; t < XT; ++t) {
-        const int token = t0 + wm * WM + 16 * t + n;
+        const int token = t0 + wm * WM + 32 * t + n;
         if (token >= a.M) continue;
-        if (a.part) {
 #pragma unroll
-            for (int w = 0; w < WT; ++w) {
-                const int m = w / (WT / MATS), r = r0 + wn * (WN / MATS) + 16 * (w % (WT / MATS)) + 4 * j;
-                if (r < a.N)
-                    *reinterpret_cast<f32x4*>(a.part + ((static_cast<size_t>(blockIdx.y) * MATS + m) * a.M + token) * a.n4 + r) = acc[w][t];
+        for (int w = 0; w < WT; ++w)
+#pragma unroll
+            for (int g = 0; g < 4 / MATS; ++g) {  // four rows of each matrix
+                const int r = r0 + (wn * WN + 32 * w) / MATS + 8 * g + 4 * j;
+                f32x4 v[MATS];
+#pragma unroll
+                for (int m = 0; m < MATS; ++m)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[m][i] = acc[w][t][8 * m + 4 * g + i];
+                if (a.part) {
+                    if (r < a.N)
+#pragma unroll
+                        for (int m = 0; m < MATS; ++m)
+                            *reinterpret_cast<f32x4*>(a.part + ((static_cast<size_t>(blockIdx.y) * MATS + m) * a.M + token) * a.n4 + r) = v[m];
+                    continue;
+                }
+                if constexpr (MATS == 2)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[0][i] = gated(v[0][i], v[1][i], a.gate);
+                float* y = a.y + static_cast<size_t>(token) * a.N + r;
+                if (a.vec && r + 3 < a.N) *reinterpret_cast<f32x4*>(y) = v[0];
+                else
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (r + i < a.N) y[i] = v[0][i];
             }
-            continue;
-        }
-#pragma unroll
-        for (int w = 0; w < WT / MATS; ++w) {
-            const int r = r0 + wn * (WN / MATS) + 16 * w + 4 * j;
-            f32x4 v = acc[w][t];
-            if constexpr (MATS == 2)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = gated(v[i], acc[w + WT / 2][t][i], a.gate);
-            float* y = a.y + static_cast<size_t>(token) * a.N + r;
-            if (a.vec && r + 3 < a.N) *reinterpret_cast<f32x4*>(y) = v;
-            else
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (r + i < a.N) y[i] = v[i];
-        }
     }
 }
 
