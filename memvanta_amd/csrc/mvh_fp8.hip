@@ -379,23 +379,28 @@ __global__ __launch_bounds__(64 * PM * PN, 2) void fp8_tile_kernel(Fp8Args a) {
 #pragma unroll
     for (int i = 0; i < SI; ++i) so[i] = static_cast<uint32_t>(min(t0 + ((i * W + wave) * 64) % TM + lane % TM, a.M - 1));
     const size_t srow = static_cast<size_t>(min(r0 + wn * (WN / MATS), a.N - 1) / kBlk) * a.blocks;  // of the wave's rows
-    // Behind the last block the last one again, so that the waits' counts hold
-    auto load = [&](Step<TM, TN>& s, int step) {
+    constexpr int LOADS = XI + WI + SI;
+    auto load = [&](Step<TM, TN>& s, int step, int i) {  // the i-th of LOADS; behind the last block the last one again
         const int kb = min(k0 + step, k1 - 1);
-#pragma unroll
-        for (int i = 0; i < XI; ++i)
+        if (i < XI) {
             load_lds<16>(xb, s.x + (i * W + wave) * 1024, xo[i], kb * kBlk);
-#pragma unroll
-        for (int i = 0; i < WI; ++i) {
-            const int m = MATS == 2 ? (i * W + wave) * 8 / PER : 0;
+        } else if (i < XI + WI) {
+            const int e = i - XI, m = MATS == 2 ? (e * W + wave) * 8 / PER : 0;
             // a last block that is short: columns of the row again, against zeros
-            const uint32_t at = wo[i] + min(static_cast<uint32_t>(kb) * kBlk + wc[i], last);
-            load_lds<16>(m ? wb[MATS - 1] : wb[0], s.w + (i * W + wave) * 1024, at, 0);
+            const uint32_t at = wo[e] + min(static_cast<uint32_t>(kb) * kBlk + wc[e], last);
+            load_lds<16>(m ? wb[MATS - 1] : wb[0], s.w + (e * W + wave) * 1024, at, 0);
+        } else {
+            const int e = i - XI - WI;
+            load_lds<4>(sb, s.xs + ((e * W + wave) * 64) % TM, so[e] * 4, kb * a.M * 4);
         }
-#pragma unroll
-        for (int i = 0; i < SI; ++i)
-            load_lds<4>(sb, s.xs + ((i * W + wave) * 64) % TM, so[i] * 4, kb * a.M * 4);
     };
+    auto load_all = [&](Step<TM, TN>& s, int step) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) load(s, step, i);
+    };
+    // Issued between products where there are many, as all waves stand still while all issue theirs together: 128 x 128
+    // alone on its CU takes 0.92 us a step, with the loads first 1.05; with few products 64 x 64 would take 0.6 and not 0.5.
+    constexpr bool SPREAD = WT * 8 >= LOADS && WT * XT >= 4;
 
     // of two matrices a tile of 32 rows takes 16 each
     const int w_row = MATS == 2 ? (n >> 4) * PER + wn * (WN / 2) + (n & 15) : wn * WN + n;
@@ -409,7 +414,7 @@ __global__ __launch_bounds__(64 * PM * PN, 2) void fp8_tile_kernel(Fp8Args a) {
 #pragma unroll
         for (int m = 0; m < MATS; ++m) ws[m] = load_const(a.ws[m] + srow + k0 + k);
         arrive();  // this step's codes are there, and nobody reads the last step's any more
-        load(next, k + 1);
+        if (!SPREAD) load_all(next, k + 1);
         float sc[MATS][XT];
 #pragma unroll
         for (int t = 0; t < XT; ++t) {
@@ -425,9 +430,15 @@ __global__ __launch_bounds__(64 * PM * PN, 2) void fp8_tile_kernel(Fp8Args a) {
             const Codes64 v = codes_at(s.w, w_row + 32 / MATS * w, j);
             f32x16 d[XT] = {};  // 32 x 32 sums of 128 products: lane (n, j) gets column n of rows 8 g + 4 j .. in values 4 g ..
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < 8; ++i) {
 #pragma unroll
                 for (int t = 0; t < XT; ++t) d[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v.h[i], x[t].h[i], d[t], 0, 0, 0);
+                if (SPREAD && w * 8 + i < LOADS) {
+                    __builtin_amdgcn_sched_barrier(0x106);  // vector and scalar operations and LDS reads may cross
+                    load(next, k + 1, w * 8 + i);
+                    __builtin_amdgcn_sched_barrier(0x106);
+                }
+            }
 #pragma unroll
             for (int t = 0; t < XT; ++t)
 #pragma unroll
@@ -435,7 +446,7 @@ __global__ __launch_bounds__(64 * PM * PN, 2) void fp8_tile_kernel(Fp8Args a) {
         }
     };
     const int steps = k1 - k0;
-    load(s0, 0);
+    load_all(s0, 0);
     for (int k = 0; k < steps; k += 2) {
         step(s0, s1, k);
         if (k + 1 < steps) step(s1, s0, k + 1);
@@ -529,7 +540,7 @@ Plan plan_of(size_t N, size_t K, size_t M, int mats) {
         const bool here = M <= 4 && M * K <= 32768 && M * (blocks * (kBlk + 4) + 16) <= 40 << 10;
         return {here ? Plan::kRowsQuantizing : Plan::kRows, 1};
     }
-    static constexpr TileCost kTiles[] = {{Plan::kTile64, 64, 64, 0.47, 0.33}, {Plan::kTile64x128, 64, 128, 0.66, 0.5}, {Plan::kTile128, 128, 128, 0.97, 0.85}};
+    static constexpr TileCost kTiles[] = {{Plan::kTile64, 64, 64, 0.47, 0.33}, {Plan::kTile64x128, 64, 128, 0.66, 0.5}, {Plan::kTile128, 128, 128, 0.92, 0.84}};
     const int blocks = static_cast<int>((K + kBlk - 1) / kBlk);
     Plan best{Plan::kTile64, 1};
     double least = 1e300;
