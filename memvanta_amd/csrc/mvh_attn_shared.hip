@@ -539,6 +539,13 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
 
 // A workgroup: a part of the prefix for a tile of all query rows, or, behind those,
 // a part of one sequence's own rows.
+//
+// 32 heads on 8 of 128, 64 sequences behind 8000 rows: 46 us, 127 MB at 2.7 TB/s; 12
+// chunks of up to 75 tokens behind 3001: 61 us, 660 TFLOP/s of products (q and weights in
+// two parts, so twice the attention's own), the matrix pipe busy 28 %, VALU 33 %: 256
+// registers leave two waves a SIMD, whose products and weights overlap in part.  32 Q8
+// sequences of 32 heads behind 12000: 49 us, 139 MB at 2.8 TB/s, VALU 42 % (int8 to
+// fp16).  5 to 6 us of each are a workgroup's way from its pages to its first rows.
 template <int KT, int NB, class P, class S>
 __global__ __launch_bounds__(256, NB > 4 ? 1 : 2) void attn_shared_kernel(SharedArgs a) {
     constexpr size_t kP = tile_bytes<NB, P>(), kS = tile_bytes<NB, S>();
@@ -593,15 +600,17 @@ __global__ __launch_bounds__(256, NB > 4 ? 1 : 2) void attn_shared_kernel(Shared
 // out row = sum over its parts.  `per` = hd / 4 threads hold a row's channels, four
 // each; `ways` such groups share the parts of a row, and 256 / per / ways rows (at
 // most kJoined) a workgroup.  The parts' weights come first, 32 threads a row: formed
-// by every thread for itself, 16 sequences behind 4000 rows took 27.7 us, not 25.1.  A part
-// without a seen row (l = 0) has no sums.
+// by every thread for itself, 16 sequences behind 4000 rows took 27.7 us, not 25.1.  A
+// part without a seen row (l = 0) has no sums.  64 sequences of 32 heads of 128 in 17
+// parts: 6 us, most of it the parts' 18 MB.
 constexpr int kSlots = 256, kJoined = 8;  // parts of a row, rows of a workgroup
 __global__ __launch_bounds__(256) void attn_shared_join(const float* __restrict__ part, float* __restrict__ out, int rows,
-                                                        int slots, int hd, int per, int ways) {
+                                                        int slots, int hd, int per, int per_magic, int way_bits, int many) {
     __shared__ float2 s_wl[kSlots * kJoined];  // weights and sums
     __shared__ float s_sum[kJoined];
     __shared__ f32x4 s_v[256];
-    const int many = 256 / per / ways, group = threadIdx.x / per, d = threadIdx.x % per * 4, in = group / ways, way = group % ways;
+    const int ways = 1 << way_bits, group = threadIdx.x * per_magic >> 16, d = (threadIdx.x - group * per) * 4;
+    const int in = group >> way_bits, way = group & (ways - 1);
     const int row0 = blockIdx.x * many, here = min(many, rows - row0);
     {
         const int row = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -613,16 +622,14 @@ __global__ __launch_bounds__(256) void attn_shared_join(const float* __restrict_
                 mine[k] = ml[k];
                 top = fmaxf(top, mine[k].x);
             }
-#pragma unroll
-        for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+        top = group_max<32>(top);
         if (row < here)
             for (int k = lane; k < slots; k += 32) {
                 const float w = mine[k].x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mine[k].x - top);
                 if (mine[k].y != 0.0f) sum = fmaf(w, mine[k].y, sum);
                 mine[k].x = w;
             }
-#pragma unroll
-        for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor(sum, x);
+        sum = group_sum<32>(sum);
         if (lane == 0) s_sum[row] = sum;
     }
     __syncthreads();
@@ -655,9 +662,8 @@ __global__ __launch_bounds__(256) void attn_shared_join(const float* __restrict_
         for (int w = 1; w < ways; ++w) v += s_v[threadIdx.x + w * per];
     }
     if (!on) return;
-    const float sum = s_sum[in];
-    *reinterpret_cast<f32x4*>(out + static_cast<size_t>(row0 + in) * hd + d) =
-        f32x4{__fdiv_rn(v[0], sum), __fdiv_rn(v[1], sum), __fdiv_rn(v[2], sum), __fdiv_rn(v[3], sum)};
+    const float per_sum = __fdiv_rn(1.0f, s_sum[in]);
+    *reinterpret_cast<f32x4*>(out + static_cast<size_t>(row0 + in) * hd + d) = v * per_sum;
 }
 
 uint32_t magic_of(size_t page_tokens) {
@@ -788,11 +794,12 @@ hipError_t launch_attn_shared(const SharedCall& call, void* scratch, hipStream_t
         if (a.part) {
             // the groups share a row's parts while each has two or more, and are at most kJoined rows
             const int rows = static_cast<int>(tokens * c.n_head), per = a.hd / 4, groups = 256 / per;
-            int ways = 1;
-            while (2 * ways <= groups && (2 * ways * 2 <= a.slots || groups / ways > kJoined)) ways *= 2;
-            const int many = groups / ways;
-            attn_shared_join<<<dim3(static_cast<unsigned>((rows + many - 1) / many)), 256, 0, st>>>(a.part, c.out, rows, a.slots, a.hd,
-                                                                                                    per, ways);
+            int bits = 0;  // of the ways
+            while (2 << bits <= groups && ((4 << bits) <= a.slots || groups >> bits > kJoined)) ++bits;
+            const int many = groups >> bits;
+            // thread / per, thread < 256: by 65536 / per, rounded up
+            attn_shared_join<<<dim3(static_cast<unsigned>((rows + many - 1) / many)), 256, 0, st>>>(a.part, c.out, rows, a.slots, a.hd, per,
+                                                                                                    (65535 + per) / per, bits, many);
             if (const hipError_t j = hipGetLastError(); j != hipSuccess) return j;
         }
     }

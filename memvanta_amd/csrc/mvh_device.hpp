@@ -95,8 +95,8 @@ __device__ __forceinline__ float group_max(float v) {
     if constexpr (N >= 32) v = fmaxf(v, swz_xor<16>(v));
     return v;
 }
-template <int N>
-__device__ __forceinline__ int group_sum(int v) {
+template <int N, class T>  // int, float
+__device__ __forceinline__ T group_sum(T v) {
     if constexpr (N >= 2) v += dpp_mov<0xb1>(v);
     if constexpr (N >= 4) v += dpp_mov<0x4e>(v);
     if constexpr (N >= 8) v += dpp_mov<0x141>(v);
