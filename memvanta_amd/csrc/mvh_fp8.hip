@@ -532,37 +532,37 @@ struct TileCost {
     int kind, tm, tn;
     double alone, each;  // us of a step of a workgroup alone on its CU, and of each of several
 };
-// Weights' bytes bound up to 16 tokens, and up to 64 where they are few: there every
-// workgroup reads all of x, and at 32 tokens and 131 MB (N 32000, K 4096) takes 45 us
-// where tiles take 37, at 48 and 45 MB 24 and 19, at 64 and 11 MB 10.5 and 12.2.
-// x is quantised within the kernel while that costs less than a launch (4 tokens, K
-// 4096: 7.9 and 8.4 us; K 11008: 18.9 and 16.5).
-//
-// Of the tiles the one with the least time by this model: steps of 128 columns that
-// cost `alone` while a CU has one workgroup, and `each` a workgroup where that is
-// more; a split of K adds a launch and two passes over its sums.  Measured (us) and
-// modelled less 4 for the launches, 333 tokens, K 11008 -> 4096: 64 x 64 whole 58 / 57,
-// in two 48 / 52; 64 x 128 in two 50 / 52, in four 45 / 47; 128 x 128 in two 53 / 51.
+// The one with the least time by models of what was measured.  Few tokens: launches,
+// the weights, and x, which every workgroup reads for its 16 rows; x is quantised
+// within the kernel while that costs less than a launch (4 tokens, K 4096: 7.7 us and
+// 7.8; K 11008: 17.8 and 14.0).  Tiles: steps of 128 columns that cost `alone` while a
+// CU has one workgroup, and `each` a workgroup where that is more; a split of K adds a
+// launch and two passes over its sums; weights that no cache holds come at 4.4 TB/s (of
+// the last, of 256 MB, faster).  Measured (us), rows and tiles, in brackets weights in that cache:
+//   N 32000, K 4096      8 tokens 31.4 and 34.7 (31.3 and 26.0), 16 37.7 and 34.1, 32 46 and 36.8 (45.0 and 26.9)
+//   two of 11008, 4096   16 25.8 and 26.7, 32 29.5 and 29.1 (27.6 and 25.4);  128000, 4096  8 115 and 131
+//   4096, 4096           32 10.3 and 14.1, 64 (12.1 and 13.4);  11008, 4096  32 20.3 and 18.2
+// and of tiles, 333 tokens, K 11008 -> 4096: 64 x 64 whole 62, in two 53; 64 x 128 in two 56, in four 49; 128 x 128 in two
+// 52.
 Plan plan_of(size_t N, size_t K, size_t M, int mats) {
-    const double mb = static_cast<double>(N) * K * mats * 1e-6;
-    if (M <= 16 || (M <= 32 && mb <= 100) || (M <= 64 && mb <= 20)) {
-        const size_t blocks = (K + kBlk - 1) / kBlk;
-        const bool here = M <= 4 && M * K <= 32768 && M * (blocks * (kBlk + 4) + 16) <= 40 << 10;
-        return {here ? Plan::kRowsQuantizing : Plan::kRows, 1};
-    }
     static constexpr TileCost kTiles[] = {{Plan::kTile64, 64, 64, 0.47, 0.33}, {Plan::kTile64x128, 64, 128, 0.66, 0.5}, {Plan::kTile128, 128, 128, 0.92, 0.84}};
     const int blocks = static_cast<int>((K + kBlk - 1) / kBlk);
+    const double mb = static_cast<double>(N) * K * 1e-6;  // of a matrix
     Plan best{Plan::kTile64, 1};
     double least = 1e300;
     for (const TileCost& t : kTiles) {
         const double tiles = static_cast<double>((M + t.tm - 1) / t.tm) * static_cast<double>((N * mats + t.tn - 1) / t.tn);
         for (int splits = 1; splits <= 8 && blocks / splits >= 4; splits *= 2) {
-            const double join = splits > 1 ? 2.0 + 8e-6 / 4 * splits * M * N * mats : 0.0;
+            const double join = splits > 1 ? 3.0 + 8e-6 / 4 * splits * M * N * mats : 0.0;
             const double us = (blocks + splits - 1) / splits * std::max(t.alone, std::ceil(tiles * splits / kCus) * t.each) + join;
             if (us < least) least = us, best = {static_cast<decltype(Plan::kind)>(t.kind), splits};
         }
     }
-    return best;
+    if (M > 64) return best;
+    const bool here = M <= 4 && M * K <= 32768 && M * (blocks * static_cast<size_t>(kBlk + 4) + 16) <= 40 << 10;
+    const double rows = (here ? 3.5 : 5.5) + 0.18 * mb * mats + 0.00375 * mb * M;
+    if (4.0 + std::max(least, mb * mats / 4.4) < rows) return best;
+    return {here ? Plan::kRowsQuantizing : Plan::kRows, 1};
 }
 
 template <int MATS, int TM, int TN, int PM, int PN>
