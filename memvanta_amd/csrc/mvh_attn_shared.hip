@@ -434,7 +434,7 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
     };
     if constexpr (DIRECT) {
         auto step = [&](int rel, const uint8_t* tile, uint8_t* other) {
-            __syncthreads();  // this tile's rows are there, and nobody reads the other any more
+            arrive();  // this tile's rows are there, and nobody reads the other any more
             if (rel + T < count) load(rel + T, other);
             look_ahead(rel);
 #pragma unroll 1
@@ -446,6 +446,7 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
             step(rel, tile0, tile1);
             if (rel + T < count) step(rel + T, tile1, tile0);
         }
+        arrive();  // no load into LDS outlives the workgroup
     } else {
         for (int rel = 0; rel < count; rel += T) {
             __syncthreads();

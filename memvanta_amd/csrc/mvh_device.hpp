@@ -197,6 +197,17 @@ __device__ __forceinline__ int query_exponent(float top) {
     return (top > 0.0f && top <= 3.402823466e38f ? max(__builtin_amdgcn_frexp_expf(top) - 1, -110) : 0) - 9;
 }
 
+// Hands tiles in LDS over: waits for this wave's loads and LDS accesses, then for the
+// other waves.  A barrier alone does not wait for loads that go straight to LDS, nor
+// does an LDS read behind it.  (s_waitcnt: vmcnt in bits 0 - 3 and 14 - 15, expcnt,
+// left alone, in 4 - 6, lgkmcnt in 8 - 11.)
+__device__ __forceinline__ void arrive() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(7 << 4);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 // 16-byte load through a pointer that is known to address global memory but
 // was itself loaded from memory (a page table): the address-space cast makes
 // it a global_load instead of a flat_load, whose LDS/VMEM counter coupling

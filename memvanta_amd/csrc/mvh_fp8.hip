@@ -304,14 +304,6 @@ __device__ __forceinline__ Codes64 codes_at(const uint8_t* rows, int row, int j)
     }
     return out;
 }
-// Waits for this wave's loads and LDS reads, then for the other waves.  (s_waitcnt: vmcnt in bits 0 - 3 and 14 - 15,
-// expcnt, left alone, in 4 - 6, lgkmcnt in 8 - 11.)
-__device__ __forceinline__ void arrive() {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(7 << 4);
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-}
 // Memory from p on, for loads that go to LDS: offsets of 32 bits, what lies `bytes` or more behind p reads as 0.  (The
 // host's pass over this file has not the device's buffer type.)
 #ifdef __HIP_DEVICE_COMPILE__
