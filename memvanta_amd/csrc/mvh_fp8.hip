@@ -139,6 +139,28 @@ __device__ __forceinline__ float gated(float g, float u, int gate) {
     return a * u;
 }
 
+// The factor xs ws of a sum c of 128 products of codes, which is 0 or 2^-18 .. 2^25.
+// Where xs ws leaves fp32's normal numbers, xs ws c need not: its power of two is then
+// split, s more = xs ws.  (xs: 0 or 2^-126 .. 2^119.2, or infinite or NaN, and so are its
+// codes NaN.)
+//   too large:  ws >= 2^8, s = xs (ws 2^-120) is 2^8 .. 2^127.2, c 2^120 overflows only
+//               where xs ws c does
+//   too small:  ws < 1, s = xs (ws 2^120) is exact to its 24 bits while xs ws c is no 0; what c
+//               2^-120 loses, below 2^-149, s < 2^-6 puts below half of fp32's last
+struct Factor {
+    float s, more;
+};
+__device__ __forceinline__ bool to_split(float s, float xs, float ws) {
+    constexpr int kZero = 0x060, kSubnormal = 0x090, kInfinite = 0x204;  // v_cmp_class
+    return __builtin_amdgcn_classf(s, kZero | kSubnormal | kInfinite) && xs != 0.0f && ws != 0.0f;
+}
+__device__ __forceinline__ Factor factor_of(float xs, float ws) {
+    const float s = xs * ws;
+    if (!to_split(s, xs, ws)) return {s, 1.0f};
+    const bool large = fabsf(s) > 1.0f;
+    return {xs * (ws * (large ? 0x1p-120f : 0x1p120f)), large ? 0x1p120f : 0x1p-120f};
+}
+
 // ---- few tokens: bound by the weights' bytes ------------------------------------
 
 // x as codes in the operand's order for tiles of 16 tokens: [tile][block][half][lane],
@@ -248,9 +270,9 @@ __global__ __launch_bounds__(64 * W) void fp8_rows_kernel(Fp8Args a) {
 #pragma unroll
                 for (int m = 0; m < MATS; ++m) {
                     const f32x4 c = dot128(w[m], x);
-                    const float s = xs * ws[m];
+                    const Factor f = factor_of(xs, ws[m]);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[m][t][i] = fmaf(s, c[i], acc[m][t][i]);
+                    for (int i = 0; i < 4; ++i) acc[m][t][i] = fmaf(f.s, c[i] * f.more, acc[m][t][i]);
                 }
             }
             now = next;
@@ -411,18 +433,21 @@ __global__ __launch_bounds__(64 * PM * PN, 2) void fp8_tile_kernel(Fp8Args a) {
     for (int w = 0; w < WT; ++w)
 #pragma unroll
         for (int t = 0; t < XT; ++t) acc[w][t] = f32x16{};
-    auto step = [&](const Step<TM, TN>& s, Step<TM, TN>& next, int k) {
-        float ws[MATS];
-#pragma unroll
-        for (int m = 0; m < MATS; ++m) ws[m] = load_const(a.ws[m] + srow + k0 + k);
-        arrive();  // this step's codes are there, and nobody reads the last step's any more
-        if (!SPREAD) load_all(next, k + 1);
-        float sc[MATS][XT];
+    // Adds a step's products: in the first round those of factors that are whole, in the second, where a wave has any,
+    // those of split ones, so that whole ones cost one operation a product's sum.
+    auto add = [&]<bool SECOND>(const Step<TM, TN>& s, Step<TM, TN>& next, int k, const float (&ws)[MATS]) {
+        Factor f[MATS][XT];
+        bool left = false;
 #pragma unroll
         for (int t = 0; t < XT; ++t) {
             const float xs = s.xs[wm * WM + 32 * t + n];
 #pragma unroll
-            for (int m = 0; m < MATS; ++m) sc[m][t] = xs * ws[m];
+            for (int m = 0; m < MATS; ++m) {
+                f[m][t] = SECOND ? factor_of(xs, ws[m]) : Factor{xs * ws[m], 1.0f};
+                const bool split = to_split(xs * ws[m], xs, ws[m]);
+                left |= split;
+                if (split != SECOND) f[m][t] = {0.0f, 1.0f};
+            }
         }
         Codes64 x[XT];
 #pragma unroll
@@ -435,7 +460,7 @@ __global__ __launch_bounds__(64 * PM * PN, 2) void fp8_tile_kernel(Fp8Args a) {
             for (int i = 0; i < 8; ++i) {
 #pragma unroll
                 for (int t = 0; t < XT; ++t) d[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v.h[i], x[t].h[i], d[t], 0, 0, 0);
-                if (SPREAD && w * 8 + i < LOADS) {
+                if (!SECOND && SPREAD && w * 8 + i < LOADS) {
                     __builtin_amdgcn_sched_barrier(0x106);  // vector and scalar operations and LDS reads may cross
                     load(next, k + 1, w * 8 + i);
                     __builtin_amdgcn_sched_barrier(0x106);
@@ -444,7 +469,22 @@ __global__ __launch_bounds__(64 * PM * PN, 2) void fp8_tile_kernel(Fp8Args a) {
 #pragma unroll
             for (int t = 0; t < XT; ++t)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) acc[w][t][i] = fmaf(sc[i * MATS / 16][t], d[t][i], acc[w][t][i]);
+                for (int i = 0; i < 16; ++i) {
+                    const Factor& by = f[i * MATS / 16][t];
+                    acc[w][t][i] = fmaf(by.s, SECOND ? d[t][i] * by.more : d[t][i], acc[w][t][i]);
+                }
+        }
+        return left;
+    };
+    auto step = [&](const Step<TM, TN>& s, Step<TM, TN>& next, int k) {
+        float ws[MATS];
+#pragma unroll
+        for (int m = 0; m < MATS; ++m) ws[m] = load_const(a.ws[m] + srow + k0 + k);
+        arrive();  // this step's codes are there, and nobody reads the last step's any more
+        if (!SPREAD) load_all(next, k + 1);
+        if (__any(add.template operator()<false>(s, next, k, ws))) {
+            asm volatile("" ::: "memory");  // the codes are read again, not held until here
+            add.template operator()<true>(s, next, k, ws);
         }
     };
     const int steps = k1 - k0;
