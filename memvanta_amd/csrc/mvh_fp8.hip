@@ -134,8 +134,9 @@ __device__ __forceinline__ float load_const(const float* p) {
     return *reinterpret_cast<entry>(reinterpret_cast<uintptr_t>(p));
 }
 
+// (1 + erf(x) is erfc(-x), which does not cancel where x is far below 0)
 __device__ __forceinline__ float gated(float g, float u, int gate) {
-    const float a = gate == kGateSilu ? __fdiv_rn(g, 1.0f + expf(-g)) : 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
+    const float a = gate == kGateSilu ? __fdiv_rn(g, 1.0f + expf(-g)) : 0.5f * g * erfcf(g * -0.70710678118654752f);
     return a * u;
 }
 
