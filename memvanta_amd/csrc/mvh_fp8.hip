@@ -134,9 +134,17 @@ __device__ __forceinline__ float load_const(const float* p) {
     return *reinterpret_cast<entry>(reinterpret_cast<uintptr_t>(p));
 }
 
-// (1 + erf(x) is erfc(-x), which does not cancel where x is far below 0)
+// g / (1 + e^-g) as g h^2 / (1 + h^2), h = e^(g/2), where g < 0: e^-g is beyond fp32 from -88.8
+// on, the quotient a normal number down to -92.  1 + erf(x) as erfc(-x), which does not
+// cancel where x is far below 0.
 __device__ __forceinline__ float gated(float g, float u, int gate) {
-    const float a = gate == kGateSilu ? __fdiv_rn(g, 1.0f + expf(-g)) : 0.5f * g * erfcf(g * -0.70710678118654752f);
+    float a;
+    if (gate == kGateSilu) {
+        const float h = expf(-0.5f * fabsf(g));
+        a = __fdiv_rn(g < 0.0f ? g * h * h : g, fmaf(h, h, 1.0f));
+    } else {
+        a = 0.5f * g * erfcf(g * -0.70710678118654752f);
+    }
     return a * u;
 }
 

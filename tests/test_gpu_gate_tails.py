@@ -52,3 +52,18 @@ def test_gelu(ctx, batch, gates):
     err = (2 * (g * g + 2) + 2 * 16 + 3) * EPS * np.abs(want) + 2.0 ** -149 * u
     assert (np.abs(y - want) <= err)[some].all(), np.abs((y - want) / want)[some].max()
     assert (y[~some] <= 0).all() and (np.abs(y[~some]) <= 1e-28).all()
+
+
+@pytest.mark.parametrize("batch", BATCHES)
+@pytest.mark.parametrize("gates", [0.5, 127 / 128])
+def test_silu(ctx, batch, gates):
+    """Down to where the activation is no normal number, -92: e^-g alone is beyond fp32 from -88.8 on.  16 steps for the
+    exponential and its square, and as many for the quotient and products."""
+    y, g, u = _run(ctx, batch, capi.MVH_GATE_SILU, gates, 2.0 ** 100)
+    some = g > -91
+    assert (g[some] < (-84, -89)[gates > 0.5] + 1).any()
+    e = np.exp(np.maximum(g, -300))
+    want = g * e / (1 + e) * u
+    err = 32 * 2 * EPS * np.abs(want)
+    assert (np.abs(y - want) <= err)[some].all(), np.abs((y - want) / want)[some].max()
+    assert (y[~some] <= 0).all() and (np.abs(y[~some]) <= 2.0 ** -124 * u).all()
