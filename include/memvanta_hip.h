@@ -225,7 +225,8 @@ int mvh_quantize_fp8(mvh_context* ctx, const float* x, size_t rows, size_t cols,
  * and y must not overlap.  Uses the context's workspace: see mvh_attn_decode for calls captured into graphs. */
 int mvh_matmul_fp8(mvh_context* ctx, const mvh_tensor* w, const float* x, float* y, size_t batch, int ptr_kind);
 /* The gated feed-forward block before its last product: y [batch][ne1] = act(x gate^T) * (x up^T), both tensors
- * MVH_TYPE_FP8_B128 of one shape, act MVH_GATE_*; x and the products as in mvh_matmul_fp8, act and the product fp32. */
+ * MVH_TYPE_FP8_B128 of one shape, act MVH_GATE_* (of an infinite gate its limit); x and the products as in mvh_matmul_fp8, act
+ * and the product fp32. */
 int mvh_gated_ffn_fp8(mvh_context* ctx, const mvh_tensor* gate, const mvh_tensor* up, int act, const float* x, float* y,
                       size_t batch, int ptr_kind);
 

@@ -10,6 +10,7 @@
 // themselves against 64 bits, 40 times what they are here.
 #include "mvh_kernels.hpp"
 
+#include <cfloat>
 #include <cmath>
 
 namespace mvh {
@@ -136,9 +137,10 @@ __device__ __forceinline__ float load_const(const float* p) {
 
 // g / (1 + e^-g) as g h^2 / (1 + h^2), h = e^(g/2), where g < 0: e^-g is beyond fp32 from -88.8
 // on, the quotient a normal number down to -92.  1 + erf(x) as erfc(-x), which does not
-// cancel where x is far below 0.
+// cancel where x is far below 0.  Of -infinity, the limit, as of the least number.
 __device__ __forceinline__ float gated(float g, float u, int gate) {
     float a;
+    g = g < -FLT_MAX ? -FLT_MAX : g;
     if (gate == kGateSilu) {
         const float h = expf(-0.5f * fabsf(g));
         a = __fdiv_rn(g < 0.0f ? g * h * h : g, fmaf(h, h, 1.0f));

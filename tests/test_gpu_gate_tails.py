@@ -67,3 +67,21 @@ def test_silu(ctx, batch, gates):
     err = 32 * 2 * EPS * np.abs(want)
     assert (np.abs(y - want) <= err)[some].all(), np.abs((y - want) / want)[some].max()
     assert (y[~some] <= 0).all() and (np.abs(y[~some]) <= 2.0 ** -124 * u).all()
+
+
+@pytest.mark.parametrize("batch", BATCHES)
+@pytest.mark.parametrize("act", [capi.MVH_GATE_SILU, capi.MVH_GATE_GELU])
+def test_infinite_gates(ctx, batch, act):
+    """A gate beyond fp32's numbers has its activation's limit: 0 below, itself above."""
+    n, k = 200, 128
+    codes = np.zeros((n, k), np.uint8)
+    codes[:, 0] = np.where(np.arange(n) % 2, 0x7e, 0xfe)  # +-448
+    ups = np.zeros((n, k), np.uint8)
+    ups[:, 0] = 0x38
+    x = np.zeros((batch, k), F)
+    x[:, 0] = F(2.0 ** 110)
+    tg, tu = _tensor(ctx, codes, np.full((2, 1), 2.0 ** 60, F)), _tensor(ctx, ups, np.full((2, 1), 2.0 ** -110, F))
+    y = ctx.gated_ffn_fp8(tg, tu, x, act)
+    assert (y[:, ::2] == 0).all() and (y[:, 1::2] == np.inf).all()
+    tg.free()
+    tu.free()
