@@ -40,7 +40,7 @@ struct SharedArgs {
     const void* const* pt_v;
     const float* q;
     float* out;
-    float* part;  // [row][slot][hd], then [row][slot][2]: sums and (m, l); null with one part
+    float* part;  // [row][slot][hd], then [row][slot][2]: means and (m, l); null with one part
     int prefix_len, n_tokens, n_head, group, kv_heads, kv_dim, hd, slots;
     int p_page, s_page;  // rows of a page
     uint32_t p_magic, s_magic;
@@ -463,18 +463,17 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
         }
     }
 
-    // the result: of the wave, or of the TW waves that shared the rows
+    // the result: of the wave, or of the TW waves that shared the rows; means, so that values near fp32's end stay in it
     const size_t gs = static_cast<size_t>(a.n_tokens) * a.n_head;
-    auto put = [&](int row, int d, f32x4 v, float top, float sum) {
+    auto put = [&](int row, int d, f32x4 mean, float top, float sum) {
         const int r = p.r0 + row;
         const size_t g = static_cast<size_t>(r / a.group) * a.n_head + kh * a.group + r % a.group;
         if (!a.part) {
-            *reinterpret_cast<f32x4*>(a.out + g * hd + d) =
-                f32x4{__fdiv_rn(v[0], sum), __fdiv_rn(v[1], sum), __fdiv_rn(v[2], sum), __fdiv_rn(v[3], sum)};
+            *reinterpret_cast<f32x4*>(a.out + g * hd + d) = mean;
             return;
         }
         const size_t at = g * a.slots + p.slot;
-        *reinterpret_cast<f32x4*>(a.part + at * hd + d) = v;
+        *reinterpret_cast<f32x4*>(a.part + at * hd + d) = mean;
         if (d == 0) {
             float* ml = a.part + gs * a.slots * hd + 2 * at;
             ml[0] = top;
@@ -485,11 +484,14 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
     for (int rt = 0; rt < RT; ++rt) {
         l[rt] = rows_sum(l[rt]);
         if (m[rt] == -__builtin_inff()) base_y[rt] = m[rt];  // nothing seen
-        if constexpr (Q8)
+        const float per_sum = l[rt] == 0.0f ? 0.0f : __fdiv_rn(1.0f, l[rt]);
 #pragma unroll
-            for (int d = 0; d < ND; ++d)
+        for (int d = 0; d < ND; ++d)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[rt][d][i] *= unit[rt];
+            for (int i = 0; i < 4; ++i) {
+                o[rt][d][i] *= per_sum;
+                if constexpr (Q8) o[rt][d][i] *= unit[rt];
+            }
     }
     if constexpr (TW == 1) {
 #pragma unroll
@@ -501,14 +503,14 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
                 if (16 * d + 4 * j < hd) put(row, 16 * d + 4 * j, o[rt][d], base_y[rt], l[rt]);
         }
     } else {
-        auto sums = [&](int w, int rt, int row) {  // [rt][16][HDP + 4] of wave w, two waves a tile
+        auto means = [&](int w, int rt, int row) {  // [rt][16][HDP + 4] of wave w, two waves a tile
             return reinterpret_cast<float*>(w < 2 ? tile0 : tile1) + (((w & 1) * RT + rt) * 16 + row) * (HDP + 4);
         };
         __syncthreads();
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
-            for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4*>(sums(wave, rt, n) + 16 * d + 4 * j) = o[rt][d];
+            for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4*>(means(wave, rt, n) + 16 * d + 4 * j) = o[rt][d];
             if (j == 0) {
                 s_ml[wave][rt][n] = base_y[rt];
                 s_ml[wave][RT + rt][n] = l[rt];
@@ -521,17 +523,21 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
             float top = s_ml[w0][rt][c];
 #pragma unroll
             for (int k = 1; k < TW; ++k) top = fmaxf(top, s_ml[w0 + k * RW][rt][c]);
-            f32x4 v = {0.f, 0.f, 0.f, 0.f};
-            float sum = 0.0f;
+            float weight[TW], sum = 0.0f;
 #pragma unroll
             for (int k = 0; k < TW; ++k) {
                 const int w = w0 + k * RW;
-                const float mine = s_ml[w][rt][c], f = mine == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mine - top);
-                if (s_ml[w][RT + rt][c] == 0.0f) continue;
-                const f32x4 x = *reinterpret_cast<const f32x4*>(sums(w, rt, c) + d);
-                sum = fmaf(f, s_ml[w][RT + rt][c], sum);
+                const float mine = s_ml[w][rt][c], own = s_ml[w][RT + rt][c];
+                weight[k] = own == 0.0f ? 0.0f : own * (mine == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mine - top));
+                sum += weight[k];
+            }
+            const float per_sum = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
+            f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = fmaf(f, x[i], v[i]);
+            for (int k = 0; k < TW; ++k) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(means(w0 + k * RW, rt, c) + d);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = fmaf(weight[k] * per_sum, x[i], v[i]);
             }
             put(row, d, v, top, sum);
         }
@@ -598,7 +604,7 @@ __global__ __launch_bounds__(256, NB > 4 ? 1 : 2) void attn_shared_kernel(Shared
     attend<KT, NB, S, true>(a, p, tile0, tile1, s_row, s_sc, reinterpret_cast<float(*)[2 * S::RT][16]>(s_ml));
 }
 
-// out row = sum over its parts.  `per` = hd / 4 threads hold a row's channels, four
+// out row = the mean of its parts' means, by their sums of weights.  `per` = hd / 4 threads hold a row's channels, four
 // each; `ways` such groups share the parts of a row, and 256 / per / ways rows (at
 // most kJoined) a workgroup.  The parts' weights come first, 32 threads a row: formed
 // by every thread for itself, 16 sequences behind 4000 rows took 27.7 us, not 25.1.  A
@@ -607,8 +613,7 @@ __global__ __launch_bounds__(256, NB > 4 ? 1 : 2) void attn_shared_kernel(Shared
 constexpr int kSlots = 256, kJoined = 8;  // parts of a row, rows of a workgroup
 __global__ __launch_bounds__(256) void attn_shared_join(const float* __restrict__ part, float* __restrict__ out, int rows,
                                                         int slots, int hd, int per, int per_magic, int way_bits, int many) {
-    __shared__ float2 s_wl[kSlots * kJoined];  // weights and sums
-    __shared__ float s_sum[kJoined];
+    __shared__ float2 s_wl[kSlots * kJoined];  // shares of the whole, and the parts' own sums
     __shared__ f32x4 s_v[256];
     const int ways = 1 << way_bits, group = threadIdx.x * per_magic >> 16, d = (threadIdx.x - group * per) * 4;
     const int in = group >> way_bits, way = group & (ways - 1);
@@ -627,11 +632,12 @@ __global__ __launch_bounds__(256) void attn_shared_join(const float* __restrict_
         if (row < here)
             for (int k = lane; k < slots; k += 32) {
                 const float w = mine[k].x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mine[k].x - top);
-                if (mine[k].y != 0.0f) sum = fmaf(w, mine[k].y, sum);
-                mine[k].x = w;
+                mine[k].x = mine[k].y != 0.0f ? w * mine[k].y : 0.0f;
+                sum += mine[k].x;
             }
-        sum = group_sum<32>(sum);
-        if (lane == 0) s_sum[row] = sum;
+        const float per_sum = __fdiv_rn(1.0f, group_sum<32>(sum));
+        if (row < here)
+            for (int k = lane; k < slots; k += 32) mine[k].x *= per_sum;
     }
     __syncthreads();
     const bool on = in < here;
@@ -663,8 +669,7 @@ __global__ __launch_bounds__(256) void attn_shared_join(const float* __restrict_
         for (int w = 1; w < ways; ++w) v += s_v[threadIdx.x + w * per];
     }
     if (!on) return;
-    const float per_sum = __fdiv_rn(1.0f, s_sum[in]);
-    *reinterpret_cast<f32x4*>(out + static_cast<size_t>(row0 + in) * hd + d) = v * per_sum;
+    *reinterpret_cast<f32x4*>(out + static_cast<size_t>(row0 + in) * hd + d) = v;
 }
 
 uint32_t magic_of(size_t page_tokens) {
