@@ -28,7 +28,7 @@ constexpr float kLift = 10.0f, kSlack = 4.0f;
 constexpr float kCoarse = 0x1p20f;
 constexpr float kLeastUnit = 0x1p-126f;
 constexpr int kAhead = 256;    // rows whose addresses are formed at a time, one a thread
-constexpr int kBatch = 128;    // sequences of a launch: their places are kernel arguments
+constexpr size_t kBatch = 128;  // sequences of a launch: their places are kernel arguments
 
 struct SharedSeq {
     const void* const* pt_k;
@@ -755,13 +755,28 @@ size_t tokens_of(const SharedCall& c) {
     for (size_t i = 0; i < c.n_seq; ++i) n += c.n_tokens[i];
     return n;
 }
+// Workgroups of the prefix's parts, whose tiles come in eights, and of the sequences' own
+size_t prefix_items(const SharedCall& c, const Cut& k) { return (k.p_splits * c.n_head_kv + 7) / 8 * 8 * k.p_tiles; }
+size_t own_items(const SharedCall& c, const Cut& k) { return c.n_seq * c.n_head_kv * k.s_tiles * k.s_splits; }
+
+// The sequences from `first` on that go in one launch: as many as its arguments hold,
+// halved until it has fewer than 2^32 threads (every sequence has the tiles of the
+// longest chunk, of every kv head).  One alone has fewer than 2^20 workgroups.
+SharedCall launch_of(const SharedCall& c, size_t first) {
+    for (size_t n = std::min(kBatch, c.n_seq - first);; n /= 2) {
+        const SharedCall s = some(c, first, n);
+        const Cut k = cut_of(s);
+        if (n == 1 || prefix_items(s, k) + own_items(s, k) < size_t{1} << 24) return s;
+    }
+}
 
 }  // namespace
 
 size_t attn_shared_scratch(const SharedCall& c) {
     size_t most = 0;
-    for (size_t at = 0; at < c.n_seq; at += kBatch) {
-        const SharedCall s = some(c, at, std::min<size_t>(kBatch, c.n_seq - at));
+    for (size_t at = 0, n; at < c.n_seq; at += n) {
+        const SharedCall s = launch_of(c, at);
+        n = s.n_seq;
         const Cut k = cut_of(s);
         if (k.slots() > 1) most = std::max(most, tokens_of(s) * c.n_head * k.slots() * (c.head_dim + 2) * 4);
     }
@@ -769,8 +784,9 @@ size_t attn_shared_scratch(const SharedCall& c) {
 }
 
 hipError_t launch_attn_shared(const SharedCall& call, void* scratch, hipStream_t st) {
-    for (size_t first = 0; first < call.n_seq; first += kBatch) {
-        const SharedCall c = some(call, first, std::min<size_t>(kBatch, call.n_seq - first));
+    for (size_t first = 0, n; first < call.n_seq; first += n) {
+        const SharedCall c = launch_of(call, first);
+        n = c.n_seq;
         const size_t tokens = tokens_of(c);
         if (!tokens) continue;
         const Cut k = cut_of(c);
@@ -784,15 +800,14 @@ hipError_t launch_attn_shared(const SharedCall& call, void* scratch, hipStream_t
         a.p_magic = magic_of(c.p_page), a.s_magic = magic_of(c.s_page);
         a.p_tiles = static_cast<int>(k.p_tiles), a.p_splits = static_cast<int>(k.p_splits), a.p_chunk = static_cast<int>(k.p_chunk);
         a.s_tiles = static_cast<int>(k.s_tiles), a.s_splits = static_cast<int>(k.s_splits), a.s_chunk = static_cast<int>(k.s_chunk);
-        a.p_items = static_cast<int>((k.p_splits * c.n_head_kv + 7) / 8 * 8 * k.p_tiles);
+        a.p_items = static_cast<int>(prefix_items(c, k));
         int row = 0;
         for (size_t i = 0; i < c.n_seq; ++i) {
             a.seq[i] = {c.seq[i].pt_k, c.seq[i].pt_v, static_cast<int>(c.pos[i]), row};
             row += static_cast<int>(c.n_tokens[i]);
         }
         a.seq[c.n_seq].row0 = row;
-        const size_t grid = a.p_items + c.n_seq * c.n_head_kv * k.s_tiles * k.s_splits;
-        if (grid > 0xffffff) return hipErrorInvalidValue;  // a launch has fewer than 2^32 threads
+        const size_t grid = a.p_items + own_items(c, k);
         const int nb = blocks_of(c.head_dim);
         const hipError_t e = c.kv_type == kKvQ8 ? run_type<kKvQ8>(nb, k, a, static_cast<unsigned>(grid), st)
                                                 : run_type<kKvF16>(nb, k, a, static_cast<unsigned>(grid), st);
