@@ -302,14 +302,15 @@ int mvh_attn_decode(mvh_context* ctx, const mvh_kv_cache* kv, size_t layer, cons
 int mvh_attn_batch(mvh_context* ctx, const mvh_kv_cache* kv, size_t layer, const float* q, size_t pos,
                    size_t n_tokens, size_t n_head, size_t n_head_kv, size_t head_dim, float* out, int ptr_kind);
 
-/* No counterpart in the reference: attention of a batch of sequences that share a prefix, whose rows are read once for
- * all of them.  Sequence i has n_tokens[i] query tokens (n_tokens NULL: one each; 0: none) at positions pos[i]..; token b
+/* No counterpart in the reference: attention of a batch of sequences that share a prefix, whose rows are read for all
+ * sequences of a launch together (up to 128; fewer where their tiles would pass a grid), not for each.  Sequence i has n_tokens[i] query tokens (n_tokens NULL: one each; 0: none) at positions pos[i]..; token b
  * of it sees rows 0..prefix_len-1 of the cache `prefix` and rows prefix_len..pos[i]+b of its own cache kvs[i], which holds
  * them at their positions (mvh_kv_write / mvh_kv_append with pos >= prefix_len; the pages below stay unallocated).  pos[i] >=
  * prefix_len; prefix may be NULL when prefix_len is 0.  F16 and Q8 caches of one type and kv_dim, the sequences' of one
  * page size; a cache may stand for several sequences, or be the prefix too.  head_dim up to 256.  q and out are rows of
  * n_head*head_dim, the tokens of sequence 0, then of 1, ..., up to 2^24 rows of a head; device q and out must be 16-byte
  * aligned and must not overlap.  kvs, pos and n_tokens are host arrays, read during the call.
+ * Scores over Q8 rows are finite for keys up to 2^113.
  * A token's bits may depend on the batch, which decides how rows are cut and joined.  A NaN or an infinity in a row makes
  * what a token that sees it gets from it NaN or infinite, and leaves other tokens alone.  For the context's workspace and
  * calls captured into graphs see mvh_attn_decode. */

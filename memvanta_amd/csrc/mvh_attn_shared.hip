@@ -547,12 +547,15 @@ __device__ __forceinline__ void attend(const SharedArgs& a, const Part& p, uint8
 // A workgroup: a part of the prefix for a tile of all query rows, or, behind those,
 // a part of one sequence's own rows.
 //
-// 32 heads on 8 of 128, 64 sequences behind 8000 rows: 46 us, 127 MB at 2.7 TB/s; 12
-// chunks of up to 75 tokens behind 3001: 61 us, 660 TFLOP/s of products (q and weights in
-// two parts, so twice the attention's own), the matrix pipe busy 28 %, VALU 33 %: 256
+// 32 heads on 8 of 128, 64 sequences behind 8000 rows: 46 us, 127 MB at 2.8 TB/s; 12
+// chunks of up to 75 tokens behind 3001: 62 us, 650 TFLOP/s of products (q and weights in
+// two parts, so twice the attention's own), the matrix pipe busy 27 %, VALU 33 %: 256
 // registers leave two waves a SIMD, whose products and weights overlap in part.  32 Q8
 // sequences of 32 heads behind 12000: 49 us, 139 MB at 2.8 TB/s, VALU 42 % (int8 to
 // fp16).  5 to 6 us of each are a workgroup's way from its pages to its first rows.
+// The Q8 shapes of 128 query rows spill at heads of 65 to 128: 12 registers, in chunks 27,
+// to 52 and 56 bytes of scratch.  With the join, 64 Q8 sequences behind 8000 rows take 55
+// us, 49 of F16; the 12 chunks 77, 62 of F16.
 template <int KT, int NB, class P, class S>
 __global__ __launch_bounds__(256, NB > 4 ? 1 : 2) void attn_shared_kernel(SharedArgs a) {
     constexpr size_t kP = tile_bytes<NB, P>(), kS = tile_bytes<NB, S>();
@@ -604,12 +607,12 @@ __global__ __launch_bounds__(256, NB > 4 ? 1 : 2) void attn_shared_kernel(Shared
     attend<KT, NB, S, true>(a, p, tile0, tile1, s_row, s_sc, reinterpret_cast<float(*)[2 * S::RT][16]>(s_ml));
 }
 
-// out row = the mean of its parts' means, by their sums of weights.  `per` = hd / 4 threads hold a row's channels, four
-// each; `ways` such groups share the parts of a row, and 256 / per / ways rows (at
-// most kJoined) a workgroup.  The parts' weights come first, 32 threads a row: formed
+// out row = the mean of its parts' means, by their sums of weights.  `per` = hd / 4
+// threads hold a row's channels, four each; `ways` such groups share the parts of a row,
+// and 256 / per / ways rows (at most kJoined) a workgroup.  The parts' weights come first, 32 threads a row: formed
 // by every thread for itself, 16 sequences behind 4000 rows took 27.7 us, not 25.1.  A
-// part without a seen row (l = 0) has no sums.  64 sequences of 32 heads of 128 in 17
-// parts: 6 us, most of it the parts' 18 MB.
+// part without a seen row (l = 0) has no mean.  64 sequences of 32 heads of 128 in 17
+// parts: 5 us, most of it the parts' 18 MB.
 constexpr int kSlots = 256, kJoined = 8;  // parts of a row, rows of a workgroup
 __global__ __launch_bounds__(256) void attn_shared_join(const float* __restrict__ part, float* __restrict__ out, int rows,
                                                         int slots, int hd, int per, int per_magic, int way_bits, int many) {

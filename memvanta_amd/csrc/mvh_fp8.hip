@@ -7,7 +7,7 @@
 // The inner sums run on the fp16 matrix pipe, which codes (4 bits each) enter
 // exactly.  The 8-bit pipe has twice its rate, but aligns eight products at a time
 // and cuts each 13 bits below the largest: sums of 128 were off by 1.4e-5 of
-// themselves against 64 bits, 40 times what they are here.
+// themselves (rms) against 64 bits, on this pipe by 9e-9.
 #include "mvh_kernels.hpp"
 
 #include <cfloat>
@@ -73,7 +73,7 @@ __device__ __forceinline__ uint32_t half_max(uint32_t m) {
 
 // x [rows][cols] -> codes (rows `pitch` apart, columns cols .. pitch zero up to the
 // last block's end) and scales[row * row_step + block * block_step]: 32 lanes a
-// block, 16 bytes each.  2048 x 11008: 21 us, 5.4 TB/s.
+// block, 16 bytes each.  2048 x 11008: 21 to 22 us, 5.2 to 5.4 TB/s.
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const float* __restrict__ x, int cols, int blocks, size_t items,
                                                             uint8_t* __restrict__ codes, size_t pitch,
                                                             float* __restrict__ scales, size_t row_step, size_t block_step) {
@@ -89,7 +89,9 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const float* __restr
     if (lane == 0) scales[row * row_step + kb * block_step] = s;
 }
 
-// The same with a scale per 128 x 128: a workgroup a block
+// The same with a scale per 128 x 128: a workgroup a block.  4096 x 11008, as weights are
+// brought to it once: 34 us, 225 MB at 6.7 TB/s, x in the last cache; 32000 x 4096: 119
+// us, 5.5 TB/s.
 __global__ __launch_bounds__(256) void quantize_tiles_kernel(const float* __restrict__ x, size_t rows, int cols, int blocks,
                                                              uint8_t* __restrict__ codes, float* __restrict__ scales) {
     __shared__ uint32_t s_top[4];
@@ -161,13 +163,13 @@ __device__ __forceinline__ float gated(float g, float u, int gate) {
 struct Factor {
     float s, more;
 };
-__device__ __forceinline__ bool to_split(float s, float xs, float ws) {
-    constexpr int kZero = 0x060, kSubnormal = 0x090, kInfinite = 0x204;  // v_cmp_class
-    return __builtin_amdgcn_classf(s, kZero | kSubnormal | kInfinite) && xs != 0.0f && ws != 0.0f;
+__device__ __forceinline__ bool unusual(float s) {  // zero, subnormal or infinite
+    return __builtin_amdgcn_classf(s, 0x060 | 0x090 | 0x204);
 }
+__device__ __forceinline__ bool to_split(float xs, float ws) { return unusual(xs * ws) && xs != 0.0f && ws != 0.0f; }
 __device__ __forceinline__ Factor factor_of(float xs, float ws) {
     const float s = xs * ws;
-    if (!to_split(s, xs, ws)) return {s, 1.0f};
+    if (!to_split(xs, ws)) return {s, 1.0f};
     const bool large = fabsf(s) > 1.0f;
     return {xs * (ws * (large ? 0x1p-120f : 0x1p120f)), large ? 0x1p120f : 0x1p-120f};
 }
@@ -195,9 +197,9 @@ __global__ __launch_bounds__(256) void quantize_operand_kernel(const float* __re
 // their way, and join through LDS.  QIN: x is quantised here, by every workgroup
 // for itself, while the first weights come; else it comes as operands.
 //
-// One token, two matrices 4096 -> 11008: 20 us, 4.5 TB/s; 8 tokens, 4096 -> 32000: 31.5
-// us, 4.2 TB/s; one token, 4096 -> 4096 (16.8 MB): 6.5 us, of which 3 are a launch's
-// start and end.  Waves wait for loads half of their time, VALU is busy for a quarter.
+// One token, two matrices 4096 -> 11008: 20.2 us, 4.5 TB/s; 8 tokens, 4096 -> 32000: 32.3
+// us, 4.1 TB/s; one token, 4096 -> 4096 (16.8 MB): 6.6 us, of which 3 are a launch's
+// start and end.  Waves wait for loads for 24 to 37 % of their time, VALU is busy for 28 to 36 %.
 template <int MATS, int TT, int W, bool QIN>
 __global__ __launch_bounds__(64 * W) void fp8_rows_kernel(Fp8Args a) {
     extern __shared__ __align__(16) uint8_t s_x[];  // QIN: codes [M][128 blocks + 16], scales [blocks][M]
@@ -367,9 +369,9 @@ __device__ __forceinline__ void load_lds(buffer_t b, void* to, uint32_t at, int 
 // twice the LDS reads, which at 64 x 64 a wave are half of the matrix pipe's time
 // already.
 //
-// 2048 tokens, K 11008 -> 4096: 159 us, 1.16 PFLOP/s, as the library's fp16 product of
-// that size, the clock held down by power (zeros for data: 20 % faster); the pipe is
-// busy 46 % of the cycles at 2.4 GHz, VALU 43 %.  64 tokens, in eight parts: 13 us, 45 MB
+// 2048 tokens, K 11008 -> 4096: 166 us, 1.11 PFLOP/s, near the library's fp16 product of
+// 8192^3 (1.16), the clock held down by power (zeros for data: 20 % faster); the pipe is
+// busy 45 % of the cycles at 2.4 GHz, VALU 43 %.  64 tokens, in eight parts: 13 us, 45 MB
 // at 3.4 TB/s; small grids wait for their loads (0.5 us a step of 64 x 64, whose
 // products take 0.2).
 template <int MATS, int TM, int TN, int PM, int PN>
@@ -444,20 +446,24 @@ __global__ __launch_bounds__(64 * PM * PN, 2) void fp8_tile_kernel(Fp8Args a) {
     for (int w = 0; w < WT; ++w)
 #pragma unroll
         for (int t = 0; t < XT; ++t) acc[w][t] = f32x16{};
-    // Adds a step's products: in the first round those of factors that are whole, in the second, where a wave has any,
-    // those of split ones, so that whole ones cost one operation a product's sum.
+    // Adds a step's products: in the first round those of usual factors, which cost one operation a product's sum, and
+    // in the second, where a wave has any, those of split ones.  Returns whether a lane has unusual ones.
     auto add = [&]<bool SECOND>(const Step<TM, TN>& s, Step<TM, TN>& next, int k, const float (&ws)[MATS]) {
         Factor f[MATS][XT];
-        bool left = false;
+        bool some = false;
 #pragma unroll
         for (int t = 0; t < XT; ++t) {
             const float xs = s.xs[wm * WM + 32 * t + n];
 #pragma unroll
             for (int m = 0; m < MATS; ++m) {
-                f[m][t] = SECOND ? factor_of(xs, ws[m]) : Factor{xs * ws[m], 1.0f};
-                const bool split = to_split(xs * ws[m], xs, ws[m]);
-                left |= split;
-                if (split != SECOND) f[m][t] = {0.0f, 1.0f};
+                const float whole = xs * ws[m];
+                if constexpr (SECOND) {
+                    f[m][t] = factor_of(xs, ws[m]);
+                    if (!to_split(xs, ws[m])) f[m][t] = {0.0f, 1.0f};
+                } else {
+                    f[m][t].s = unusual(whole) ? 0.0f : whole;
+                    some |= unusual(whole);
+                }
             }
         }
         Codes64 x[XT];
@@ -485,7 +491,7 @@ __global__ __launch_bounds__(64 * PM * PN, 2) void fp8_tile_kernel(Fp8Args a) {
                     acc[w][t][i] = fmaf(by.s, SECOND ? d[t][i] * by.more : d[t][i], acc[w][t][i]);
                 }
         }
-        return left;
+        return some;
     };
     auto step = [&](const Step<TM, TN>& s, Step<TM, TN>& next, int k) {
         float ws[MATS];
@@ -494,8 +500,13 @@ __global__ __launch_bounds__(64 * PM * PN, 2) void fp8_tile_kernel(Fp8Args a) {
         arrive();  // this step's codes are there, and nobody reads the last step's any more
         if (!SPREAD) load_all(next, k + 1);
         if (__any(add.template operator()<false>(s, next, k, ws))) {
-            asm volatile("" ::: "memory");  // the codes are read again, not held until here
-            add.template operator()<true>(s, next, k, ws);
+            asm volatile("" ::: "memory");  // scales and codes are read again, not held until here
+            bool split = false;  // and not rows or blocks of zeros
+#pragma unroll
+            for (int t = 0; t < XT; ++t)
+#pragma unroll
+                for (int m = 0; m < MATS; ++m) split |= to_split(s.xs[wm * WM + 32 * t + n], ws[m]);
+            if (__any(split)) add.template operator()<true>(s, next, k, ws);
         }
     };
     const int steps = k1 - k0;
@@ -582,9 +593,9 @@ struct TileCost {
 // CU has one workgroup, and `each` a workgroup where that is more; a split of K adds a
 // launch and two passes over its sums; weights that no cache holds come at 4.4 TB/s (of
 // the last, of 256 MB, faster).  Measured (us), rows and tiles, in brackets weights in that cache:
-//   N 32000, K 4096      8 tokens 31.4 and 34.7 (31.3 and 26.0), 16 37.7 and 34.1, 32 46 and 36.8 (45.0 and 26.9)
-//   two of 11008, 4096   16 25.8 and 26.7, 32 29.5 and 29.1 (27.6 and 25.4);  128000, 4096  8 115 and 131
-//   4096, 4096           32 10.3 and 14.1, 64 (12.1 and 13.4);  11008, 4096  32 20.3 and 18.2
+//   N 32000, K 4096      8 tokens 33.2 and 34.1 (31.5 and 25.9), 16 36.8 and 34.8, 32 46 and 36.9 (44.7 and 26.0)
+//   two of 11008, 4096   16 25.2 and 26.2, 32 29.9 and 28.6 (28.3 and 24.9);  128000, 4096  8 117 and 131
+//   4096, 4096           32 10.1 and 14.1, 64 (13.5 and 13.9);  4096, 11008  32 19.6 and 20.0
 // and of tiles, 333 tokens, K 11008 -> 4096: 64 x 64 whole 62, in two 53; 64 x 128 in two 56, in four 49; 128 x 128 in two
 // 52.
 Plan plan_of(size_t N, size_t K, size_t M, int mats) {
