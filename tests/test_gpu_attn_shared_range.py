@@ -2,8 +2,7 @@
 import numpy as np
 import pytest
 
-from test_gpu_attn_shared import F16, Q8, F, _Batch
-from memvanta_amd import capi
+from test_gpu_attn_shared import Q8, F, _Batch
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -29,4 +28,16 @@ def test_rows_of_both_ends(ctx, n_tokens):
         return k, v * F(2.0) ** rng.choice([-110, 0, 123], (len(v), 1)).astype(F)
     b = _Batch(ctx, rng, Q8, 200, [210, 300, 230][: len(n_tokens)], n_tokens, 4, 2, 64, value=value)
     b.check()
+    b.close()
+
+
+@pytest.mark.parametrize("power", [-110, -60, 60, 100, 110])
+@pytest.mark.parametrize("heads,kv_heads,hd", [(4, 2, 64), (2, 2, 256)])
+@pytest.mark.parametrize("prefix,n_tokens", [(300, [1] * 5), (33, [65, 1, 40])])
+def test_sizes_of_keys(ctx, power, heads, kv_heads, hd, prefix, n_tokens):
+    """Keys up to 2^113 and queries that make ordinary scores of them."""
+    rng = np.random.default_rng(power + 200)
+    b = _Batch(ctx, rng, Q8, prefix, [prefix + 20 + i for i in range(len(n_tokens))], n_tokens, heads, kv_heads, hd,
+               value=lambda k, v: (k * F(2.0 ** power), v))
+    b.check((b.q * F(2.0 ** -power)).astype(F))
     b.close()
